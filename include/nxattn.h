@@ -278,6 +278,52 @@ int nxa_ssm_io_bwd(int64_t nb, int32_t L, int32_t d, int32_t n, int32_t dtype, c
                    void* ddelta, float* dA, void* dB, void* dC, float* dD,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention over packed sequences: nseq sequences of any lengths (zero too)
+ * laid end to end along the T rows of q, k and v, sequence s at rows
+ * offsets[s] .. offsets[s + 1] - 1; every query attends the keys of its own
+ * sequence (causal: those up to itself).  H query heads, H / Hk of which
+ * share a key-value head: query head h reads head h / (H / Hk).  No
+ * counterpart in the reference.
+ * q [H, T, D], k [Hk, T, D], v [Hk, T, Dv], o [H, T, Dv] with unit stride
+ * over the head dim and any head and row strides (whole 16-byte chunks; 64
+ * rows must span less than 2^32 bytes); head dims as in nxa_desc.
+ * offsets: nseq + 1 int32 on the device, non-decreasing in 0 .. T; values
+ * outside are taken as the nearest bound and a sequence that ends before it
+ * starts as empty (with decreasing offsets rows may belong to two sequences
+ * and hold either's result).  Rows of no sequence (before offsets[0], from
+ * offsets[nseq] on) are never read and their o, dq, dk, dv are zero.
+ * lse [H, T] (natural log; may be NULL in the forward): rows of no sequence
+ * are not written. */
+typedef struct {
+  int32_t T, nseq, H, Hk, D, Dv;
+  int32_t io_dtype;       /* nxa_dtype of every tensor but lse               */
+  int32_t causal;
+  float scale;
+  int64_t q_str[2];       /* head and row strides                            */
+  int64_t k_str[2];
+  int64_t v_str[2];
+  int64_t o_str[2];
+} nxa_packed_desc;
+
+/* Host-only validation (no GPU needed). */
+int nxa_packed_check(const nxa_packed_desc* desc);
+
+int nxa_packed_fwd(const nxa_packed_desc* desc, const void* q, const void* k, const void* v,
+                   const int32_t* offsets, void* o, float* lse, void* stream);
+
+/* Bytes of the backward's workspace (256-byte aligned; scratch of one call):
+ * two fp32 values a query row. */
+size_t nxa_packed_workspace_bytes(const nxa_packed_desc* desc);
+
+/* dq, dk, dv (strides of their own) from dout; o and lse as the forward left
+ * them.  dk and dv are summed over the query heads that share them, in a
+ * fixed order. */
+int nxa_packed_bwd(const nxa_packed_desc* desc, const void* q, const void* k, const void* v,
+                   const int32_t* offsets, const void* o, const float* lse, const void* dout,
+                   const int64_t* do_str, void* dq, const int64_t* dq_str, void* dk,
+                   const int64_t* dk_str, void* dv, const int64_t* dv_str, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 /* Message of the last failure on this thread ("" if none). */
 const char* nxa_last_error(void);
 

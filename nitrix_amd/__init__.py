@@ -21,6 +21,11 @@ from .attention import (
     scaled_dot_product_attention,
     scaled_dot_product_attention_hip,
 )
+from .packed import (
+    packed_attention,
+    packed_attention_hip,
+    reference_packed_attention,
+)
 from .ssm import (
     reference_selective_scan,
     selective_scan,
@@ -32,7 +37,10 @@ __all__ = [
     'NitrixBackendError',
     'NitrixBackendFallback',
     'default_scale',
+    'packed_attention',
+    'packed_attention_hip',
     'qk_rms_norm',
+    'reference_packed_attention',
     'reference_scaled_dot_product_attention',
     'reference_selective_scan',
     'reproducible',

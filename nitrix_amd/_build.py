@@ -46,6 +46,8 @@ HIPCC_FLAGS = [
 FILE_FLAGS = {
     'nxa_fwd16_wide.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
     'nxa_bwd16_wide.hip': ['-mllvm', '-amdgpu-sched-strategy=max-ilp'],
+    'nxa_packed_fwd16_wide.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
+    'nxa_packed_bwd16_wide.hip': ['-mllvm', '-amdgpu-sched-strategy=max-ilp'],
 }
 
 

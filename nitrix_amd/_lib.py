@@ -67,6 +67,10 @@ EXPORTS = (
     'nxa_ssm_io_workspace_bytes',
     'nxa_ssm_io_fwd',
     'nxa_ssm_io_bwd',
+    'nxa_packed_check',
+    'nxa_packed_fwd',
+    'nxa_packed_workspace_bytes',
+    'nxa_packed_bwd',
     'nxa_last_error',
     'nxa_profile_enable',
     'nxa_profile_read',
@@ -74,6 +78,7 @@ EXPORTS = (
 )
 
 _I64x3 = ctypes.c_int64 * 3
+I64x2 = ctypes.c_int64 * 2
 
 
 class NxaDesc(ctypes.Structure):
@@ -96,6 +101,26 @@ class NxaDesc(ctypes.Structure):
         ('bias_str', _I64x3),
         ('mask_str', _I64x3),
         ('Dv', ctypes.c_int32),
+    ]
+
+
+class NxaPackedDesc(ctypes.Structure):
+    """Mirror of ``nxa_packed_desc``."""
+
+    _fields_ = [
+        ('T', ctypes.c_int32),
+        ('nseq', ctypes.c_int32),
+        ('H', ctypes.c_int32),
+        ('Hk', ctypes.c_int32),
+        ('D', ctypes.c_int32),
+        ('Dv', ctypes.c_int32),
+        ('io_dtype', ctypes.c_int32),
+        ('causal', ctypes.c_int32),
+        ('scale', ctypes.c_float),
+        ('q_str', I64x2),
+        ('k_str', I64x2),
+        ('v_str', I64x2),
+        ('o_str', I64x2),
     ]
 
 
@@ -175,6 +200,18 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nxa_ssm_io_bwd.restype = ctypes.c_int
     lib.nxa_ssm_io_bwd.argtypes = (
         [i64, i32, i32, i32, i32] + [vp] * 15 + [ctypes.c_size_t, vp]
+    )
+    pp = ctypes.POINTER(NxaPackedDesc)
+    s2 = ctypes.POINTER(ctypes.c_int64)
+    lib.nxa_packed_check.restype = ctypes.c_int
+    lib.nxa_packed_check.argtypes = [pp]
+    lib.nxa_packed_fwd.restype = ctypes.c_int
+    lib.nxa_packed_fwd.argtypes = [pp] + [vp] * 7
+    lib.nxa_packed_workspace_bytes.restype = ctypes.c_size_t
+    lib.nxa_packed_workspace_bytes.argtypes = [pp]
+    lib.nxa_packed_bwd.restype = ctypes.c_int
+    lib.nxa_packed_bwd.argtypes = (
+        [pp] + [vp] * 7 + [s2] + [vp, s2] * 3 + [vp, ctypes.c_size_t, vp]
     )
     lib.nxa_last_error.restype = ctypes.c_char_p
     lib.nxa_last_error.argtypes = []

@@ -23,8 +23,43 @@
 // row r at c ^ swz32(r)), which keeps both access patterns free of bank
 // conflicts: 16 consecutive rows of 16-byte reads, and 32 consecutive
 // columns of rows r and r + 4 (r % 8 < 4) of 4-byte reads.
+//
+// With NXA_PACKED defined (nxa_packed32.hip includes this file) the kernels
+// run over packed sequences (nxa_packed.h), each block on its tile's sequence
+// as on a dense problem; a dK / dV block streams the query tiles of every
+// query head that shares its keys, one head after the other: tile t is tile
+// t % gcnt (from gfirst on) of head t / gcnt.
 #include "nxa_common.h"
 #include "nxa_launch.h"
+#ifdef NXA_PACKED
+#include "nxa_packed.h"
+#endif
+
+// Tile i of a block's active tiles, its class, the first query row of tile
+// t, and the row strides that a dense problem's gradients share with q, k
+// and v, and dO with o.
+#ifdef NXA_PACKED
+// Without the dense kernels' runtime branches a tile would be one scheduling
+// region, which costs the compiler's ordering of the products minutes a
+// kernel: the phases are kept apart instead.
+#define NXA_PHASE __builtin_amdgcn_sched_barrier(0)
+#define NXA_TILE_AT(i) (i)
+#define NXA_CLASS_AT(i) 3
+#define NXA_TILE_ROW(t) (gfirst + (t) % gcnt) * BQ
+#define NXA_DK_STRIDE grp.dk_rs
+#define NXA_DV_STRIDE grp.dv_rs
+#define NXA_DO_STRIDE pp.do_str[2]
+#define NXA_DQ_STRIDE pp.dq_str[2]
+#else
+#define NXA_PHASE (void)0
+#define NXA_TILE_AT(i) (int)(lst[i] & 0xffff)
+#define NXA_CLASS_AT(i) (int)(lst[i] >> 16)
+#define NXA_TILE_ROW(t) t * BQ
+#define NXA_DK_STRIDE p.k_str[2]
+#define NXA_DV_STRIDE p.v_str[2]
+#define NXA_DO_STRIDE p.o_str[2]
+#define NXA_DQ_STRIDE p.q_str[2]
+#endif
 
 namespace nxa {
 
@@ -326,18 +361,31 @@ __device__ __forceinline__ void fwd32_tile(const Params& p, const F32Offsets<DP>
 // reference, so the result is exact.
 // ---------------------------------------------------------------------------
 template <int DP, bool HAS_BIAS, bool CAUSAL>
+#ifdef NXA_PACKED
+__global__ __launch_bounds__(256, 1) void fwd32_kernel(const PackedParams pp) {
+#else
 __global__ __launch_bounds__(256, 1) void fwd32_kernel(const Params p) {
+#endif
   constexpr int BM = 128, BN = DP > 128 ? 32 : 64, NC = DP / 8, NDB = DP / 32;
   constexpr int TILE = BN * DP * 4;
   constexpr int STAGE = 2 * TILE;  // K, V
   using S = F32Stream<DP, 4, BN, (DP > 128)>;
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+#ifndef NXA_PACKED
   __shared__ uint32_t lst[kF32MaxTiles];
+#endif
 
+#ifdef NXA_PACKED
+  Params p;
+  int qt;
+  if (!packed_query_block<float>(pp, BM, p, qt)) return;
+  constexpr int b = 0, h = 0;
+#else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);
   const int bh = vid / p.nqt;
   const int qt = p.nqt - 1 - (vid % p.nqt);  // longest (causal) blocks first
   const int b = bh / p.H, h = bh % p.H;
+#endif
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c32 = lane & 31;
@@ -352,9 +400,13 @@ __global__ __launch_bounds__(256, 1) void fwd32_kernel(const Params p) {
 
   const int k_end = CAUSAL ? min(p.Lk, q0 + BM) : p.Lk;
   const int nk = (k_end + BN - 1) / BN;
+#ifdef NXA_PACKED
+  const int n = nk;
+#else
   const int n = list_tiles(lst, nk, wave, lane, [&](int t) -> int {
     return p.has_tilemap ? tile_class(p, b, h, q0, q0 + BM, t * BN, t * BN + BN) : 3;
   });
+#endif
 
   f32x4 qf[NC];
   {
@@ -382,7 +434,7 @@ __global__ __launch_bounds__(256, 1) void fwd32_kernel(const Params p) {
   lo.init(g, c32);
   const uint32_t lds0 = lds_offset(smem);
   auto issue = [&](int i, int st) NXA_INLINE {
-    const int t = i < n ? (int)(lst[i] & 0xffff) : nk;
+    const int t = i < n ? NXA_TILE_AT(i) : nk;
     const uint32_t at = lds0 + st * STAGE;
     const i32x4 rk = tile_rsrc<BN>(kp, p.k_str[2], t * BN, p.Lk, p.D);
     const i32x4 rv = tile_rsrc<BN>(vp, p.v_str[2], t * BN, p.Lk, p.Dv);
@@ -399,7 +451,7 @@ __global__ __launch_bounds__(256, 1) void fwd32_kernel(const Params p) {
   for (int i = 0; i < n; ++i) {
     const int st = i & 1;
     const uint32_t at = lds0 + st * STAGE;
-    const int t = (int)(lst[i] & 0xffff), cls = (int)(lst[i] >> 16);
+    const int t = NXA_TILE_AT(i), cls = NXA_CLASS_AT(i);
     const int k0 = t * BN;
     issue(i + 1, st ^ 1);
 
@@ -436,18 +488,31 @@ __global__ __launch_bounds__(256, 1) void fwd32_kernel(const Params p) {
 // Four times the blocks of the 32-query grid, the same arithmetic per tile.
 // ---------------------------------------------------------------------------
 template <bool HAS_BIAS, bool CAUSAL>
+#ifdef NXA_PACKED
+__global__ __launch_bounds__(256, 1) void fwd32s_kernel(const PackedParams pp) {
+#else
 __global__ __launch_bounds__(256, 1) void fwd32s_kernel(const Params p) {
+#endif
   constexpr int DP = 64, BM = 32, BN = 64, NC = DP / 8, NDB = DP / 32, NW = 4;
   constexpr int TILE = BN * DP * 4;
   using S = F32Stream<DP, 1>;
   __shared__ __attribute__((aligned(16))) char smem[NW * 2 * TILE];
+#ifndef NXA_PACKED
   __shared__ uint32_t lst[kF32MaxTiles];
+#endif
   static_assert(NW * 64 * (NDB * 16 + 2) * 4 <= NW * 2 * TILE, "the merge fits the stages");
 
+#ifdef NXA_PACKED
+  Params p;
+  int qt;
+  if (!packed_query_block<float>(pp, BM, p, qt)) return;
+  constexpr int b = 0, h = 0;
+#else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);
   const int bh = vid / p.nqt;
   const int qt = p.nqt - 1 - (vid % p.nqt);
   const int b = bh / p.H, h = bh % p.H;
+#endif
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c32 = lane & 31;
@@ -460,9 +525,13 @@ __global__ __launch_bounds__(256, 1) void fwd32s_kernel(const Params p) {
   const float* vp = (const float*)p.v + b * p.v_str[0] + h * p.v_str[1];
   const int k_end = CAUSAL ? min(p.Lk, q0 + BM) : p.Lk;
   const int nk = (k_end + BN - 1) / BN;
+#ifdef NXA_PACKED
+  const int n = nk;
+#else
   const int n = list_tiles(lst, nk, wave, lane, [&](int t) -> int {
     return p.has_tilemap ? tile_class(p, b, h, q0, q0 + BM, t * BN, t * BN + BN) : 3;
   });
+#endif
 
   f32x4 qf[NC];
   {
@@ -490,7 +559,7 @@ __global__ __launch_bounds__(256, 1) void fwd32s_kernel(const Params p) {
   lo.init(g, c32);
   const uint32_t at = lds_offset(smem) + wave * 2 * TILE;  // this wave's K, V
   for (int i = wave; i < n; i += NW) {
-    const int t = (int)(lst[i] & 0xffff), cls = (int)(lst[i] >> 16);
+    const int t = NXA_TILE_AT(i), cls = NXA_CLASS_AT(i);
     const i32x4 rk = tile_rsrc(kp, p.k_str[2], t * BN, p.Lk, p.D);
     const i32x4 rv = tile_rsrc(vp, p.v_str[2], t * BN, p.Lk, p.Dv);
 #pragma unroll
@@ -570,7 +639,11 @@ enum : int { kF32Dv = 1, kF32Dk = 2, kF32Both = 3 };
 // a stage of their own; their sums are added in LDS in a fixed order.
 // ---------------------------------------------------------------------------
 template <int DP, bool CAUSAL, int OUT = kF32Both, bool SPLIT = false>
+#ifdef NXA_PACKED
+__global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const PackedParams pp) {
+#else
 __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params p) {
+#endif
   constexpr bool DV = OUT & kF32Dv, DK = OUT & kF32Dk;
   static_assert(OUT == kF32Both || DP > 128, "split launches are for head dim 256");
   static_assert(!SPLIT || (OUT == kF32Both && DP == 64), "the merge is of dV and dK at head dim 64");
@@ -581,12 +654,22 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
   constexpr int STAGE = 2 * TILE + 2 * BQ * 4;  // Q, dO, -lse log2(e), -delta
   using S = F32Stream<DP, NW, BQ, (DP > 128)>;
   __shared__ __attribute__((aligned(16))) char smem[(SPLIT ? 4 : 2) * STAGE];
+#ifndef NXA_PACKED
   __shared__ uint32_t lst[kF32MaxTiles];
+#endif
 
+#ifdef NXA_PACKED
+  Params p;
+  int kt;
+  PackedGroup grp;
+  if (!packed_key_block<float>(pp, BNK, p, kt, grp)) return;
+  constexpr int b = 0, h = 0;
+#else
   const int vid = xcd_remap(blockIdx.x, p.nbh, p.nkt);
   const int bh = p.bh0 + vid / p.nkt;
   const int kt = vid % p.nkt;
   const int b = bh / p.H, h = bh % p.H;
+#endif
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c32 = lane & 31;
@@ -597,17 +680,28 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
   const bool kok = key < p.Lk;
   const int kc = kok ? key : p.Lk - 1;
 
+#ifdef NXA_PACKED
+  // (those of the group's first head)
+  const float *qp0 = (const float*)p.q, *dop0 = (const float*)p.dout;
+  const float *nlp0 = p.nlse2, *ndp0 = p.ndelta;
+#else
   const float* qp = (const float*)p.q + b * p.q_str[0] + h * p.q_str[1];
   const float* dop = (const float*)p.dout + b * p.o_str[0] + h * p.o_str[1];
   const float* nlp = p.nlse2 + ((int64_t)b * p.H + h) * p.Lq;
   const float* ndp = p.ndelta + ((int64_t)b * p.H + h) * p.Lq;
+#endif
 
+#ifdef NXA_PACKED
+  const int gfirst = CAUSAL ? kblk0 / BQ : 0, gcnt = (p.Lq + BQ - 1) / BQ - gfirst;
+  const int nq = grp.heads * gcnt, n = nq;
+#else
   const int nq = (p.Lq + BQ - 1) / BQ;
   const int n = list_tiles(lst, nq, wave, lane, [&](int t) -> int {
     const int q0 = t * BQ;
     if (CAUSAL && q0 + BQ - 1 < kblk0) return 0;
     return p.has_tilemap ? tile_class(p, b, h, q0, q0 + BQ, kblk0, kblk0 + BNK) : 3;
   });
+#endif
 
   // Stationary K and V rows of the lane's key (B operands; V only where dP
   // is formed).
@@ -632,7 +726,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
 
   S qs, ds_;
   qs.init(p.q_str[2], p.D, cw, lane);
-  ds_.init(p.o_str[2], p.Dv, cw, lane);
+  ds_.init(NXA_DO_STRIDE, p.Dv, cw, lane);
   F32Offsets<DP> lo;
   lo.init(g, c32);
   const uint32_t lds0 = lds_offset(smem);
@@ -641,11 +735,20 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
   // CNT Q and CNT dO copies, and BQ / NW rows of -lse log2(e) and -delta per
   // wave (lanes 0 .. BQ / NW - 1).
   auto issue = [&](int i, int st) NXA_INLINE {
+#ifdef NXA_PACKED
+    const int64_t hd = i < n ? i / gcnt : 0;
+    const int q0 = i < n ? NXA_TILE_ROW(i) : p.Lq;
+    const float* const qp = qp0 + hd * grp.q_hs;
+    const float* const dop = dop0 + hd * grp.do_hs;
+    const float* const nlp = nlp0 + hd * grp.row_hs;
+    const float* const ndp = ndp0 + hd * grp.row_hs;
+#else
     const int t = i < n ? (int)(lst[i] & 0xffff) : nq;
     const int q0 = t * BQ;
+#endif
     const uint32_t at = lds0 + st * STAGE;
     const i32x4 rq = tile_rsrc<BQ>(qp, p.q_str[2], q0, p.Lq, p.D);
-    const i32x4 ro = tile_rsrc<BQ>(dop, p.o_str[2], q0, p.Lq, p.Dv);
+    const i32x4 ro = tile_rsrc<BQ>(dop, NXA_DO_STRIDE, q0, p.Lq, p.Dv);
 #pragma unroll
     for (int m = 0; m < S::CNT; ++m) {
       qs.issue(rq, at, m, cw);
@@ -668,6 +771,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
   const bool full_db = p.dbias_mode == kDbiasFull;
 
   if (!SPLIT && n > 0) issue(0, 0);
+#ifndef NXA_PACKED
   if (DK && full_db && kok) {
     // A full dbias gets zeros where no query of a tile keeps this key block.
     int li = 0;
@@ -681,6 +785,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
         store_db32(p, dbbase + (int64_t)q * p.dbias_str[2], 0.f);
     }
   }
+#endif
   if constexpr (!SPLIT) {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     __syncthreads();
@@ -688,8 +793,8 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
   for (int i = SPLIT ? wave : 0; i < n; i += SPLIT ? 4 : 1) {
     const int st = SPLIT ? wave : i & 1;
     const uint32_t at = lds0 + st * STAGE;
-    const int t = (int)(lst[i] & 0xffff), cls = (int)(lst[i] >> 16);
-    const int q0 = t * BQ;
+    const int t = NXA_TILE_AT(i), cls = NXA_CLASS_AT(i);
+    const int q0 = NXA_TILE_ROW(t);
     if constexpr (SPLIT) {
       // Only this wave reads its stage: its own wait publishes the copies.
       // (The wait is no memory operation to the compiler and no barrier
@@ -760,6 +865,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
     }
     f32x16* s = acc;
     f32x16* dp = acc + NQB;
+    NXA_PHASE;
 
     // P and dS, element by element (the query is the accumulator row).
     typedef __attribute__((address_space(3))) f32x4 lds_f4;
@@ -797,6 +903,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
         }
       }
 
+    NXA_PHASE;
     // dV^T += dO^T P and dK^T += Q^T dS (A operands read transposed), in
     // halves of the head dim: four accumulators (dV and dK of two 32-column
     // blocks) interleaved, the fragments of the next step read during this
@@ -833,6 +940,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
 #pragma unroll
     for (int hb = 0; hb < (OUT == kF32Both ? NDB : 0); hb += 2) {
       constexpr int NA = NDB >= 2 ? 4 : 2, NS = 4 * NQB;
+      NXA_PHASE;
       f32x16 o[NA];
 #pragma unroll
       for (int u = 0; u < NA / 2; ++u) {
@@ -910,8 +1018,8 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
     for (int r = 0; r < 16; ++r) o[r] = total(wave * 16 + r);
     if (kok) {
       const bool is_k = wave & 1;
-      float* op = is_k ? (float*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * p.k_str[2]
-                       : (float*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * p.v_str[2];
+      float* op = is_k ? (float*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * NXA_DK_STRIDE
+                       : (float*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * NXA_DV_STRIDE;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int d0 = (wave >> 1) * 32 + 8 * c + 4 * g;
@@ -927,8 +1035,8 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
   }
 
   if (kok) {
-    float* dkp = (float*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * p.k_str[2];
-    float* dvp = (float*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * p.v_str[2];
+    float* dkp = (float*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * NXA_DK_STRIDE;
+    float* dvp = (float*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * NXA_DV_STRIDE;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -952,19 +1060,32 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
 // SPLIT as in dK / dV: 32 queries a block, every fourth 32-key tile a wave.
 // ---------------------------------------------------------------------------
 template <int DP, bool CAUSAL, bool SPLIT = false>
+#ifdef NXA_PACKED
+__global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const PackedParams pp) {
+#else
 __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p) {
+#endif
   constexpr int NW = SPLIT ? 1 : 4;  // waves that share a tile
   constexpr int BM = 32 * NW, BN = DP > 128 || SPLIT ? 32 : 64, NKB = BN / 32, NC = DP / 8, NDB = DP / 32;
   constexpr int TILE = BN * DP * 4;
   constexpr int STAGE = 2 * TILE;  // K, V
   using S = F32Stream<DP, NW, BN, (DP > 128)>;
   __shared__ __attribute__((aligned(16))) char smem[(SPLIT ? 4 : 2) * STAGE];
+#ifndef NXA_PACKED
   __shared__ uint32_t lst[kF32MaxTiles];
+#endif
 
+#ifdef NXA_PACKED
+  Params p;
+  int qt;
+  if (!packed_query_block<float>(pp, BM, p, qt)) return;
+  constexpr int b = 0, h = 0;
+#else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);
   const int bh = vid / p.nqt;
   const int qt = p.nqt - 1 - (vid % p.nqt);  // longest (causal) blocks first
   const int b = bh / p.H, h = bh % p.H;
+#endif
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c32 = lane & 31;
@@ -980,14 +1101,18 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
 
   const int k_end = CAUSAL ? min(p.Lk, q0 + BM) : p.Lk;
   const int nk = (k_end + BN - 1) / BN;
+#ifdef NXA_PACKED
+  const int n = nk;
+#else
   const int n = list_tiles(lst, nk, wave, lane, [&](int t) -> int {
     return p.has_tilemap ? tile_class(p, b, h, q0, q0 + BM, t * BN, t * BN + BN) : 3;
   });
+#endif
 
   f32x4 qf[NC], df[NC];
   {
     const float* qr = (const float*)p.q + b * p.q_str[0] + h * p.q_str[1] + (int64_t)qc * p.q_str[2];
-    const float* dr = (const float*)p.dout + b * p.o_str[0] + h * p.o_str[1] + (int64_t)qc * p.o_str[2];
+    const float* dr = (const float*)p.dout + b * p.o_str[0] + h * p.o_str[1] + (int64_t)qc * NXA_DO_STRIDE;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int d = 8 * c + 4 * g;
@@ -1011,7 +1136,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
   lo.init(g, c32);
   const uint32_t lds0 = lds_offset(smem);
   auto issue = [&](int i, int st) NXA_INLINE {
-    const int t = i < n ? (int)(lst[i] & 0xffff) : nk;
+    const int t = i < n ? NXA_TILE_AT(i) : nk;
     const uint32_t at = lds0 + st * STAGE;
     const i32x4 rk = tile_rsrc<BN>(kp, p.k_str[2], t * BN, p.Lk, p.D);
     const i32x4 rv = tile_rsrc<BN>(vp, p.v_str[2], t * BN, p.Lk, p.Dv);
@@ -1033,7 +1158,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
   for (int i = SPLIT ? wave : 0; i < n; i += SPLIT ? 4 : 1) {
     const int st = SPLIT ? wave : i & 1;
     const uint32_t at = lds0 + st * STAGE;
-    const int t = (int)(lst[i] & 0xffff), cls = (int)(lst[i] >> 16);
+    const int t = NXA_TILE_AT(i), cls = NXA_CLASS_AT(i);
     const int k0 = t * BN;
     if constexpr (SPLIT) {
       // Only this wave reads its stage: its own wait publishes the copies.
@@ -1082,6 +1207,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
     }
     f32x16* s = acc;
     f32x16* dp = acc + NKB;
+    NXA_PHASE;
 
     const bool need_mask = p.has_mask && !(cls & 2);
     const bool diag = CAUSAL && (k0 + BN - 1 > qw0);
@@ -1109,6 +1235,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
         }
       }
 
+    NXA_PHASE;
     // dQ^T += K^T dS^T, the accumulators of a group of NDH column blocks
     // interleaved (all NDB at once, or, at head dim 256, one half and then
     // the other, which halves the read-ahead registers), fragments read a
@@ -1168,7 +1295,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
       const int f = wave * 16 + r;
       o[r] = (slot(f, 0) + slot(f, 1)) + (slot(f, 2) + slot(f, 3));
     }
-    float* dqp = (float*)p.dq + b * p.q_str[0] + h * p.q_str[1] + (int64_t)qrow * p.q_str[2];
+    float* dqp = (float*)p.dq + b * p.q_str[0] + h * p.q_str[1] + (int64_t)qrow * NXA_DQ_STRIDE;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int d0 = wave * 32 + 8 * c + 4 * g;
@@ -1178,7 +1305,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
   }
 
   if (qok) {
-    float* dqp = (float*)p.dq + b * p.q_str[0] + h * p.q_str[1] + (int64_t)qrow * p.q_str[2];
+    float* dqp = (float*)p.dq + b * p.q_str[0] + h * p.q_str[1] + (int64_t)qrow * NXA_DQ_STRIDE;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -1189,6 +1316,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
   }
 }
 
+#ifndef NXA_PACKED
 // Launchers: false when the problem is outside what these kernels take
 // (more streamed tiles than a block lists).
 bool launch_fwd32(Params p, int dp, hipStream_t stream) {
@@ -1310,5 +1438,6 @@ bool launch_dq32(Params p, int dp, hipStream_t stream) {
   }
   return true;
 }
+#endif
 
 }  // namespace nxa

@@ -23,12 +23,36 @@
 //
 // Kernel and launcher templates; instantiated by nxa_bwd16.hip (head dims
 // 64 and 128) and nxa_bwd16_wide.hip (256, compiled with flags of its own).
+// With NXA_PACKED defined (nxa_packed_bwd16.hip, nxa_packed_bwd16_wide.hip)
+// the kernels run over packed sequences (nxa_packed.h), each block on its
+// tile's sequence as on a dense problem; a dK / dV block streams the query
+// tiles of every query head that shares its keys, one head after the other:
+// tile t is tile t % gcnt (from gfirst on) of head t / gcnt.
 #pragma once
 
 #include "nxa_common.h"
 #include "nxa_launch.h"
+#ifdef NXA_PACKED
+#include "nxa_packed.h"
+#endif
 
 #include <type_traits>
+
+// First query row of a dK / dV block's tile t; row strides of dO and of the
+// gradients, which a dense problem shares with o, q, k and v.
+#ifdef NXA_PACKED
+#define NXA_TILE_ROW(t) (gfirst + (t) % gcnt) * BQ
+#define NXA_DK_STRIDE grp.dk_rs
+#define NXA_DV_STRIDE grp.dv_rs
+#define NXA_DO_STRIDE pp.do_str[2]
+#define NXA_DQ_STRIDE pp.dq_str[2]
+#else
+#define NXA_TILE_ROW(t) t * BQ
+#define NXA_DK_STRIDE p.k_str[2]
+#define NXA_DV_STRIDE p.v_str[2]
+#define NXA_DO_STRIDE p.o_str[2]
+#define NXA_DQ_STRIDE p.q_str[2]
+#endif
 
 namespace nxa {
 
@@ -165,7 +189,11 @@ __device__ __forceinline__ float load_bias1(const Params& p, int64_t off) {
 //
 // ---------------------------------------------------------------------------
 template <typename T, int DP, bool HAS_BIAS, bool CAUSAL, int DBM>
+#ifdef NXA_PACKED
+__global__ __launch_bounds__(512, 1) void dkdv16_kernel(const PackedParams pp) {
+#else
 __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
+#endif
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int EPC = 8, KC = 16;
@@ -183,6 +211,13 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
   __shared__ uint8_t acls[kMaxBwdTiles], tcls[kMaxBwdTiles];
   __shared__ int sched_s[4];
 
+#ifdef NXA_PACKED
+  Params p;
+  int kt;
+  PackedGroup grp;
+  if (!packed_key_block<T>(pp, BNK, p, kt, grp)) return;
+  constexpr int b = 0, h = 0;
+#else
   const int vid = xcd_remap(blockIdx.x, p.nbh, p.nkt);
   const int bh = p.bh0 + vid / p.nkt;
   const int b = bh / p.H, h = bh % p.H;
@@ -190,6 +225,7 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
   // blocks are the longest and come first in index order).
   const int kt = p.order ? ordered_tile(p, b, h, p.ord_k128, vid % p.nkt, p.nkt)
                          : vid % p.nkt;
+#endif
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform
   const bool pw = wave < 4;                                   // role (uniform)
@@ -200,21 +236,40 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
   const bool kok = key < p.Lk;
   const int kc = kok ? key : p.Lk - 1;
 
+#ifdef NXA_PACKED
+  // (those of the group's first head)
+  const T *qp0 = (const T*)p.q, *dop0 = (const T*)p.dout;
+  const float *nlp0 = p.nlse2, *ndp0 = p.ndelta;
+#else
   const T* qp = (const T*)p.q + b * p.q_str[0] + h * p.q_str[1];
   const T* dop = (const T*)p.dout + b * p.o_str[0] + h * p.o_str[1];
   const float* nlp = p.nlse2 + ((int64_t)b * p.H + h) * p.Lq;
   const float* ndp = p.ndelta + ((int64_t)b * p.H + h) * p.Lq;
+#endif
+#ifdef NXA_PACKED
+  const int64_t qs = p.q_str[2], os = grp.do_rs;
+#else
   const int64_t qs = p.q_str[2], os = p.o_str[2];
+#endif
 
   // Query-tile classes (0 = nothing kept for this key block).
+#ifdef NXA_PACKED
+  const int gfirst = CAUSAL ? kblk0 / BQ : 0, gcnt = (p.Lq + BQ - 1) / BQ - gfirst;
+  const int nq = grp.heads * gcnt;
+#else
   const int nq = (p.Lq + BQ - 1) / BQ;
+#endif
   auto tclass_g = [&](int t) -> int {
     const int q0 = t * BQ;
     if (CAUSAL && q0 + BQ - 1 < kblk0) return 0;
     if (!p.has_tilemap) return 3;
     return tile_class(p, b, h, q0, q0 + BQ, kblk0, kblk0 + BNK);
   };
+#ifdef NXA_PACKED
+  const QTiles tl = {nq, 0, nq, 3, false, true, act, acls, tcls};
+#else
   const QTiles tl = build_qtiles(act, acls, tcls, sched_s, nq, tid, NW * 64, tclass_g);
+#endif
 
   // Stationary B operands for this lane's key: K (P wave) or V (dS wave).
   Frag bfr[NC];
@@ -294,7 +349,14 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
     i32x4 q, d, r;  // Q rows, dO rows, per-row values (-lse2 or -delta)
   };
   auto tile_src = [&](int t) NXA_INLINE -> TileSrc {
-    const int q0 = t < nq ? t * BQ : p.Lq;
+#ifdef NXA_PACKED
+    const int64_t hd = t < nq ? t / gcnt : 0;
+    const T* const qp = qp0 + hd * grp.q_hs;
+    const T* const dop = dop0 + hd * grp.do_hs;
+    const float* const nlp = nlp0 + hd * grp.row_hs;
+    const float* const ndp = ndp0 + hd * grp.row_hs;
+#endif
+    const int q0 = t < nq ? NXA_TILE_ROW(t) : p.Lq;
     // Rows of this tile that exist (0: empty ranges).  Each range covers
     // only the tile's own rows, so its byte size stays below 64 row strides,
     // which the host bounds below 2^32 bytes.
@@ -458,7 +520,7 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
   // `par`, then dV^T += dO^T P.
   auto p_tile = [&](int t, int cls, int st, int par, Frag (&pf)[2][FPB]) NXA_INLINE {
     const uint32_t at = lds0 + st * STAGE_BYTES;
-    const int q0 = t * BQ;
+    const int q0 = NXA_TILE_ROW(t);
     __builtin_amdgcn_s_setprio(DKDV_PRIO);  // the exp pass depends on these
     f32x16 x[2], rows[2];
     row_products(at, x, rows, [](int) {});
@@ -540,7 +602,7 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
   auto ds_lag = [&](int t, int st, int par, f32x16 (&x)[2], const TileSrc& s,
                     int stn) NXA_INLINE {
     const uint32_t at = lds0 + st * STAGE_BYTES;
-    const int q0 = t * BQ;
+    const int q0 = NXA_TILE_ROW(t);
     Frag pf[2][FPB];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
@@ -693,7 +755,7 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
   }
   if (kok) {
     if (!pw) {
-      T* dkp = (T*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * p.k_str[2];
+      T* dkp = (T*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * NXA_DK_STRIDE;
       const float sc = p.qk_norm ? 1.0f : p.scale;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -703,7 +765,7 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
           if (d0 < p.D) store4(dkp + d0, acc[db], 4 * c, sc);
         }
     } else {
-      T* dvp = (T*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * p.v_str[2];
+      T* dvp = (T*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * NXA_DV_STRIDE;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -734,7 +796,11 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
 // tile between its row products.
 // ---------------------------------------------------------------------------
 template <typename T, bool HAS_BIAS, bool CAUSAL, int DBM>
+#ifdef NXA_PACKED
+__global__ __launch_bounds__(256, 1) void dkdv256_kernel(const PackedParams pp) {
+#else
 __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
+#endif
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int DP = 256, EPC = 8, KC = 16;
@@ -750,6 +816,13 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
   __shared__ uint8_t acls[kMaxBwdTiles], tcls[kMaxBwdTiles];
   __shared__ int sched_s[4];
 
+#ifdef NXA_PACKED
+  Params p;
+  int kt;
+  PackedGroup grp;
+  if (!packed_key_block<T>(pp, BNK, p, kt, grp)) return;
+  constexpr int b = 0, h = 0;
+#else
   const int vid = xcd_remap(blockIdx.x, p.nbh, p.nkt);
   const int bh = p.bh0 + vid / p.nkt;
   const int b = bh / p.H, h = bh % p.H;
@@ -757,6 +830,7 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
   // blocks are the longest and come first in index order).
   const int kt = p.order ? ordered_tile(p, b, h, p.ord_k128, vid % p.nkt, p.nkt)
                          : vid % p.nkt;
+#endif
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform
   const int g = lane >> 5, c32 = lane & 31;
@@ -766,21 +840,40 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
   const bool kok = key < p.Lk;
   const int kc = kok ? key : p.Lk - 1;
 
+#ifdef NXA_PACKED
+  // (those of the group's first head)
+  const T *qp0 = (const T*)p.q, *dop0 = (const T*)p.dout;
+  const float *nlp0 = p.nlse2, *ndp0 = p.ndelta;
+#else
   const T* qp = (const T*)p.q + b * p.q_str[0] + h * p.q_str[1];
   const T* dop = (const T*)p.dout + b * p.o_str[0] + h * p.o_str[1];
   const float* nlp = p.nlse2 + ((int64_t)b * p.H + h) * p.Lq;
   const float* ndp = p.ndelta + ((int64_t)b * p.H + h) * p.Lq;
+#endif
+#ifdef NXA_PACKED
+  const int64_t qs = p.q_str[2], os = grp.do_rs;
+#else
   const int64_t qs = p.q_str[2], os = p.o_str[2];
+#endif
 
   // Query-tile classes (0 = nothing kept for this key block), as in dkdv16.
+#ifdef NXA_PACKED
+  const int gfirst = CAUSAL ? kblk0 / BQ : 0, gcnt = (p.Lq + BQ - 1) / BQ - gfirst;
+  const int nq = grp.heads * gcnt;
+#else
   const int nq = (p.Lq + BQ - 1) / BQ;
+#endif
   auto tclass_g = [&](int t) -> int {
     const int q0 = t * BQ;
     if (CAUSAL && q0 + BQ - 1 < kblk0) return 0;
     if (!p.has_tilemap) return 3;
     return tile_class(p, b, h, q0, q0 + BQ, kblk0, kblk0 + BNK);
   };
+#ifdef NXA_PACKED
+  const QTiles tl = {nq, 0, nq, 3, false, true, act, acls, tcls};
+#else
   const QTiles tl = build_qtiles(act, acls, tcls, sched_s, nq, tid, NW * 64, tclass_g);
+#endif
 
   // Stationary B operands of this lane's key: K (for S) and V (for dP).
   Frag kf[NC], vf[NC];
@@ -835,7 +928,14 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
     i32x4 q, d, r;
   };
   auto tile_src = [&](int t) NXA_INLINE -> TileSrc {
-    const int q0 = t < nq ? t * BQ : p.Lq;
+#ifdef NXA_PACKED
+    const int64_t hd = t < nq ? t / gcnt : 0;
+    const T* const qp = qp0 + hd * grp.q_hs;
+    const T* const dop = dop0 + hd * grp.do_hs;
+    const float* const nlp = nlp0 + hd * grp.row_hs;
+    const float* const ndp = ndp0 + hd * grp.row_hs;
+#endif
+    const int q0 = t < nq ? NXA_TILE_ROW(t) : p.Lq;
     const int rows = min(p.Lq - q0, BQ);  // 0: empty ranges
     TileSrc s;
     s.q = make_rsrc(qp + (int64_t)q0 * qs,
@@ -896,7 +996,7 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
   // ride along with the row products.
   auto tile = [&](int t, int cls, int st, const TileSrc& s, int stn) NXA_INLINE {
     const uint32_t at = lds0 + st * STAGE_BYTES;
-    const int q0 = t * BQ;
+    const int q0 = NXA_TILE_ROW(t);
     copy(s, stn, NCPY);
     // Per-row values of rows 8c + 4g .. +3: -delta seeds dP, -lse2 the logits.
     f32x16 xs, xp, rl;
@@ -1079,8 +1179,8 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
       for (int e = 0; e < 16; ++e) dk[db][e] = gy[db][e];
   }
   if (kok) {
-    T* dkp = (T*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * p.k_str[2];
-    T* dvp = (T*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * p.v_str[2];
+    T* dkp = (T*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * NXA_DK_STRIDE;
+    T* dvp = (T*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * NXA_DV_STRIDE;
     const float sc = p.qk_norm ? 1.0f : p.scale;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -1112,7 +1212,11 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
 // per 32-key block, as in the forward; other biases take the element pass.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int BMODE, bool CAUSAL>
+#ifdef NXA_PACKED
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const PackedParams pp) {
+#else
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const Params p) {
+#endif
   using M = Mma<T>;
   using Frag = typename M::Frag;
   using MB = Mma<bf16>;  // the ones-column product of -delta
@@ -1135,6 +1239,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const Param
   __shared__ uint32_t ainfo[kMaxBwdTiles];  // active key tiles, in order: index | class << 30
   __shared__ int nact_s;
 
+#ifdef NXA_PACKED
+  Params p;
+  int qt;
+  if (!packed_query_block<T>(pp, BM, p, qt)) return;
+  constexpr int b = 0, h = 0;
+#else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);
   const int bh = vid / p.nqt;
   const int b = bh / p.H, h = bh % p.H;
@@ -1142,6 +1252,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const Param
   // query blocks, which see the most keys.
   const int qt = p.order ? ordered_tile(p, b, h, p.ord_q128, vid % p.nqt, p.nqt)
                          : p.nqt - 1 - (vid % p.nqt);
+#endif
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform
   const int g = lane >> 5, c32 = lane & 31;
@@ -1195,7 +1306,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const Param
     const T* qp = (const T*)p.q + b * p.q_str[0] + h * p.q_str[1] +
                   (int64_t)qc * p.q_str[2];
     const T* dop = (const T*)p.dout + b * p.o_str[0] + h * p.o_str[1] +
-                   (int64_t)qc * p.o_str[2];
+                   (int64_t)qc * NXA_DO_STRIDE;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int d = c * KC + g * EPC;
@@ -1537,7 +1648,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const Param
       for (int e = 0; e < 16; ++e) dq[db][e] = gy[db][e];
   }
   if (qok) {
-    T* dqp = (T*)p.dq + b * p.q_str[0] + h * p.q_str[1] + (int64_t)qrow * p.q_str[2];
+    T* dqp = (T*)p.dq + b * p.q_str[0] + h * p.q_str[1] + (int64_t)qrow * NXA_DQ_STRIDE;
     const float sc = p.qk_norm ? 1.0f : p.scale;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -1552,6 +1663,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const Param
 // ---------------------------------------------------------------------------
 // Launchers.
 // ---------------------------------------------------------------------------
+#ifndef NXA_PACKED
 template <typename T, int DP, bool HB, bool CA, int DBM>
 static void launch_dkdv16_t(Params p, hipStream_t stream) {
   p.nkt = (p.Lk + 127) / 128;
@@ -1619,5 +1731,6 @@ static void launch_dq16_flags(const Params& p, hipStream_t stream) {
   else if (p.fwd_bias == kFbRow) launch_dq16_c<T, DP, kFbRow>(p, stream);
   else launch_dq16_c<T, DP, kFbValu>(p, stream);
 }
+#endif
 
 }  // namespace nxa

@@ -1361,3 +1361,5 @@ int nxa_profile_reset(void) {
 }
 
 }  // extern "C"
+
+#include "nxa_capi_packed.h"

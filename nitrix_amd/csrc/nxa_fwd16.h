@@ -47,10 +47,17 @@
 //
 // Kernel and launcher templates; instantiated by nxa_fwd16.hip (head dims
 // 64 and 128) and nxa_fwd16_wide.hip (256, compiled with flags of its own).
+// With NXA_PACKED defined (nxa_packed_fwd16.hip, nxa_packed_fwd16_wide.hip)
+// the kernel runs over packed sequences: its grid is that of nxa_packed.h,
+// and each block works on its tile's sequence as on a dense problem of one
+// head.
 #pragma once
 
 #include "nxa_common.h"
 #include "nxa_launch.h"
+#ifdef NXA_PACKED
+#include "nxa_packed.h"
+#endif
 
 #include <type_traits>
 
@@ -126,7 +133,11 @@ struct FwdRing {
 // 4 waves and one block per CU, so that each wave has the 512 registers that
 // its stationary Q (64) and O (128) need.
 template <typename T, int DP, int NW, int BMODE, bool CAUSAL>
+#ifdef NXA_PACKED
+__global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const PackedParams pp) {
+#else
 __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const Params p) {
+#endif
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int EPC = 8, KC = 16;
@@ -159,6 +170,12 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const 
   __shared__ int mslot_kt[kMaskSlots];
   __shared__ uint32_t mslot_w[kMaskSlots * 16];
 
+#ifdef NXA_PACKED
+  Params p;
+  int qt;
+  if (!packed_query_block<T>(pp, BM, p, qt)) return;
+  constexpr int b = 0, h = 0;
+#else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);
   const int bh = vid / p.nqt;
   const int b = bh / p.H, h = bh % p.H;
@@ -167,6 +184,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const 
   const int qt = p.order ? ordered_tile(p, b, h, BM == 128 ? p.ord_q128 : p.ord_q256,
                                         vid % p.nqt, p.nqt)
                          : p.nqt - 1 - (vid % p.nqt);
+#endif
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform
   const int g = lane >> 5, c32 = lane & 31;
@@ -945,6 +963,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const 
   }
 }
 
+#ifndef NXA_PACKED
 template <typename T, int DP, int NW, int BMODE, bool CA>
 static void launch_fwd16_t(Params p, hipStream_t stream) {
   constexpr int BM = NW * 32;
@@ -991,5 +1010,6 @@ static void launch_fwd16_flags(const Params& p, hipStream_t stream) {
     default: launch_fwd16_nw<T, DP, kFbNone>(p, stream); break;
   }
 }
+#endif
 
 }  // namespace nxa

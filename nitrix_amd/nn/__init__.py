@@ -5,9 +5,12 @@ from ..attention import (
     reference_scaled_dot_product_attention,
     scaled_dot_product_attention,
 )
+from ..packed import packed_attention, reference_packed_attention
 from ..ssm import reference_selective_scan, selective_scan
 
 __all__ = [
+    'packed_attention',
+    'reference_packed_attention',
     'reference_scaled_dot_product_attention',
     'reference_selective_scan',
     'scaled_dot_product_attention',

@@ -324,6 +324,88 @@ int nxa_packed_bwd(const nxa_packed_desc* desc, const void* q, const void* k, co
                    const int64_t* dk_str, void* dv, const int64_t* dv_str, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/* Paged key-value cache.  A pool is P pages of PS token slots for each of Hk
+ * heads: k_pages [P, Hk, PS, D], v_pages [P, Hk, PS, Dv], unit stride over the
+ * head dim, any page, head and slot strides (whole 16-byte chunks; 64 slots
+ * must span less than 2^32 bytes).  A page table holds, row by row, the pages
+ * of each sequence in order: token j of sequence b is slot j % PS of page
+ * table[b][j / PS].  An entry outside 0 .. P - 1 is no page.  Page tables,
+ * lengths, counts and row numbers are int32 on the device; ones outside their
+ * range are skipped, never followed.  No counterpart in the reference. */
+typedef struct {
+  int32_t P, Hk, PS, D, Dv;
+  int32_t io_dtype;       /* nxa_dtype of the pool, q, k, v and o            */
+  int64_t k_str[3];       /* page, head and slot strides                     */
+  int64_t v_str[3];
+} nxa_pool_desc;
+
+/* Host-only validation (no GPU needed). */
+int nxa_pool_check(const nxa_pool_desc* desc);
+
+/* Attention of one new token a sequence: o[b, h] = softmax(scale q[b, h] . k)
+ * v over the first lengths[b] tokens of sequence b (at most M * PS; a negative
+ * length is zero), key-value head h / (H / Hk).  q [B, H, D], o [B, H, Dv]
+ * with sequence and head strides.  Tokens in no page take no part; a row
+ * without tokens (or whose scores are all -inf) is zero.  The workspace
+ * (16-byte aligned) is scratch of one call. */
+size_t nxa_paged_workspace_bytes(const nxa_pool_desc* desc, int32_t B, int32_t M, int32_t H);
+int nxa_paged_fwd(const nxa_pool_desc* desc, const void* k_pages, const void* v_pages,
+                  const void* q, const int64_t* q_str, const int32_t* table, int64_t table_rs,
+                  const int32_t* lengths, int32_t B, int32_t M, int32_t H, float scale, void* o,
+                  const int64_t* o_str, void* workspace, size_t workspace_bytes, void* stream);
+
+/* New tokens k [Hk, T, D], v [Hk, T, Dv] (head and token strides) into their
+ * pages.  With offsets (B + 1, as nxa_packed_desc) token t of sequence s goes
+ * to position starts[s] + t - offsets[s]; without (T = B) token s to
+ * starts[s].  Tokens of no sequence, outside the table or in no page are
+ * dropped.  Of tokens meant for one slot (rows that share a page there) either
+ * may stay, by 16-byte chunks. */
+int nxa_pages_write(const nxa_pool_desc* desc, void* k_pages, void* v_pages, const void* k,
+                    const int64_t* k_str, const void* v, const int64_t* v_str, int64_t T,
+                    const int32_t* table, int64_t table_rs, const int32_t* starts,
+                    const int32_t* offsets, int32_t B, int32_t M, void* stream);
+
+/* Page src[i] to page dst[i], both lists on the host.  Pages outside the pool
+ * are NXA_E_ARG; the caller sees to it that no page is a target twice or both
+ * a source and a target. */
+int nxa_pages_copy(const nxa_pool_desc* desc, void* k_pages, void* v_pages, const int32_t* src,
+                   const int32_t* dst, int32_t n, void* stream);
+
+/* Page management on contiguous tables [B, M], with reference counts refs [P]:
+ * how many table entries name a page (none: it is free).  Results go to
+ * arrays of their own.
+ * free: the n listed rows (a row listed twice counts once) give their pages
+ * back, become -1 and of length zero.
+ * extend: row b grows by counts[b] tokens (negative: none; at most to M * PS);
+ * columns that these reach and that hold no page take free pages, lowest
+ * first, in row and column order.  Where pages run out a row's length ends
+ * with its last token that has one.  Workspace: P * 4 bytes.
+ * fork: row dst[i] becomes a copy of row src[i], for n pairs (of those with
+ * one target the last counts; src[i] == dst[i] does nothing): whole pages are
+ * shared, the tokens of a partly filled last page copied to a free page
+ * (lowest first, in order of i; without one the row ends with its whole
+ * pages).  The target's former pages are given back, but not handed out by
+ * this call.
+ * compact: n live pages end up in 0 .. n - 1: the k-th live page from n on is
+ * copied to the k-th free one below n, and table entries and counts follow. */
+int nxa_pages_free(int32_t B, int32_t M, int32_t P, const int32_t* table,
+                   const int32_t* lengths, const int32_t* refs, const int32_t* rows, int32_t n,
+                   int32_t* table_out, int32_t* lengths_out, int32_t* refs_out, void* stream);
+int nxa_pages_extend(int32_t B, int32_t M, int32_t P, int32_t PS, const int32_t* table,
+                     const int32_t* lengths, const int32_t* refs, const int32_t* counts,
+                     int32_t* table_out, int32_t* lengths_out, int32_t* refs_out,
+                     void* workspace, size_t workspace_bytes, void* stream);
+size_t nxa_pages_fork_workspace_bytes(int32_t B, int32_t P, int32_t n);
+int nxa_pages_fork(const nxa_pool_desc* desc, void* k_pages, void* v_pages, int32_t B, int32_t M,
+                   const int32_t* table, const int32_t* lengths, const int32_t* refs,
+                   const int32_t* src, const int32_t* dst, int32_t n, int32_t* table_out,
+                   int32_t* lengths_out, int32_t* refs_out, void* workspace,
+                   size_t workspace_bytes, void* stream);
+size_t nxa_pages_compact_workspace_bytes(int32_t P);
+int nxa_pages_compact(const nxa_pool_desc* desc, void* k_pages, void* v_pages, int64_t entries,
+                      const int32_t* table, const int32_t* refs, int32_t* table_out,
+                      int32_t* refs_out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Message of the last failure on this thread ("" if none). */
 const char* nxa_last_error(void);
 

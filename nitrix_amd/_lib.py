@@ -71,6 +71,17 @@ EXPORTS = (
     'nxa_packed_fwd',
     'nxa_packed_workspace_bytes',
     'nxa_packed_bwd',
+    'nxa_pool_check',
+    'nxa_paged_workspace_bytes',
+    'nxa_paged_fwd',
+    'nxa_pages_write',
+    'nxa_pages_copy',
+    'nxa_pages_free',
+    'nxa_pages_extend',
+    'nxa_pages_fork_workspace_bytes',
+    'nxa_pages_fork',
+    'nxa_pages_compact_workspace_bytes',
+    'nxa_pages_compact',
     'nxa_last_error',
     'nxa_profile_enable',
     'nxa_profile_read',
@@ -121,6 +132,21 @@ class NxaPackedDesc(ctypes.Structure):
         ('k_str', I64x2),
         ('v_str', I64x2),
         ('o_str', I64x2),
+    ]
+
+
+class NxaPoolDesc(ctypes.Structure):
+    """Mirror of ``nxa_pool_desc``."""
+
+    _fields_ = [
+        ('P', ctypes.c_int32),
+        ('Hk', ctypes.c_int32),
+        ('PS', ctypes.c_int32),
+        ('D', ctypes.c_int32),
+        ('Dv', ctypes.c_int32),
+        ('io_dtype', ctypes.c_int32),
+        ('k_str', _I64x3),
+        ('v_str', _I64x3),
     ]
 
 
@@ -213,6 +239,34 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nxa_packed_bwd.argtypes = (
         [pp] + [vp] * 7 + [s2] + [vp, s2] * 3 + [vp, ctypes.c_size_t, vp]
     )
+    dl = ctypes.POINTER(NxaPoolDesc)
+    sz = ctypes.c_size_t
+    lib.nxa_pool_check.restype = ctypes.c_int
+    lib.nxa_pool_check.argtypes = [dl]
+    lib.nxa_paged_workspace_bytes.restype = sz
+    lib.nxa_paged_workspace_bytes.argtypes = [dl, i32, i32, i32]
+    lib.nxa_paged_fwd.restype = ctypes.c_int
+    lib.nxa_paged_fwd.argtypes = [
+        dl, vp, vp, vp, s2, vp, i64, vp, i32, i32, i32, ctypes.c_float, vp, s2, vp, sz, vp,
+    ]
+    lib.nxa_pages_write.restype = ctypes.c_int
+    lib.nxa_pages_write.argtypes = [dl, vp, vp, vp, s2, vp, s2, i64, vp, i64, vp, vp, i32, i32, vp]
+    lib.nxa_pages_copy.restype = ctypes.c_int
+    lib.nxa_pages_copy.argtypes = [dl, vp, vp, vp, vp, i32, vp]
+    lib.nxa_pages_free.restype = ctypes.c_int
+    lib.nxa_pages_free.argtypes = [i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, vp, vp]
+    lib.nxa_pages_extend.restype = ctypes.c_int
+    lib.nxa_pages_extend.argtypes = [i32] * 4 + [vp] * 8 + [sz, vp]
+    lib.nxa_pages_fork_workspace_bytes.restype = sz
+    lib.nxa_pages_fork_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.nxa_pages_fork.restype = ctypes.c_int
+    lib.nxa_pages_fork.argtypes = (
+        [dl, vp, vp, i32, i32] + [vp] * 5 + [i32] + [vp] * 4 + [sz, vp]
+    )
+    lib.nxa_pages_compact_workspace_bytes.restype = sz
+    lib.nxa_pages_compact_workspace_bytes.argtypes = [i32]
+    lib.nxa_pages_compact.restype = ctypes.c_int
+    lib.nxa_pages_compact.argtypes = [dl, vp, vp, i64] + [vp] * 5 + [sz, vp]
     lib.nxa_last_error.restype = ctypes.c_char_p
     lib.nxa_last_error.argtypes = []
     lib.nxa_profile_enable.restype = ctypes.c_int

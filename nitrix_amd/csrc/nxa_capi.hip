@@ -1363,3 +1363,4 @@ int nxa_profile_reset(void) {
 }  // extern "C"
 
 #include "nxa_capi_packed.h"
+#include "nxa_capi_paged.h"

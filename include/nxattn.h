@@ -289,8 +289,7 @@ int nxa_ssm_io_bwd(int64_t nb, int32_t L, int32_t d, int32_t n, int32_t dtype, c
  * rows must span less than 2^32 bytes); head dims as in nxa_desc.
  * offsets: nseq + 1 int32 on the device, non-decreasing in 0 .. T; values
  * outside are taken as the nearest bound and a sequence that ends before it
- * starts as empty (with decreasing offsets rows may belong to two sequences
- * and hold either's result).  Rows of no sequence (before offsets[0], from
+ * starts as empty (with decreasing offsets what rows hold is not defined).  Rows of no sequence (before offsets[0], from
  * offsets[nseq] on) are never read and their o, dq, dk, dv are zero.
  * lse [H, T] (natural log; may be NULL in the forward): rows of no sequence
  * are not written. */
@@ -312,7 +311,8 @@ int nxa_packed_fwd(const nxa_packed_desc* desc, const void* q, const void* k, co
                    const int32_t* offsets, void* o, float* lse, void* stream);
 
 /* Bytes of the backward's workspace (256-byte aligned; scratch of one call):
- * two fp32 values a query row. */
+ * two fp32 values a query row and, for few tokens and key-value heads, fp32
+ * partial sums of dk and dv. */
 size_t nxa_packed_workspace_bytes(const nxa_packed_desc* desc);
 
 /* dq, dk, dv (strides of their own) from dout; o and lse as the forward left

@@ -378,7 +378,7 @@ __global__ __launch_bounds__(256, 1) void fwd32_kernel(const Params p) {
 #ifdef NXA_PACKED
   Params p;
   int qt;
-  if (!packed_query_block<float>(pp, BM, p, qt)) return;
+  if (!packed_query_block<float, CAUSAL>(pp, BM, p, qt)) return;
   constexpr int b = 0, h = 0;
 #else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);
@@ -505,7 +505,7 @@ __global__ __launch_bounds__(256, 1) void fwd32s_kernel(const Params p) {
 #ifdef NXA_PACKED
   Params p;
   int qt;
-  if (!packed_query_block<float>(pp, BM, p, qt)) return;
+  if (!packed_query_block<float, CAUSAL>(pp, BM, p, qt)) return;
   constexpr int b = 0, h = 0;
 #else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);
@@ -662,7 +662,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dkdv32_kernel(const Params
   Params p;
   int kt;
   PackedGroup grp;
-  if (!packed_key_block<float>(pp, BNK, p, kt, grp)) return;
+  if (!packed_key_block<float, CAUSAL>(pp, BNK, p, kt, grp)) return;
   constexpr int b = 0, h = 0;
 #else
   const int vid = xcd_remap(blockIdx.x, p.nbh, p.nkt);
@@ -1078,7 +1078,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 1) void dq32_kernel(const Params p
 #ifdef NXA_PACKED
   Params p;
   int qt;
-  if (!packed_query_block<float>(pp, BM, p, qt)) return;
+  if (!packed_query_block<float, CAUSAL>(pp, BM, p, qt)) return;
   constexpr int b = 0, h = 0;
 #else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);

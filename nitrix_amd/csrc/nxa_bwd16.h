@@ -215,7 +215,7 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
   Params p;
   int kt;
   PackedGroup grp;
-  if (!packed_key_block<T>(pp, BNK, p, kt, grp)) return;
+  if (!packed_key_block<T, CAUSAL>(pp, BNK, p, kt, grp)) return;
   constexpr int b = 0, h = 0;
 #else
   const int vid = xcd_remap(blockIdx.x, p.nbh, p.nkt);
@@ -754,6 +754,18 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
       for (int e = 0; e < 16; ++e) acc[db][e] = gy[db][e];
   }
   if (kok) {
+#ifdef NXA_PACKED
+    if (grp.dk_part) {
+      float* op = pw ? grp.dv_part + (int64_t)key * grp.dv_rs : grp.dk_part + (int64_t)key * grp.dk_rs;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int d0 = db * 32 + 8 * c + 4 * g;
+          if (d0 < (pw ? p.Dv : p.D)) store4(op + d0, acc[db], 4 * c, pw ? 1.0f : p.scale);
+        }
+    } else
+#endif
     if (!pw) {
       T* dkp = (T*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * NXA_DK_STRIDE;
       const float sc = p.qk_norm ? 1.0f : p.scale;
@@ -820,7 +832,7 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
   Params p;
   int kt;
   PackedGroup grp;
-  if (!packed_key_block<T>(pp, BNK, p, kt, grp)) return;
+  if (!packed_key_block<T, CAUSAL>(pp, BNK, p, kt, grp)) return;
   constexpr int b = 0, h = 0;
 #else
   const int vid = xcd_remap(blockIdx.x, p.nbh, p.nkt);
@@ -1178,6 +1190,21 @@ __global__ __launch_bounds__(256, 1) void dkdv256_kernel(const Params p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) dk[db][e] = gy[db][e];
   }
+#ifdef NXA_PACKED
+  if (kok && grp.dk_part) {
+    float* dkp = grp.dk_part + (int64_t)key * grp.dk_rs;
+    float* dvp = grp.dv_part + (int64_t)key * grp.dv_rs;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int d0 = db * 32 + 8 * c + 4 * g;
+        if (d0 < p.D) store4(dkp + d0, dk[db], 4 * c, p.scale);
+        if (d0 < p.Dv) store4(dvp + d0, dv[db], 4 * c, 1.0f);
+      }
+    return;
+  }
+#endif
   if (kok) {
     T* dkp = (T*)p.dk + b * p.k_str[0] + h * p.k_str[1] + (int64_t)key * NXA_DK_STRIDE;
     T* dvp = (T*)p.dv + b * p.v_str[0] + h * p.v_str[1] + (int64_t)key * NXA_DV_STRIDE;
@@ -1242,7 +1269,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const Param
 #ifdef NXA_PACKED
   Params p;
   int qt;
-  if (!packed_query_block<T>(pp, BM, p, qt)) return;
+  if (!packed_query_block<T, CAUSAL>(pp, BM, p, qt)) return;
   constexpr int b = 0, h = 0;
 #else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);

@@ -122,7 +122,8 @@ int nxa_packed_fwd(const nxa_packed_desc* d, const void* q, const void* k, const
 
 size_t nxa_packed_workspace_bytes(const nxa_packed_desc* d) {
   if (check_packed(d)) return 0;
-  return 2 * align256((size_t)d->H * d->T * 4);
+  const nxa::PackedParams p = packed_params(d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+  return 2 * align256((size_t)d->H * d->T * 4) + 4 * nxa::packed_part_floats(p);
 }
 
 int nxa_packed_bwd(const nxa_packed_desc* d, const void* q, const void* k, const void* v,
@@ -156,8 +157,11 @@ int nxa_packed_bwd(const nxa_packed_desc* d, const void* q, const void* k, const
   set_strides(p.dq_str, dq_str);
   set_strides(p.dk_str, dk_str);
   set_strides(p.dv_str, dv_str);
+  const size_t rows = align256((size_t)d->H * d->T * 4);
   p.nlse2 = (float*)workspace;
-  p.ndelta = (float*)((char*)workspace + need / 2);
+  p.ndelta = (float*)((char*)workspace + rows);
+  p.parts = nxa::packed_parts(p);
+  p.dkv_part = (float*)((char*)workspace + 2 * rows);
   hipStream_t s = (hipStream_t)stream;
   return launch("packed_bwd", s, [&] { nxa::launch_packed_bwd(p, d->io_dtype, packed_dp(d), s); });
 }

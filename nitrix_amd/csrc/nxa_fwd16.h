@@ -121,7 +121,12 @@ struct FwdRing {
   static constexpr bool TILE_BIAS = BMODE == kFbTile;
   static_assert(DP <= 128 || (NW == 4 && !TILE_BIAS), "head dim 256: 4 waves, no bias tiles");
   static constexpr bool LAG = NW == 8 && !(TILE_BIAS && DP == 128);
+#ifdef NXA_PACKED
+  // (two blocks of 4 waves share a CU's LDS at head dim 128)
+  static constexpr int NST = DP > 128 || (DP == 128 && NW == 4) ? 2 : 4;
+#else
   static constexpr int NST = DP > 128 ? 2 : TILE_BIAS ? (LAG ? 3 : 2) : 4;  // K/V stages
+#endif
   static constexpr int AHEAD = LAG ? NST - 2 : NST - 1;      // K/V tiles ahead
   static constexpr int NSTB = TILE_BIAS ? (LAG ? 3 : 2) : 1;  // bias stages
   static constexpr int AHEADB = TILE_BIAS ? NSTB - 1 : 0;     // bias tiles ahead
@@ -173,7 +178,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const 
 #ifdef NXA_PACKED
   Params p;
   int qt;
-  if (!packed_query_block<T>(pp, BM, p, qt)) return;
+  if (!packed_query_block<T, CAUSAL>(pp, BM, p, qt)) return;
   constexpr int b = 0, h = 0;
 #else
   const int vid = xcd_remap(blockIdx.x, p.B * p.H, p.nqt);

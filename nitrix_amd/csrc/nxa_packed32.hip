@@ -32,8 +32,40 @@ __global__ __launch_bounds__(256) void packed_delta32_kernel(const PackedParams 
   }
 }
 
+// Head dim 64: the kernels whose four waves share 32 rows and split the
+// streamed tiles, against 128 rows a block and 32 a wave.  The first have four
+// times the blocks and waste fewer rows at a sequence's end, the second read
+// every tile once for four waves.  By 128-row blocks and tokens a sequence,
+// 8 heads on 2 unless said, us of the pass, large block -> change with the
+// split one: forward, 192 blocks (6 heads) of one sequence of 4096 1430 - 59,
+// causal 1487 - 159; 256 blocks 1434 + 16, sequences of 512 225 + 33; 20 volumes
+// of 250 tokens (235 blocks) 352 - 8.  dQ: 256 blocks, 512 tokens 225 - 4, causal
+// 224 - 19, 4096 1434 - 52, causal 1495 - 251; 1024 blocks, 512 tokens 760 + 19,
+// 2048 2737 - 17, causal 1589 - 43; volumes 352 - 49.  dK / dV: 64 blocks 374 -
+// 94; 256 blocks, all keys, 512 tokens 225 + 19, 4096 1434 + 57, causal 224 - 9,
+// 1495 - 306; volumes 352 - 15; 1024 blocks, causal 531 + 93.
+static int64_t blocks128(const PackedParams& p, int heads) { return (int64_t)heads * p.T / 128; }
+static bool split_fwd(const PackedParams& p) { return blocks128(p, p.Hk * p.G) < 240; }
+static bool split_dq(const PackedParams& p) {
+  const int64_t n = blocks128(p, p.Hk * p.G);
+  return n <= 512 || (n <= 1024 && p.T / p.nseq >= 2048);
+}
+static bool split_dkdv(const PackedParams& p) {
+  const int64_t n = blocks128(p, p.Hk * p.parts);
+  return n <= 128 || (n <= 256 && (p.causal || p.T / p.nseq < 320));
+}
+
 template <int DP, bool CA>
 static void launch_packed_fwd32_t(PackedParams p, hipStream_t stream) {
+  if constexpr (DP == 64) {
+    if (split_fwd(p)) {
+      p.slots = packed_slots(p, 32);
+      p.nwork = p.Hk * p.G * p.slots;
+      hipLaunchKernelGGL((fwd32s_kernel<false, CA>), dim3(p.nwork + kPackedZeroBlocks), dim3(256),
+                         0, stream, p);
+      return;
+    }
+  }
   p.slots = packed_slots(p, 128);
   p.nwork = p.Hk * p.G * p.slots;
   hipLaunchKernelGGL((fwd32_kernel<DP, false, CA>), dim3(p.nwork + kPackedZeroBlocks), dim3(256),
@@ -47,9 +79,26 @@ static void launch_packed_bwd32_t(PackedParams p, hipStream_t stream) {
   const int64_t rows = (int64_t)p.Hk * p.G * p.T;
   hipLaunchKernelGGL(packed_delta32_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0,
                      stream, p);
-  hipLaunchKernelGGL((dq32_kernel<DP, CA>), dim3(p.nwork + kPackedZeroBlocks), dim3(256), 0,
-                     stream, p);
-  const dim3 grid(p.Hk * p.slots);
+  PackedParams s = p;  // over 32-row tiles
+  s.slots = packed_slots(p, 32);
+  s.nwork = p.Hk * p.G * s.slots;
+  if constexpr (DP == 64) {
+    if (split_dq(p))
+      hipLaunchKernelGGL((dq32_kernel<DP, CA, true>), dim3(s.nwork + kPackedZeroBlocks), dim3(256),
+                         0, stream, s);
+    else
+      hipLaunchKernelGGL((dq32_kernel<DP, CA>), dim3(p.nwork + kPackedZeroBlocks), dim3(256), 0,
+                         stream, p);
+    if (split_dkdv(p)) {
+      hipLaunchKernelGGL((dkdv32_kernel<DP, CA, kF32Both, true>), dim3(p.Hk * p.parts * s.slots),
+                         dim3(256), 0, stream, s);
+      return;
+    }
+  } else {
+    hipLaunchKernelGGL((dq32_kernel<DP, CA>), dim3(p.nwork + kPackedZeroBlocks), dim3(256), 0,
+                       stream, p);
+  }
+  const dim3 grid(p.Hk * p.parts * p.slots);
   if constexpr (DP > 128) {
     hipLaunchKernelGGL((dkdv32_kernel<DP, CA, kF32Dv>), grid, dim3(256), 0, stream, p);
     hipLaunchKernelGGL((dkdv32_kernel<DP, CA, kF32Dk>), grid, dim3(256), 0, stream, p);

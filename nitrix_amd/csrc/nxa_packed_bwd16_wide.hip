@@ -11,8 +11,8 @@ static void launch_packed_wide_t(PackedParams p, hipStream_t stream) {
   p.nwork = p.Hk * p.G * p.slots;
   hipLaunchKernelGGL((dq16_kernel<T, 256, kFbNone, CA>), dim3(p.nwork + kPackedZeroBlocks),
                      dim3(256), 0, stream, p);
-  hipLaunchKernelGGL((dkdv256_kernel<T, false, CA, kDbNone>), dim3(p.Hk * p.slots), dim3(256), 0,
-                     stream, p);
+  hipLaunchKernelGGL((dkdv256_kernel<T, false, CA, kDbNone>), dim3(p.Hk * p.parts * p.slots),
+                     dim3(256), 0, stream, p);
 }
 
 void launch_packed_bwd16_wide(const PackedParams& p, int io_dtype, hipStream_t stream) {

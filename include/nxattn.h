@@ -292,7 +292,11 @@ int nxa_ssm_io_bwd(int64_t nb, int32_t L, int32_t d, int32_t n, int32_t dtype, c
  * starts as empty (with decreasing offsets what rows hold is not defined).  Rows of no sequence (before offsets[0], from
  * offsets[nseq] on) are never read and their o, dq, dk, dv are zero.
  * lse [H, T] (natural log; may be NULL in the forward): rows of no sequence
- * are not written. */
+ * are not written.
+ * o_lo (bf16, fp16; o's strides; may be NULL, and is ignored in fp32): what the
+ * rounding of o to 16 bits left, written by the forward for the backward's
+ * delta = sum o dO; without it delta is taken from the rounded o.  Rows of no
+ * sequence are not written. */
 typedef struct {
   int32_t T, nseq, H, Hk, D, Dv;
   int32_t io_dtype;       /* nxa_dtype of every tensor but lse               */
@@ -308,19 +312,19 @@ typedef struct {
 int nxa_packed_check(const nxa_packed_desc* desc);
 
 int nxa_packed_fwd(const nxa_packed_desc* desc, const void* q, const void* k, const void* v,
-                   const int32_t* offsets, void* o, float* lse, void* stream);
+                   const int32_t* offsets, void* o, void* o_lo, float* lse, void* stream);
 
 /* Bytes of the backward's workspace (256-byte aligned; scratch of one call):
  * two fp32 values a query row and, for few tokens and key-value heads, fp32
  * partial sums of dk and dv. */
 size_t nxa_packed_workspace_bytes(const nxa_packed_desc* desc);
 
-/* dq, dk, dv (strides of their own) from dout; o and lse as the forward left
- * them.  dk and dv are summed over the query heads that share them, in a
+/* dq, dk, dv (strides of their own) from dout; o, o_lo and lse as the forward
+ * left them.  dk and dv are summed over the query heads that share them, in a
  * fixed order. */
 int nxa_packed_bwd(const nxa_packed_desc* desc, const void* q, const void* k, const void* v,
-                   const int32_t* offsets, const void* o, const float* lse, const void* dout,
-                   const int64_t* do_str, void* dq, const int64_t* dq_str, void* dk,
+                   const int32_t* offsets, const void* o, const void* o_lo, const float* lse,
+                   const void* dout, const int64_t* do_str, void* dq, const int64_t* dq_str, void* dk,
                    const int64_t* dk_str, void* dv, const int64_t* dv_str, void* workspace,
                    size_t workspace_bytes, void* stream);
 

@@ -232,12 +232,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nxa_packed_check.restype = ctypes.c_int
     lib.nxa_packed_check.argtypes = [pp]
     lib.nxa_packed_fwd.restype = ctypes.c_int
-    lib.nxa_packed_fwd.argtypes = [pp] + [vp] * 7
+    lib.nxa_packed_fwd.argtypes = [pp] + [vp] * 8
     lib.nxa_packed_workspace_bytes.restype = ctypes.c_size_t
     lib.nxa_packed_workspace_bytes.argtypes = [pp]
     lib.nxa_packed_bwd.restype = ctypes.c_int
     lib.nxa_packed_bwd.argtypes = (
-        [pp] + [vp] * 7 + [s2] + [vp, s2] * 3 + [vp, ctypes.c_size_t, vp]
+        [pp] + [vp] * 8 + [s2] + [vp, s2] * 3 + [vp, ctypes.c_size_t, vp]
     )
     dl = ctypes.POINTER(NxaPoolDesc)
     sz = ctypes.c_size_t

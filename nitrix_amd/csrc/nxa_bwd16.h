@@ -560,6 +560,24 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
 #pragma unroll
       for (int f = 0; f < FPB; ++f) {
         pf[qb][f] = M::pack(x[qb], f);
+#ifdef NXA_PACKED
+        // fp16 P and fp16 dS would round twice at the same place: P in [0, 2)
+        // crosses in 16 bits of its own, 4 of exponent and 12 of mantissa (the
+        // float bits of P 2^-112, whose exponents end at 15), a quarter of
+        // fp16's step everywhere.
+        if constexpr (std::is_same<T, f16>::value) {
+          u32x4 px;
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const uint32_t lo = __float_as_uint(x[qb][8 * f + e] * 0x1p-112f) + 0x400u;
+            const uint32_t hi = __float_as_uint(x[qb][8 * f + e + 1] * 0x1p-112f) + 0x400u;
+            px[e >> 1] = lo >> 11 | (hi << 5 & 0xffff0000u);
+          }
+          *(lds_pfrag*)(uintptr_t)(poff + par * PB_BYTES + (qb * FPB + f) * 1024) =
+              __builtin_bit_cast(f16x8, px);
+          continue;
+        }
+#endif
         // The exchange carries P in fp16 whatever T is: P <= 1 here, fp16
         // holds it with more mantissa than bf16, and the dS wave multiplies
         // it in one mixed-precision FMA.
@@ -619,7 +637,16 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
           // fp16 P times fp32: an FMA with a zero addend on the converted
           // half, which the compiler emits as one mixed-precision
           // v_fma_mix_f32 (exact conversion, one rounding).
+#ifdef NXA_PACKED
+          float pe = (float)pb[e];
+          if constexpr (std::is_same<T, f16>::value) {
+            const uint32_t w = __builtin_bit_cast(u32x4, pb)[e >> 1];
+            pe = __uint_as_float(e & 1 ? w >> 5 & 0x07fff800u : (w & 0xffffu) << 11) * 0x1p112f;
+          }
+          const float ds = __builtin_fmaf(pe, x[qb][r], 0.0f);
+#else
           const float ds = __builtin_fmaf((float)pb[e], x[qb][r], 0.0f);
+#endif
           x[qb][r] = ds;
           if constexpr (DBM == kDbFull) {
             const int q = q0 + qb * 32 + 8 * (r >> 2) + 4 * g + (r & 3);
@@ -1357,6 +1384,18 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void dq16_kernel(const Param
 #pragma unroll
       for (int e = 0; e < EPC; ++e) dacc = __builtin_fmaf((float)of[e], (float)df[c][e], dacc);
     }
+#ifdef NXA_PACKED
+    if (const T* lo = packed_o_lo<T>(p)) {
+      lo += (int64_t)qc * p.o_str[2];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int d = c * KC + g * EPC;
+        const Frag lf = (qok && d < p.Dv) ? ld16(lo + d) : zero_frag<T>();
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) dacc = __builtin_fmaf((float)lf[e], (float)df[c][e], dacc);
+      }
+    }
+#endif
   }
   const float ndlt = -(dacc + shfl_xor32(dacc));
   const float neg_lse2 = -p.lse[rowid] * kLog2e;

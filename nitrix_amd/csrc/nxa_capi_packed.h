@@ -107,7 +107,7 @@ extern "C" {
 int nxa_packed_check(const nxa_packed_desc* desc) { return check_packed(desc); }
 
 int nxa_packed_fwd(const nxa_packed_desc* d, const void* q, const void* k, const void* v,
-                   const int32_t* offsets, void* o, float* lse, void* stream) {
+                   const int32_t* offsets, void* o, void* o_lo, float* lse, void* stream) {
   int rc = check_packed(d);
   if (!rc) rc = check_ptr16("q", q);
   if (!rc) rc = check_ptr16("k", k);
@@ -115,7 +115,9 @@ int nxa_packed_fwd(const nxa_packed_desc* d, const void* q, const void* k, const
   if (!rc) rc = check_ptr16("o", o);
   if (rc) return rc;
   if (!offsets) return fail(NXA_E_ARG, "offsets is NULL");
-  const nxa::PackedParams p = packed_params(d, q, k, v, offsets, o, lse);
+  if (o_lo && (uintptr_t)o_lo % 16) return fail(NXA_E_LAYOUT, "o_lo must be 16-byte aligned");
+  nxa::PackedParams p = packed_params(d, q, k, v, offsets, o, lse);
+  p.o_lo = d->io_dtype == NXA_F32 ? nullptr : o_lo;
   hipStream_t s = (hipStream_t)stream;
   return launch("packed_fwd", s, [&] { nxa::launch_packed_fwd(p, d->io_dtype, packed_dp(d), s); });
 }
@@ -127,7 +129,8 @@ size_t nxa_packed_workspace_bytes(const nxa_packed_desc* d) {
 }
 
 int nxa_packed_bwd(const nxa_packed_desc* d, const void* q, const void* k, const void* v,
-                   const int32_t* offsets, const void* o, const float* lse, const void* dout,
+                   const int32_t* offsets, const void* o, const void* o_lo, const float* lse,
+                   const void* dout,
                    const int64_t* do_str, void* dq, const int64_t* dq_str, void* dk,
                    const int64_t* dk_str, void* dv, const int64_t* dv_str, void* workspace,
                    size_t workspace_bytes, void* stream) {
@@ -148,7 +151,9 @@ int nxa_packed_bwd(const nxa_packed_desc* d, const void* q, const void* k, const
   if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)
     return fail(NXA_E_WORKSPACE, "workspace of %zu bytes, %zu needed (256-byte aligned)",
                 workspace ? workspace_bytes : (size_t)0, need);
+  if (o_lo && (uintptr_t)o_lo % 16) return fail(NXA_E_LAYOUT, "o_lo must be 16-byte aligned");
   nxa::PackedParams p = packed_params(d, q, k, v, offsets, o, lse);
+  p.o_lo = d->io_dtype == NXA_F32 ? nullptr : const_cast<void*>(o_lo);
   p.dout = dout;
   p.dq = dq;
   p.dk = dk;

@@ -965,6 +965,27 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const 
       }
     if (g == 0 && p.lse)
       p.lse[((int64_t)b * p.H + h) * p.Lq + qrow] = (m_ref + __log2f(l)) * kLn2;
+#ifdef NXA_PACKED
+    // For the backward's delta = sum O dO: what the rounding of O left.  (Of
+    // delta's own size, a rounded O would leave dS of short sequences, where
+    // dP and delta nearly cancel, little but noise.)
+    if (T* lo = packed_o_lo<T>(p)) {
+      lo += (int64_t)qrow * p.o_str[2];
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int d0 = db * 32 + 8 * c + 4 * g;
+          f32x16 rest;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = oacc[db][4 * c + j] * inv;
+            rest[j] = x - (float)(T)x;
+          }
+          if (d0 < p.Dv) store4(lo + d0, rest, 0, 1.0f);
+        }
+    }
+#endif
   }
 }
 

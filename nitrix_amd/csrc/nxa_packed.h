@@ -35,6 +35,7 @@ struct PackedParams : Params {
   int slots;           // tile slots of the launching kernel
   int nwork;           // blocks with a slot; those behind zero the unowned rows
   int64_t do_str[3], dq_str[3], dk_str[3], dv_str[3];
+  void* o_lo;          // what rounding o to 16 bits left (o's strides), or null
   // dK / dV of a group of query heads in `parts` blocks, each over some of
   // them, whose fp32 sums go to dkv_part ([parts][Hk][T][D], then the same of
   // dV) and are added up afterwards (1: one block takes them all).
@@ -209,6 +210,13 @@ __device__ __forceinline__ PackedTile packed_tile(const PackedParams& pp, int ra
   return packed_find(pp, keys ? rank : pp.slots - 1 - rank, rows);
 }
 
+// The rows of o_lo that go with p.o (a packed problem has no qk-norm, whose
+// output pointer carries them).
+template <typename T>
+__device__ __forceinline__ T* packed_o_lo(const Params& p) {
+  return (T*)p.qn_out;
+}
+
 // Blocks of the forward and dQ kernels: one query tile of one query head.
 // False: nothing to do.
 template <typename T, bool CAUSAL>
@@ -237,7 +245,9 @@ __device__ __forceinline__ bool packed_query_block(const PackedParams& pp, int r
   p.q = (const T*)pp.q + hq * pp.q_str[1] + r0 * pp.q_str[2];
   p.k = (const T*)pp.k + hk * pp.k_str[1] + r0 * pp.k_str[2];
   p.v = (const T*)pp.v + hk * pp.v_str[1] + r0 * pp.v_str[2];
-  p.o = (T*)pp.o + hq * pp.o_str[1] + r0 * pp.o_str[2];
+  const int64_t ro = hq * pp.o_str[1] + r0 * pp.o_str[2];
+  p.o = (T*)pp.o + ro;
+  p.qn_out = pp.o_lo ? (T*)pp.o_lo + ro : nullptr;  // (packed_o_lo)
   const int64_t row = (int64_t)hq * pp.T + r0;
   if (pp.lse) p.lse = pp.lse + row;
   if (pp.dq) {

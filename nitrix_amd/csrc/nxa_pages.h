@@ -13,7 +13,7 @@ struct WriteParams : PoolParams {
   const int* table;
   int64_t table_rs;
   int64_t T;
-  int B, M, es, per;
+  int B, M, es;
 };
 
 // Page pairs in kernel arguments: no copy to the device, no buffer to keep.
@@ -40,6 +40,7 @@ struct RowsParams {
 };
 
 constexpr int kCompactPages = 4096;  // pages of a counting block
+constexpr int kCompactFew = 8;
 struct CompactParams {
   const int *table, *refs;
   int *table_out, *refs_out;
@@ -48,7 +49,7 @@ struct CompactParams {
   int P, Hk, PS;
 };
 
-void launch_pages_write(WriteParams p, hipStream_t stream);
+void launch_pages_write(const WriteParams& p, hipStream_t stream);
 void launch_pages_copy(const PoolParams& p, int es, const CopyPairs& pairs, hipStream_t stream);
 void launch_pages_free(const RowsParams& p, hipStream_t stream);
 void launch_pages_extend(const RowsParams& p, hipStream_t stream);

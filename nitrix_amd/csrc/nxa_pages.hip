@@ -103,17 +103,19 @@ __device__ int find_free(const int* refs, int P, int need, int* list, int* wsum)
 }  // namespace
 
 // ---------------------------------------------------------------------------
-// New tokens into their pages.  A wave takes kWriteTokens tokens in turn:
-// finds the token's sequence (64 probes a step among the offsets), its page,
-// and moves the rows of every head.
+// New tokens into their pages, a wave each: it finds the token's sequence (64
+// probes a step among the offsets) and page, and moves the rows of every head.
+// Bound by HBM: 16384 tokens of 8 heads of 128, 67 MB read and written, 27 us
+// (5.0 TB/s, the rate of a copy).  2 and 4 tokens a wave, one after the other,
+// wait for one another's lookups (34 and 36 us, 30.5 with one); the rows are
+// read once, past the caches (30.5 -> 27).
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void pages_write_kernel(const WriteParams p) {
   const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= p.T) return;
   const int ck = p.D * p.es / 16, cv = p.Dv * p.es / 16, all = p.Hk * (ck + cv);
-  for (int i = 0; i < p.per; ++i) {
-    const int64_t t = w * p.per + i;
-    if (t >= p.T) return;
+  {
     int s = (int)t;
     int64_t pos = 0;
     if (p.offsets) {
@@ -127,13 +129,13 @@ __global__ __launch_bounds__(256) void pages_write_kernel(const WriteParams p) {
         hi = min(lo + step, hi);
       }
       s = __builtin_amdgcn_readfirstlane(lo);
-      if (s >= p.B || p.offsets[s] > t) continue;
+      if (s >= p.B || p.offsets[s] > t) return;
       pos = t - p.offsets[s];
     }
     pos += p.starts[s];
-    if (pos < 0 || pos >= (int64_t)p.M * p.PS) continue;
+    if (pos < 0 || pos >= (int64_t)p.M * p.PS) return;
     const int page = p.table[s * p.table_rs + pos / p.PS];
-    if (!is_page(page, p.P)) continue;
+    if (!is_page(page, p.P)) return;
     const int slot = (int)(pos % p.PS);
     const char* ks = (const char*)p.ks + t * p.ks_str[1] * p.es;
     const char* vs = (const char*)p.vs + t * p.vs_str[1] * p.es;
@@ -146,7 +148,8 @@ __global__ __launch_bounds__(256) void pages_write_kernel(const WriteParams p) {
       const int h = y / cpr, c = 16 * (y - h * cpr);
       const char* src = key ? ks + h * p.ks_str[0] * p.es : vs + h * p.vs_str[0] * p.es;
       char* dst = key ? kd + h * p.k_str[1] * p.es : vd + h * p.v_str[1] * p.es;
-      *reinterpret_cast<u32x4*>(dst + c) = *reinterpret_cast<const u32x4*>(src + c);
+      *reinterpret_cast<u32x4*>(dst + c) =
+          __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + c));
     }
   }
 }
@@ -324,9 +327,10 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(const RowsParams p, con
 
 // ---------------------------------------------------------------------------
 // Compaction.  n live pages: the k-th live page from n on moves into the k-th
-// dead one below n.  Counting blocks of kCompactPages pages; then each block
+// dead one below n.  Blocks of kCompactPages pages are counted; then each block
 // adds up the counts before it and lists its movers and holes; then pages,
-// table and counts move.
+// table and counts move.  (Up to kCompactFew blocks count for themselves: a
+// launch of 3 us less.)
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(1024) void pages_count_kernel(const CompactParams p) {
   __shared__ int wsum[16];
@@ -342,11 +346,25 @@ __global__ __launch_bounds__(1024) void pages_count_kernel(const CompactParams p
 __global__ __launch_bounds__(1024) void pages_plan_kernel(const CompactParams p) {
   __shared__ int wsum[16];
   const int tid = threadIdx.x, nb = (p.P + kCompactPages - 1) / kCompactPages;
-  // Live pages in all (n), before this block, and before the block of page n.
+  const bool few = nb <= kCompactFew;  // (then not counted before)
+  // Live pages in all (n) and before this block.
   int part[2] = {0, 0};
-  for (int i = tid; i < nb; i += 1024) {
-    part[0] += p.counts[i];
-    part[1] += i < (int)blockIdx.x ? p.counts[i] : 0;
+  if (few) {
+    for (int i = 0; i < nb; ++i) {
+      int c = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = i * kCompactPages + 4 * tid + e;
+        c += at < p.P && p.refs[at] > 0;
+      }
+      part[0] += c;
+      part[1] += i < (int)blockIdx.x ? c : 0;
+    }
+  } else {
+    for (int i = tid; i < nb; i += 1024) {
+      part[0] += p.counts[i];
+      part[1] += i < (int)blockIdx.x ? p.counts[i] : 0;
+    }
   }
   int n, before;
   block_scan(part[0], wsum, n);
@@ -354,7 +372,13 @@ __global__ __launch_bounds__(1024) void pages_plan_kernel(const CompactParams p)
   // Live pages below n: those before its block and those of its block.
   const int bn = n / kCompactPages;
   int x = 0;
-  for (int i = tid; i < bn; i += 1024) x += p.counts[i];
+  if (few) {
+    for (int i = 0; i < bn; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x += p.refs[i * kCompactPages + 4 * tid + e] > 0;
+  } else {
+    for (int i = tid; i < bn; i += 1024) x += p.counts[i];
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int at = bn * kCompactPages + 4 * tid + i;
@@ -417,12 +441,8 @@ __global__ __launch_bounds__(256) void pages_move_kernel(const CompactParams p,
 // ---------------------------------------------------------------------------
 // Launchers.
 // ---------------------------------------------------------------------------
-void launch_pages_write(WriteParams p, hipStream_t stream) {
-  // Tokens a wave: enough that its lookups overlap the rows it moves, few
-  // enough that a small batch still spreads over the CUs.
-  p.per = p.T >= 16384 ? 4 : p.T >= 4096 ? 2 : 1;
-  const int64_t waves = (p.T + p.per - 1) / p.per;
-  hipLaunchKernelGGL(pages_write_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream, p);
+void launch_pages_write(const WriteParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(pages_write_kernel, dim3((unsigned)((p.T + 3) / 4)), dim3(256), 0, stream, p);
 }
 
 void launch_pages_copy(const PoolParams& p, int es, const CopyPairs& pairs, hipStream_t stream) {
@@ -460,7 +480,8 @@ void launch_pages_fork(const RowsParams& p, const PoolParams& pool, int es, hipS
 void launch_pages_compact(const CompactParams& p, const PoolParams& pool, int es,
                           hipStream_t stream) {
   const int nb = (p.P + kCompactPages - 1) / kCompactPages;
-  hipLaunchKernelGGL(pages_count_kernel, dim3(nb), dim3(1024), 0, stream, p);
+  if (nb > kCompactFew)
+    hipLaunchKernelGGL(pages_count_kernel, dim3(nb), dim3(1024), 0, stream, p);
   hipLaunchKernelGGL(pages_plan_kernel, dim3(nb), dim3(1024), 0, stream, p);
   hipLaunchKernelGGL(pages_move_kernel, dim3(2048), dim3(256), 0, stream, p, pool, es);
 }

@@ -16,6 +16,7 @@ axis; the reference has no counterpart.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional
 
@@ -28,6 +29,7 @@ from .attention import (
     _IO_DTYPES,
     _MAX_HEAD_DIM,
     HipNotTileable,
+    _ptr,
     _row_stride_ok,
     default_scale,
     reference_scaled_dot_product_attention,
@@ -166,6 +168,24 @@ def _empty_like(x: torch.Tensor, d: int) -> torch.Tensor:
     return torch.empty((h, t, d), dtype=x.dtype, device=x.device)
 
 
+_SAME_DEVICE = contextlib.nullcontext()
+# (the public current_stream() builds a Stream object, 2 us of a call's 20)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
+def _on(device: torch.device):
+    """Context in which ``device`` is current, for launches on its streams."""
+    if device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    if _raw_stream is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
+
+
 def _desc(q, k, v, o, offsets, scale, causal) -> _lib.NxaPackedDesc:
     desc = _lib.NxaPackedDesc()
     desc.H, desc.T, desc.D = q.shape
@@ -181,41 +201,45 @@ def _desc(q, k, v, o, offsets, scale, causal) -> _lib.NxaPackedDesc:
     return desc
 
 
-def _forward(q, k, v, offsets, scale, causal, want_lse):
+def _forward(q, k, v, offsets, scale, causal, train):
+    """The output and, for a backward, the log-sum-exp and what the rounding of
+    the output left (16-bit types)."""
     o = _empty_like(q, v.shape[2])
-    lse = None
-    if want_lse:
+    lse = o_lo = None
+    if train:
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        if q.dtype != torch.float32:
+            o_lo = _empty_like(q, v.shape[2])
     desc = _desc(q, k, v, o, offsets, scale, causal)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         _lib.check(
             _lib.lib().nxa_packed_fwd(
                 ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                offsets.data_ptr(), o.data_ptr(), None if lse is None else lse.data_ptr(),
-                torch.cuda.current_stream(q.device).cuda_stream,
+                offsets.data_ptr(), o.data_ptr(), _ptr(o_lo), _ptr(lse),
+                _stream(q.device),
             )
         )
-    return o, lse
+    return o, o_lo, lse
 
 
 class _PackedHip(torch.autograd.Function):
     """``(q, k, v, offsets) -> out``; the residuals are the inputs as the
-    kernels read them, the output and the log-sum-exp, kept with
+    kernels read them, the output with its rounding, and the log-sum-exp, kept with
     ``save_for_backward`` (an in-place change between forward and backward
     raises); the backward is not itself differentiable."""
 
     @staticmethod
     def forward(ctx, q, k, v, offsets, scale, causal):
         kq, kk, kv = _kernel_layout(q), _kernel_layout(k), _kernel_layout(v)
-        o, lse = _forward(kq, kk, kv, offsets, scale, causal, True)
+        o, o_lo, lse = _forward(kq, kk, kv, offsets, scale, causal, True)
         ctx.args = (scale, causal)
-        ctx.save_for_backward(kq, kk, kv, offsets, o, lse)
+        ctx.save_for_backward(kq, kk, kv, offsets, o, o_lo, lse)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, offsets, o, lse = ctx.saved_tensors
+        q, k, v, offsets, o, o_lo, lse = ctx.saved_tensors
         dout = _kernel_layout(dout)
         dq, dk, dv = (_empty_like(x, x.shape[2]) for x in (q, k, v))
         desc = _desc(q, k, v, o, offsets, *ctx.args)
@@ -223,14 +247,14 @@ class _PackedHip(torch.autograd.Function):
         need = lib.nxa_packed_workspace_bytes(ctypes.byref(desc))
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         strides = [_lib.I64x2(*x.stride()[:2]) for x in (dout, dq, dk, dv)]
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             _lib.check(
                 lib.nxa_packed_bwd(
                     ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                    offsets.data_ptr(), o.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                    offsets.data_ptr(), o.data_ptr(), _ptr(o_lo), lse.data_ptr(), dout.data_ptr(),
                     strides[0], dq.data_ptr(), strides[1], dk.data_ptr(), strides[2],
                     dv.data_ptr(), strides[3], ws.data_ptr(), ws.numel(),
-                    torch.cuda.current_stream(q.device).cuda_stream,
+                    _stream(q.device),
                 )
             )
         return dq, dk, dv, None, None, None

@@ -31,6 +31,7 @@ lengths and counts are returned anew.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 from typing import Optional, Sequence, Union
@@ -46,7 +47,7 @@ from .attention import (
     _row_stride_ok,
     default_scale,
 )
-from .packed import _empty_like, _kernel_layout
+from .packed import _empty_like, _kernel_layout, _on, _stream
 
 __all__ = [
     'compact_pages',
@@ -79,7 +80,7 @@ def _check_pool(name, k_pages, v_pages, written=False) -> None:
             f'{name}: k_pages and v_pages must share device and dtype; got {k_pages.device} '
             f'{k_pages.dtype}, {v_pages.device} {v_pages.dtype}.'
         )
-    if written and any(
+    if written and (0 in k_pages.stride() or 0 in v_pages.stride()) and any(
         s == 0 and n > 1 for x in (k_pages, v_pages) for s, n in zip(x.stride(), x.shape)
     ):
         raise ValueError(f'{name}: pages that share memory (a zero stride) cannot be written.')
@@ -88,12 +89,14 @@ def _check_pool(name, k_pages, v_pages, written=False) -> None:
 def _check_ints(name, device, **arrays) -> None:
     """int32 arrays of the given shapes (None: any size) on ``device``."""
     for arg, (x, shape) in arrays.items():
-        ok = x.ndim == len(shape) and all(s is None or s == n for s, n in zip(shape, x.shape))
+        have = tuple(x.shape)
+        ok = have == tuple(shape)
+        if not ok and len(have) == len(shape):
+            ok = all(s is None or s == n for s, n in zip(shape, have))
         if x.dtype != torch.int32 or not ok:
             want = ', '.join('n' if s is None else str(s) for s in shape)
             raise ValueError(
-                f'{name}: {arg} must be int32 of shape ({want}); got {x.dtype} of shape '
-                f'{tuple(x.shape)}.'
+                f'{name}: {arg} must be int32 of shape ({want}); got {x.dtype} of shape {have}.'
             )
         if x.device != device:
             raise ValueError(f'{name}: {arg} is on {x.device}, expected {device}.')
@@ -116,18 +119,21 @@ def _check_fused(k_pages, v_pages, *others) -> None:
         raise HipNotTileable(
             f'fused paged kernels support bfloat16, float16 and float32; got {k_pages.dtype}.'
         )
-    epc = 16 // k_pages.element_size()
+    es = k_pages.element_size()
+    epc = 16 // es
     for x in (k_pages, v_pages):
-        if x.shape[3] > _MAX_HEAD_DIM or x.shape[3] % epc:
+        d = x.shape[3]
+        if d > _MAX_HEAD_DIM or d % epc:
             raise HipNotTileable(
                 f'fused paged kernels require head dims <= {_MAX_HEAD_DIM} and multiples of '
-                f'{epc}; got {x.shape[3]}.'
+                f'{epc}; got {d}.'
             )
+        s0, s1, s2, s3 = x.stride()
         if (
-            x.stride(3) != 1
-            or any(s % epc for s in x.stride()[:3])
+            s3 != 1
+            or (s0 | s1 | s2) % epc
             or x.data_ptr() % 16
-            or not _row_stride_ok(x.stride(2), x.element_size())
+            or not _row_stride_ok(s2, es)
         ):
             raise HipNotTileable(
                 f'fused paged kernels need 16-byte aligned rows; got strides {x.stride()}.'
@@ -148,10 +154,6 @@ def _pool_desc(k_pages, v_pages) -> _lib.NxaPoolDesc:
     return desc
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _workspace(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
@@ -168,7 +170,7 @@ def _dispatch(name, backend, device, fused, reference, shapes, dtype):
     ``reference``."""
     if resolve_backend(backend, device) == 'hip':
         try:
-            with torch.cuda.device(device):
+            with _on(device):
                 return fused()
         except HipNotTileable as exc:
             fallback(
@@ -684,18 +686,19 @@ def compact_pages(
     )
 
 
-def _page_list(arg, pages, limit) -> torch.Tensor:
-    x = torch.as_tensor(pages)
-    if x.numel() == 0:
-        x = x.reshape(-1).to(torch.int32)
-    if x.device.type != 'cpu' or x.ndim != 1 or x.is_floating_point() or x.dtype == torch.bool:
-        raise ValueError(
-            f'copy_pages: {arg} must be a list or host tensor of page numbers; got '
-            f'{x.dtype} of shape {tuple(x.shape)} on {x.device}.'
-        )
-    if x.numel() and (int(x.min()) < 0 or int(x.max()) >= limit):
+def _page_list(arg, pages, limit) -> array.array:
+    """A list or host tensor of page numbers as C ints."""
+    if isinstance(pages, torch.Tensor):
+        if pages.device.type != 'cpu':
+            raise ValueError(f'copy_pages: {arg} must be on the host; it is on {pages.device}.')
+        pages = pages.tolist()
+    try:
+        x = array.array('i', pages)
+    except (TypeError, OverflowError) as exc:
+        raise ValueError(f'copy_pages: {arg} must be a list of page numbers ({exc}).') from None
+    if x and (min(x) < 0 or max(x) >= limit):
         raise ValueError(f'copy_pages: {arg} names pages outside the pool of {limit}.')
-    return x.to(torch.int32).contiguous()
+    return x
 
 
 def copy_pages(
@@ -716,13 +719,14 @@ def copy_pages(
     _check_written('copy_pages', k_pages, v_pages)
     s = _page_list('src', src, k_pages.shape[0])
     d = _page_list('dst', dst, k_pages.shape[0])
-    if s.numel() != d.numel():
-        raise ValueError(f'copy_pages: {s.numel()} sources for {d.numel()} targets.')
-    if d.numel() != d.unique().numel():
+    if len(s) != len(d):
+        raise ValueError(f'copy_pages: {len(s)} sources for {len(d)} targets.')
+    targets = set(d)
+    if len(targets) != len(d):
         raise ValueError('copy_pages: a page is the target of two copies.')
-    if torch.isin(d, s).any():
+    if not targets.isdisjoint(s):
         raise ValueError('copy_pages: a page is both a source and a target.')
-    if s.numel() == 0:
+    if not s:
         return
     dev = k_pages.device
 
@@ -731,8 +735,8 @@ def copy_pages(
         desc = _pool_desc(k_pages, v_pages)
         _lib.check(
             _lib.lib().nxa_pages_copy(
-                ctypes.byref(desc), k_pages.data_ptr(), v_pages.data_ptr(), s.data_ptr(),
-                d.data_ptr(), s.numel(), _stream(dev),
+                ctypes.byref(desc), k_pages.data_ptr(), v_pages.data_ptr(), s.buffer_info()[0],
+                d.buffer_info()[0], len(s), _stream(dev),
             )
         )
         _touched(k_pages, v_pages)
@@ -740,6 +744,6 @@ def copy_pages(
     def reference():
         with torch.no_grad():
             for pages in (k_pages, v_pages):
-                pages[d.long().to(dev)] = pages[s.long().to(dev)]
+                pages[torch.tensor(d, device=dev)] = pages[torch.tensor(s, device=dev)]
 
     _dispatch('copy_pages', backend, dev, fused, reference, (tuple(k_pages.shape),), k_pages.dtype)

@@ -4,7 +4,7 @@ Every tolerance is a bound computed element by element beside the expected
 value, from the roundings the kernels make: u = eps(T) / 2 for each rounding
 to the I/O type (the probabilities and dS as matrix operands, the outputs;
 zero times anything for float32, whose operands are not rounded), 2^-11 for
-the fp16 copy of P inside dK / dV, 2^-16 for delta as a pair of bf16 terms,
+the fp16 copy of P inside dK / dV (bf16; fp16 has a finer one), 2^-16 for delta as a pair of bf16 terms,
 2^-24 a step for float32 sums.  fp16 numbers below 2^-14 are 2^-24 apart, so
 there half a step is 2^-25 however small the value: an absolute term for the
 fp16 copy of P (both 16-bit types) and for P and dS as fp16 operands.
@@ -63,7 +63,9 @@ def _bounds(q, k, v, do, scale, causal, u, dt):
     delta = (o * do).sum(-1, keepdims=True)
     ds = p * (dp - delta)
     edp = (dv_ + 8) * E24 * np.einsum('gid,jd->gij', ado, av)
-    edl = ((to * ado).sum(-1, keepdims=True) + (dv_ + 8) * E24 * (np.abs(o) * ado).sum(-1, keepdims=True)
+    # (delta is taken from o with its rounding kept apart: u^2 of it is left)
+    tod = to - u * (1 - 2 * u) * np.abs(o)
+    edl = ((tod * ado).sum(-1, keepdims=True) + (dv_ + 8) * E24 * (np.abs(o) * ado).sum(-1, keepdims=True)
            + (0 if f32 else 2.0 ** -16) * np.abs(delta))
     tds = np.abs(ds) * (rp + (0 if f32 else 2.0 ** -11) + u) + p * (edp + edl) * (1 + rp)
     tds = tds + sub + subx * (np.abs(dp - delta) + edp + edl)
@@ -283,6 +285,20 @@ def test_gradients_by_differences():
         # for independent signs), and step^2 / 6 of a third derivative of
         # order |w| ~ 40.
         assert abs(num - ana) <= 2e-3 + 40 * step ** 2 / 6
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16', 'f32'])
+def test_single_tokens_have_no_score_gradients(dtype):
+    """A softmax over one key does not depend on q and k: dP = delta, and what
+    their roundings leave of dQ and dK is far below a rounding of o."""
+    n, d = 300, 128
+    q, k, v = _tokens(n, 2, 2, d, d, DT[dtype], 17)
+    do = _tokens(n, 2, 2, d, d, DT[dtype], 18)[0]
+    got = _train(q, k, v, _off(range(n + 1)), do, causal=True)
+    _check(q, k, v, list(range(n + 1)), got, 1 / math.sqrt(d), True, do)
+    for g in got[1:3]:
+        # delta as two bf16 terms: 2^-16 of |o||do| ~ 11, times |k| / sqrt(d)
+        assert g.abs().max() < 2.0 ** -16 * 60 * 4.5 / math.sqrt(d) * 2
 
 
 def test_many_tiny_sequences():

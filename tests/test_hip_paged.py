@@ -333,7 +333,7 @@ def _same(got, want):
 
 @pytest.mark.parametrize('b, m, p, ps, hk, seed', [
     (9, 5, 30, 3, 2, 0), (9, 5, 30, 16, 1, 1), (64, 33, 1500, 16, 2, 2), (1, 1, 1, 8, 1, 3),
-    (1300, 9, 9000, 4, 1, 4), (40, 300, 20000, 2, 1, 5),
+    (1300, 9, 9000, 4, 1, 4), (40, 300, 20000, 2, 1, 5), (30, 700, 40000, 2, 1, 6),
 ])
 def test_page_management(b, m, p, ps, hk, seed):
     rng = np.random.default_rng(seed)

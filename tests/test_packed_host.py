@@ -172,15 +172,16 @@ def test_c_entries_refuse_before_any_launch():
     lib = _lib.lib()
     d = _desc()
     P, s = 1 << 12, _lib.I64x2(6400, 64)
-    assert lib.nxa_packed_fwd(ctypes.byref(d), P, P, P, None, P, None, None) == _lib.NXA_E_ARG
-    assert lib.nxa_packed_fwd(ctypes.byref(d), P + 8, P, P, P, P, None, None) == _lib.NXA_E_LAYOUT
-    assert lib.nxa_packed_fwd(None, P, P, P, P, P, None, None) == _lib.NXA_E_ARG
+    assert lib.nxa_packed_fwd(ctypes.byref(d), P, P, P, None, P, None, None, None) == _lib.NXA_E_ARG
+    assert lib.nxa_packed_fwd(ctypes.byref(d), P + 8, P, P, P, P, None, None, None) == _lib.NXA_E_LAYOUT
+    assert lib.nxa_packed_fwd(None, P, P, P, P, P, None, None, None) == _lib.NXA_E_ARG
+    assert lib.nxa_packed_fwd(ctypes.byref(d), P, P, P, P, P, P + 4, None, None) == _lib.NXA_E_LAYOUT
     need = lib.nxa_packed_workspace_bytes(ctypes.byref(d))
     assert need >= 2 * 8 * 100 * 4
     assert lib.nxa_packed_workspace_bytes(ctypes.byref(_desc(T=0))) == 0
 
     def bwd(ws, n, lse=P, st=s):
-        return lib.nxa_packed_bwd(ctypes.byref(d), P, P, P, P, P, lse, P, s, P, st, P, s, P, s,
+        return lib.nxa_packed_bwd(ctypes.byref(d), P, P, P, P, P, None, lse, P, s, P, st, P, s, P, s,
                                   ws, n, None)
     assert bwd(None, need) == _lib.NXA_E_WORKSPACE
     assert bwd(P, need - 1) == _lib.NXA_E_WORKSPACE

@@ -59,18 +59,18 @@ int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
   // Units of the largest table, in 31 bits a head.
   const int64_t room = (int64_t)M * d->PS;
   const int64_t len = room < INT32_MAX ? room : INT32_MAX;
-  const int64_t tiles = (int64_t)B * ((len + nxa::kPagedKeys - 1) / nxa::kPagedKeys);
+  const int64_t tiles = (int64_t)B * ((len + nxa::kPagedKeys - 1) / nxa::kPagedKeys + nxa::kStartUnits);
   const int64_t rows = (int64_t)B * d->Hk * plan->strips;
   if (tiles >= (int64_t)1 << 31 || rows >= (int64_t)1 << 31)
     return fail(NXA_E_SHAPE, "%d sequences of up to %lld tokens exceed 2^31 tiles", B,
                 (long long)len);
-  plan->nblk = nxa::paged_blocks(tiles * d->Hk * plan->strips);
+  plan->nblk = nxa::paged_whole(room) ? 0 : nxa::paged_blocks(tiles * d->Hk * plan->strips);
   return NXA_OK;
 }
 
 size_t paged_workspace(const nxa_pool_desc* d, const PagedPlan& plan) {
   const int dp = nxa::paged_dp(d->D > d->Dv ? d->D : d->Dv);
-  return (size_t)2 * plan.nblk * nxa::paged_part_floats(dp) * 4;
+  return (size_t)plan.nblk * (2 * nxa::paged_part_floats(dp) * 4 + sizeof(int4));
 }
 
 // Free, extend and fork: contiguous tables, results in arrays of their own.
@@ -158,7 +158,8 @@ int nxa_paged_fwd(const nxa_pool_desc* d, const void* k_pages, const void* v_pag
   p.strips = plan.strips;
   p.nblk = plan.nblk;
   p.scale_log2 = scale * nxa::kLog2e;
-  p.part = (float*)workspace;
+  p.joins = (int4*)workspace;
+  p.part = (float*)(p.joins + plan.nblk);
   hipStream_t s = (hipStream_t)stream;
   return launch("paged_fwd", s, [&] { nxa::launch_paged(p, d->io_dtype, s); });
 }

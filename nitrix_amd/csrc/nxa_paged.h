@@ -28,16 +28,22 @@ struct PagedParams : PoolParams {
   int64_t table_rs;
   int B, M, G;
   int strips;        // of 16 query heads that share a key-value head
-  int nblk;          // blocks that share the work
+  int nblk;          // blocks that share the work; 0: a block a row
   float scale_log2;
   float* part;       // [2 nblk] partial results (paged_part_floats each)
+  int4* joins;       // [nblk] the row that starts in a block and goes on in the next:
+                     // sequence, head, pieces (0: none), its first piece
 };
 
 constexpr int kPagedKeys = 128;    // keys of a work unit
+constexpr int kStartUnits = 1;     // what starting on a row costs, in units
 constexpr int kPagedBlocks = 512;  // most blocks that share the work
 // One partial result: [16 heads][DP] sums, then a maximum and a sum a head.
 constexpr int paged_part_floats(int dp) { return 16 * dp + 32; }
 int paged_dp(int m);               // padded head dim
+// Whether a block takes a whole row (sequence and key-value head) of up to
+// `room` tokens, and else how many share the units.
+bool paged_whole(int64_t room);
 int paged_blocks(int64_t most_units);
 void launch_paged(const PagedParams& p, int io_dtype, hipStream_t stream);
 

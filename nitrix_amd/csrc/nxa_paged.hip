@@ -10,21 +10,23 @@
 //    device knows, are numbered through and shared evenly by at most 512
 //    blocks (two a CU): block i takes units [U i / N, U (i + 1) / N), whatever
 //    sequences these belong to.  One long sequence and many ragged ones load
-//    the chip alike.  A (sequence, head) that one block holds whole is
-//    finished there; the pieces of the others (at most two a block) go to the
-//    workspace, and a second kernel joins them in order.
+//    the chip alike.  Starting on a row counts as one unit more (64 sequences of
+//    up to 8192 tokens 112 -> 102 us, 256 of up to 2048 166 -> 139).  A
+//    (sequence, head) that one block holds whole is finished there; the pieces
+//    of the others (at most two a block) go to the workspace, and a second
+//    kernel joins them in order.  Where the table has room for few tokens
+//    (paged_whole) each row is a block's own and nothing is joined.
 //  * K and V go from memory to registers in the layout that the matrix
 //    instructions read: no LDS, no barrier in the loop, and each of a
 //    block's four waves streams its own tokens with NB steps of 16 tokens
-//    in flight.
+//    in flight, past the caches (each row is read once): 64 sequences of up to
+//    8192 tokens, 578 MB, 131 -> 122 us, 150,000 tokens of two, 613 MB, 120 ->
+//    107 us (5.7 TB/s); 4 steps in flight against 3: 122 -> 119 us, 5: 148.
 //  * S^T = K Q^T (16x16 products): a lane's A operand is 16 bytes of one key's
 //    row, loaded as they are.  O^T = V^T P^T needs four keys of one column in a
 //    lane: lane (g, c) loads DPL = DP / 16 columns from DPL c on of keys 4 g ..
 //    4 g + 3 and interleaves them (v_perm); S^T's accumulator holds P^T for
 //    just these keys, so P never leaves its lane.
-//    The loads are marked non-temporal (each row is read once): 64 sequences of
-//    up to 8192 tokens, 578 MB, 131 -> 122 us, 150,000 tokens of two, 613 MB,
-//    120 -> 107 us (5.7 TB/s); 4 steps in flight against 3: 122 -> 119 us, 5: 148.
 //  * Loads go through buffer resources that end at the step's last token (and
 //    are empty where the table has no page): what lies behind a sequence, be it
 //    NaN, reads as zero.
@@ -58,15 +60,20 @@ __device__ __forceinline__ int paged_len(const PagedParams& p, int b) {
   const int n = p.lengths[b];
   return n < 0 ? 0 : n > room ? (int)room : n;
 }
-__device__ __forceinline__ int paged_tiles(const PagedParams& p, int b) {
-  return (int)(((int64_t)paged_len(p, b) + kPagedKeys - 1) / kPagedKeys);
+__device__ __forceinline__ int paged_tiles(int len) {
+  return (int)(((int64_t)len + kPagedKeys - 1) / kPagedKeys);
+}
+// Units of a (sequence, head): its tiles after kStartUnits for starting on it.
+__device__ __forceinline__ int paged_units(const PagedParams& p, int b) {
+  const int n = paged_tiles(paged_len(p, b));
+  return n ? n + kStartUnits : 0;
 }
 __device__ __forceinline__ void paged_prefix(const PagedParams& p, int* pre, int* wsum) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = (p.B + 255) / 256;
   int n = 0;
   for (int i = 0; i < per; ++i)
-    if (tid * per + i < p.B) n += paged_tiles(p, tid * per + i);
+    if (tid * per + i < p.B) n += paged_units(p, tid * per + i);
   int x = n;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -87,6 +94,13 @@ __device__ __forceinline__ void paged_prefix(const PagedParams& p, int* pre, int
 // (the join takes a piece from every block between a row's first and last).
 __device__ __forceinline__ int busy_blocks(const PagedParams& p, int64_t units) {
   return (int)min((int64_t)p.nblk, units);
+}
+// o of a sequence without tokens.
+template <typename T>
+__device__ __forceinline__ void paged_zero(const PagedParams& p, int b) {
+  T* op = (T*)p.o + b * p.o_str[0];
+  for (int i = threadIdx.x; i < p.Hk * p.G * p.Dv; i += 256)
+    op[(i / p.Dv) * p.o_str[1] + i % p.Dv] = (T)0.f;
 }
 // First unit of block i of n.
 __device__ __forceinline__ int64_t first_unit(int64_t units, int i, int n) { return units * i / n; }
@@ -196,17 +210,32 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
   const int g = lane >> 4, c = lane & 15;
   const int HV = p.Hk * p.strips;
 
-  paged_prefix(p, pre, wsum);
-  const int64_t units = (int64_t)__builtin_amdgcn_readfirstlane(pre[256]) * HV;
-  const int nblk = busy_blocks(p, units);
-  if ((int)blockIdx.x >= nblk) return;
-  int64_t u = first_unit(units, blockIdx.x, nblk);
-  const int64_t u0 = u, u1 = first_unit(units, blockIdx.x + 1, nblk);
-
-  // The sequence of unit u: the last group that starts at or before it, then
-  // along the group.
-  int b, before;
-  {
+  // The units of this block, u .. u1, numbered from `before` tiles of sequences
+  // before b on.
+  int64_t u, u1, units = 0;
+  int b, before, nblk = 0;
+  if (p.nblk == 0) {
+    b = blockIdx.x / HV;
+    before = 0;
+    const int n = paged_units(p, b), hv = blockIdx.x % HV;
+    if (n == 0) {
+      if (hv == 0) paged_zero<T>(p, b);
+      return;
+    }
+    u = (int64_t)hv * n;
+    u1 = u + n;
+  } else {
+    for (int i = blockIdx.x; i < p.B; i += p.nblk)
+      if (paged_len(p, i) == 0) paged_zero<T>(p, i);
+    if (tid == 0) p.joins[blockIdx.x] = {0, 0, 0, 0};
+    paged_prefix(p, pre, wsum);
+    units = (int64_t)__builtin_amdgcn_readfirstlane(pre[256]) * HV;
+    nblk = busy_blocks(p, units);
+    if ((int)blockIdx.x >= nblk) return;
+    u = first_unit(units, blockIdx.x, nblk);
+    u1 = first_unit(units, blockIdx.x + 1, nblk);
+    // The sequence of unit u: the last group that starts at or before it, then
+    // along the group.
     const int x = (int)(u / HV);
     int lo = 0, hi = 256;
     while (hi - lo > 1) {
@@ -216,10 +245,11 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
     }
     b = lo * ((p.B + 255) / 256);
     before = pre[lo];
-    for (int n; before + (n = paged_tiles(p, b)) <= x; ++b) before += n;
+    for (int n; before + (n = paged_units(p, b)) <= x; ++b) before += n;
     b = __builtin_amdgcn_readfirstlane(b);
     before = __builtin_amdgcn_readfirstlane(before);
   }
+  const int64_t u0 = u;
 
   // Per-lane byte offsets inside a step.  K: key c, 16-byte chunk g + 4 j.  V:
   // key 4 g + j, columns DPL c ...  Columns past the head dim are taken from
@@ -237,15 +267,16 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
 
   while (u < u1) {
     const int len = __builtin_amdgcn_readfirstlane(paged_len(p, b));
-    const int n = (int)(((int64_t)len + kPagedKeys - 1) / kPagedKeys);
-    if (n == 0) {
+    if (len == 0) {
       ++b;
       continue;
     }
+    const int n = paged_tiles(len) + kStartUnits;
     const int64_t rem = u - (int64_t)before * HV;
     const int hv = __builtin_amdgcn_readfirstlane((int)(rem / n));
-    const int t0 = __builtin_amdgcn_readfirstlane((int)(rem % n));
-    const int t1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)n, t0 + (u1 - u)));
+    const int v0 = __builtin_amdgcn_readfirstlane((int)(rem % n));
+    const int v1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)n, v0 + (u1 - u)));
+    const int t0 = max(v0 - kStartUnits, 0), t1 = max(v1 - kStartUnits, 0);  // tiles
     const int hk = hv / p.strips, h0 = (hv % p.strips) * 16;
     const int heads = min(16, p.G - h0);
 
@@ -444,7 +475,7 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
         for (int w = 0; w < kWaves; ++w)
           x[f] = __builtin_fmaf(ms[(w * FIELDS + 4 * f + wave) * 64 + lane], sc[w], x[f]);
       }
-      if (t0 == 0 && t1 == n) {
+      if (v0 == 0 && v1 == n) {
         // (no page of the row valid: no keys, zero)
         const float inv = lt > 0.f || lt != lt ? 1.0f / lt : 0.f;
         if (c < heads && d0 < p.Dv) {
@@ -454,7 +485,14 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
             if (d0 + f < p.Dv) op[f] = (T)(x[f] * inv);
         }
       } else if (c < heads) {
-        float* part = p.part + (2 * (int64_t)blockIdx.x + (u > u0 ? 1 : 0)) * paged_part_floats(DP);
+        const int slot = 2 * blockIdx.x + (u > u0 ? 1 : 0);
+        if (v0 == 0 && tid == 0) {
+          // The row's last unit is the block j's with first_unit(j) <= it.
+          const int64_t z = u + n - 1;
+          const int last = (int)(((z + 1) * nblk - 1) / units);
+          p.joins[blockIdx.x] = {b, hv, last - (int)blockIdx.x + 1, slot};
+        }
+        float* part = p.part + (int64_t)slot * paged_part_floats(DP);
 #pragma unroll
         for (int f = 0; f < NF; ++f) part[c * DP + d0 + f] = x[f];
         if (wave == 0 && g == 0) {
@@ -463,45 +501,28 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
         }
       }
     }
-    u += t1 - t0;
-    if (hv == HV - 1 && t1 == n) {
+    u += v1 - v0;
+    if (hv == HV - 1 && v1 == n) {
       before += n;
       ++b;
     }
   }
 }
 
-// Joins the pieces of each (sequence, key-value head, strip) that several
-// blocks shared, in the blocks' order, and zeroes the rows of empty sequences.
+// Joins the pieces of the rows that several blocks shared, in the blocks'
+// order: block i the row that starts in block i.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p) {
-  __shared__ int pre[257], wsum[kWaves];
   __shared__ float wgt[kPagedBlocks * 16];
   __shared__ float inv_s[16];
   __shared__ float acc_s[256 * 4];
-  const int tid = threadIdx.x;
-  const int HV = p.Hk * p.strips;
-  const int b = blockIdx.x / HV, hv = blockIdx.x % HV;
+  const int tid = threadIdx.x, j0 = blockIdx.x;
+  const int4 row = p.joins[j0];
+  const int b = row.x, hv = row.y, np = row.z, first = row.w;
+  if (np == 0) return;
   const int hk = hv / p.strips, h0 = (hv % p.strips) * 16, heads = min(16, p.G - h0);
-  const int n = paged_tiles(p, b);
   T* op = (T*)p.o + b * p.o_str[0] + ((int64_t)hk * p.G + h0) * p.o_str[1];
-  if (n == 0) {
-    for (int i = tid; i < heads * p.Dv; i += 256) op[(i / p.Dv) * p.o_str[1] + i % p.Dv] = (T)0.f;
-    return;
-  }
-  paged_prefix(p, pre, wsum);
-  const int per = (p.B + 255) / 256;
-  int before = pre[b / per];
-  for (int i = b / per * per; i < b; ++i) before += paged_tiles(p, i);
-  const int64_t units = (int64_t)pre[256] * HV;
-  const int64_t a = (int64_t)before * HV + (int64_t)hv * n, z = a + n - 1;
-  // The block of a unit: first_unit(j) <= unit < first_unit(j + 1).
-  const int nblk = busy_blocks(p, units);
-  const int j0 = (int)(((a + 1) * nblk - 1) / units), j1 = (int)(((z + 1) * nblk - 1) / units);
-  if (j0 == j1) return;
-  const int np = j1 - j0 + 1;
-  // (the first piece is its block's second result unless the row starts it)
-  const int first = 2 * j0 + (a > first_unit(units, j0, nblk) ? 1 : 0);
+  // (the later pieces are their blocks' first results)
   auto piece = [&](int i) {
     return p.part + (int64_t)(i == 0 ? first : 2 * (j0 + i)) * paged_part_floats(DP);
   };
@@ -568,18 +589,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p) {
 
 int paged_dp(int m) { return m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256; }
 
+// Rows of up to 1024 tokens gain less from several blocks than the join costs:
+// us in a graph, split and whole, head dim 128, 8 heads: one sequence of 256
+// 12.5 / 8.0, 1024 12.6 / 14.6 (24.5 / 22.0 with the host's work), 2048 13.6 /
+// 31.6; 64 of up to 512 26 / 17, 1024 33 / 27, 2048 47 / 44, 4096 62 / 81; 256 of
+// up to 1024 90 / 83, 2048 139 / 138.
+bool paged_whole(int64_t room) { return room <= 1024; }
+
 int paged_blocks(int64_t most_units) {
   return (int)(most_units < kPagedBlocks ? most_units : kPagedBlocks);
 }
 
 template <typename T, int DP>
 static void launch_paged_t(const PagedParams& p, hipStream_t stream) {
-  const dim3 grid(p.nblk), block(256);
+  const dim3 grid(p.nblk ? p.nblk : p.B * p.Hk * p.strips), block(256);
   if (p.PS % kStepKeys == 0)
     hipLaunchKernelGGL((paged_kernel<T, DP, true>), grid, block, 0, stream, p);
   else
     hipLaunchKernelGGL((paged_kernel<T, DP, false>), grid, block, 0, stream, p);
-  hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3(p.B * p.Hk * p.strips), block, 0, stream, p);
+  if (p.nblk)
+    hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3(p.nblk), block, 0, stream, p);
 }
 
 template <typename T>

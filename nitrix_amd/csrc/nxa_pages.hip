@@ -100,6 +100,26 @@ __device__ int find_free(const int* refs, int P, int need, int* list, int* wsum)
   return min(found, need);
 }
 
+// The state that the results start from, by one block of 1024 threads, whose
+// later writes and counts come after it.
+__device__ __forceinline__ void start_alone(const RowsParams& p) {
+  auto copy = [](int* dst, const int* src, int n) NXA_INLINE {
+    int done = 0;
+    if ((((uintptr_t)dst | (uintptr_t)src) & 15) == 0) {
+      done = n & ~3;
+#pragma unroll 4
+      for (int i = 4 * threadIdx.x; i < done; i += 4096)
+        *reinterpret_cast<int4*>(dst + i) = *reinterpret_cast<const int4*>(src + i);
+    }
+    for (int i = done + threadIdx.x; i < n; i += 1024) dst[i] = src[i];
+  };
+  copy(p.table_out, p.table, p.B * p.M);
+  copy(p.refs_out, p.refs, p.P);
+  copy(p.lengths_out, p.lengths, p.B);
+  __threadfence();
+  __syncthreads();
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -193,6 +213,30 @@ __global__ __launch_bounds__(256) void pages_free_kernel(const RowsParams p) {
   if (tid == 0) p.lengths_out[r] = 0;
 }
 
+// The same by one block, of up to kFreeAlone rows.
+__global__ __launch_bounds__(1024) void pages_free_alone_kernel(const RowsParams p) {
+  __shared__ int rows[kFreeAlone];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int mine = tid < p.n ? p.rows[tid] : -1;
+  rows[tid] = mine;
+  start_alone(p);
+  bool first = (unsigned)mine < (unsigned)p.B;
+  for (int i = 0; i < tid && first; ++i) first = rows[i] != mine;
+  __syncthreads();
+  rows[tid] = first ? mine : -1;
+  __syncthreads();
+  for (int i = tid >> 6; i < p.n; i += 16) {
+    const int r = rows[i];
+    if (r < 0) continue;
+    for (int c = lane; c < p.M; c += 64) {
+      const int e = p.table[(int64_t)r * p.M + c];
+      if (is_page(e, p.P)) atomicAdd(p.refs_out + e, -1);
+      p.table_out[(int64_t)r * p.M + c] = -1;
+    }
+    if (lane == 0) p.lengths_out[r] = 0;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Rows grown: the new tokens' missing pages are numbered through in row and
 // column order and the k-th takes the k-th free page.  One block.
@@ -200,6 +244,7 @@ __global__ __launch_bounds__(256) void pages_free_kernel(const RowsParams p) {
 __global__ __launch_bounds__(1024) void pages_extend_kernel(const RowsParams p) {
   __shared__ int wsum[16];
   const int tid = threadIdx.x;
+  if (p.start) start_alone(p);
   const int per = (p.B + 1023) / 1024;
   const int64_t room = (int64_t)p.M * p.PS;
   // Columns [first, last) of row r that its new tokens reach.
@@ -254,6 +299,7 @@ __global__ __launch_bounds__(1024) void pages_extend_kernel(const RowsParams p) 
 __global__ __launch_bounds__(1024) void pages_fork_plan_kernel(const RowsParams p) {
   __shared__ int wsum[16];
   const int tid = threadIdx.x;
+  if (p.start) start_alone(p);
   int* winner = p.work + p.n;          // [B]
   int* list = winner + p.B;            // [min(n, P)]
   for (int r = tid; r < p.B; r += 1024) winner[r] = -1;
@@ -449,7 +495,10 @@ void launch_pages_copy(const PoolParams& p, int es, const CopyPairs& pairs, hipS
   hipLaunchKernelGGL(pages_copy_kernel, dim3(pairs.n * p.Hk), dim3(256), 0, stream, p, es, pairs);
 }
 
-static void launch_start(const RowsParams& p, hipStream_t stream) {
+// Whether the one-block kernel of the call copies the state itself; else a
+// launch of its own does.
+static int launch_start(const RowsParams& p, bool one_block, hipStream_t stream) {
+  if (one_block && (int64_t)p.B * p.M + p.P + p.B <= kStartAlone) return 1;
   StartParams s = {};
   s.src[0] = p.table, s.dst[0] = p.table_out, s.n[0] = (int64_t)p.B * p.M;
   s.src[1] = p.refs, s.dst[1] = p.refs_out, s.n[1] = p.P;
@@ -458,20 +507,22 @@ static void launch_start(const RowsParams& p, hipStream_t stream) {
   const int64_t blocks = (most + 1023) / 1024;
   hipLaunchKernelGGL(pages_start_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256),
                      0, stream, s);
+  return 0;
 }
 
 void launch_pages_free(const RowsParams& p, hipStream_t stream) {
-  launch_start(p, stream);
-  if (p.n > 0) hipLaunchKernelGGL(pages_free_kernel, dim3(p.n), dim3(256), 0, stream, p);
+  if (launch_start(p, p.n <= kFreeAlone, stream))
+    hipLaunchKernelGGL(pages_free_alone_kernel, dim3(1), dim3(1024), 0, stream, p);
+  else if (p.n > 0) hipLaunchKernelGGL(pages_free_kernel, dim3(p.n), dim3(256), 0, stream, p);
 }
 
-void launch_pages_extend(const RowsParams& p, hipStream_t stream) {
-  launch_start(p, stream);
+void launch_pages_extend(RowsParams p, hipStream_t stream) {
+  p.start = launch_start(p, true, stream);
   hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, stream, p);
 }
 
-void launch_pages_fork(const RowsParams& p, const PoolParams& pool, int es, hipStream_t stream) {
-  launch_start(p, stream);
+void launch_pages_fork(RowsParams p, const PoolParams& pool, int es, hipStream_t stream) {
+  p.start = launch_start(p, p.n > 0, stream);
   if (p.n == 0) return;
   hipLaunchKernelGGL(pages_fork_plan_kernel, dim3(1), dim3(1024), 0, stream, p);
   hipLaunchKernelGGL(pages_fork_kernel, dim3(p.n, 1 + pool.Hk), dim3(256), 0, stream, p, pool, es);

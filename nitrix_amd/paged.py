@@ -89,14 +89,14 @@ def _check_pool(name, k_pages, v_pages, written=False) -> None:
 def _check_ints(name, device, **arrays) -> None:
     """int32 arrays of the given shapes (None: any size) on ``device``."""
     for arg, (x, shape) in arrays.items():
-        have = tuple(x.shape)
-        ok = have == tuple(shape)
-        if not ok and len(have) == len(shape):
-            ok = all(s is None or s == n for s, n in zip(shape, have))
+        have = x.shape
+        ok = have == shape or (
+            len(have) == len(shape) and all(s is None or s == n for s, n in zip(shape, have))
+        )
         if x.dtype != torch.int32 or not ok:
             want = ', '.join('n' if s is None else str(s) for s in shape)
             raise ValueError(
-                f'{name}: {arg} must be int32 of shape ({want}); got {x.dtype} of shape {have}.'
+                f'{name}: {arg} must be int32 of shape ({want}); got {x.dtype} of shape {tuple(have)}.'
             )
         if x.device != device:
             raise ValueError(f'{name}: {arg} is on {x.device}, expected {device}.')

@@ -246,10 +246,10 @@ def test_c_pool_check(kw, code):
 def test_c_entries_refuse_before_any_launch():
     lib, P, s = _lib.lib(), 1 << 12, _lib.I64x2(128, 64)
     d = ctypes.byref(_pool())
-    need = lib.nxa_paged_workspace_bytes(d, 4, 8, 6)
-    assert need > 0 and lib.nxa_paged_workspace_bytes(d, 4, 8, 5) == 0
+    need = lib.nxa_paged_workspace_bytes(d, 4, 100, 6)
+    assert need > 0 and lib.nxa_paged_workspace_bytes(d, 4, 100, 5) == 0
 
-    def att(B=4, M=8, H=6, ws=P, n=need, table=P, q=P, pool=d, rs=8):
+    def att(B=4, M=100, H=6, ws=P, n=need, table=P, q=P, pool=d, rs=8):
         return lib.nxa_paged_fwd(pool, P, P, q, s, table, rs, P, B, M, H, 0.1, P, s, ws, n, None)
     assert att(H=5) == _lib.NXA_E_SHAPE
     assert att(B=0) == _lib.NXA_E_SHAPE

@@ -154,6 +154,9 @@ __device__ __forceinline__ PackedTile packed_find(const PackedParams& pp, int sl
   r.start = __builtin_amdgcn_readfirstlane(packed_offset(pp, lo));
   r.len = max(__builtin_amdgcn_readfirstlane(packed_offset(pp, lo + 1)) - r.start, 0);
   r.tile = slot - (r.start / tile_rows + lo);
+  // (offsets that decrease can end the search at a sequence behind the slot,
+  // whose tiles before its first row are other sequences' rows)
+  if (r.tile < 0) r.len = r.tile = 0;
   return r;
 }
 

@@ -325,6 +325,21 @@ def test_offsets_out_of_order_or_range_stay_in_bounds():
     _check(q, k, v, [0, 100, 200], got, 0.125, True, do)
 
 
+def test_many_offsets_out_of_order_stay_in_bounds():
+    """As above for more sequences than are ranked, whose tiles are searched
+    for: offsets that jump send the search to a sequence behind its slot."""
+    t = 4000
+    q, k, v = _tokens(t, 2, 1, 64, 64, torch.bfloat16, 60)
+    do = torch.randn_like(q)
+    for seed in range(3):
+        ends = np.random.default_rng(seed).integers(0, t, 301).tolist()
+        got = _train(q, k, v, _off(ends), do, causal=True)
+        torch.cuda.synchronize()
+        assert all(x.shape[1] == t for x in got)
+    ends = sorted(ends)  # as many in order
+    _check(q, k, v, ends, _train(q, k, v, _off(ends), do, causal=True), 0.125, True, do)
+
+
 def test_repeated_calls_agree_and_streams_do_not_mix():
     ends = _ends([300, 200, 11])
     sets = [(_tokens(511, 4, 2, 64, 64, torch.bfloat16, 20 + i)) for i in range(2)]

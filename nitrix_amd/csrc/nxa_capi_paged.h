@@ -6,12 +6,17 @@
 
 namespace {
 
+// (page and slot numbers plus what a block steps by stay in 31 bits)
+constexpr int kMostPages = 1 << 30;
+
 int check_pool(const nxa_pool_desc* d) {
   if (!d) return fail(NXA_E_ARG, "pool descriptor is NULL");
   if (!known_dtype(d->io_dtype))
     return fail(NXA_E_DTYPE, "io_dtype %d is not NXA_BF16, NXA_F16 or NXA_F32", d->io_dtype);
   if (d->P <= 0 || d->Hk <= 0 || d->PS <= 0)
     return fail(NXA_E_SHAPE, "extents must be positive (P=%d Hk=%d PS=%d)", d->P, d->Hk, d->PS);
+  if (d->P > kMostPages || d->PS > kMostPages)
+    return fail(NXA_E_SHAPE, "P=%d, PS=%d: at most 2^30 pages of 2^30 tokens", d->P, d->PS);
   const int es = esize(d->io_dtype);
   int rc = check_head_dim("D", d->D, 16 / es);
   if (!rc) rc = check_head_dim("Dv", d->Dv, 16 / es);
@@ -79,6 +84,10 @@ int check_rows(int B, int M, int P, int PS, const void* table, const void* lengt
                const void* refs_out) {
   if (B <= 0 || M <= 0 || P <= 0 || PS <= 0)
     return fail(NXA_E_SHAPE, "extents must be positive (B=%d M=%d P=%d PS=%d)", B, M, P, PS);
+  if (P > kMostPages || B > kMostPages)
+    return fail(NXA_E_SHAPE, "B=%d, P=%d: at most 2^30 rows and pages", B, P);
+  if ((int64_t)M * PS >= (int64_t)1 << 31)
+    return fail(NXA_E_SHAPE, "a row of %d pages of %d tokens has room for 2^31 or more", M, PS);
   if (!table || !lengths || !refs || !table_out || !lengths_out || !refs_out)
     return fail(NXA_E_ARG, "a table, lengths or refs pointer is NULL");
   if (table == table_out || lengths == lengths_out || refs == refs_out)
@@ -292,7 +301,7 @@ int nxa_pages_fork(const nxa_pool_desc* d, void* k_pages, void* v_pages, int32_t
 }
 
 size_t nxa_pages_compact_workspace_bytes(int32_t P) {
-  if (P <= 0) return 0;
+  if (P <= 0 || P > kMostPages) return 0;
   const size_t nb = ((size_t)P + nxa::kCompactPages - 1) / nxa::kCompactPages;
   return (nb + 4 + 3 * (size_t)P) * 4;
 }

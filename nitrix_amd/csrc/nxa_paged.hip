@@ -362,9 +362,12 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
                                           (uint32_t)__shfl((int)(uint32_t)vr, src, 64));
             const bool vok = (hv_rows >> src & 1) && voff[x] != 0xffffff00u;
             const char* at = (const char*)(vb + row) + (vok ? voff[x] : 0u);
+            // (of a lane's 16-byte chunks some may lie behind the row's end)
 #pragma unroll
             for (int w = 0; w < NV; ++w)
-              r.v[x].w[w] = vok ? reinterpret_cast<const uint32_t*>(at)[w] : 0u;
+              r.v[x].w[w] = vok && DPL * c + (w & ~3) * (4 / ES) < p.Dv
+                                ? reinterpret_cast<const uint32_t*>(at)[w]
+                                : 0u;
           }
         }
       };

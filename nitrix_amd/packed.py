@@ -134,6 +134,8 @@ def _check_tileable(q, k, v) -> None:
             f'fused packed attention needs one dtype for q, k, v; got {q.dtype}, {k.dtype}, '
             f'{v.dtype}.'
         )
+    if q.shape[1] >> 31:
+        raise HipNotTileable(f'fused packed attention numbers rows in 31 bits; got t={q.shape[1]}.')
     epc = 16 // q.element_size()
     for name, n in (('d', q.shape[-1]), ('d_v', v.shape[-1])):
         if n > _MAX_HEAD_DIM or n % epc != 0 or n == 0:
@@ -306,7 +308,8 @@ def packed_attention(
     ``scale`` defaults to ``1/sqrt(d)``.  Tokens of no sequence (before
     ``offsets[0]``, from ``offsets[-1]`` on) give zero, take no part in
     anything and get zero gradients, whatever they hold; a NaN or infinity
-    inside a sequence stays in that sequence.  Differentiable in q, k and v; gradients of k and v are summed over the heads that share
+    inside a sequence stays in that sequence.  Differentiable
+    in q, k and v; gradients of k and v are summed over the heads that share
     them.
 
     ``backend`` as in :func:`scaled_dot_product_attention`.  The fused engine

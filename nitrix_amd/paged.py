@@ -104,8 +104,11 @@ def _check_ints(name, device, **arrays) -> None:
 
 def _check_table(name, device, page_table, **arrays) -> None:
     _check_ints(name, device, page_table=(page_table, (None, None)), **arrays)
-    if 0 in page_table.shape:
-        raise ValueError(f'{name}: page_table must not be empty; got {tuple(page_table.shape)}.')
+    if 0 in page_table.shape or max(page_table.shape) >> 30:
+        raise ValueError(
+            f'{name}: page_table must not be empty nor have 2^30 rows or columns; got '
+            f'{tuple(page_table.shape)}.'
+        )
 
 
 def _check_written(name, *tensors) -> None:
@@ -138,6 +141,9 @@ def _check_fused(k_pages, v_pages, *others) -> None:
             raise HipNotTileable(
                 f'fused paged kernels need 16-byte aligned rows; got strides {x.stride()}.'
             )
+    p, hk, ps, _ = k_pages.shape
+    if (p | hk | ps) >> 30:
+        raise HipNotTileable('fused paged kernels number up to 2^30 pages, heads and slots.')
     for x in others:
         if x.dtype != k_pages.dtype:
             raise HipNotTileable(f'fused paged kernels need one dtype; got {x.dtype}.')
@@ -281,8 +287,8 @@ def paged_attention(
     b = q.shape[0]
     _check_ints('paged_attention', q.device, page_table=(page_table, (b, None)),
                 lengths=(lengths, (b,)))
-    if page_table.shape[1] == 0:
-        raise ValueError('paged_attention: page_table has no columns.')
+    if not 0 < page_table.shape[1] < 1 << 30:
+        raise ValueError('paged_attention: page_table has no columns, or 2^30 or more.')
     scale = float(default_scale(q.shape[2]) if scale is None else scale)
     args = (q, k_pages, v_pages, page_table, lengths, scale)
     if b == 0:

@@ -375,6 +375,40 @@ def test_page_management(b, m, p, ps, hk, seed):
     np.testing.assert_array_equal(v.cpu().numpy(), hostv)
 
 
+@pytest.mark.parametrize('b, m, p, ps', [(5, 200, 700, 4), (70, 40, 3000, 3), (1500, 20, 9000, 2),
+                                          (1, 3000, 2500, 1), (40, 65, 30, 8)])
+def test_rows_that_grow_by_prompts(b, m, p, ps):
+    """Rows that grow by many columns next to ones that grow by few or none;
+    some columns hold a page already, and the pages may run out."""
+    rng = np.random.default_rng(b)
+    table = np.full((b, m), -1, np.int32)
+    lengths = np.minimum(rng.integers(0, 3 * ps, b), m * ps).astype(np.int32)
+    refs = (rng.random(p) < 0.2).astype(np.int32)
+    held = rng.permutation(p)[:p // 10]
+    cells = rng.permutation(b * m)[:len(held)]
+    table.reshape(-1)[cells] = held[:len(cells)]
+    refs[held[:len(cells)]] = 1
+    counts = np.where(rng.random(b) < 0.5, rng.integers(0, 2 * ps, b), rng.integers(0, m * ps, b))
+    want = plain.extend(table, lengths, refs, counts, ps)
+    got = nx.extend_sequences(_i32(table), _i32(lengths), _i32(refs), _i32(counts), ps,
+                              backend='hip')
+    _same(got, want)
+
+
+@pytest.mark.parametrize('dtype, d, dv, ps', [
+    ('bf16', 256, 248, 9), ('f16', 64, 136, 1), ('f32', 128, 100, 7), ('f32', 16, 252, 3),
+])
+def test_values_that_end_inside_a_lane(dtype, d, dv, ps):
+    """Pages that are no multiple of a step, and head dims of v that are no
+    multiple of the columns a lane takes: the pool's very last row is used."""
+    lens = [ps * 7, 40, 1]
+    k, v, table = _setup(DT[dtype], lens, 2, d, dv, ps, spare=0, nan=False)
+    assert (table == k.shape[0] - 1).any()
+    q = _rand((3, 4, d), DT[dtype], 5)
+    out = nx.paged_attention(q, k, v, _i32(table), _i32(lens), backend='hip')
+    _check(out, q, k, v, table, lens, 1 / math.sqrt(d))
+
+
 def test_management_of_nothing():
     t, n, c = _i32([[0, -1], [1, -1]]), _i32([3, 4]), _i32([1, 1, 0])
     k = _rand((3, 1, 4, 8), torch.bfloat16, 1)

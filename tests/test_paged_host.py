@@ -231,6 +231,8 @@ def _pool(**kw):
     ({}, _lib.NXA_OK),
     (dict(P=0), _lib.NXA_E_SHAPE),
     (dict(PS=0), _lib.NXA_E_SHAPE),
+    (dict(P=(1 << 30) + 1), _lib.NXA_E_SHAPE),
+    (dict(PS=(1 << 30) + 1), _lib.NXA_E_SHAPE),
     (dict(Dv=0), _lib.NXA_E_SHAPE),
     (dict(D=12), _lib.NXA_E_UNSUPPORTED),
     (dict(D=512), _lib.NXA_E_UNSUPPORTED),
@@ -271,6 +273,10 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.nxa_pages_free(2, 2, 4, P, P, P, None, 1, 2 * P, 2 * P, 2 * P, None) == _lib.NXA_E_ARG
     assert lib.nxa_pages_extend(2, 2, 4, 8, P, P, P, P, 2 * P, 2 * P, 2 * P, P, 15,
                                 None) == _lib.NXA_E_WORKSPACE
+    assert lib.nxa_pages_extend(2, 1 << 20, 4, 1 << 11, P, P, P, P, 2 * P, 2 * P, 2 * P, P, 16,
+                                None) == _lib.NXA_E_SHAPE
+    assert lib.nxa_pages_free(2, 2, (1 << 30) + 1, P, P, P, P, 1, 2 * P, 2 * P, 2 * P,
+                              None) == _lib.NXA_E_SHAPE
     assert lib.nxa_pages_fork(d, P, P, 2, 2, P, P, P, P, P, 1, 2 * P, 2 * P, 2 * P, None, 0,
                               None) == _lib.NXA_E_WORKSPACE
     assert lib.nxa_pages_compact(d, P, P, 4, P, P, 2 * P, 2 * P, P, 8, None) == _lib.NXA_E_WORKSPACE

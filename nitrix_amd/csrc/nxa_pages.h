@@ -45,6 +45,10 @@ struct RowsParams {
 // it on the host, with three launches less.
 constexpr int64_t kStartAlone = 32768;
 constexpr int kFreeAlone = 1024;  // rows that the single block frees
+// Columns of a grown row that a thread takes alone, a row's wave 64 a step.  us
+// in a graph, thread / wave: 64 rows of 12 columns 15 / 17, 24 20 / 17, 48 33 / 17,
+// 500 246 / 51; 512 of 12 24 / 62, 100 172 / 108; one of 6000 1723 / 66.
+constexpr int kLaneColumns = 32;
 
 constexpr int kCompactPages = 4096;  // pages of a counting block
 constexpr int kCompactFew = 8;

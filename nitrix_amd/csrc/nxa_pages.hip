@@ -239,11 +239,15 @@ __global__ __launch_bounds__(1024) void pages_free_alone_kernel(const RowsParams
 
 // ---------------------------------------------------------------------------
 // Rows grown: the new tokens' missing pages are numbered through in row and
-// column order and the k-th takes the k-th free page.  One block.
+// column order and the k-th takes the k-th free page.  One block: a thread
+// takes its rows' columns one after the other (a new token or a few reach one
+// or two); rows whose tokens reach more than kLaneColumns (prompts) are taken
+// by a wave each, 64 columns a step, their counts and first ranks passed
+// through lengths_out.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(1024) void pages_extend_kernel(const RowsParams p) {
   __shared__ int wsum[16];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (p.start) start_alone(p);
   const int per = (p.B + 1023) / 1024;
   const int64_t room = (int64_t)p.M * p.PS;
@@ -254,39 +258,94 @@ __global__ __launch_bounds__(1024) void pages_extend_kernel(const RowsParams p) 
     first = (int)((len + p.PS - 1) / p.PS);
     last = (int)((grown + p.PS - 1) / p.PS);
   };
+  auto missing = [&](int r, int64_t c) { return !is_page(p.table[(int64_t)r * p.M + c], p.P); };
   int need = 0;
+  bool wide = false;
   for (int i = 0; i < per; ++i) {
     const int r = tid * per + i;
     if (r >= p.B) break;
     int a, b;
     int64_t g;
     span(r, a, b, g);
-    for (int c = a; c < b; ++c) need += !is_page(p.table[(int64_t)r * p.M + c], p.P);
+    if (b - a > kLaneColumns) {
+      wide = true;
+      continue;
+    }
+    for (int c = a; c < b; ++c) need += missing(r, c);
+  }
+  wide = __syncthreads_or(wide);
+  if (wide) {
+    for (int r = wave; r < p.B; r += 16) {
+      int a, b, n = 0;
+      int64_t g;
+      span(r, a, b, g);
+      if (b - a <= kLaneColumns) continue;
+#pragma unroll 4
+      for (int64_t c = a; c < b; c += 64)
+        n += (int)__popcll(__ballot(c + lane < b && missing(r, min(c + lane, (int64_t)b - 1))));
+      if (lane == 0) p.lengths_out[r] = n;
+    }
+    __syncthreads();
+    for (int i = 0; i < per; ++i) {
+      const int r = tid * per + i;
+      if (r >= p.B) break;
+      int a, b;
+      int64_t g;
+      span(r, a, b, g);
+      if (b - a > kLaneColumns) need += p.lengths_out[r];
+    }
   }
   int total;
   int rank = block_scan(need, wsum, total) - need;
   const int got = find_free(p.refs, p.P, min(total, p.P), p.work, wsum);
   __threadfence_block();
+  // Column c of row r without a page, the k-th of all; false where the pages
+  // have run out.
+  auto take = [&](int r, int64_t c, int k) {
+    const int page = k < got ? p.work[k] : -1;
+    p.table_out[(int64_t)r * p.M + c] = page;
+    if (page >= 0) p.refs_out[page] = 1;
+    return page >= 0;
+  };
   for (int i = 0; i < per; ++i) {
     const int r = tid * per + i;
     if (r >= p.B) break;
     int a, b;
     int64_t g;
     span(r, a, b, g);
+    if (b - a > kLaneColumns) {
+      const int n = p.lengths_out[r];
+      p.lengths_out[r] = rank;
+      rank += n;
+      continue;
+    }
     for (int c = a; c < b; ++c) {
-      if (is_page(p.table[(int64_t)r * p.M + c], p.P)) continue;
-      if (rank < got) {
-        const int page = p.work[rank];
-        p.table_out[(int64_t)r * p.M + c] = page;
-        p.refs_out[page] = 1;
-      } else {
-        // Out of pages: the row ends with the tokens that have one.
-        p.table_out[(int64_t)r * p.M + c] = -1;
-        g = min(g, (int64_t)c * p.PS);
-      }
+      if (!missing(r, c)) continue;
+      // Out of pages: the row ends with the tokens that have one.
+      if (!take(r, c, rank)) g = min(g, (int64_t)c * p.PS);
       ++rank;
     }
     p.lengths_out[r] = (int)g;
+  }
+  if (!wide) return;
+  __syncthreads();
+  for (int r = wave; r < p.B; r += 16) {
+    int a, b;
+    int64_t g;
+    span(r, a, b, g);
+    if (b - a <= kLaneColumns) continue;
+    int k = p.lengths_out[r];
+    for (int64_t c0 = a; c0 < b; c0 += 64) {
+      const int64_t c = c0 + lane;
+      const bool miss = c < b && missing(r, c);
+      const uint64_t m = __ballot(miss);
+      bool out = false;
+      if (miss) out = !take(r, c, k + (int)__popcll(m & ((1ull << lane) - 1)));
+      const uint64_t none = __ballot(out);
+      if (none) g = min(g, (c0 + (int)__builtin_ctzll(none)) * p.PS);
+      k += (int)__popcll(m);
+    }
+    if (lane == 0) p.lengths_out[r] = (int)g;
   }
 }
 

@@ -314,7 +314,9 @@ def packed_attention(
 
     ``backend`` as in :func:`scaled_dot_product_attention`.  The fused engine
     never reads the offsets on the host: a captured graph may be replayed
-    with other offsets (and lengths) in the same tensor.
+    with other offsets (and lengths) in the same tensor.  Capture forward and
+    backward together, with no eager graph of the same leaves alive: torch ties
+    a leaf's accumulation to the stream of the first graph that uses it.
     """
     _validate(q, k, v, offsets)
     resolved_scale = default_scale(q.shape[-1]) if scale is None else scale

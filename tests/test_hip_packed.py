@@ -378,6 +378,41 @@ def test_graph_replay_with_other_offsets():
             assert torch.equal(out, packed_attention(q, k, v, _off(e), causal=True, backend='hip'))
 
 
+@pytest.mark.parametrize('dtype, h, hk, t', [('bf16', 8, 1, 700), ('f16', 4, 2, 300),
+                                             ('f32', 2, 1, 300)])
+def test_captured_training_step(dtype, h, hk, t):
+    """Forward and backward captured together, replayed with other inputs and
+    offsets and eager calls in between: the bytes of an eager step."""
+    dt = {'bf16': torch.bfloat16, 'f16': torch.float16, 'f32': torch.float32}[dtype]
+    q, k, v = _tokens(t, h, hk, 64, 64, dt, 70)
+    do = torch.randn_like(q)
+    off = _off([0, t // 3, t])
+    ins = [x.requires_grad_(True) for x in (q, k, v)]
+
+    def step():
+        out = packed_attention(*ins, off, causal=True, backend='hip')
+        return (out, *torch.autograd.grad(out, ins, do))
+
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        out = step()
+    for i, ends in enumerate(([0, t // 3, t], [0, 1, t], [5, t - 80, t - 7])):
+        off.copy_(_off(ends))
+        with torch.no_grad():
+            for x, y in zip(ins, _tokens(t, h, hk, 64, 64, dt, 80 + i)):
+                x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.detach().clone() for x in out]
+        want = _train(q, k, v, _off(ends), do, causal=True)
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
 def test_rows_past_2_31_elements():
     """A row stride that puts late tokens beyond 2^31 elements (and 2^32
     bytes) of the operands' base."""

@@ -147,7 +147,9 @@ def _check_tileable(q, k, v) -> None:
 
 def _kernel_layout(x: torch.Tensor) -> torch.Tensor:
     """``x`` (h, t, d) itself where the kernels can read it in place, else a
-    contiguous copy."""
+    contiguous copy.  (``contiguous()`` would be no copy of a contiguous view
+    off a 16-byte boundary, nor of one whose only odd stride is that of an
+    axis of size one.)"""
     h_str, t_str, d_str = x.stride()
     epc = 16 // x.element_size()
     if (
@@ -158,7 +160,7 @@ def _kernel_layout(x: torch.Tensor) -> torch.Tensor:
         and _row_stride_ok(t_str, x.element_size())
     ):
         return x
-    return x.contiguous()
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _empty_like(x: torch.Tensor, d: int) -> torch.Tensor:

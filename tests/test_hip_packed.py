@@ -446,3 +446,28 @@ def test_in_place_change_between_the_passes_raises():
     off += 1
     with pytest.raises(RuntimeError, match='modified by an inplace'):
         out.sum().backward()
+
+
+def _off_by_one(x):
+    """The same numbers, contiguous, one element past a 16-byte boundary."""
+    flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+    y = flat[1:].view(x.shape)
+    y.copy_(x)
+    assert y.is_contiguous() and y.data_ptr() % 16
+    return y
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f32'])
+@pytest.mark.parametrize('t, h, hk', [(85, 4, 2), (1, 2, 1), (40, 1, 1)])
+def test_contiguous_operands_off_a_boundary(dtype, t, h, hk):
+    """Slices of flat buffers, the cotangent's among them."""
+    ends = _ends([t - t // 3, t // 3])
+    q, k, v = _tokens(t, h, hk, 64, 64, DT[dtype], 90)
+    do = _tokens(t, h, h, 64, 64, DT[dtype], 91)[0]
+    want = _train(q, k, v, _off(ends), do, causal=True)
+    ins = [_off_by_one(x) for x in (q, k, v)]
+    got = _train(*ins, _off(ends), _off_by_one(do), causal=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(packed_attention(*ins, _off(ends), causal=True, backend='hip'), want[0])

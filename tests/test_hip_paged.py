@@ -532,3 +532,29 @@ def test_serving_run():
             assert (refs[:live] > 0).all() and int(table.max()) < live
     counted = np.bincount(table.cpu().numpy()[table.cpu().numpy() >= 0], minlength=p)
     np.testing.assert_array_equal(refs.cpu().numpy(), counted)
+
+
+def test_contiguous_operands_off_a_boundary():
+    """Slices of flat buffers, and one sequence whose axis has an odd stride."""
+    lens = [70, 3]
+    k, v, table = _setup(torch.bfloat16, lens, 2, 64, 64, 16)
+
+    def off_by_one(x):
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape)
+        y.copy_(x)
+        return y
+
+    q = _rand((2, 4, 64), torch.bfloat16, 8)
+    want = nx.paged_attention(q, k, v, _i32(table), _i32(lens), backend='hip')
+    got = nx.paged_attention(off_by_one(q), k, v, _i32(table), _i32(lens), backend='hip')
+    assert torch.equal(got, want)
+    one = torch.as_strided(q, (1, 4, 64), (257, 64, 1))
+    assert one.is_contiguous()
+    got = nx.paged_attention(one, k, v, _i32(table[:1]), _i32(lens[:1]), backend='hip')
+    _check(got, q[:1], k, v, table[:1], lens[:1], 0.125)
+    new = [_rand((2, 2, 64), torch.bfloat16, 9 + i) for i in range(2)]
+    pools = [[x.clone() for x in (k, v)] for _ in range(2)]
+    for p, toks in zip(pools, (new, [off_by_one(x) for x in new])):
+        nx.write_pages(*p, *toks, _i32(table), _i32([70, 3]), backend='hip')
+    for a, b in zip(*pools):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))

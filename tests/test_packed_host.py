@@ -188,3 +188,24 @@ def test_c_entries_refuse_before_any_launch():
     assert bwd(P + 16, need) == _lib.NXA_E_WORKSPACE
     assert bwd(P, need, lse=None) == _lib.NXA_E_ARG
     assert bwd(P, need, st=_lib.I64x2(6400, 63)) == _lib.NXA_E_LAYOUT
+
+
+def _readable(x):
+    epc = 16 // x.element_size()
+    return (x.data_ptr() % 16 == 0 and x.stride(2) == 1 and x.stride(0) % epc == 0
+            and x.stride(1) % epc == 0)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_contiguous_views_the_kernels_cannot_read_are_copied(dtype):
+    """Slices of a flat buffer off a 16-byte boundary, and axes of size one
+    whose stride is no multiple of 16 bytes, count as contiguous."""
+    flat = torch.randn(1 + 4 * 10 * 8).to(dtype)
+    views = [flat[1:].view(4, 10, 8), flat[1:1 + 80].view(1, 10, 8), flat[1:1 + 32].view(4, 1, 8),
+             torch.as_strided(flat, (1, 10, 8), (83, 8, 1)),
+             torch.as_strided(flat, (4, 1, 8), (8, 9, 1)),
+             torch.as_strided(flat, (1, 1, 8), (3, 1 << 27, 1))]
+    for x in views:
+        assert x.is_contiguous() and not _readable(x)
+        y = _kernel_layout(x)
+        assert _readable(y) and torch.equal(x, y)

@@ -80,6 +80,13 @@ def qk_rms_norm(z: torch.Tensor) -> torch.Tensor:
     return (zf * torch.rsqrt(ms + _QK_RMS_EPS)).to(z.dtype)
 
 
+def _copied(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous copy, also of a tensor that counts as contiguous but the
+    kernels cannot read in place: a slice of a flat buffer off a 16-byte
+    boundary, an axis of size one with an odd stride."""
+    return x.clone(memory_format=torch.contiguous_format)
+
+
 def _rms_norm_rows(x: torch.Tensor):
     """``nxa_rms_norm_fwd`` over the rows of ``x``: returns ``(y, x2, rstd)``
     with ``y`` normalised in ``x.dtype`` (shape of ``x``, contiguous), ``x2``
@@ -87,10 +94,9 @@ def _rms_norm_rows(x: torch.Tensor):
     when ``x`` is already laid out so) and ``rstd`` the fp32 per-row
     ``rsqrt(mean(x^2) + eps)``."""
     d = x.shape[-1]
-    epc = 4 if x.dtype == torch.float32 else 8
     x2 = x.reshape(-1, d)
-    if not x2.is_contiguous() or x2.data_ptr() % 16 or d % epc:
-        x2 = x2.contiguous()
+    if not x2.is_contiguous() or x2.data_ptr() % 16 or x2.stride(0) != d:
+        x2 = _copied(x2)
     rows = x2.shape[0]
     y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
     rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
@@ -123,7 +129,7 @@ class _RmsNormHip(torch.autograd.Function):
         rows, d = x2.shape
         dy2 = dy.reshape(rows, d)
         if not dy2.is_contiguous() or dy2.data_ptr() % 16:
-            dy2 = dy2.contiguous()
+            dy2 = _copied(dy2)
         dx = torch.empty((rows, d), dtype=x2.dtype, device=x2.device)
         stream = torch.cuda.current_stream(x2.device).cuda_stream
         _lib.check(
@@ -305,7 +311,7 @@ def _as_bhld(x: torch.Tensor, lead: Sequence[int], nb: int, epc: int) -> torch.T
     else:
         y = x.expand(*lead, L, d).reshape(nb, h, L, d)
     if not _layout_ok(y, epc):
-        y = y.contiguous()
+        y = _copied(y)
     return y
 
 
@@ -318,7 +324,7 @@ def _as_bhst(
     else:
         y = x.expand(*lead, s, t).reshape(nb, h, s, t)
     if (y.stride(-1) != 1 and t != 1) or not _row_stride_ok(y.stride(-2), y.element_size()):
-        y = y.contiguous()
+        y = _copied(y)
     return y
 
 
@@ -492,7 +498,7 @@ def _backward(prep: _Prepared, o, lse, fwd_ws, dout, want_dbias: bool, norm=None
         prep.desc.v_str[:] = v.stride()[:3]
     dout = dout.reshape(prep.nb, prep.h, prep.s, prep.dv)
     if not dout.is_contiguous() or dout.data_ptr() % 16 != 0:
-        dout = dout.contiguous()
+        dout = _copied(dout)
     dq = torch.empty_like(q, memory_format=torch.contiguous_format)
     dk = torch.empty_like(k, memory_format=torch.contiguous_format)
     dv = torch.empty_like(v, memory_format=torch.contiguous_format)
@@ -613,7 +619,7 @@ class _SdpaNormHip(torch.autograd.Function):
         d = q.shape[-1]
         q2 = q.reshape(-1, d)
         if not q2.is_contiguous() or q2.data_ptr() % 16:
-            q2 = q2.contiguous()
+            q2 = _copied(q2)
         for_bwd = any(ctx.needs_input_grad[:4])
         qn = torch.empty_like(q2) if for_bwd else None
         rq = (torch.empty((q2.shape[0],), dtype=torch.float32, device=q.device)

@@ -238,3 +238,33 @@ def test_shared_bias_gradient_memory_is_bounded():
     e = float((got - bf.grad).abs().max() / bf.grad.abs().max())
     print(f'  dbias relerr vs reference engine {e:.2e}', flush=True)
     assert e <= 2e-2
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('qk_norm', [False, True])
+def test_contiguous_operands_off_a_boundary(dtype, qk_norm):
+    """Slices of flat buffers one element past a 16-byte boundary, the
+    cotangent's among them, give the bytes of aligned operands."""
+    def off_by_one(x):
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape)
+        y.copy_(x)
+        assert y.is_contiguous() and y.data_ptr() % 16
+        return y
+
+    ins = [_rand((2, 2, n, 64), dtype, n) for n in (50, 70, 71)]
+    ins[2] = ins[2][:, :, :70].contiguous()
+    do = _rand((2, 2, 50, 64), dtype, 9)
+
+    def step(tensors, cotangent):
+        ts = [x.detach().requires_grad_(True) for x in tensors]
+        out = scaled_dot_product_attention(*ts, qk_norm=qk_norm, backend='hip')
+        return (out, *torch.autograd.grad(out, ts, cotangent))
+
+    want = step(ins, do)
+    got = step([off_by_one(x) for x in ins], off_by_one(do))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    one = scaled_dot_product_attention(*(off_by_one(x[:1, :1, :1]) for x in ins), qk_norm=qk_norm,
+                                       backend='hip')
+    assert torch.equal(one, scaled_dot_product_attention(
+        *(x[:1, :1, :1].clone() for x in ins), qk_norm=qk_norm, backend='hip'))

@@ -128,3 +128,21 @@ def test_a_bias_that_does_not_broadcast_still_raises():
     bias = torch.randn(6, 4, 8, 8)
     with pytest.raises(RuntimeError):
         A._Prepared(q, k, v, bias, None, 0.125, False)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_contiguous_operands_the_kernels_cannot_read_are_copied(dtype):
+    """Slices of a flat buffer off a 16-byte boundary, and axes of size one
+    whose stride is no multiple of 16 bytes, count as contiguous."""
+    epc = 4 if dtype == torch.float32 else 8
+    flat = torch.randn(1 + 2 * 3 * 10 * 8).to(dtype)
+    for x, lead in ((flat[1:].view(2, 3, 10, 8), (2, 3)),
+                    (torch.as_strided(flat, (1, 3, 10, 8), (241, 80, 8, 1)), (1, 3)),
+                    (torch.as_strided(flat, (2, 3, 1, 8), (24, 8, 9, 1)), (2, 3)),
+                    (torch.as_strided(flat, (2, 3, 1, 8), (24, 8, 1 << 27, 1)), (2, 3))):
+        assert x.is_contiguous() and not A._layout_ok(x, epc)
+        y = A._as_bhld(x, lead, lead[0], epc)
+        assert A._layout_ok(y, epc) and torch.equal(x, y)
+    row = torch.as_strided(flat, (1, 1, 1, 8), (8, 8, 1 << 31, 1))
+    bias = A._as_bhst(row, (1, 1), 1, 1, 8)
+    assert A._row_stride_ok(bias.stride(-2), bias.element_size()) and torch.equal(bias, row)

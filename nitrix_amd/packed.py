@@ -29,6 +29,7 @@ from .attention import (
     _IO_DTYPES,
     _MAX_HEAD_DIM,
     HipNotTileable,
+    _has_tangent,
     _ptr,
     _row_stride_ok,
     default_scale,
@@ -244,6 +245,8 @@ class _PackedHip(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, offsets, o, o_lo, lse = ctx.saved_tensors
+        if _has_tangent(dout):
+            raise RuntimeError('packed_attention: the backward pass is not itself differentiable.')
         dout = _kernel_layout(dout)
         dq, dk, dv = (_empty_like(x, x.shape[2]) for x in (q, k, v))
         desc = _desc(q, k, v, o, offsets, *ctx.args)
@@ -274,9 +277,11 @@ def packed_attention_hip(
     causal: bool = False,
 ) -> torch.Tensor:
     """Fused packed attention on gfx950.  Raises :class:`HipNotTileable` for
-    types and head dims outside the supported set; differentiable in q, k
-    and v."""
+    types and head dims outside the supported set and for forward-mode
+    derivatives; differentiable in q, k and v."""
     _check_tileable(q, k, v)
+    if _has_tangent(q, k, v):
+        raise HipNotTileable('fused packed attention has no forward-mode derivative.')
     _lib.lib()  # a missing library is an error here, not a fallback
     offsets = offsets.contiguous()
     scale, causal = float(scale), bool(causal)
@@ -314,7 +319,8 @@ def packed_attention(
     in q, k and v; gradients of k and v are summed over the heads that share
     them.
 
-    ``backend`` as in :func:`scaled_dot_product_attention`.  The fused engine
+    ``backend`` as in :func:`scaled_dot_product_attention`; forward-mode
+    derivatives are left to the reference engine.  The fused engine
     never reads the offsets on the host: a captured graph may be replayed
     with other offsets (and lengths) in the same tensor.  Capture forward and
     backward together, with no eager graph of the same leaves alive: torch ties

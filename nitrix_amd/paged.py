@@ -44,6 +44,7 @@ from .attention import (
     _IO_DTYPES,
     _MAX_HEAD_DIM,
     HipNotTileable,
+    _has_tangent,
     _row_stride_ok,
     default_scale,
 )
@@ -114,6 +115,8 @@ def _check_table(name, device, page_table, **arrays) -> None:
 def _check_written(name, *tensors) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError(f'{name} is not differentiable; detach its inputs or use no_grad.')
+    if _has_tangent(*tensors):
+        raise ValueError(f'{name} is not differentiable; its inputs carry forward-mode tangents.')
 
 
 def _check_fused(k_pages, v_pages, *others) -> None:
@@ -225,6 +228,8 @@ def _paged_hip(q, k_pages, v_pages, page_table, lengths, scale):
     _check_fused(k_pages, v_pages, q)
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k_pages, v_pages)):
         raise HipNotTileable('fused paged attention has no backward pass.')
+    if _has_tangent(q, k_pages, v_pages):
+        raise HipNotTileable('fused paged attention has no forward-mode derivative.')
     q = _kernel_layout(q)
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
@@ -269,7 +274,8 @@ def paged_attention(
 
     The fused engine takes bfloat16, float16 and float32, head dims up to 256
     (multiples of 8, 4 in float32) and pages of any number of slots (a
-    multiple of 16 is fastest); it has no backward pass.
+    multiple of 16 is fastest); derivatives, backward and forward mode, are the
+    reference engine's.
     """
     _check_pool('paged_attention', k_pages, v_pages)
     if q.ndim != 3 or q.shape[2] != k_pages.shape[3]:

@@ -471,3 +471,23 @@ def test_contiguous_operands_off_a_boundary(dtype, t, h, hk):
         assert torch.equal(a, b)
     with torch.no_grad():
         assert torch.equal(packed_attention(*ins, _off(ends), causal=True, backend='hip'), want[0])
+
+
+def test_forward_mode_falls_back_loudly():
+    from torch.autograd import forward_ad
+
+    q, k, v = _tokens(60, 4, 2, 32, 32, torch.float32, 92)
+    off = _off([0, 25, 60])
+    with forward_ad.dual_level():
+        ins = [forward_ad.make_dual(x, torch.randn_like(x)) for x in (q, k, v)]
+        nx.reset_fallback_state()
+        with pytest.warns(nx.NitrixBackendFallback, match='forward-mode'):
+            got = forward_ad.unpack_dual(packed_attention(*ins, off, causal=True))
+        want = forward_ad.unpack_dual(packed_attention(*ins, off, causal=True, backend='jax'))
+        for a, b in zip(got, want):
+            assert a is not None and torch.equal(a, b)
+    # a cotangent with a tangent: the backward has no derivative
+    ts = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    out = packed_attention(*ts, off, backend='hip')
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match='not itself differentiable'):
+        torch.autograd.grad(out, ts, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))

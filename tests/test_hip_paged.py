@@ -558,3 +558,19 @@ def test_contiguous_operands_off_a_boundary():
         nx.write_pages(*p, *toks, _i32(table), _i32([70, 3]), backend='hip')
     for a, b in zip(*pools):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def test_forward_mode_falls_back_loudly():
+    from torch.autograd import forward_ad
+
+    lens = [20, 7]
+    k, v, table = _setup(torch.float32, lens, 1, 64, 64, 16, nan=False)
+    q = _rand((2, 2, 64), torch.float32, 1)
+    with forward_ad.dual_level():
+        args = (forward_ad.make_dual(q, torch.ones_like(q)), k, v, _i32(table), _i32(lens))
+        nx.reset_fallback_state()
+        with pytest.warns(nx.NitrixBackendFallback, match='forward-mode'):
+            got = forward_ad.unpack_dual(nx.paged_attention(*args))
+        want = forward_ad.unpack_dual(nx.paged_attention(*args, backend='jax'))
+        for a, b in zip(got, want):
+            assert a is not None and torch.equal(a, b)

@@ -209,3 +209,26 @@ def test_contiguous_views_the_kernels_cannot_read_are_copied(dtype):
         assert x.is_contiguous() and not _readable(x)
         y = _kernel_layout(x)
         assert _readable(y) and torch.equal(x, y)
+
+
+def test_forward_mode_is_left_to_the_reference_engine():
+    """A tensor with a tangent need not have requires_grad: the fused engine
+    declines it, the reference engine's tangent is that of differences."""
+    from torch.autograd import forward_ad
+
+    from nitrix_amd.packed import packed_attention_hip
+
+    off = torch.tensor([0, 4, 7], dtype=torch.int32)
+    ins = [torch.from_numpy(x) for x in _inputs(4, 2, 7, 8, seed=3)]
+    for i in range(3):
+        t = torch.from_numpy(np.random.default_rng(i).standard_normal(ins[i].shape))
+        with forward_ad.dual_level():
+            dual = [forward_ad.make_dual(x, t) if n == i else x for n, x in enumerate(ins)]
+            out, tangent = forward_ad.unpack_dual(packed_attention(*dual, off, causal=True))
+            with pytest.raises(HipNotTileable, match='forward-mode'):
+                packed_attention_hip(*(x.float() for x in dual), off, scale=1.0)
+        ahead, behind = (packed_attention(*(x + s * t if n == i else x for n, x in enumerate(ins)),
+                                          off, causal=True) for s in (2.0 ** -14, -2.0 ** -14))
+        # (float64: rounding 2^-53 / 2^-14 of values of order one, and 2^-28 of
+        # a third derivative of some hundred)
+        torch.testing.assert_close(tangent, (ahead - behind) * 2.0 ** 13, atol=1e-5, rtol=0)

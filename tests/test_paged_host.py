@@ -281,3 +281,31 @@ def test_c_entries_refuse_before_any_launch():
                               None) == _lib.NXA_E_WORKSPACE
     assert lib.nxa_pages_compact(d, P, P, 4, P, P, 2 * P, 2 * P, P, 8, None) == _lib.NXA_E_WORKSPACE
     assert lib.nxa_pages_compact(d, P, P, 4, P, P, P, 2 * P, P, 1 << 20, None) == _lib.NXA_E_ARG
+
+
+def test_forward_mode_is_left_to_the_reference_engine_or_refused():
+    """A tensor with a tangent need not have requires_grad."""
+    from torch.autograd import forward_ad
+
+    from nitrix_amd.paged import HipNotTileable, _paged_hip
+
+    a = _args()
+    a['k_pages'], a['v_pages'] = torch.randn(5, 2, 4, 8), torch.randn(5, 2, 4, 8)
+    t, n, c = _i32(np.zeros((3, 2))), _i32([3, 4, 5]), _i32([1, 0, 1, 1, 0])
+    with forward_ad.dual_level():
+        for name in ('q', 'k_pages', 'v_pages'):
+            x = a[name]
+            dual = {**a, name: forward_ad.make_dual(x, torch.randn_like(x))}
+            assert forward_ad.unpack_dual(nx.paged_attention(**dual)).tangent is not None
+            with pytest.raises(HipNotTileable, match='forward-mode'):
+                _paged_hip(*dual.values(), 1.0)
+        k = forward_ad.make_dual(torch.randn(2, 3, 8), torch.randn(2, 3, 8))
+        pool = forward_ad.make_dual(a['k_pages'].clone(), torch.randn(5, 2, 4, 8))
+        v = torch.zeros(2, 3, 8)
+        for call in (lambda: nx.write_pages(a['k_pages'], a['v_pages'], k, v, t, n),
+                     lambda: nx.write_pages(pool, a['v_pages'], v, v, t, n),
+                     lambda: nx.fork_sequences(pool, a['v_pages'], t, n, c, _i32([0]), _i32([1])),
+                     lambda: nx.compact_pages(pool, a['v_pages'], t, c),
+                     lambda: nx.copy_pages(pool, a['v_pages'], [0], [1])):
+            with pytest.raises(ValueError, match='forward-mode'):
+                call()

@@ -75,6 +75,15 @@ def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
     return any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)
 
 
+_NO_TANGENT = 'fused attention has no forward-mode derivative.'
+
+
+def _no_tangent_back(name: str, cotangent: torch.Tensor) -> None:
+    """The backward kernels see a cotangent's values alone."""
+    if _has_tangent(cotangent):
+        raise RuntimeError(f'{name}: the backward pass is not itself differentiable.')
+
+
 def default_scale(head_dim: int) -> float:
     """``1 / sqrt(d)`` (``_reference.py:35-49``)."""
     return 1.0 / math.sqrt(float(head_dim))
@@ -137,6 +146,7 @@ class _RmsNormHip(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x2, rstd = ctx.saved_tensors
+        _no_tangent_back('qk_norm', dy)
         rows, d = x2.shape
         dy2 = dy.reshape(rows, d)
         if not dy2.is_contiguous() or dy2.data_ptr() % 16:
@@ -499,6 +509,7 @@ def _backward(prep: _Prepared, o, lse, fwd_ws, dout, want_dbias: bool, norm=None
     taken with respect to the raw ones); returns flattened
     ``(dq, dk, dv, dbias_kernel)``."""
     lib = _lib.lib()
+    _no_tangent_back('scaled_dot_product_attention', dout)
     # dK / dV are written per (b, h): broadcast q / k / v are materialised.
     q = prep.q if all(x != 0 for x in prep.q.stride()[:2]) else prep.q.contiguous()
     k = prep.k if all(x != 0 for x in prep.k.stride()[:2]) else prep.k.contiguous()
@@ -682,11 +693,13 @@ def scaled_dot_product_attention_hip(
 ) -> torch.Tensor:
     """Fused attention on gfx950 (``attention.py:768-824`` counterpart).
 
-    Raises :class:`HipNotTileable` for shapes outside the supported set; the
-    dispatcher turns that into a loud fallback.  Differentiable in q, k, v and
-    bias.
+    Raises :class:`HipNotTileable` for shapes outside the supported set and
+    for forward-mode derivatives; the dispatcher turns that into a loud
+    fallback.  Differentiable in q, k, v and bias.
     """
     _check_tileable(q, k, v)
+    if _has_tangent(q, k, v, bias):
+        raise HipNotTileable(_NO_TANGENT)
     _lib.lib()  # a missing library is an error here, not a fallback
     if not (torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (q, k, v, bias))):
@@ -758,6 +771,8 @@ def scaled_dot_product_attention(
     resolved = resolve_backend(backend, q.device)
     if resolved == 'hip':
         try:
+            if qk_norm and _has_tangent(q, k, v, bias):
+                raise HipNotTileable(_NO_TANGENT)
             if qk_norm and _norm_fusable(q, k, v):
                 _check_tileable(q, k, v)
                 _lib.lib()

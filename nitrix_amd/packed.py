@@ -30,6 +30,7 @@ from .attention import (
     _MAX_HEAD_DIM,
     HipNotTileable,
     _has_tangent,
+    _no_tangent_back,
     _ptr,
     _row_stride_ok,
     default_scale,
@@ -245,8 +246,7 @@ class _PackedHip(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, offsets, o, o_lo, lse = ctx.saved_tensors
-        if _has_tangent(dout):
-            raise RuntimeError('packed_attention: the backward pass is not itself differentiable.')
+        _no_tangent_back('packed_attention', dout)
         dout = _kernel_layout(dout)
         dq, dk, dv = (_empty_like(x, x.shape[2]) for x in (q, k, v))
         desc = _desc(q, k, v, o, offsets, *ctx.args)

@@ -40,7 +40,7 @@ from ._backend import (
     reproducible_enabled,
     resolve_backend,
 )
-from .attention import HipNotTileable
+from .attention import HipNotTileable, _no_tangent_back
 
 __all__ = [
     'reference_selective_scan',
@@ -421,6 +421,7 @@ class _ScanHip(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _no_tangent_back('selective_scan', dy)
         prep = ctx.prep
         prep.x, prep.delta, prep.A, prep.B, prep.C, prep.D, state = ctx.saved_tensors
         dx, ddelta, dA, dB, dC, dD = _scan_backward(prep, state, dy)

@@ -268,3 +268,20 @@ def test_contiguous_operands_off_a_boundary(dtype, qk_norm):
                                        backend='hip')
     assert torch.equal(one, scaled_dot_product_attention(
         *(x[:1, :1, :1].clone() for x in ins), qk_norm=qk_norm, backend='hip'))
+
+
+@pytest.mark.parametrize('qk_norm', [False, True])
+def test_forward_mode_falls_back_loudly(qk_norm):
+    from torch.autograd import forward_ad
+
+    q, k, v = (_rand((1, 2, 30, 32), torch.float32, s) for s in (1, 2, 3))
+    with forward_ad.dual_level():
+        ins = [forward_ad.make_dual(x, torch.ones_like(x)) for x in (q, k, v)]
+        with warnings.catch_warnings(record=True) as rec:
+            warnings.simplefilter('always')
+            got = forward_ad.unpack_dual(scaled_dot_product_attention(*ins, qk_norm=qk_norm))
+        assert len(_fallbacks(rec)) == 1
+        want = forward_ad.unpack_dual(
+            scaled_dot_product_attention(*ins, qk_norm=qk_norm, backend='jax'))
+    for a, b in zip(got, want):
+        assert a is not None and torch.equal(a, b)

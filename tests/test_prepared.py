@@ -146,3 +146,20 @@ def test_contiguous_operands_the_kernels_cannot_read_are_copied(dtype):
     row = torch.as_strided(flat, (1, 1, 1, 8), (8, 8, 1 << 31, 1))
     bias = A._as_bhst(row, (1, 1), 1, 1, 8)
     assert A._row_stride_ok(bias.stride(-2), bias.element_size()) and torch.equal(bias, row)
+
+
+def test_the_fused_engine_declines_forward_mode():
+    """A tensor with a tangent need not have requires_grad: the kernels, which
+    see values alone, would drop the derivative."""
+    from torch.autograd import forward_ad
+
+    q, k, v = (torch.randn(1, 2, 5, 8) for _ in range(3))
+    bias = torch.randn(5, 5)
+    with forward_ad.dual_level():
+        for i in range(4):
+            a = [forward_ad.make_dual(x, torch.ones_like(x)) if n == i else x
+                 for n, x in enumerate((q, k, v, bias))]
+            with pytest.raises(A.HipNotTileable, match='forward-mode'):
+                A.scaled_dot_product_attention_hip(*a[:3], bias=a[3], scale=1.0)
+        with pytest.raises(RuntimeError, match='not itself differentiable'):
+            A._no_tangent_back('x', forward_ad.make_dual(q, q))

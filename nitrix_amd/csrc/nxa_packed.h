@@ -36,8 +36,8 @@ struct PackedParams : Params {
   int nwork;           // blocks with a slot; those behind zero the unowned rows
   int64_t do_str[3], dq_str[3], dk_str[3], dv_str[3];
   void* o_lo;          // what rounding o to 16 bits left (o's strides), or null
-  // dK / dV of a group of query heads in `parts` blocks, each over some of
-  // them, whose fp32 sums go to dkv_part ([parts][Hk][T][D], then the same of
+  // dK / dV of a group of query heads in `parts` blocks, each over one or more
+  // of them, whose fp32 sums go to dkv_part ([parts][Hk][T][D], then the same of
   // dV) and are added up afterwards (1: one block takes them all).
   int parts;
   float* dkv_part;
@@ -45,7 +45,7 @@ struct PackedParams : Params {
 
 // What a dK / dV block streams besides its own sequence's base pointers.
 struct PackedGroup {
-  int heads;                   // query heads of the group
+  int heads;                   // query heads of the group (1 or more)
   int64_t q_hs, do_hs, row_hs; // from one head to the next (row_hs: nlse2, ndelta)
   int64_t do_rs, dk_rs, dv_rs; // row strides
   float *dk_part, *dv_part;    // this block's rows of dkv_part, or null
@@ -319,7 +319,9 @@ inline int packed_parts(const PackedParams& p) {
   const int64_t mean = (int64_t)p.Hk * p.T;
   const int64_t want = p.T / p.nseq >= 1024 ? 131072 : 65536;
   const int64_t parts = (want + mean - 1) / mean;
-  return (int)(parts < p.G ? parts : p.G);
+  // (as many as it takes with the heads of the largest: none without a head)
+  const int per = parts < p.G ? (int)((p.G + parts - 1) / parts) : 1;
+  return (p.G + per - 1) / per;
 }
 inline size_t packed_part_floats(const PackedParams& p) {
   const int parts = packed_parts(p);

@@ -232,3 +232,22 @@ def test_forward_mode_is_left_to_the_reference_engine():
         # (float64: rounding 2^-53 / 2^-14 of values of order one, and 2^-28 of
         # a third derivative of some hundred)
         torch.testing.assert_close(tangent, (ahead - behind) * 2.0 ** 13, atol=1e-5, rtol=0)
+
+
+def test_no_part_of_a_group_is_without_a_head():
+    """Blocks that share a group's query heads take ceil(G / parts) each: the
+    workspace has as many planes of dk and dv as that takes."""
+    lib, seen = _lib.lib(), set()
+    for g in range(1, 41):
+        for t in [65536 // n + 1 for n in range(1, 41)] + [512, 100000, 130000]:
+            for nseq in (1, 200):
+                d = _desc(T=t, nseq=nseq, H=g, Hk=1, D=8, Dv=8)
+                rows = -(-g * t * 4 // 256) * 256
+                more = lib.nxa_packed_workspace_bytes(ctypes.byref(d)) - 2 * rows
+                parts, odd = divmod(more, 4 * t * 16)
+                assert odd == 0 and parts != 1 and parts <= g
+                parts = max(parts, 1)
+                per = -(-g // parts)
+                assert (parts - 1) * per < g, (g, t, nseq, parts)
+                seen.add((g, parts))
+    assert {(7, 4), (16, 1), (16, 4), (16, 6), (16, 8), (16, 16), (5, 3)} <= seen

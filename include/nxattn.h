@@ -308,7 +308,9 @@ typedef struct {
   int64_t o_str[2];
 } nxa_packed_desc;
 
-/* Host-only validation (no GPU needed). */
+/* Host-only validation (no GPU needed).  A launch holds less than 2^32
+ * threads: NXA_E_SHAPE for extents beyond (some 2^24 (head, sequence) pairs or
+ * 2^31 (head, row) pairs, less in a backward, whose workspace size is then 0). */
 int nxa_packed_check(const nxa_packed_desc* desc);
 
 int nxa_packed_fwd(const nxa_packed_desc* desc, const void* q, const void* k, const void* v,
@@ -362,7 +364,7 @@ int nxa_paged_fwd(const nxa_pool_desc* desc, const void* k_pages, const void* v_
  * pages.  With offsets (B + 1, as nxa_packed_desc) token t of sequence s goes
  * to position starts[s] + t - offsets[s]; without (T = B) token s to
  * starts[s].  Tokens of no sequence, outside the table or in no page are
- * dropped.  Of tokens meant for one slot (rows that share a page there) either
+ * dropped.  T < 2^26.  Of tokens meant for one slot (rows that share a page there) either
  * may stay, by 16-byte chunks. */
 int nxa_pages_write(const nxa_pool_desc* desc, void* k_pages, void* v_pages, const void* k,
                     const int64_t* k_str, const void* v, const int64_t* v_str, int64_t T,
@@ -378,13 +380,13 @@ int nxa_pages_copy(const nxa_pool_desc* desc, void* k_pages, void* v_pages, cons
 /* Page management on contiguous tables [B, M], with reference counts refs [P]:
  * how many table entries name a page (none: it is free).  Results go to
  * arrays of their own.
- * free: the n listed rows (a row listed twice counts once) give their pages
+ * free: the n < 2^24 listed rows (a row listed twice counts once) give their pages
  * back, become -1 and of length zero.
  * extend: row b grows by counts[b] tokens (negative: none; at most to M * PS);
  * columns that these reach and that hold no page take free pages, lowest
  * first, in row and column order.  Where pages run out a row's length ends
  * with its last token that has one.  Workspace: P * 4 bytes.
- * fork: row dst[i] becomes a copy of row src[i], for n pairs (of those with
+ * fork: row dst[i] becomes a copy of row src[i], for n < 2^24 pairs (of those with
  * one target the last counts; src[i] == dst[i] does nothing): whole pages are
  * shared, the tokens of a partly filled last page copied to a free page
  * (lowest first, in order of i; without one the row ends with its whole

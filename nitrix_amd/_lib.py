@@ -162,6 +162,10 @@ class NxaError(RuntimeError):
         self.code = code
 
 
+class NxaShapeError(NxaError):
+    """``NXA_E_SHAPE``: extents the library declines, before any launch."""
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -314,7 +318,7 @@ def check(rc: int) -> None:
     """Raise :class:`NxaError` with the library's message for rc != 0."""
     if rc != NXA_OK:
         msg = lib().nxa_last_error().decode('utf-8', 'replace')
-        raise NxaError(rc, msg)
+        raise (NxaShapeError if rc == NXA_E_SHAPE else NxaError)(rc, msg)
 
 
 def profile_enable(on: bool) -> None:

@@ -53,11 +53,7 @@ int check_packed(const nxa_packed_desc* d) {
   if (!rc) rc = check_strides("k", d->k_str, 2, es);
   if (!rc) rc = check_strides("v", d->v_str, 2, es);
   if (!rc) rc = check_strides("o", d->o_str, 2, es);
-  if (rc) return rc;
-  // Blocks of a grid (32-row tiles at most) in 31 bits.
-  if ((int64_t)d->H * ((int64_t)d->T / 32 + d->nseq + 1) >= (int64_t)1 << 31)
-    return fail(NXA_E_SHAPE, "H * (T / 32 + nseq) exceeds 2^31 blocks");
-  return NXA_OK;
+  return rc;
 }
 
 void set_strides(int64_t (&dst)[3], const int64_t* src) {
@@ -100,15 +96,28 @@ int packed_dp(const nxa_packed_desc* d) {
   return m <= 64 ? 64 : m <= 128 ? 128 : 256;
 }
 
+int check_packed_grid(const nxa_packed_desc* d, bool bwd) {
+  nxa::PackedParams p = packed_params(d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+  p.parts = nxa::packed_parts(p);
+  const int64_t threads = bwd ? nxa::packed_bwd_threads(p, d->io_dtype, packed_dp(d))
+                              : nxa::packed_fwd_threads(p, d->io_dtype, packed_dp(d));
+  if (threads >= (int64_t)1 << 32)
+    return fail(NXA_E_SHAPE, "H=%d T=%d nseq=%d exceed a grid of 2^32 threads", d->H, d->T, d->nseq);
+  return NXA_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
-int nxa_packed_check(const nxa_packed_desc* desc) { return check_packed(desc); }
+int nxa_packed_check(const nxa_packed_desc* desc) {
+  const int rc = check_packed(desc);
+  return rc ? rc : check_packed_grid(desc, false);
+}
 
 int nxa_packed_fwd(const nxa_packed_desc* d, const void* q, const void* k, const void* v,
                    const int32_t* offsets, void* o, void* o_lo, float* lse, void* stream) {
-  int rc = check_packed(d);
+  int rc = nxa_packed_check(d);
   if (!rc) rc = check_ptr16("q", q);
   if (!rc) rc = check_ptr16("k", k);
   if (!rc) rc = check_ptr16("v", v);
@@ -123,7 +132,7 @@ int nxa_packed_fwd(const nxa_packed_desc* d, const void* q, const void* k, const
 }
 
 size_t nxa_packed_workspace_bytes(const nxa_packed_desc* d) {
-  if (check_packed(d)) return 0;
+  if (check_packed(d) || check_packed_grid(d, true)) return 0;
   const nxa::PackedParams p = packed_params(d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
   return 2 * align256((size_t)d->H * d->T * 4) + 4 * nxa::packed_part_floats(p);
 }
@@ -135,6 +144,7 @@ int nxa_packed_bwd(const nxa_packed_desc* d, const void* q, const void* k, const
                    const int64_t* dk_str, void* dv, const int64_t* dv_str, void* workspace,
                    size_t workspace_bytes, void* stream) {
   int rc = check_packed(d);
+  if (!rc) rc = check_packed_grid(d, true);
   const void* ptrs[8] = {q, k, v, o, dout, dq, dk, dv};
   const char* names[8] = {"q", "k", "v", "o", "dout", "dq", "dk", "dv"};
   for (int i = 0; i < 8 && !rc; ++i) rc = check_ptr16(names[i], ptrs[i]);

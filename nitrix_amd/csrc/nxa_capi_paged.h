@@ -8,6 +8,8 @@ namespace {
 
 // (page and slot numbers plus what a block steps by stay in 31 bits)
 constexpr int kMostPages = 1 << 30;
+// (a grid holds less than 2^32 threads: 64 a token written, 256 a listed row)
+constexpr int kMostTokens = 1 << 26, kMostListed = 1 << 24;
 
 int check_pool(const nxa_pool_desc* d) {
   if (!d) return fail(NXA_E_ARG, "pool descriptor is NULL");
@@ -69,7 +71,8 @@ int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
   if (tiles >= (int64_t)1 << 31 || rows >= (int64_t)1 << 31)
     return fail(NXA_E_SHAPE, "%d sequences of up to %lld tokens exceed 2^31 tiles", B,
                 (long long)len);
-  plan->nblk = nxa::paged_whole(room) ? 0 : nxa::paged_blocks(tiles * d->Hk * plan->strips);
+  // (a block a row where a grid of less than 2^32 threads holds them)
+  plan->nblk = nxa::paged_whole(room) && rows < 1 << 24 ? 0 : nxa::paged_blocks(tiles * d->Hk * plan->strips);
   return NXA_OK;
 }
 
@@ -185,7 +188,8 @@ int nxa_pages_write(const nxa_pool_desc* d, void* k_pages, void* v_pages, const 
   if (rc) return rc;
   if (!table || !starts || !k_str || !v_str)
     return fail(NXA_E_ARG, "table, starts and the strides must not be NULL");
-  if (T <= 0 || T >= (int64_t)1 << 31) return fail(NXA_E_SHAPE, "T=%lld", (long long)T);
+  if (T <= 0 || T >= kMostTokens)
+    return fail(NXA_E_SHAPE, "T=%lld: 1 to 2^26 - 1 tokens a call", (long long)T);
   if (!offsets && T != B)
     return fail(NXA_E_SHAPE, "without offsets one token a sequence is written: T=%lld, B=%d",
                 (long long)T, B);
@@ -218,7 +222,7 @@ int nxa_pages_copy(const nxa_pool_desc* d, void* k_pages, void* v_pages, const i
   if (!rc) rc = check_pool_ptrs(k_pages, v_pages);
   if (rc) return rc;
   if (n < 0 || (n > 0 && (!src || !dst))) return fail(NXA_E_ARG, "n=%d pairs", n);
-  if ((int64_t)nxa::kCopyPairs * d->Hk >= (int64_t)1 << 31)
+  if ((int64_t)(n < nxa::kCopyPairs ? n : nxa::kCopyPairs) * d->Hk * 256 >= (int64_t)1 << 32)
     return fail(NXA_E_SHAPE, "Hk=%d exceeds the grid", d->Hk);
   for (int i = 0; i < n; ++i)
     if (src[i] < 0 || src[i] >= d->P || dst[i] < 0 || dst[i] >= d->P)
@@ -245,6 +249,7 @@ int nxa_pages_free(int32_t B, int32_t M, int32_t P, const int32_t* table, const 
   const int rc = check_rows(B, M, P, 1, table, lengths, refs, table_out, lengths_out, refs_out);
   if (rc) return rc;
   if (n < 0 || (n > 0 && !rows)) return fail(NXA_E_ARG, "n=%d rows", n);
+  if (n >= kMostListed) return fail(NXA_E_SHAPE, "n=%d: less than 2^24 rows a call", n);
   nxa::RowsParams p = rows_params(B, M, P, 1, table, lengths, refs, table_out, lengths_out, refs_out);
   p.rows = rows;
   p.n = n;
@@ -284,6 +289,7 @@ int nxa_pages_fork(const nxa_pool_desc* d, void* k_pages, void* v_pages, int32_t
     rc = check_rows(B, M, d->P, d->PS, table, lengths, refs, table_out, lengths_out, refs_out);
   if (rc) return rc;
   if (n < 0 || (n > 0 && (!src || !dst))) return fail(NXA_E_ARG, "n=%d forks", n);
+  if (n >= kMostListed) return fail(NXA_E_SHAPE, "n=%d: less than 2^24 forks a call", n);
   if (d->Hk >= 65535) return fail(NXA_E_SHAPE, "Hk=%d exceeds the grid", d->Hk);
   rc = need_workspace(workspace, workspace_bytes, n ? nxa_pages_fork_workspace_bytes(B, d->P, n) : 0);
   if (rc) return rc;

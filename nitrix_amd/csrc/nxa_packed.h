@@ -330,6 +330,16 @@ inline size_t packed_part_floats(const PackedParams& p) {
 void launch_packed_parts(const PackedParams& p, int io_dtype, hipStream_t stream);
 
 inline int packed_slots(const PackedParams& p, int tile_rows) { return p.T / tile_rows + p.nseq; }
+// Threads of a launch with a block a slot of `heads` heads (and the zeroing
+// ones), and of the largest launch of a forward and of a backward: a grid holds
+// less than 2^32.
+inline int64_t packed_threads(const PackedParams& p, int64_t heads, int tile_rows, int threads) {
+  return (heads * ((int64_t)p.T / tile_rows + p.nseq) + kPackedZeroBlocks) * threads;
+}
+int64_t packed_fwd_threads(const PackedParams& p, int io_dtype, int dp);
+int64_t packed_bwd_threads(const PackedParams& p, int io_dtype, int dp);
+int64_t packed_fwd32_threads(const PackedParams& p, int dp);
+int64_t packed_bwd32_threads(const PackedParams& p, int dp);
 
 void launch_packed_fwd(const PackedParams& p, int io_dtype, int dp, hipStream_t stream);
 void launch_packed_bwd(const PackedParams& p, int io_dtype, int dp, hipStream_t stream);

@@ -55,6 +55,17 @@ static bool split_dkdv(const PackedParams& p) {
   return n <= 128 || (n <= 256 && (p.causal || p.T / p.nseq < 320));
 }
 
+int64_t packed_fwd32_threads(const PackedParams& p, int dp) {
+  return packed_threads(p, (int64_t)p.Hk * p.G, dp == 64 && split_fwd(p) ? 32 : 128, 256);
+}
+int64_t packed_bwd32_threads(const PackedParams& p, int dp) {
+  const int64_t delta = ((int64_t)p.Hk * p.G * p.T + 15) / 16 * 256;
+  const int64_t dq = packed_threads(p, (int64_t)p.Hk * p.G, dp == 64 && split_dq(p) ? 32 : 128, 256);
+  const int64_t dkdv = packed_threads(p, (int64_t)p.Hk * p.parts, dp == 64 && split_dkdv(p) ? 32 : 128, 256);
+  const int64_t most = dq > dkdv ? dq : dkdv;
+  return delta > most ? delta : most;
+}
+
 template <int DP, bool CA>
 static void launch_packed_fwd32_t(PackedParams p, hipStream_t stream) {
   if constexpr (DP == 64) {

@@ -17,6 +17,13 @@ static void launch_packed_t(PackedParams p, hipStream_t stream) {
                      dim3(512), 0, stream, p);
 }
 
+int64_t packed_bwd_threads(const PackedParams& p, int io_dtype, int dp) {
+  if (io_dtype == kF32) return packed_bwd32_threads(p, dp);
+  const int64_t dq = packed_threads(p, (int64_t)p.Hk * p.G, 128, 256);
+  const int64_t dkdv = packed_threads(p, (int64_t)p.Hk * p.parts, 128, dp == 256 ? 256 : 512);
+  return dq > dkdv ? dq : dkdv;
+}
+
 template <typename T>
 static void launch_packed_d(const PackedParams& p, int dp, hipStream_t stream) {
   if (dp == 64) {

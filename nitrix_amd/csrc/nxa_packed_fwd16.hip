@@ -33,6 +33,12 @@ static bool four_waves(const PackedParams& p) {
   return p.T / p.nseq < (p.causal ? 3000 : 1400);
 }
 
+int64_t packed_fwd_threads(const PackedParams& p, int io_dtype, int dp) {
+  if (io_dtype == kF32) return packed_fwd32_threads(p, dp);
+  const int nw = dp == 128 && !four_waves(p) ? 8 : 4;
+  return packed_threads(p, (int64_t)p.Hk * p.G, nw * 32, nw * 64);
+}
+
 template <typename T>
 static void launch_packed_d(const PackedParams& p, int dp, hipStream_t stream) {
   if (dp == 64) launch_packed_t<T, 64, 4>(p, stream);

@@ -208,24 +208,29 @@ def _desc(q, k, v, o, offsets, scale, causal) -> _lib.NxaPackedDesc:
 
 
 def _forward(q, k, v, offsets, scale, causal, train):
-    """The output and, for a backward, the log-sum-exp and what the rounding of
-    the output left (16-bit types)."""
+    """The output and, for a backward, what the rounding of the output left
+    (16-bit types), the log-sum-exp and the bytes of the backward's workspace."""
     o = _empty_like(q, v.shape[2])
-    lse = o_lo = None
+    lse = o_lo = need = None
     if train:
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
         if q.dtype != torch.float32:
             o_lo = _empty_like(q, v.shape[2])
     desc = _desc(q, k, v, o, offsets, scale, causal)
+    lib = _lib.lib()
+    if train:
+        need = lib.nxa_packed_workspace_bytes(ctypes.byref(desc))
+        if need == 0:
+            raise HipNotTileable(lib.nxa_last_error().decode('utf-8', 'replace'))
     with _on(q.device):
         _lib.check(
-            _lib.lib().nxa_packed_fwd(
+            lib.nxa_packed_fwd(
                 ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 offsets.data_ptr(), o.data_ptr(), _ptr(o_lo), _ptr(lse),
                 _stream(q.device),
             )
         )
-    return o, o_lo, lse
+    return o, o_lo, lse, need
 
 
 class _PackedHip(torch.autograd.Function):
@@ -237,7 +242,7 @@ class _PackedHip(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, scale, causal):
         kq, kk, kv = _kernel_layout(q), _kernel_layout(k), _kernel_layout(v)
-        o, o_lo, lse = _forward(kq, kk, kv, offsets, scale, causal, True)
+        o, o_lo, lse, ctx.need = _forward(kq, kk, kv, offsets, scale, causal, True)
         ctx.args = (scale, causal)
         ctx.save_for_backward(kq, kk, kv, offsets, o, o_lo, lse)
         return o
@@ -251,8 +256,7 @@ class _PackedHip(torch.autograd.Function):
         dq, dk, dv = (_empty_like(x, x.shape[2]) for x in (q, k, v))
         desc = _desc(q, k, v, o, offsets, *ctx.args)
         lib = _lib.lib()
-        need = lib.nxa_packed_workspace_bytes(ctypes.byref(desc))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = torch.empty(ctx.need, dtype=torch.uint8, device=q.device)
         strides = [_lib.I64x2(*x.stride()[:2]) for x in (dout, dq, dk, dv)]
         with _on(q.device):
             _lib.check(
@@ -332,7 +336,7 @@ def packed_attention(
     if resolved == 'hip' and q.shape[1] > 0:
         try:
             return packed_attention_hip(q, k, v, offsets, scale=resolved_scale, causal=causal)
-        except HipNotTileable as exc:
+        except (HipNotTileable, _lib.NxaShapeError) as exc:
             fallback(
                 function='packed_attention',
                 requested='hip',

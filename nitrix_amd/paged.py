@@ -181,7 +181,7 @@ def _dispatch(name, backend, device, fused, reference, shapes, dtype):
         try:
             with _on(device):
                 return fused()
-        except HipNotTileable as exc:
+        except (HipNotTileable, _lib.NxaShapeError) as exc:
             fallback(
                 function=name,
                 requested='hip',

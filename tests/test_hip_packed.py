@@ -491,3 +491,21 @@ def test_forward_mode_falls_back_loudly():
     out = packed_attention(*ts, off, backend='hip')
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match='not itself differentiable'):
         torch.autograd.grad(out, ts, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+def test_more_sequences_than_a_grid_holds_fall_back():
+    """64 heads of 2^18 sequences: 2^32 threads forward; of 2^17: backward."""
+    q, k, v = _tokens(40, 64, 64, 8, 8, torch.float32, 93)
+    off = torch.full(((1 << 18) + 1,), 40, dtype=torch.int32, device=_dev())
+    off[0], off[1] = 0, 25
+    nx.reset_fallback_state()
+    with pytest.warns(nx.NitrixBackendFallback, match='grid'):
+        out = packed_attention(q, k, v, off, causal=True)
+    _check(q, k, v, [0, 25, 40], (out,), 1 / math.sqrt(8), True)
+    fewer = off[:(1 << 17) + 1]
+    b = [x.to(torch.bfloat16) for x in (q, k, v)]
+    _check(*b, [0, 25, 40], (packed_attention(*b, fewer, causal=True, backend='hip'),),
+           1 / math.sqrt(8), True)
+    nx.reset_fallback_state()
+    with pytest.warns(nx.NitrixBackendFallback, match='grid'):
+        packed_attention(b[0].requires_grad_(True), b[1], b[2], fewer, causal=True)

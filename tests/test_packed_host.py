@@ -251,3 +251,51 @@ def test_no_part_of_a_group_is_without_a_head():
                 assert (parts - 1) * per < g, (g, t, nseq, parts)
                 seen.add((g, parts))
     assert {(7, 4), (16, 1), (16, 4), (16, 6), (16, 8), (16, 16), (5, 3)} <= seen
+
+
+@pytest.mark.parametrize('kw, fwd, bwd', [
+    # 128 rows and 256 threads a block, 512 in dK / dV
+    (dict(H=64, Hk=64, T=64, nseq=(1 << 18) - 1), True, False),
+    (dict(H=64, Hk=64, T=64, nseq=1 << 18), False, False),
+    (dict(H=64, Hk=64, T=64, nseq=(1 << 17) - 1), True, True),
+    (dict(H=64, Hk=64, T=64, nseq=1 << 17), True, False),
+    (dict(H=2, Hk=2, T=(1 << 30) - 128 * 18, nseq=1), True, False),
+    (dict(H=2, Hk=2, T=(1 << 29) - 128 * 18, nseq=1), True, True),
+    # 8 waves: 256 rows and 512 threads
+    (dict(H=2, Hk=2, T=(1 << 30) - 256 * 18, nseq=1, D=128), True, False),
+    (dict(H=2, Hk=2, T=1 << 30, nseq=1, D=128), False, False),
+    # float32: -delta of 16 rows a block of 256
+    (dict(H=2, Hk=2, T=(1 << 27) - 16, nseq=1, io_dtype=_lib.NXA_F32), True, True),
+    (dict(H=2, Hk=2, T=1 << 27, nseq=1, io_dtype=_lib.NXA_F32), True, False),
+    # ... and 32-row blocks where they are few
+    (dict(H=1, Hk=1, T=1000, nseq=(1 << 24) - 64, io_dtype=_lib.NXA_F32), True, True),
+    (dict(H=1, Hk=1, T=1000, nseq=(1 << 24) - 62, io_dtype=_lib.NXA_F32), False, False),
+])
+def test_extents_past_a_grid_are_declined(kw, fwd, bwd):
+    """A launch holds less than 2^32 threads."""
+    lib, d = _lib.lib(), _desc(**kw)
+    assert lib.nxa_packed_check(ctypes.byref(d)) == (_lib.NXA_OK if fwd else _lib.NXA_E_SHAPE)
+    assert (lib.nxa_packed_workspace_bytes(ctypes.byref(d)) > 0) == bwd
+    P, s = 1 << 12, _lib.I64x2(6400, 64)
+    if not fwd:
+        assert lib.nxa_packed_fwd(ctypes.byref(d), P, P, P, P, P, None, None,
+                                  None) == _lib.NXA_E_SHAPE
+    if not bwd:
+        assert lib.nxa_packed_bwd(ctypes.byref(d), P, P, P, P, P, None, P, P, s, P, s, P, s, P, s,
+                                  P, 1 << 40, None) == _lib.NXA_E_SHAPE
+
+
+def test_extents_the_library_declines_fall_back(monkeypatch):
+    from nitrix_amd import packed
+
+    def declined(*args, **kw):
+        _lib.check(_lib.lib().nxa_packed_check(ctypes.byref(_desc(T=0))))
+
+    monkeypatch.setattr(packed, 'resolve_backend', lambda *a: 'hip')
+    monkeypatch.setattr(packed, 'packed_attention_hip', declined)
+    q, k, v = (torch.from_numpy(x) for x in _inputs(4, 2, 7, 8))
+    off = torch.tensor([0, 7], dtype=torch.int32)
+    nx.reset_fallback_state()
+    with pytest.warns(nx.NitrixBackendFallback, match='must be positive'):
+        out = packed_attention(q, k, v, off)
+    assert torch.equal(out, reference_packed_attention(q, k, v, off))

@@ -3,6 +3,7 @@ refusals, and the C ABI's checks (CPU only)."""
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import _paged_plain as plain
@@ -309,3 +310,32 @@ def test_forward_mode_is_left_to_the_reference_engine_or_refused():
                      lambda: nx.copy_pages(pool, a['v_pages'], [0], [1])):
             with pytest.raises(ValueError, match='forward-mode'):
                 call()
+
+
+def test_extents_past_a_grid_are_declined(monkeypatch):
+    """A launch holds less than 2^32 threads; attention's rows past 2^24 are
+    shared by its blocks instead of one each."""
+    lib, P, s = _lib.lib(), 1 << 12, _lib.I64x2(128, 64)
+    d = _pool()
+    small = lib.nxa_paged_workspace_bytes(ctypes.byref(d), (1 << 23) - 1, 1, 2)
+    assert small == 0 and lib.nxa_paged_workspace_bytes(ctypes.byref(d), 1 << 23, 1, 2) > 0
+    w = lib.nxa_pages_write
+    assert w(ctypes.byref(d), P, P, P, s, P, s, 1 << 26, P, 8, P, P, 4, 8, None) == _lib.NXA_E_SHAPE
+    n = 1 << 24
+    assert lib.nxa_pages_free(2, 2, 4, P, P, P, P, n, 2 * P, 2 * P, 2 * P, None) == _lib.NXA_E_SHAPE
+    assert lib.nxa_pages_fork(ctypes.byref(d), P, P, 2, 2, P, P, P, P, P, n, 2 * P, 2 * P, 2 * P, P,
+                              1 << 40, None) == _lib.NXA_E_SHAPE
+    ints = (ctypes.c_int32 * 400)(*range(400))
+    many = _pool(Hk=41944, P=400, k_str=(0, 1024, 64), v_str=(0, 1024, 64))
+    assert lib.nxa_pages_copy(ctypes.byref(many), P, P, ints, ints, 400, None) == _lib.NXA_E_SHAPE
+
+    from nitrix_amd import paged
+
+    def declined():
+        _lib.check(lib.nxa_pool_check(ctypes.byref(_pool(P=0))))
+
+    monkeypatch.setattr(paged, 'resolve_backend', lambda *a: 'hip')
+    monkeypatch.setattr(paged, '_on', lambda dev: contextlib.nullcontext())
+    nx.reset_fallback_state()
+    with pytest.warns(nx.NitrixBackendFallback, match='must be positive'):
+        assert paged._dispatch('f', 'auto', None, declined, lambda: 7, (), None) == 7

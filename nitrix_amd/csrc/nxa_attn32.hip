@@ -45,16 +45,16 @@
 #define NXA_PHASE __builtin_amdgcn_sched_barrier(0)
 #define NXA_TILE_AT(i) (i)
 #define NXA_CLASS_AT(i) 3
-#define NXA_TILE_ROW(t) (gfirst + (t) % gcnt) * BQ
+#define NXA_TILE_ROW(t) ((gfirst + (t) % gcnt) * BQ)
 #define NXA_DK_STRIDE grp.dk_rs
 #define NXA_DV_STRIDE grp.dv_rs
 #define NXA_DO_STRIDE pp.do_str[2]
 #define NXA_DQ_STRIDE pp.dq_str[2]
 #else
 #define NXA_PHASE (void)0
-#define NXA_TILE_AT(i) (int)(lst[i] & 0xffff)
-#define NXA_CLASS_AT(i) (int)(lst[i] >> 16)
-#define NXA_TILE_ROW(t) t * BQ
+#define NXA_TILE_AT(i) ((int)(lst[i] & 0xffff))
+#define NXA_CLASS_AT(i) ((int)(lst[i] >> 16))
+#define NXA_TILE_ROW(t) ((t) * BQ)
 #define NXA_DK_STRIDE p.k_str[2]
 #define NXA_DV_STRIDE p.v_str[2]
 #define NXA_DO_STRIDE p.o_str[2]

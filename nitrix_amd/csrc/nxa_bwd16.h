@@ -41,13 +41,13 @@
 // First query row of a dK / dV block's tile t; row strides of dO and of the
 // gradients, which a dense problem shares with o, q, k and v.
 #ifdef NXA_PACKED
-#define NXA_TILE_ROW(t) (gfirst + (t) % gcnt) * BQ
+#define NXA_TILE_ROW(t) ((gfirst + (t) % gcnt) * BQ)
 #define NXA_DK_STRIDE grp.dk_rs
 #define NXA_DV_STRIDE grp.dv_rs
 #define NXA_DO_STRIDE pp.do_str[2]
 #define NXA_DQ_STRIDE pp.dq_str[2]
 #else
-#define NXA_TILE_ROW(t) t * BQ
+#define NXA_TILE_ROW(t) ((t) * BQ)
 #define NXA_DK_STRIDE p.k_str[2]
 #define NXA_DV_STRIDE p.v_str[2]
 #define NXA_DO_STRIDE p.o_str[2]

@@ -116,17 +116,14 @@ __device__ __forceinline__ void vm_wait_le(int n) {
 // barriers t and t+1, so the stage of tile t-1 receives tile t + NST - 1.
 // Head dim 256 (4-wave blocks, one per CU): two 64 KB K / V stages, one tile
 // ahead; no bias-tile ring (LDS is full).
-template <int DP, int NW, int BMODE>
+template <int DP, int NW, int BMODE, bool PACKED>
 struct FwdRing {
   static constexpr bool TILE_BIAS = BMODE == kFbTile;
   static_assert(DP <= 128 || (NW == 4 && !TILE_BIAS), "head dim 256: 4 waves, no bias tiles");
   static constexpr bool LAG = NW == 8 && !(TILE_BIAS && DP == 128);
-#ifdef NXA_PACKED
-  // (two blocks of 4 waves share a CU's LDS at head dim 128)
-  static constexpr int NST = DP > 128 || (DP == 128 && NW == 4) ? 2 : 4;
-#else
-  static constexpr int NST = DP > 128 ? 2 : TILE_BIAS ? (LAG ? 3 : 2) : 4;  // K/V stages
-#endif
+  // K/V stages (packed: two blocks of 4 waves share a CU's LDS at head dim 128)
+  static constexpr int NST = DP > 128 || (PACKED && DP == 128 && NW == 4) ? 2
+                             : TILE_BIAS ? (LAG ? 3 : 2) : 4;
   static constexpr int AHEAD = LAG ? NST - 2 : NST - 1;      // K/V tiles ahead
   static constexpr int NSTB = TILE_BIAS ? (LAG ? 3 : 2) : 1;  // bias stages
   static constexpr int AHEADB = TILE_BIAS ? NSTB - 1 : 0;     // bias tiles ahead
@@ -147,7 +144,11 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const 
   using Frag = typename M::Frag;
   constexpr int EPC = 8, KC = 16;
   constexpr int BM = NW * 32, BN = 64;
-  using R = FwdRing<DP, NW, BMODE>;
+#ifdef NXA_PACKED
+  using R = FwdRing<DP, NW, BMODE, true>;
+#else
+  using R = FwdRing<DP, NW, BMODE, false>;
+#endif
   constexpr int NST = R::NST, AHEAD = R::AHEAD, NSTB = R::NSTB, AHEADB = R::AHEADB;
   constexpr bool VALU_BIAS = BMODE == kFbValu;
   constexpr bool MFMA_BIAS = BMODE == kFbRow || BMODE == kFbTile;

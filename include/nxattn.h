@@ -380,18 +380,18 @@ int nxa_pages_copy(const nxa_pool_desc* desc, void* k_pages, void* v_pages, cons
 /* Page management on contiguous tables [B, M], with reference counts refs [P]:
  * how many table entries name a page (none: it is free).  Results go to
  * arrays of their own.
- * free: the n < 2^24 listed rows (a row listed twice counts once) give their pages
- * back, become -1 and of length zero.
+ * free: the n < 2^24 listed rows (a row listed twice counts once) give their
+ * pages back, become -1 and of length zero.
  * extend: row b grows by counts[b] tokens (negative: none; at most to M * PS);
  * columns that these reach and that hold no page take free pages, lowest
  * first, in row and column order.  Where pages run out a row's length ends
  * with its last token that has one.  Workspace: P * 4 bytes.
- * fork: row dst[i] becomes a copy of row src[i], for n < 2^24 pairs (of those with
- * one target the last counts; src[i] == dst[i] does nothing): whole pages are
+ * fork: row dst[i] becomes a copy of row src[i], for n < 2^24 pairs (of those
+ * with one target the last counts; src[i] == dst[i] does nothing): whole pages are
  * shared, the tokens of a partly filled last page copied to a free page
- * (lowest first, in order of i; without one the row ends with its whole
- * pages).  The target's former pages are given back, but not handed out by
- * this call.
+ * (lowest first, in order of i; without one, or where the source has no such
+ * page, the row ends with its whole pages).  The target's former pages are
+ * given back, but not handed out by this call.
  * compact: n live pages end up in 0 .. n - 1: the k-th live page from n on is
  * copied to the k-th free one below n, and table entries and counts follow. */
 int nxa_pages_free(int32_t B, int32_t M, int32_t P, const int32_t* table,

@@ -352,8 +352,7 @@ __global__ __launch_bounds__(1024) void pages_extend_kernel(const RowsParams p) 
 // ---------------------------------------------------------------------------
 // Forks.  First a block settles which entries count (of those that name one
 // row as their target the last) and gives each that needs it a free page.
-// work[i]: -2 does not count, -1 no page needed (or none left: `short_` says
-// so), else the page.
+// work[i]: -2 does not count, -1 no page needed (or none left), else the page.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(1024) void pages_fork_plan_kernel(const RowsParams p) {
   __shared__ int wsum[16];
@@ -372,9 +371,11 @@ __global__ __launch_bounds__(1024) void pages_fork_plan_kernel(const RowsParams 
   __syncthreads();
   const int per = (p.n + 1023) / 1024;
   const int64_t room = (int64_t)p.M * p.PS;
+  // (a partly filled last page of a source that has that page)
   auto wants = [&](int i) {
-    const int64_t len = min(max((int64_t)p.lengths[p.rows[i]], (int64_t)0), room);
-    return len % p.PS != 0;
+    const int s = p.rows[i];
+    const int64_t len = min(max((int64_t)p.lengths[s], (int64_t)0), room);
+    return len % p.PS != 0 && is_page(p.table[(int64_t)s * p.M + len / p.PS], p.P);
   };
   int need = 0;
   for (int k = 0; k < per; ++k) {

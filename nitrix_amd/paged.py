@@ -472,17 +472,16 @@ def _reference_fork(k_pages, v_pages, page_table, lengths, refs, src, dst):
     src, dst = src[ok].long(), dst[ok].long()
     length = lengths[src].long().clamp(0, m * ps)
     full, rest = length // ps, length % ps
-    fresh = _handed_out(refs, rest > 0)
+    last_page = page_table[src, full.clamp(max=m - 1)]
+    fresh = _handed_out(refs, (rest > 0) & (last_page >= 0) & (last_page < p))
     got = fresh >= 0
     col = torch.arange(m, device=src.device)[None]
     rows = torch.where(col < full[:, None], page_table[src], -1)
     rows = torch.where((rows >= 0) & (rows < p), rows, -1)
     rows = torch.where((col == full[:, None]) & got[:, None], fresh[:, None], rows)
     out_refs = _counted(rows, _counted(page_table[dst], refs, -1), 1)
-    last_page = page_table[src, full.clamp(max=m - 1)]
-    copied = got & (last_page >= 0) & (last_page < p)
     slot = torch.arange(ps, device=src.device)[None] < rest[:, None]
-    f, s = torch.nonzero(copied[:, None] & slot, as_tuple=True)
+    f, s = torch.nonzero(got[:, None] & slot, as_tuple=True)
     with torch.no_grad():
         for pages in (k_pages, v_pages):
             pages[fresh[f].long(), :, s] = pages[last_page[f].long(), :, s]
@@ -616,12 +615,12 @@ def fork_sequences(
 
     Whole pages are shared (their counts grow).  The tokens in a partly filled
     last page are copied, in place, to a free page (the lowest first, in order
-    of ``i``), so that the two rows can grow apart; where none is left the new
-    row ends with its whole pages.  The target's former pages no longer count
-    for it, but are not handed out by the same call.  Sources are taken as
-    they were before the call.  Of several pairs with one target the last
-    counts; ``src[i] == dst[i]`` and numbers outside the table are ignored.
-    Returns the new ``(page_table, lengths, refs)``."""
+    of ``i``), so that the two rows can grow apart; where none is left, or the
+    source's tokens there are in no page, the new row ends with its whole
+    pages.  The target's former pages no longer count for it, but are not
+    handed out by the same call.  Sources are taken as they were before the
+    call.  Of several pairs with one target the last counts; ``src[i] ==
+    dst[i]`` and numbers outside the table are ignored.  Returns the new ``(page_table, lengths, refs)``."""
     _check_pool('fork_sequences', k_pages, v_pages, written=True)
     dev = page_table.device
     _check_table('fork_sequences', k_pages.device, page_table,

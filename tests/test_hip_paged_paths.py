@@ -242,3 +242,25 @@ def test_write_offsets_out_of_order_store_nothing_else():
             for buf, x in pools:
                 assert (buf[:edge] == 7).all() and (buf[-edge:] == 7).all(), (off, starts)
                 assert (x[other] == 7).all(), (off, starts)
+
+
+@pytest.mark.parametrize('wide', [4, 9000])
+def test_fork_of_a_row_whose_last_tokens_are_in_no_page(wide):
+    """As on the reference engine; the state copied by the call's own block or
+    by a launch before it."""
+    rng = np.random.default_rng(wide)
+    b, p, ps = 12, 60, 4
+    table = np.full((b, wide), -1, np.int32)
+    table[:6, :4] = rng.permutation(p)[:24].reshape(6, 4)
+    lengths = np.array([13, 16, 9, 7, 14, 5] + [0] * 6, np.int32)
+    table[0, 3], table[2, 2], table[4, 3] = -1, p, -2 ** 31
+    refs = np.bincount(table[(table >= 0) & (table < p)], minlength=p).astype(np.int32)
+    src, dst = [0, 1, 2, 3, 4, 5], [6, 7, 8, 9, 10, 11]
+    pools = [_rand((p, 2, ps, 16), torch.float32, i) for i in (1, 2)]
+    host = [x.clone().cpu() for x in pools]
+    got = nx.fork_sequences(*pools, *(_i32(x) for x in (table, lengths, refs, src, dst)), backend='hip')
+    args = [torch.tensor(x, dtype=torch.int32) for x in (table, lengths, refs, src, dst)]
+    want = nx.fork_sequences(*host, *args)
+    for a, w in zip((*got, *pools), (*want, *host)):
+        assert torch.equal(a.cpu(), w)
+    assert got[1][6:].tolist() == [12, 16, 8, 7, 12, 5]

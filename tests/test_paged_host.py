@@ -339,3 +339,15 @@ def test_extents_past_a_grid_are_declined(monkeypatch):
     nx.reset_fallback_state()
     with pytest.warns(nx.NitrixBackendFallback, match='must be positive'):
         assert paged._dispatch('f', 'auto', None, declined, lambda: 7, (), None) == 7
+
+
+def test_fork_of_a_row_whose_last_tokens_are_in_no_page():
+    """Nothing to copy: the new row ends with its whole pages instead of a page
+    of whatever a free one holds, and no page is handed out for it."""
+    table = _i32([[0, 1, -1, -1], [2, 9, -1, -1], [3, 4, -1, -1], [-1] * 4, [-1] * 4, [-1] * 4])
+    lengths, refs = _i32([10, 6, 7, 0, 0, 0]), _i32([1, 1, 1, 1, 1, 0, 0, 0])
+    k = torch.arange(8.).reshape(8, 1, 1, 1).expand(8, 1, 4, 4).contiguous()
+    t, n, c = nx.fork_sequences(k, -k, table, lengths, refs, _i32([0, 1, 2]), _i32([3, 4, 5]))
+    assert t[3:].tolist() == [[0, 1, -1, -1], [2, -1, -1, -1], [3, 5, -1, -1]]
+    assert n.tolist() == [10, 6, 7, 8, 4, 7] and c.tolist() == [2, 2, 2, 2, 1, 1, 0, 0]
+    assert (k[5, :, :3] == 4).all() and (k[6:] > 5).all()

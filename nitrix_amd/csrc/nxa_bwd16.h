@@ -56,6 +56,8 @@
 
 namespace nxa {
 
+// The largest P of a packed fp16 backward's exchange: 16 bits of ones.
+constexpr float kMostP16 = 0x1.fffp0f;
 constexpr int kMaxBwdTiles = 1024;
 // dQ's packed tile entries: key-tile index in the low 30 bits (and the
 // index past the last active tile), class in the top 2.
@@ -569,11 +571,12 @@ __global__ __launch_bounds__(512, 1) void dkdv16_kernel(const Params p) {
           u32x4 px;
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
-            const uint32_t lo = __float_as_uint(x[qb][8 * f + e] * 0x1p-112f) + 0x400u;
-            const uint32_t hi = __float_as_uint(x[qb][8 * f + e + 1] * 0x1p-112f) + 0x400u;
-            // (a P of 2 or more, which only an lse past 2^23 leaves, or NaN, does
-            // not reach its neighbour)
-            px[e >> 1] = (lo >> 11 & 0xffffu) | (hi << 5 & 0xffff0000u);
+            // (a P of 2 or more, which only an lse past 2^23 leaves, counts as 2,
+            // and so does a NaN, whose delta is NaN)
+            const float pl = fminf(x[qb][8 * f + e], kMostP16), ph = fminf(x[qb][8 * f + e + 1], kMostP16);
+            const uint32_t lo = __float_as_uint(pl * 0x1p-112f) + 0x400u;
+            const uint32_t hi = __float_as_uint(ph * 0x1p-112f) + 0x400u;
+            px[e >> 1] = lo >> 11 | (hi << 5 & 0xffff0000u);
           }
           *(lds_pfrag*)(uintptr_t)(poff + par * PB_BYTES + (qb * FPB + f) * 1024) =
               __builtin_bit_cast(f16x8, px);

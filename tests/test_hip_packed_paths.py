@@ -289,3 +289,36 @@ def test_offsets_out_of_order_store_nothing_beside_the_outputs(dtype, h, hk, d, 
         torch.cuda.synchronize()
         for name, x in dict(o=o, o_lo=o_lo, lse=lse, dq=dq, dk=dk, dv=dv, ws=ws).items():
             assert x.untouched_around(), (name, ends[:8])
+
+
+def test_float16_probabilities_past_two_saturate():
+    """Scores past 2^23, whose log-sum-exp in float32 leaves P of 2 and more
+    where 1/2 is right: as an operand of dS such a P counts as 2 and does not
+    wrap.  dV of one query shows the P that the kernel sees."""
+    n, d, scale = 256, 64, 8.0
+    g = torch.Generator().manual_seed(5)
+    q = (256 * (1 + torch.arange(n) / 256.0))[:, None, None].expand(n, 2, d)
+    k = torch.full((n, 2, d), 256.0)
+    v0 = torch.randn(n, 1, d, generator=g)
+    v = torch.cat((v0, -v0), 1)  # the output and delta are zero
+    do = torch.zeros(n, 2, d)
+    do[:, 1] = torch.randn(n, d, generator=g)
+    q, k, v, do = (x.reshape(1, 2 * n, d).to(torch.float16).to(_dev()) for x in (q, k, v, do))
+    got = _train(q, k, v, _off(range(0, 2 * n + 1, 2)), do, scale=scale)
+    o, _, dk, dv = (x.double().reshape(n, 2, d) for x in got)
+    q, v, do = (x.double().reshape(n, 2, d) for x in (q, v, do))
+    assert (o == 0).all()
+    top = do[:, 1:].abs().argmax(-1, keepdim=True)
+    p = dv.gather(2, top.expand(n, 2, 1)) / do[:, 1:].gather(2, top)  # [n, 2, 1]
+    assert int((p > 2.01).sum()) > 10 and int((p < 1.9).sum()) > 10
+    ds = p.clamp(max=2) * (v * do[:, 1:]).sum(-1, keepdim=True)
+    want = scale * ds * q[:, 1:]
+    # roundings of 2^-11: P as dV's operand and dV, P's exchange, dS, dK; dP in
+    # float32 of 64 terms; 2^-12 for the largest P below 2
+    tol = 6 * 2.0 ** -11 * want.abs() + scale * q[:, 1:] * p * 2.0 ** -16
+    near = (dk - want).abs() <= tol
+    # a dK past fp16's largest number, 65504, is infinite, as it is to round
+    # (|want| up to 8 * 512 * 2 * |v . do|, some 2e5); 2^-8: tol next to there
+    edge = 65504 * (1 - 2.0 ** -8)
+    past = (want.abs() >= edge) & (dk.abs() >= edge) & (dk.sign() == want.sign())
+    assert (near | past).all() and int(near.sum()) > dk.numel() // 2

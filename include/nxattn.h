@@ -289,8 +289,9 @@ int nxa_ssm_io_bwd(int64_t nb, int32_t L, int32_t d, int32_t n, int32_t dtype, c
  * rows must span less than 2^32 bytes); head dims as in nxa_desc.
  * offsets: nseq + 1 int32 on the device, non-decreasing in 0 .. T; values
  * outside are taken as the nearest bound and a sequence that ends before it
- * starts as empty (with decreasing offsets what rows hold is not defined).  Rows of no sequence (before offsets[0], from
- * offsets[nseq] on) are never read and their o, dq, dk, dv are zero.
+ * starts as empty (with decreasing offsets what rows hold is not defined).
+ * Rows of no sequence (before offsets[0], from offsets[nseq] on) are never
+ * read and their o, dq, dk, dv are zero.
  * lse [H, T] (natural log; may be NULL in the forward): rows of no sequence
  * are not written.
  * o_lo (bf16, fp16; o's strides; may be NULL, and is ignored in fp32): what the
@@ -383,8 +384,8 @@ int nxa_pages_copy(const nxa_pool_desc* desc, void* k_pages, void* v_pages, cons
  * free: the n < 2^24 listed rows (a row listed twice counts once) give their
  * pages back, become -1 and of length zero.
  * extend: row b grows by counts[b] tokens (negative: none; at most to M * PS);
- * columns that these reach and that hold no page take free pages, lowest
- * first, in row and column order.  Where pages run out a row's length ends
+ * columns behind the row's last token that these reach and that hold no page
+ * take free pages, lowest first, in row and column order.  Where pages run out a row's length ends
  * with its last token that has one.  Workspace: P * 4 bytes.
  * fork: row dst[i] becomes a copy of row src[i], for n < 2^24 pairs (of those
  * with one target the last counts; src[i] == dst[i] does nothing): whole pages are

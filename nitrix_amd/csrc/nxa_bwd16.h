@@ -20,6 +20,13 @@
 //   come out of one FMA per element, S * scale * log2(e) - lse * log2(e), on
 //   the exact fp32 products (scaling Q or K before the 16-bit rounding would
 //   perturb every logit by 2^-9 of its size in bf16).
+// * P and dS enter their products (dV; dK and dQ) in T, what the matrix core
+//   multiplies at full rate; what they are made of, sums and statistics stay in
+//   fp32.  As two terms of T each would double those products: packed, 16384
+//   tokens of 11 documents, 16 heads on 4, head dim 128, a training step (its
+//   forward's P alike) with one term / two 1093 / 1409 us, errors relative to
+//   float64 bf16 o 0.0021 / 0.0016, dq and dk 0.0024 / 0.0017, dv 0.0023 / 0.0017
+//   (the right ones are those of P and dS in fp32), fp16 an eighth of these.
 //
 // Kernel and launcher templates; instantiated by nxa_bwd16.hip (head dims
 // 64 and 128) and nxa_bwd16_wide.hip (256, compiled with flags of its own).

@@ -72,7 +72,9 @@ int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
     return fail(NXA_E_SHAPE, "%d sequences of up to %lld tokens exceed 2^31 tiles", B,
                 (long long)len);
   // (a block a row where a grid of less than 2^32 threads holds them)
-  plan->nblk = nxa::paged_whole(room) && rows < 1 << 24 ? 0 : nxa::paged_blocks(tiles * d->Hk * plan->strips);
+  plan->nblk = nxa::paged_whole(room) && rows < 1 << 24
+                   ? 0
+                   : nxa::paged_blocks(tiles * d->Hk * plan->strips);
   return NXA_OK;
 }
 

@@ -698,6 +698,12 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void fwd16_kernel(const 
   // P = exp2(S cc - m_ref) of the tile, packed to the T reduction fragments
   // of P V; returns this lane's half-row sum of P (four chains per block).
   // S is left intact, so a tile can be redone against another reference.
+  // P enters the product in T, as the reference engine's weights do; its sum
+  // stays in fp32.  As two terms of T it would cost half as many products
+  // again for an error that only a packed call shows: relative to float64,
+  // one term / two (and P in fp32), bf16 0.0020 to 0.0021 / 0.0016, fp16
+  // 0.00022 to 0.00024 / 0.00019; packed, head dim 128, 8192 tokens of 16 prompts
+  // 96 / 118 us, a prompt of 29,859 tokens 2942 / 4147.
   Frag pf[2][FPB];
   auto exp_tile = [&](float cc) NXA_INLINE -> float {
     const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;

@@ -44,6 +44,19 @@ __global__ __launch_bounds__(256) void packed_delta32_kernel(const PackedParams 
 // 2048 2737 - 17, causal 1589 - 43; volumes 352 - 49.  dK / dV: 64 blocks 374 -
 // 94; 256 blocks, all keys, 512 tokens 225 + 19, 4096 1434 + 57, causal 224 - 9,
 // 1495 - 306; volumes 352 - 15; 1024 blocks, causal 531 + 93.
+// Between the counts (8 heads of their own keys, sequences of one length, us of
+// the pass, split / large).  Forward, 256 tokens a sequence: 96 blocks 21 / 25,
+// 160 31 / 26, 200 59 / 52, 224 39 / 26, 240 40 / 27, 288 49 / 44; some 1100
+// tokens: 96 75 / 123, 160 95 / 104, 200 121 / 90, 224 122 / 101, 240 123 / 105,
+// 288 152 / 168; the same causal 40 / 123, 59 / 104, 68 / 88, 78 / 98, 83 / 104,
+// 94 / 102.  Backward, all keys, the rule of dK / dV alone changed: 144 blocks
+// of 192 tokens 94 / 93, 329 123 / 111; 176 of 201 105 / 93, 352 129 / 113; 208 of
+// 195 110 / 136, 256 112 / 94, 332 145 / 123; 240 of 192 112 / 117, 256 114 / 96,
+// 320 146 / 167, 426 180 / 219.  So from 130 to 240 blocks sequences that are all
+// short or all alike lose to the large forward block, by up to 17 us; where their
+// lengths differ (the volumes above, the usual call) the split one gains, and
+// the host does not know the lengths.  The 320 tokens of dK / dV lie among
+// crossings that move with the rounding up to whole blocks and rounds.
 static int64_t blocks128(const PackedParams& p, int heads) { return (int64_t)heads * p.T / 128; }
 static bool split_fwd(const PackedParams& p) { return blocks128(p, p.Hk * p.G) < 240; }
 static bool split_dq(const PackedParams& p) {
@@ -60,8 +73,9 @@ int64_t packed_fwd32_threads(const PackedParams& p, int dp) {
 }
 int64_t packed_bwd32_threads(const PackedParams& p, int dp) {
   const int64_t delta = ((int64_t)p.Hk * p.G * p.T + 15) / 16 * 256;
-  const int64_t dq = packed_threads(p, (int64_t)p.Hk * p.G, dp == 64 && split_dq(p) ? 32 : 128, 256);
-  const int64_t dkdv = packed_threads(p, (int64_t)p.Hk * p.parts, dp == 64 && split_dkdv(p) ? 32 : 128, 256);
+  const int64_t q = (int64_t)p.Hk * p.G, k = (int64_t)p.Hk * p.parts;
+  const int64_t dq = packed_threads(p, q, dp == 64 && split_dq(p) ? 32 : 128, 256);
+  const int64_t dkdv = packed_threads(p, k, dp == 64 && split_dkdv(p) ? 32 : 128, 256);
   const int64_t most = dq > dkdv ? dq : dkdv;
   return delta > most ? delta : most;
 }

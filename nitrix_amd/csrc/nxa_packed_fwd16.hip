@@ -7,7 +7,8 @@
 namespace nxa {
 
 // The dense kernel's ring is a type of its own.
-static_assert(FwdRing<128, 4, kFbNone, true>::NST == 2 && FwdRing<128, 4, kFbNone, false>::NST == 4);
+static_assert(FwdRing<128, 4, kFbNone, true>::NST == 2 &&
+              FwdRing<128, 4, kFbNone, false>::NST == 4);
 
 template <typename T, int DP, int NW>
 static void launch_packed_t(PackedParams p, hipStream_t stream) {

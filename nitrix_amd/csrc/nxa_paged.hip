@@ -51,9 +51,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float xor16(float x) { return __shfl_xor(x, 16, 64); }
 
-// Sum of the sequences' units a head (tiles of 128 tokens) before each of 256
-// consecutive groups of sequences, into pre[0 .. 256] (LDS); tiles of one
-// sequence by paged_tiles.
+// Tokens of sequence b, and tiles of so many.
 __device__ __forceinline__ int paged_len(const PagedParams& p, int b) {
   // (a length beyond the table's room counts as the room)
   const int64_t room = (int64_t)p.M * p.PS;
@@ -68,6 +66,8 @@ __device__ __forceinline__ int paged_units(const PagedParams& p, int b) {
   const int n = paged_tiles(paged_len(p, b));
   return n ? n + kStartUnits : 0;
 }
+// Sum of the sequences' units a head before each of 256 consecutive groups of
+// sequences, into pre[0 .. 256] (LDS).
 __device__ __forceinline__ void paged_prefix(const PagedParams& p, int* pre, int* wsum) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = (p.B + 255) / 256;

@@ -40,9 +40,13 @@ struct RowsParams {
   int start;          // the kernel itself copies what the results start from
 };
 
-// Up to so many numbers a single block copies the state itself: free, fork and
-// extend of 64 rows of 128 entries and 4096 pages, 66 -> 57 us a step, most of
-// it on the host, with three launches less.
+// Up to so many numbers a single block copies the state itself, which saves a
+// launch and the host 2 to 3 us of it.  us a call of free, fork, extend, alone /
+// with the launch: 4112 numbers 15.0 / 17.2, 26.0 / 28.6, 16.3 / 18.8; 28448 14.4 /
+// 16.7, 25.4 / 28.1, 16.0 / 18.6; 36928 14.3 / 16.7, 25.5 / 28.1, 16.0 / 18.5; 65600
+// 18.4 / 16.7, 25.5 / 28.1, 16.1 / 18.7; 196736 37.4 / 17.1, 27.7 / 28.0, 20.7 / 18.7.
+// (In a captured graph, without the host, the launch is the faster: 7.3 / 4.9,
+// 12.1 / 10.5, 7.7 / 6.1 at 4112, 11.2 / 4.8, 14.4 / 11.1, 9.5 / 6.1 at 28448.)
 constexpr int64_t kStartAlone = 32768;
 constexpr int kFreeAlone = 1024;  // rows that the single block frees
 // Columns of a grown row that a thread takes alone, a row's wave 64 a step.  us

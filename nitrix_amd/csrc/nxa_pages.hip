@@ -135,42 +135,40 @@ __global__ __launch_bounds__(256) void pages_write_kernel(const WriteParams p) {
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= p.T) return;
   const int ck = p.D * p.es / 16, cv = p.Dv * p.es / 16, all = p.Hk * (ck + cv);
-  {
-    int s = (int)t;
-    int64_t pos = 0;
-    if (p.offsets) {
-      int lo = 0, hi = p.B + 1;  // last s with offsets[s] <= t
-      while (hi - lo > 1) {
-        const int step = (hi - lo + 63) / 64;
-        const int x = lo + lane * step;
-        const int cnt = (int)__popcll(__ballot(x < hi && p.offsets[x] <= t));
-        if (cnt == 0) break;  // before the first sequence
-        lo += (cnt - 1) * step;
-        hi = min(lo + step, hi);
-      }
-      s = __builtin_amdgcn_readfirstlane(lo);
-      if (s >= p.B || p.offsets[s] > t) return;
-      pos = t - p.offsets[s];
+  int s = (int)t;
+  int64_t pos = 0;
+  if (p.offsets) {
+    int lo = 0, hi = p.B + 1;  // last s with offsets[s] <= t
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64;
+      const int x = lo + lane * step;
+      const int cnt = (int)__popcll(__ballot(x < hi && p.offsets[x] <= t));
+      if (cnt == 0) break;  // before the first sequence
+      lo += (cnt - 1) * step;
+      hi = min(lo + step, hi);
     }
-    pos += p.starts[s];
-    if (pos < 0 || pos >= (int64_t)p.M * p.PS) return;
-    const int page = p.table[s * p.table_rs + pos / p.PS];
-    if (!is_page(page, p.P)) return;
-    const int slot = (int)(pos % p.PS);
-    const char* ks = (const char*)p.ks + t * p.ks_str[1] * p.es;
-    const char* vs = (const char*)p.vs + t * p.vs_str[1] * p.es;
-    char* kd = (char*)p.k + (page * p.k_str[0] + slot * p.k_str[2]) * p.es;
-    char* vd = (char*)p.v + (page * p.v_str[0] + slot * p.v_str[2]) * p.es;
+    s = __builtin_amdgcn_readfirstlane(lo);
+    if (s >= p.B || p.offsets[s] > t) return;
+    pos = t - p.offsets[s];
+  }
+  pos += p.starts[s];
+  if (pos < 0 || pos >= (int64_t)p.M * p.PS) return;
+  const int page = p.table[s * p.table_rs + pos / p.PS];
+  if (!is_page(page, p.P)) return;
+  const int slot = (int)(pos % p.PS);
+  const char* ks = (const char*)p.ks + t * p.ks_str[1] * p.es;
+  const char* vs = (const char*)p.vs + t * p.vs_str[1] * p.es;
+  char* kd = (char*)p.k + (page * p.k_str[0] + slot * p.k_str[2]) * p.es;
+  char* vd = (char*)p.v + (page * p.v_str[0] + slot * p.v_str[2]) * p.es;
 #pragma unroll 4
-    for (int x = lane; x < all; x += 64) {
-      const bool key = x < p.Hk * ck;
-      const int y = key ? x : x - p.Hk * ck, cpr = key ? ck : cv;
-      const int h = y / cpr, c = 16 * (y - h * cpr);
-      const char* src = key ? ks + h * p.ks_str[0] * p.es : vs + h * p.vs_str[0] * p.es;
-      char* dst = key ? kd + h * p.k_str[1] * p.es : vd + h * p.v_str[1] * p.es;
-      *reinterpret_cast<u32x4*>(dst + c) =
-          __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + c));
-    }
+  for (int x = lane; x < all; x += 64) {
+    const bool key = x < p.Hk * ck;
+    const int y = key ? x : x - p.Hk * ck, cpr = key ? ck : cv;
+    const int h = y / cpr, c = 16 * (y - h * cpr);
+    const char* src = key ? ks + h * p.ks_str[0] * p.es : vs + h * p.vs_str[0] * p.es;
+    char* dst = key ? kd + h * p.k_str[1] * p.es : vd + h * p.v_str[1] * p.es;
+    *reinterpret_cast<u32x4*>(dst + c) =
+        __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + c));
   }
 }
 

@@ -20,8 +20,8 @@ graph.
 
 With :func:`~nitrix_amd.packed.packed_attention` for the prompts they serve a
 model: prompt keys and values are written while their attention runs packed,
-then each new token is written and attends its sequence's pages.  Nothing
-here is differentiable.  The reference has no counterpart; engines and
+then each new token is written and attends its sequence's pages.  The fused
+engine has no derivatives.  The reference has no counterpart; engines and
 ``backend`` as in :func:`~nitrix_amd.attention.scaled_dot_product_attention`
 (``'jax'``: the same functions in stock tensor ops).
 
@@ -563,8 +563,8 @@ def extend_sequences(
 ):
     """Room for ``counts[i]`` (int32 ``(b,)``) more tokens in each sequence.
 
-    Columns that the new tokens reach and that hold no page take free pages,
-    the lowest first, in row and then column order; lengths grow by the counts
+    Columns behind the row's last token that the new ones reach and that hold
+    no page take free pages, the lowest first, in row and then column order; lengths grow by the counts
     (below zero: none; at most to the table's room).  Where the pages run out, a
     row's length ends with its last token that has a page.  Returns the new
     ``(page_table, lengths, refs)``; the tokens themselves are then written at

@@ -65,7 +65,7 @@ PEAK_HBM_GBS = 8000.0
 # TRAFFIC_SRC is the fingerprint (_src_fingerprint) of the attention kernel
 # sources the passes ran; when the sources differ, the figure describes other
 # kernels and is reported as stale (traffic null, the old figure beside it).
-TRAFFIC_SRC = '6a6f897873f2b7b9'
+TRAFFIC_SRC = '738d21595883162f'
 MEASURED_TRAFFIC = {
     'c1': ('fwd', 6113962),
     'c2': ('dkdv', 910714325),

@@ -413,6 +413,92 @@ int nxa_pages_compact(const nxa_pool_desc* desc, void* k_pages, void* v_pages, i
                       const int32_t* table, const int32_t* refs, int32_t* table_out,
                       int32_t* refs_out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Quantised paged key-value cache.  A row (token and head) of D elements is
+ * held as codes of 4 or 8 bits with a scale s and a minimum z of io_dtype T: z =
+ * min, s = T((max - min) * r) in fp32 with r = 1 / (2^bits - 1) rounded to it, code
+ * = rint((x - z) / s) (the exact quotient, ties to even) in 0 .. 2^bits - 1, and
+ * stands for z + s code.  A row
+ * that holds NaN or infinity, or whose range is infinite, stands for NaN.
+ * k_pages [P, Hk, PS, D bits / 8] and v_pages [P, Hk, PS, Dv bits / 8] are bytes
+ * (4 bits: element 2 i in the low half of byte i), scales [P, Hk, PS, 4] of T
+ * hold k's s and z and v's s and z.  The slots of a (page, head) lie end to end;
+ * page and head strides are multiples of 4 bytes (codes) and 4 elements (scales).
+ * D and Dv are multiples of 8 up to 256.  Pointers are 16-byte aligned.  Page
+ * tables and the rest as for nxa_pool_desc.  No counterpart in the reference. */
+typedef struct {
+  int32_t P, Hk, PS, D, Dv;
+  int32_t io_dtype;       /* nxa_dtype of scales, q, k, v and o              */
+  int32_t bits;           /* 4 or 8                                          */
+  int64_t k_str[2];       /* page and head strides: bytes                    */
+  int64_t v_str[2];       /* bytes                                           */
+  int64_t s_str[2];       /* elements                                        */
+} nxa_quant_pool_desc;
+
+/* Host-only validation (no GPU needed). */
+int nxa_quant_pool_check(const nxa_quant_pool_desc* desc);
+
+/* New tokens into their pages as nxa_pages_write does, quantised. */
+int nxa_quant_write(const nxa_quant_pool_desc* desc, void* k_pages, void* v_pages, void* scales,
+                    const void* k, const int64_t* k_str, const void* v, const int64_t* v_str,
+                    int64_t T, const int32_t* table, int64_t table_rs, const int32_t* starts,
+                    const int32_t* offsets, int32_t B, int32_t M, void* stream);
+
+/* The tokens that nxa_quant_write's arguments name, back into k [Hk, T, D] and v
+ * [Hk, T, Dv]; zero for tokens of no sequence, outside the table or in no page. */
+int nxa_quant_read(const nxa_quant_pool_desc* desc, const void* k_pages, const void* v_pages,
+                   const void* scales, void* k, const int64_t* k_str, void* v,
+                   const int64_t* v_str, int64_t T, const int32_t* table, int64_t table_rs,
+                   const int32_t* starts, const int32_t* offsets, int32_t B, int32_t M,
+                   void* stream);
+
+/* nxa_paged_fwd over quantised pages.  M * PS < 2^31 - 4096. */
+size_t nxa_quant_paged_workspace_bytes(const nxa_quant_pool_desc* desc, int32_t B, int32_t M,
+                                       int32_t H);
+int nxa_quant_paged_fwd(const nxa_quant_pool_desc* desc, const void* k_pages, const void* v_pages,
+                        const void* scales, const void* q, const int64_t* q_str,
+                        const int32_t* table, int64_t table_rs, const int32_t* lengths, int32_t B,
+                        int32_t M, int32_t H, float scale, void* o, const int64_t* o_str,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* nxa_pages_copy, nxa_pages_fork and nxa_pages_compact (with their workspaces)
+ * over quantised pages. */
+int nxa_quant_copy(const nxa_quant_pool_desc* desc, void* k_pages, void* v_pages, void* scales,
+                   const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+int nxa_quant_fork(const nxa_quant_pool_desc* desc, void* k_pages, void* v_pages, void* scales,
+                   int32_t B, int32_t M, const int32_t* table, const int32_t* lengths,
+                   const int32_t* refs, const int32_t* src, const int32_t* dst, int32_t n,
+                   int32_t* table_out, int32_t* lengths_out, int32_t* refs_out, void* workspace,
+                   size_t workspace_bytes, void* stream);
+int nxa_quant_compact(const nxa_quant_pool_desc* desc, void* k_pages, void* v_pages, void* scales,
+                      int64_t entries, const int32_t* table, const int32_t* refs,
+                      int32_t* table_out, int32_t* refs_out, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Rotary positions.  q [B, H, T, D] and k [B, Hk, T, D] (Hk = 0: none), batch, head
+ * and token strides, unit stride over D (at most 256).  Of a row at position p
+ * pair i < R / 2, elements (i, i + R / 2) or, interleaved, (2 i, 2 i + 1), turns by p
+ * frequencies[i] radians and is multiplied by scale: a' = scale (a cos - b sin),
+ * b' = scale (b cos + a sin); inverse turns back (the gradient).  Elements from R on
+ * are copied.  positions [B, T] are int32 (pos64: int64) with batch and token
+ * strides, frequencies [R / 2] doubles, both on the device.  Outputs must not
+ * overlap the inputs.  B ceil(T / 4) < 2^24.  No counterpart in the reference. */
+typedef struct {
+  int32_t B, T, H, Hk, D, R;
+  int32_t io_dtype;       /* nxa_dtype of q, k and the outputs               */
+  int32_t interleaved, inverse, pos64;
+  float scale;
+  int64_t pos_str[2];
+  int64_t q_str[3];
+  int64_t k_str[3];
+  int64_t q_out_str[3];
+  int64_t k_out_str[3];
+} nxa_rotary_desc;
+
+/* Host-only validation (no GPU needed). */
+int nxa_rotary_check(const nxa_rotary_desc* desc);
+int nxa_rotary(const nxa_rotary_desc* desc, const void* q, const void* k, const void* positions,
+               const double* frequencies, void* q_out, void* k_out, void* stream);
+
 /* Message of the last failure on this thread ("" if none). */
 const char* nxa_last_error(void);
 

@@ -82,6 +82,16 @@ EXPORTS = (
     'nxa_pages_fork',
     'nxa_pages_compact_workspace_bytes',
     'nxa_pages_compact',
+    'nxa_quant_pool_check',
+    'nxa_quant_write',
+    'nxa_quant_read',
+    'nxa_quant_paged_workspace_bytes',
+    'nxa_quant_paged_fwd',
+    'nxa_quant_copy',
+    'nxa_quant_fork',
+    'nxa_quant_compact',
+    'nxa_rotary_check',
+    'nxa_rotary',
     'nxa_last_error',
     'nxa_profile_enable',
     'nxa_profile_read',
@@ -147,6 +157,46 @@ class NxaPoolDesc(ctypes.Structure):
         ('io_dtype', ctypes.c_int32),
         ('k_str', _I64x3),
         ('v_str', _I64x3),
+    ]
+
+
+class NxaQuantPoolDesc(ctypes.Structure):
+    """Mirror of ``nxa_quant_pool_desc``."""
+
+    _fields_ = [
+        ('P', ctypes.c_int32),
+        ('Hk', ctypes.c_int32),
+        ('PS', ctypes.c_int32),
+        ('D', ctypes.c_int32),
+        ('Dv', ctypes.c_int32),
+        ('io_dtype', ctypes.c_int32),
+        ('bits', ctypes.c_int32),
+        ('k_str', I64x2),
+        ('v_str', I64x2),
+        ('s_str', I64x2),
+    ]
+
+
+class NxaRotaryDesc(ctypes.Structure):
+    """Mirror of ``nxa_rotary_desc``."""
+
+    _fields_ = [
+        ('B', ctypes.c_int32),
+        ('T', ctypes.c_int32),
+        ('H', ctypes.c_int32),
+        ('Hk', ctypes.c_int32),
+        ('D', ctypes.c_int32),
+        ('R', ctypes.c_int32),
+        ('io_dtype', ctypes.c_int32),
+        ('interleaved', ctypes.c_int32),
+        ('inverse', ctypes.c_int32),
+        ('pos64', ctypes.c_int32),
+        ('scale', ctypes.c_float),
+        ('pos_str', I64x2),
+        ('q_str', _I64x3),
+        ('k_str', _I64x3),
+        ('q_out_str', _I64x3),
+        ('k_out_str', _I64x3),
     ]
 
 
@@ -271,6 +321,31 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nxa_pages_compact_workspace_bytes.argtypes = [i32]
     lib.nxa_pages_compact.restype = ctypes.c_int
     lib.nxa_pages_compact.argtypes = [dl, vp, vp, i64] + [vp] * 5 + [sz, vp]
+    dq = ctypes.POINTER(NxaQuantPoolDesc)
+    lib.nxa_quant_pool_check.restype = ctypes.c_int
+    lib.nxa_quant_pool_check.argtypes = [dq]
+    for move in (lib.nxa_quant_write, lib.nxa_quant_read):
+        move.restype = ctypes.c_int
+        move.argtypes = [dq, vp, vp, vp, vp, s2, vp, s2, i64, vp, i64, vp, vp, i32, i32, vp]
+    lib.nxa_quant_paged_workspace_bytes.restype = sz
+    lib.nxa_quant_paged_workspace_bytes.argtypes = [dq, i32, i32, i32]
+    lib.nxa_quant_paged_fwd.restype = ctypes.c_int
+    lib.nxa_quant_paged_fwd.argtypes = [
+        dq, vp, vp, vp, vp, s2, vp, i64, vp, i32, i32, i32, ctypes.c_float, vp, s2, vp, sz, vp,
+    ]
+    lib.nxa_quant_copy.restype = ctypes.c_int
+    lib.nxa_quant_copy.argtypes = [dq, vp, vp, vp, vp, vp, i32, vp]
+    lib.nxa_quant_fork.restype = ctypes.c_int
+    lib.nxa_quant_fork.argtypes = (
+        [dq, vp, vp, vp, i32, i32] + [vp] * 5 + [i32] + [vp] * 4 + [sz, vp]
+    )
+    lib.nxa_quant_compact.restype = ctypes.c_int
+    lib.nxa_quant_compact.argtypes = [dq, vp, vp, vp, i64] + [vp] * 5 + [sz, vp]
+    dr = ctypes.POINTER(NxaRotaryDesc)
+    lib.nxa_rotary_check.restype = ctypes.c_int
+    lib.nxa_rotary_check.argtypes = [dr]
+    lib.nxa_rotary.restype = ctypes.c_int
+    lib.nxa_rotary.argtypes = [dr] + [vp] * 7
     lib.nxa_last_error.restype = ctypes.c_char_p
     lib.nxa_last_error.argtypes = []
     lib.nxa_profile_enable.restype = ctypes.c_int

@@ -1364,3 +1364,5 @@ int nxa_profile_reset(void) {
 
 #include "nxa_capi_packed.h"
 #include "nxa_capi_paged.h"
+#include "nxa_capi_quant.h"
+#include "nxa_capi_rotary.h"

@@ -59,28 +59,34 @@ struct PagedPlan {
   int strips, nblk;
 };
 
-int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
-  if (H <= 0 || H % d->Hk != 0)
-    return fail(NXA_E_SHAPE, "H=%d must be a positive multiple of Hk=%d", H, d->Hk);
-  plan->strips = (H / d->Hk + 15) / 16;
+int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t), PagedPlan* plan) {
+  if (H <= 0 || H % Hk != 0)
+    return fail(NXA_E_SHAPE, "H=%d must be a positive multiple of Hk=%d", H, Hk);
+  plan->strips = (H / Hk + 15) / 16;
   // Units of the largest table, in 31 bits a head.
-  const int64_t room = (int64_t)M * d->PS;
+  const int64_t room = (int64_t)M * PS;
   const int64_t len = room < INT32_MAX ? room : INT32_MAX;
   const int64_t tiles = (int64_t)B * ((len + nxa::kPagedKeys - 1) / nxa::kPagedKeys + nxa::kStartUnits);
-  const int64_t rows = (int64_t)B * d->Hk * plan->strips;
+  const int64_t rows = (int64_t)B * Hk * plan->strips;
   if (tiles >= (int64_t)1 << 31 || rows >= (int64_t)1 << 31)
     return fail(NXA_E_SHAPE, "%d sequences of up to %lld tokens exceed 2^31 tiles", B,
                 (long long)len);
   // (a block a row where a grid of less than 2^32 threads holds them)
-  plan->nblk = nxa::paged_whole(room) && rows < 1 << 24
-                   ? 0
-                   : nxa::paged_blocks(tiles * d->Hk * plan->strips);
+  plan->nblk =
+      whole(room) && rows < 1 << 24 ? 0 : nxa::paged_blocks(tiles * Hk * plan->strips);
   return NXA_OK;
 }
 
-size_t paged_workspace(const nxa_pool_desc* d, const PagedPlan& plan) {
-  const int dp = nxa::paged_dp(d->D > d->Dv ? d->D : d->Dv);
+int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
+  return plan_paged(d->Hk, d->PS, B, M, H, nxa::paged_whole, plan);
+}
+
+size_t paged_workspace(int dp, const PagedPlan& plan) {
   return (size_t)plan.nblk * (2 * nxa::paged_part_floats(dp) * 4 + sizeof(int4));
+}
+
+size_t paged_workspace(const nxa_pool_desc* d, const PagedPlan& plan) {
+  return paged_workspace(nxa::paged_dp(d->D > d->Dv ? d->D : d->Dv), plan);
 }
 
 // Free, extend and fork: contiguous tables, results in arrays of their own.
@@ -122,6 +128,94 @@ int need_workspace(const void* ws, size_t have, size_t need) {
     return fail(NXA_E_WORKSPACE, "workspace of %zu bytes, %zu needed (16-byte aligned)",
                 ws ? have : (size_t)0, need);
   return NXA_OK;
+}
+
+size_t fork_workspace(int B, int P, int n) {
+  if (B <= 0 || P <= 0 || n < 0) return 0;
+  return ((size_t)n + B + (n < P ? n : P)) * 4;
+}
+
+size_t compact_workspace(int P) {
+  if (P <= 0 || P > kMostPages) return 0;
+  const size_t nb = ((size_t)P + nxa::kCompactPages - 1) / nxa::kCompactPages;
+  return (nb + 4 + 3 * (size_t)P) * 4;
+}
+
+// Copies, forks and compaction of a checked pool: PoolParams, es its elements'
+// bytes, or QuantPool, es its scales'.
+template <typename Pool>
+int pages_copy(const char* name, const Pool& p, int es, const int32_t* src, const int32_t* dst,
+               int n, void* stream) {
+  if (n < 0 || (n > 0 && (!src || !dst))) return fail(NXA_E_ARG, "n=%d pairs", n);
+  if ((int64_t)(n < nxa::kCopyPairs ? n : nxa::kCopyPairs) * p.Hk * 256 >= (int64_t)1 << 32)
+    return fail(NXA_E_SHAPE, "Hk=%d exceeds the grid", p.Hk);
+  for (int i = 0; i < n; ++i)
+    if (src[i] < 0 || src[i] >= p.P || dst[i] < 0 || dst[i] >= p.P)
+      return fail(NXA_E_ARG, "pair %d (%d -> %d) is outside the pool's %d pages", i, src[i],
+                  dst[i], p.P);
+  hipStream_t s = (hipStream_t)stream;
+  return launch(name, s, [&] {
+    nxa::CopyPairs c;
+    for (int i = 0; i < n; i += c.n) {
+      c.n = n - i < nxa::kCopyPairs ? n - i : nxa::kCopyPairs;
+      memcpy(c.src, src + i, c.n * sizeof(int));
+      memcpy(c.dst, dst + i, c.n * sizeof(int));
+      nxa::launch_pages_copy(p, es, c, s);
+    }
+  });
+}
+
+template <typename Pool>
+int pages_fork(const char* name, const Pool& pool, int es, int B, int M, const int32_t* table,
+               const int32_t* lengths, const int32_t* refs, const int32_t* src,
+               const int32_t* dst, int n, int32_t* table_out, int32_t* lengths_out,
+               int32_t* refs_out, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc =
+      check_rows(B, M, pool.P, pool.PS, table, lengths, refs, table_out, lengths_out, refs_out);
+  if (rc) return rc;
+  if (n < 0 || (n > 0 && (!src || !dst))) return fail(NXA_E_ARG, "n=%d forks", n);
+  if (n >= kMostListed) return fail(NXA_E_SHAPE, "n=%d: less than 2^24 forks a call", n);
+  if (pool.Hk >= 65535) return fail(NXA_E_SHAPE, "Hk=%d exceeds the grid", pool.Hk);
+  rc = need_workspace(workspace, workspace_bytes, n ? fork_workspace(B, pool.P, n) : 0);
+  if (rc) return rc;
+  nxa::RowsParams p =
+      rows_params(B, M, pool.P, pool.PS, table, lengths, refs, table_out, lengths_out, refs_out);
+  p.rows = src;
+  p.counts = dst;
+  p.n = n;
+  p.work = (int*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  return launch(name, s, [&] { nxa::launch_pages_fork(p, pool, es, s); });
+}
+
+template <typename Pool>
+int pages_compact(const char* name, const Pool& pool, int es, int64_t entries,
+                  const int32_t* table, const int32_t* refs, int32_t* table_out,
+                  int32_t* refs_out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (entries < 0) return fail(NXA_E_SHAPE, "%lld table entries", (long long)entries);
+  if ((entries && (!table || !table_out)) || !refs || !refs_out)
+    return fail(NXA_E_ARG, "a table or refs pointer is NULL");
+  if ((entries && table == table_out) || refs == refs_out)
+    return fail(NXA_E_ARG, "results need arrays of their own");
+  const int rc = need_workspace(workspace, workspace_bytes, compact_workspace(pool.P));
+  if (rc) return rc;
+  nxa::CompactParams p = {};
+  p.table = table;
+  p.refs = refs;
+  p.table_out = table_out;
+  p.refs_out = refs_out;
+  p.entries = entries;
+  p.P = pool.P;
+  p.Hk = pool.Hk;
+  p.PS = pool.PS;
+  int* w = (int*)workspace;
+  p.movers = w;
+  p.holes = w + p.P;
+  p.mover_rank = w + 2 * (size_t)p.P;
+  p.info = w + 3 * (size_t)p.P;
+  p.counts = p.info + 4;
+  hipStream_t s = (hipStream_t)stream;
+  return launch(name, s, [&] { nxa::launch_pages_compact(p, pool, es, s); });
 }
 
 }  // namespace
@@ -223,26 +317,9 @@ int nxa_pages_copy(const nxa_pool_desc* d, void* k_pages, void* v_pages, const i
   int rc = check_pool(d);
   if (!rc) rc = check_pool_ptrs(k_pages, v_pages);
   if (rc) return rc;
-  if (n < 0 || (n > 0 && (!src || !dst))) return fail(NXA_E_ARG, "n=%d pairs", n);
-  if ((int64_t)(n < nxa::kCopyPairs ? n : nxa::kCopyPairs) * d->Hk * 256 >= (int64_t)1 << 32)
-    return fail(NXA_E_SHAPE, "Hk=%d exceeds the grid", d->Hk);
-  for (int i = 0; i < n; ++i)
-    if (src[i] < 0 || src[i] >= d->P || dst[i] < 0 || dst[i] >= d->P)
-      return fail(NXA_E_ARG, "pair %d (%d -> %d) is outside the pool's %d pages", i, src[i],
-                  dst[i], d->P);
   nxa::PoolParams p = {};
   set_pool(p, d, k_pages, v_pages);
-  const int es = esize(d->io_dtype);
-  hipStream_t s = (hipStream_t)stream;
-  return launch("pages_copy", s, [&] {
-    nxa::CopyPairs c;
-    for (int i = 0; i < n; i += c.n) {
-      c.n = n - i < nxa::kCopyPairs ? n - i : nxa::kCopyPairs;
-      memcpy(c.src, src + i, c.n * sizeof(int));
-      memcpy(c.dst, dst + i, c.n * sizeof(int));
-      nxa::launch_pages_copy(p, es, c, s);
-    }
-  });
+  return pages_copy("pages_copy", p, esize(d->io_dtype), src, dst, n, stream);
 }
 
 int nxa_pages_free(int32_t B, int32_t M, int32_t P, const int32_t* table, const int32_t* lengths,
@@ -276,8 +353,7 @@ int nxa_pages_extend(int32_t B, int32_t M, int32_t P, int32_t PS, const int32_t*
 }
 
 size_t nxa_pages_fork_workspace_bytes(int32_t B, int32_t P, int32_t n) {
-  if (B <= 0 || P <= 0 || n < 0) return 0;
-  return ((size_t)n + B + (n < P ? n : P)) * 4;
+  return fork_workspace(B, P, n);
 }
 
 int nxa_pages_fork(const nxa_pool_desc* d, void* k_pages, void* v_pages, int32_t B, int32_t M,
@@ -287,32 +363,14 @@ int nxa_pages_fork(const nxa_pool_desc* d, void* k_pages, void* v_pages, int32_t
                    size_t workspace_bytes, void* stream) {
   int rc = check_pool(d);
   if (!rc) rc = check_pool_ptrs(k_pages, v_pages);
-  if (!rc)
-    rc = check_rows(B, M, d->P, d->PS, table, lengths, refs, table_out, lengths_out, refs_out);
   if (rc) return rc;
-  if (n < 0 || (n > 0 && (!src || !dst))) return fail(NXA_E_ARG, "n=%d forks", n);
-  if (n >= kMostListed) return fail(NXA_E_SHAPE, "n=%d: less than 2^24 forks a call", n);
-  if (d->Hk >= 65535) return fail(NXA_E_SHAPE, "Hk=%d exceeds the grid", d->Hk);
-  rc = need_workspace(workspace, workspace_bytes, n ? nxa_pages_fork_workspace_bytes(B, d->P, n) : 0);
-  if (rc) return rc;
-  nxa::RowsParams p =
-      rows_params(B, M, d->P, d->PS, table, lengths, refs, table_out, lengths_out, refs_out);
-  p.rows = src;
-  p.counts = dst;
-  p.n = n;
-  p.work = (int*)workspace;
   nxa::PoolParams pool = {};
   set_pool(pool, d, k_pages, v_pages);
-  hipStream_t s = (hipStream_t)stream;
-  return launch("pages_fork", s,
-                [&] { nxa::launch_pages_fork(p, pool, esize(d->io_dtype), s); });
+  return pages_fork("pages_fork", pool, esize(d->io_dtype), B, M, table, lengths, refs, src, dst, n,
+                    table_out, lengths_out, refs_out, workspace, workspace_bytes, stream);
 }
 
-size_t nxa_pages_compact_workspace_bytes(int32_t P) {
-  if (P <= 0 || P > kMostPages) return 0;
-  const size_t nb = ((size_t)P + nxa::kCompactPages - 1) / nxa::kCompactPages;
-  return (nb + 4 + 3 * (size_t)P) * 4;
-}
+size_t nxa_pages_compact_workspace_bytes(int32_t P) { return compact_workspace(P); }
 
 int nxa_pages_compact(const nxa_pool_desc* d, void* k_pages, void* v_pages, int64_t entries,
                       const int32_t* table, const int32_t* refs, int32_t* table_out,
@@ -320,33 +378,10 @@ int nxa_pages_compact(const nxa_pool_desc* d, void* k_pages, void* v_pages, int6
   int rc = check_pool(d);
   if (!rc) rc = check_pool_ptrs(k_pages, v_pages);
   if (rc) return rc;
-  if (entries < 0) return fail(NXA_E_SHAPE, "%lld table entries", (long long)entries);
-  if ((entries && (!table || !table_out)) || !refs || !refs_out)
-    return fail(NXA_E_ARG, "a table or refs pointer is NULL");
-  if ((entries && table == table_out) || refs == refs_out)
-    return fail(NXA_E_ARG, "results need arrays of their own");
-  rc = need_workspace(workspace, workspace_bytes, nxa_pages_compact_workspace_bytes(d->P));
-  if (rc) return rc;
-  nxa::CompactParams p = {};
-  p.table = table;
-  p.refs = refs;
-  p.table_out = table_out;
-  p.refs_out = refs_out;
-  p.entries = entries;
-  p.P = d->P;
-  p.Hk = d->Hk;
-  p.PS = d->PS;
-  int* w = (int*)workspace;
-  p.movers = w;
-  p.holes = w + p.P;
-  p.mover_rank = w + 2 * (size_t)p.P;
-  p.info = w + 3 * (size_t)p.P;
-  p.counts = p.info + 4;
   nxa::PoolParams pool = {};
   set_pool(pool, d, k_pages, v_pages);
-  hipStream_t s = (hipStream_t)stream;
-  return launch("pages_compact", s,
-                [&] { nxa::launch_pages_compact(p, pool, esize(d->io_dtype), s); });
+  return pages_compact("pages_compact", pool, esize(d->io_dtype), entries, table, refs, table_out,
+                       refs_out, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

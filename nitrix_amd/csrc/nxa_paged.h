@@ -46,5 +46,7 @@ int paged_dp(int m);               // padded head dim
 bool paged_whole(int64_t room);
 int paged_blocks(int64_t most_units);
 void launch_paged(const PagedParams& p, int io_dtype, hipStream_t stream);
+// The second kernel alone, for pieces of dp = 64, 128 or 256 columns.
+void launch_paged_join(const PagedParams& p, int io_dtype, int dp, hipStream_t stream);
 
 }  // namespace nxa

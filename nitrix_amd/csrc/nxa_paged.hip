@@ -35,7 +35,7 @@
 // more than 2^kSlack; sums and outputs accumulate against the same maximum in
 // fp32.  In 16 bits P enters the second product as a pair of terms, so that of
 // its rounding 2^-16 (bf16) is left; fp32 pools are multiplied in fp32.
-#include "nxa_paged.h"
+#include "nxa_paged_units.h"
 
 #include <type_traits>
 
@@ -43,67 +43,9 @@ namespace nxa {
 
 namespace {
 
-constexpr float kSlack = 8.0f;
-constexpr int kWaves = 4;
 constexpr int kStepKeys = 16;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float xor16(float x) { return __shfl_xor(x, 16, 64); }
-
-// Tokens of sequence b, and tiles of so many.
-__device__ __forceinline__ int paged_len(const PagedParams& p, int b) {
-  // (a length beyond the table's room counts as the room)
-  const int64_t room = (int64_t)p.M * p.PS;
-  const int n = p.lengths[b];
-  return n < 0 ? 0 : n > room ? (int)room : n;
-}
-__device__ __forceinline__ int paged_tiles(int len) {
-  return (int)(((int64_t)len + kPagedKeys - 1) / kPagedKeys);
-}
-// Units of a (sequence, head): its tiles after kStartUnits for starting on it.
-__device__ __forceinline__ int paged_units(const PagedParams& p, int b) {
-  const int n = paged_tiles(paged_len(p, b));
-  return n ? n + kStartUnits : 0;
-}
-// Sum of the sequences' units a head before each of 256 consecutive groups of
-// sequences, into pre[0 .. 256] (LDS).
-__device__ __forceinline__ void paged_prefix(const PagedParams& p, int* pre, int* wsum) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (p.B + 255) / 256;
-  int n = 0;
-  for (int i = 0; i < per; ++i)
-    if (tid * per + i < p.B) n += paged_units(p, tid * per + i);
-  int x = n;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) wsum[wave] = x;
-  __syncthreads();
-  int base = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) base += w < wave ? wsum[w] : 0;
-  pre[tid + 1] = base + x;
-  if (tid == 0) pre[0] = 0;
-  __syncthreads();
-}
-
-// Blocks that get work: at most one a unit, so that none of them is empty
-// (the join takes a piece from every block between a row's first and last).
-__device__ __forceinline__ int busy_blocks(const PagedParams& p, int64_t units) {
-  return (int)min((int64_t)p.nblk, units);
-}
-// o of a sequence without tokens.
-template <typename T>
-__device__ __forceinline__ void paged_zero(const PagedParams& p, int b) {
-  T* op = (T*)p.o + b * p.o_str[0];
-  for (int i = threadIdx.x; i < p.Hk * p.G * p.Dv; i += 256)
-    op[(i / p.Dv) * p.o_str[1] + i % p.Dv] = (T)0.f;
-}
-// First unit of block i of n.
-__device__ __forceinline__ int64_t first_unit(int64_t units, int i, int n) { return units * i / n; }
 
 template <typename T>
 struct Step;  // products of one 16-token step
@@ -146,32 +88,6 @@ struct Step<f16> {
     return f32x4{(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
   }
 };
-
-constexpr int kNonTemporal = 2;  // cache policy of a buffer load
-
-// N dwords from a buffer resource at a byte offset (zero past its end).
-template <int N>
-struct Words {
-  uint32_t w[N];
-};
-template <int N>
-__device__ __forceinline__ Words<N> buf_load(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-  Words<N> x;
-  if constexpr (N == 1) {
-    x.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kNonTemporal);
-  } else if constexpr (N == 2) {
-    const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, kNonTemporal);
-    x.w[0] = y[0], x.w[1] = y[1];
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, kNonTemporal);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x.w[i + j] = y[j];
-    }
-  }
-  return x;
-}
 
 // Loads of one step in flight, and how they are consumed.
 template <typename T, int DP>
@@ -622,6 +538,22 @@ static void launch_paged_d(const PagedParams& p, hipStream_t stream) {
     case 128: launch_paged_t<T, 128>(p, stream); break;
     default: launch_paged_t<T, 256>(p, stream); break;
   }
+}
+
+template <typename T>
+static void launch_join_d(const PagedParams& p, int dp, hipStream_t stream) {
+  const dim3 grid(p.nblk), block(256);
+  switch (dp) {
+    case 64: hipLaunchKernelGGL((paged_join_kernel<T, 64>), grid, block, 0, stream, p); break;
+    case 128: hipLaunchKernelGGL((paged_join_kernel<T, 128>), grid, block, 0, stream, p); break;
+    default: hipLaunchKernelGGL((paged_join_kernel<T, 256>), grid, block, 0, stream, p); break;
+  }
+}
+
+void launch_paged_join(const PagedParams& p, int io_dtype, int dp, hipStream_t stream) {
+  if (io_dtype == kF32) launch_join_d<float>(p, dp, stream);
+  else if (io_dtype == kF16) launch_join_d<f16>(p, dp, stream);
+  else launch_join_d<bf16>(p, dp, stream);
 }
 
 void launch_paged(const PagedParams& p, int io_dtype, hipStream_t stream) {

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "nxa_paged.h"
+#include "nxa_quant.h"
 
 namespace nxa {
 
@@ -65,11 +66,14 @@ struct CompactParams {
 };
 
 void launch_pages_write(const WriteParams& p, hipStream_t stream);
-void launch_pages_copy(const PoolParams& p, int es, const CopyPairs& pairs, hipStream_t stream);
+// (Pool: PoolParams, es its elements' bytes, or QuantPool, es its scales')
+template <typename Pool>
+void launch_pages_copy(const Pool& p, int es, const CopyPairs& pairs, hipStream_t stream);
 void launch_pages_free(const RowsParams& p, hipStream_t stream);
 void launch_pages_extend(RowsParams p, hipStream_t stream);
-void launch_pages_fork(RowsParams p, const PoolParams& pool, int es, hipStream_t stream);
-void launch_pages_compact(const CompactParams& p, const PoolParams& pool, int es,
-                          hipStream_t stream);
+template <typename Pool>
+void launch_pages_fork(RowsParams p, const Pool& pool, int es, hipStream_t stream);
+template <typename Pool>
+void launch_pages_compact(const CompactParams& p, const Pool& pool, int es, hipStream_t stream);
 
 }  // namespace nxa

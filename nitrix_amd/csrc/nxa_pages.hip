@@ -52,6 +52,34 @@ __device__ __forceinline__ void copy_head(const PoolParams& p, int es, int from,
             p.v_str[2] * es, tid, threads);
 }
 
+// `bytes` (a multiple of 4, as the addresses are) from src to dst.
+__device__ __forceinline__ void copy_span(char* dst, const char* src, int64_t bytes, int tid,
+                                          int threads) {
+  int64_t done = 0;
+  if ((((uintptr_t)dst | (uintptr_t)src) & 15) == 0) {
+    done = bytes & ~(int64_t)15;
+#pragma unroll 4
+    for (int64_t i = 16 * (int64_t)tid; i < done; i += 16 * threads)
+      *reinterpret_cast<u32x4*>(dst + i) = *reinterpret_cast<const u32x4*>(src + i);
+  }
+  for (int64_t i = done + 4 * tid; i < bytes; i += 4 * threads)
+    *reinterpret_cast<uint32_t*>(dst + i) = *reinterpret_cast<const uint32_t*>(src + i);
+}
+
+// The same of a quantised pool, whose slots lie end to end; es: a scale's bytes.
+__device__ __forceinline__ void copy_head(const QuantPool& p, int es, int from, int to, int head,
+                                          int rows, int tid, int threads) {
+  char* k = (char*)p.k + head * p.k_str[1];
+  char* v = (char*)p.v + head * p.v_str[1];
+  char* s = (char*)p.sc + head * p.sc_str[1] * es;
+  copy_span(k + to * p.k_str[0], k + from * p.k_str[0], (int64_t)rows * (p.D * p.bits / 8), tid,
+            threads);
+  copy_span(v + to * p.v_str[0], v + from * p.v_str[0], (int64_t)rows * (p.Dv * p.bits / 8), tid,
+            threads);
+  copy_span(s + to * p.sc_str[0] * es, s + from * p.sc_str[0] * es, (int64_t)rows * 4 * es, tid,
+            threads);
+}
+
 __device__ __forceinline__ bool is_page(int e, int P) { return (unsigned)e < (unsigned)P; }
 
 // Inclusive sum over a block of 1024 threads; `total` the block's.
@@ -175,7 +203,8 @@ __global__ __launch_bounds__(256) void pages_write_kernel(const WriteParams p) {
 // ---------------------------------------------------------------------------
 // Page copies named by the host, a block a (pair, head).
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void pages_copy_kernel(const PoolParams p, int es,
+template <typename Pool>
+__global__ __launch_bounds__(256) void pages_copy_kernel(const Pool p, int es,
                                                          const CopyPairs pairs) {
   const int i = blockIdx.x / p.Hk, h = blockIdx.x % p.Hk;
   copy_head(p, es, pairs.src[i], pairs.dst[i], h, p.PS, threadIdx.x, 256);
@@ -401,7 +430,8 @@ __global__ __launch_bounds__(1024) void pages_fork_plan_kernel(const RowsParams 
 
 // Then blocks (i, 0) write the rows and counts, and blocks (i, 1 + h) copy
 // head h of the partly filled last page.
-__global__ __launch_bounds__(256) void pages_fork_kernel(const RowsParams p, const PoolParams pool,
+template <typename Pool>
+__global__ __launch_bounds__(256) void pages_fork_kernel(const RowsParams p, const Pool pool,
                                                          int es) {
   const int i = blockIdx.x, tid = threadIdx.x;
   const int fresh = p.work[i];
@@ -517,8 +547,9 @@ __global__ __launch_bounds__(1024) void pages_plan_kernel(const CompactParams p)
   }
 }
 
-__global__ __launch_bounds__(256) void pages_move_kernel(const CompactParams p,
-                                                         const PoolParams pool, int es) {
+template <typename Pool>
+__global__ __launch_bounds__(256) void pages_move_kernel(const CompactParams p, const Pool pool,
+                                                         int es) {
   const int tid = threadIdx.x;
   const int n = p.info[0], moves = p.info[1];
   auto where = [&](int e) { return e >= n && p.refs[e] > 0 ? p.holes[p.mover_rank[e]] : e; };
@@ -549,8 +580,9 @@ void launch_pages_write(const WriteParams& p, hipStream_t stream) {
   hipLaunchKernelGGL(pages_write_kernel, dim3((unsigned)((p.T + 3) / 4)), dim3(256), 0, stream, p);
 }
 
-void launch_pages_copy(const PoolParams& p, int es, const CopyPairs& pairs, hipStream_t stream) {
-  hipLaunchKernelGGL(pages_copy_kernel, dim3(pairs.n * p.Hk), dim3(256), 0, stream, p, es, pairs);
+template <typename Pool>
+void launch_pages_copy(const Pool& p, int es, const CopyPairs& pairs, hipStream_t stream) {
+  hipLaunchKernelGGL(pages_copy_kernel<Pool>, dim3(pairs.n * p.Hk), dim3(256), 0, stream, p, es, pairs);
 }
 
 // Whether the one-block kernel of the call copies the state itself; else a
@@ -579,20 +611,29 @@ void launch_pages_extend(RowsParams p, hipStream_t stream) {
   hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, stream, p);
 }
 
-void launch_pages_fork(RowsParams p, const PoolParams& pool, int es, hipStream_t stream) {
+template <typename Pool>
+void launch_pages_fork(RowsParams p, const Pool& pool, int es, hipStream_t stream) {
   p.start = launch_start(p, p.n > 0, stream);
   if (p.n == 0) return;
   hipLaunchKernelGGL(pages_fork_plan_kernel, dim3(1), dim3(1024), 0, stream, p);
-  hipLaunchKernelGGL(pages_fork_kernel, dim3(p.n, 1 + pool.Hk), dim3(256), 0, stream, p, pool, es);
+  hipLaunchKernelGGL(pages_fork_kernel<Pool>, dim3(p.n, 1 + pool.Hk), dim3(256), 0, stream, p, pool,
+                     es);
 }
 
-void launch_pages_compact(const CompactParams& p, const PoolParams& pool, int es,
-                          hipStream_t stream) {
+template <typename Pool>
+void launch_pages_compact(const CompactParams& p, const Pool& pool, int es, hipStream_t stream) {
   const int nb = (p.P + kCompactPages - 1) / kCompactPages;
   if (nb > kCompactFew)
     hipLaunchKernelGGL(pages_count_kernel, dim3(nb), dim3(1024), 0, stream, p);
   hipLaunchKernelGGL(pages_plan_kernel, dim3(nb), dim3(1024), 0, stream, p);
-  hipLaunchKernelGGL(pages_move_kernel, dim3(2048), dim3(256), 0, stream, p, pool, es);
+  hipLaunchKernelGGL(pages_move_kernel<Pool>, dim3(2048), dim3(256), 0, stream, p, pool, es);
 }
+
+template void launch_pages_copy(const PoolParams&, int, const CopyPairs&, hipStream_t);
+template void launch_pages_copy(const QuantPool&, int, const CopyPairs&, hipStream_t);
+template void launch_pages_fork(RowsParams, const PoolParams&, int, hipStream_t);
+template void launch_pages_fork(RowsParams, const QuantPool&, int, hipStream_t);
+template void launch_pages_compact(const CompactParams&, const PoolParams&, int, hipStream_t);
+template void launch_pages_compact(const CompactParams&, const QuantPool&, int, hipStream_t);
 
 }  // namespace nxa

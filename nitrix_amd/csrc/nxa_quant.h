@@ -1,0 +1,51 @@
+// Quantised paged key-value cache: parameter blocks and launchers of
+// nxa_qpages.hip (writing and reading back) and nxa_qpaged.hip (one new token a
+// sequence attends its pages).
+//
+// A row (token and head) of D elements is held as codes of 4 or 8 bits with a
+// scale s and a minimum z of the model's type T: s = T((max - min) * float(1 /
+// (2^bits - 1))), code = rint((x - z) / s), value = z + s code.  Pools: k codes [P, Hk, PS,
+// D bits / 8 bytes], v codes likewise, scales [P, Hk, PS, 4] of T (k's s and z,
+// v's s and z); the slots of a page and head lie end to end, so that a step of an
+// attention is one run of each.  In 4 bits element 2 i is the low half of byte i.
+#pragma once
+
+#include "nxa_paged.h"
+
+namespace nxa {
+
+// A pool of codes: k and v of PoolParams with strides in bytes, and the scales
+// with strides in elements.
+struct QuantPool : PoolParams {
+  void* sc;
+  int64_t sc_str[2];  // page, head
+  int bits;
+};
+
+// Written (ks / vs to the pool) or read back (the pool to ks / vs).
+struct QuantMoveParams {
+  QuantPool pool;
+  void *ks, *vs;                 // [Hk, T, D], [Hk, T, Dv]
+  int64_t ks_str[2], vs_str[2];  // head, token
+  const int* offsets;            // [B + 1], or null: token s is sequence s's
+  const int* starts;             // [B]
+  const int* table;
+  int64_t table_rs;
+  int64_t T;
+  int B, M;
+};
+
+struct QuantPagedParams : PagedParams {  // k_str, v_str in bytes
+  const void* sc;
+  int64_t sc_str[2];
+  int bits;
+};
+
+int qpaged_dp(int m);  // padded head dim
+bool qpaged_whole(int64_t room);
+
+void launch_quant_write(const QuantMoveParams& p, int io_dtype, hipStream_t stream);
+void launch_quant_read(const QuantMoveParams& p, int io_dtype, hipStream_t stream);
+void launch_quant_paged(const QuantPagedParams& p, int io_dtype, hipStream_t stream);
+
+}  // namespace nxa

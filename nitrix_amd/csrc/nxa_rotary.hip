@@ -1,0 +1,146 @@
+// Rotary positions: pairs of a row's elements turned by an angle that grows
+// with the row's position,
+//   a' = c (a cos pw - b sin pw),   b' = c (b cos pw + a sin pw),
+// pair i of the half layout being elements i and i + R / 2, of the interleaved
+// one 2 i and 2 i + 1; elements from R on are copied.  The backward pass is the
+// same with the sines' sign turned.
+//
+// Bound by HBM: 6 operations on 4 bytes read and 4 written (16 bits).  What
+// could cost more is the sine and cosine of each pair, which all heads of a
+// token share: a block takes a few tokens with all their heads, forms each pair's
+// once and keeps them in LDS.  Angles are turns in 64 bits, p (w / 2 pi), of which
+// the fraction goes on in 32 bits: a position of 10^9 costs no accuracy.
+#include "nxa_rotary.h"
+
+namespace nxa {
+
+namespace {
+
+__device__ __forceinline__ int64_t rotary_position(const RotaryParams& p, int b, int t) {
+  const int64_t at = b * p.pos_str[0] + t * p.pos_str[1];
+  return p.pos64 ? ((const int64_t*)p.positions)[at] : ((const int*)p.positions)[at];
+}
+
+// c cos and c sin of pair i at a position.
+__device__ __forceinline__ float2 rotary_turn(const RotaryParams& p, int64_t pos, int i) {
+  constexpr double kInvTwoPi = 0.15915494309189533577;
+  const double turns = (double)pos * (p.freq[i] * kInvTwoPi);
+  const float f = (float)(2.0 * (turns - __builtin_rint(turns)));
+  float s, c;
+  sincospif(f, &s, &c);
+  return float2{c * p.scale, (p.inverse ? -s : s) * p.scale};
+}
+
+template <typename T>
+struct alignas(16) Chunk {
+  static constexpr int N = 16 / sizeof(T);
+  T x[N];
+};
+
+}  // namespace
+
+// Rows as 16-byte chunks: an item is a pair of chunks that turn together (half
+// layout), one chunk of pairs (interleaved) or one that is copied.  TB tokens a
+// block.
+template <typename T, bool IL, int TB>
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
+  constexpr int N = Chunk<T>::N;
+  __shared__ float2 cs[TB * kRotaryMaxDim / 2];
+  const int tid = threadIdx.x, half = p.R / 2;
+  const int blocks = (p.T + TB - 1) / TB;
+  const int b = blockIdx.x / blocks, t0 = (blockIdx.x % blocks) * TB;
+  const int nt = min(TB, p.T - t0);
+  for (int i = tid; i < nt * half; i += 256) {
+    const int t = i / half, j = i - t * half;
+    cs[t * (kRotaryMaxDim / 2) + j] = rotary_turn(p, rotary_position(p, b, t0 + t), j);
+  }
+  __syncthreads();
+  const int turned = IL ? p.R / N : half / N;
+  const int per = turned + (p.D - p.R) / N, heads = p.H[0] + p.H[1];
+  const int total = nt * heads * per;
+  for (int i = tid; i < total; i += 256) {
+    const int row = i / per, c = i - row * per;
+    const int t = row / heads, hh = row - t * heads;
+    const int w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
+    const T* x = (const T*)p.x[w] + b * p.x_str[w][0] + h * p.x_str[w][1] + (t0 + t) * p.x_str[w][2];
+    T* y = (T*)p.y[w] + b * p.y_str[w][0] + h * p.y_str[w][1] + (t0 + t) * p.y_str[w][2];
+    const float2* at = cs + t * (kRotaryMaxDim / 2);
+    if (c >= turned) {
+      const int d = p.R + (c - turned) * N;
+      *reinterpret_cast<u32x4*>(y + d) = *reinterpret_cast<const u32x4*>(x + d);
+    } else if (IL) {
+      Chunk<T> a = *reinterpret_cast<const Chunk<T>*>(x + c * N);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        const float2 k = at[c * (N / 2) + e];
+        const float u = (float)a.x[2 * e], v = (float)a.x[2 * e + 1];
+        a.x[2 * e] = (T)(u * k.x - v * k.y);
+        a.x[2 * e + 1] = (T)(v * k.x + u * k.y);
+      }
+      *reinterpret_cast<Chunk<T>*>(y + c * N) = a;
+    } else {
+      Chunk<T> a = *reinterpret_cast<const Chunk<T>*>(x + c * N);
+      Chunk<T> o = *reinterpret_cast<const Chunk<T>*>(x + half + c * N);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float2 k = at[c * N + e];
+        const float u = (float)a.x[e], v = (float)o.x[e];
+        a.x[e] = (T)(u * k.x - v * k.y);
+        o.x[e] = (T)(v * k.x + u * k.y);
+      }
+      *reinterpret_cast<Chunk<T>*>(y + c * N) = a;
+      *reinterpret_cast<Chunk<T>*>(y + half + c * N) = o;
+    }
+  }
+}
+
+// Any head dim, rotated part, strides and alignment: a pair or an element an
+// item.
+template <typename T, int TB>
+__global__ __launch_bounds__(256) void rotary_any_kernel(const RotaryParams p) {
+  __shared__ float2 cs[TB * kRotaryMaxDim / 2];
+  const int tid = threadIdx.x, half = p.R / 2;
+  const int blocks = (p.T + TB - 1) / TB;
+  const int b = blockIdx.x / blocks, t0 = (blockIdx.x % blocks) * TB;
+  const int nt = min(TB, p.T - t0);
+  for (int i = tid; i < nt * half; i += 256) {
+    const int t = i / half, j = i - t * half;
+    cs[t * (kRotaryMaxDim / 2) + j] = rotary_turn(p, rotary_position(p, b, t0 + t), j);
+  }
+  __syncthreads();
+  const int per = half + p.D - p.R, heads = p.H[0] + p.H[1];
+  const int total = nt * heads * per;
+  for (int i = tid; i < total; i += 256) {
+    const int row = i / per, c = i - row * per;
+    const int t = row / heads, hh = row - t * heads;
+    const int w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
+    const T* x = (const T*)p.x[w] + b * p.x_str[w][0] + h * p.x_str[w][1] + (t0 + t) * p.x_str[w][2];
+    T* y = (T*)p.y[w] + b * p.y_str[w][0] + h * p.y_str[w][1] + (t0 + t) * p.y_str[w][2];
+    if (c >= half) {
+      y[half + c] = x[half + c];
+      continue;
+    }
+    const int d0 = p.interleaved ? 2 * c : c, d1 = p.interleaved ? 2 * c + 1 : c + half;
+    const float2 k = cs[t * (kRotaryMaxDim / 2) + c];
+    const float u = (float)x[d0], v = (float)x[d1];
+    y[d0] = (T)(u * k.x - v * k.y);
+    y[d1] = (T)(v * k.x + u * k.y);
+  }
+}
+
+template <typename T>
+static void launch_rotary_t(const RotaryParams& p, bool chunks, hipStream_t stream) {
+  constexpr int TB = 4;
+  const dim3 grid((unsigned)((int64_t)p.B * ((p.T + TB - 1) / TB))), block(256);
+  if (!chunks) hipLaunchKernelGGL((rotary_any_kernel<T, TB>), grid, block, 0, stream, p);
+  else if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, true, TB>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((rotary_kernel<T, false, TB>), grid, block, 0, stream, p);
+}
+
+void launch_rotary(const RotaryParams& p, int io_dtype, bool chunks, hipStream_t stream) {
+  if (io_dtype == kF32) launch_rotary_t<float>(p, chunks, stream);
+  else if (io_dtype == kF16) launch_rotary_t<f16>(p, chunks, stream);
+  else launch_rotary_t<bf16>(p, chunks, stream);
+}
+
+}  // namespace nxa

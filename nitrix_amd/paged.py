@@ -40,6 +40,8 @@ import torch
 
 from . import _lib
 from ._backend import NitrixBackendError, fallback, resolve_backend
+from ._quant_pool import _check_fused as _check_fused_quantized
+from ._quant_pool import _check_quantized, _quant_desc
 from .attention import (
     _IO_DTYPES,
     _MAX_HEAD_DIM,
@@ -161,6 +163,39 @@ def _pool_desc(k_pages, v_pages) -> _lib.NxaPoolDesc:
     desc.k_str[:] = k_pages.stride()[:3]
     desc.v_str[:] = v_pages.stride()[:3]
     return desc
+
+
+class _Moved:
+    """A pool whose pages an operator moves: ``k_pages`` and ``v_pages``, of
+    codes with their ``scales`` where these are given."""
+
+    def __init__(self, name, k_pages, v_pages, scales):
+        if scales is None:
+            _check_pool(name, k_pages, v_pages, written=True)
+            self.tensors = (k_pages, v_pages)
+        else:
+            _check_quantized(name, k_pages, v_pages, scales, written=True)
+            self.tensors = (k_pages, v_pages, scales)
+        _check_written(name, *self.tensors)
+        self.k_pages, self.scales = k_pages, scales
+        self.dtype = k_pages.dtype if scales is None else scales.dtype
+
+    def call(self, what, *args):
+        """``nxa_pages_<what>`` or ``nxa_quant_<what>`` on the pool."""
+        if self.scales is None:
+            _check_fused(*self.tensors)
+            desc, kind = _pool_desc(*self.tensors), 'pages'
+        else:
+            # (bytes are moved, whatever they stand for)
+            bits = 4 if any(x.shape[3] % 8 for x in self.tensors[:2]) else 8
+            _check_fused_quantized(*self.tensors, bits)
+            desc, kind = _quant_desc(*self.tensors, bits), 'quant'
+        _lib.check(
+            getattr(_lib.lib(), f'nxa_{kind}_{what}')(
+                ctypes.byref(desc), *(x.data_ptr() for x in self.tensors), *args
+            )
+        )
+        _touched(*self.tensors)
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor:
@@ -460,9 +495,9 @@ def _reference_extend(page_table, lengths, refs, counts, page_size):
     return table, torch.minimum(grown, first * page_size).to(torch.int32), refs
 
 
-def _reference_fork(k_pages, v_pages, page_table, lengths, refs, src, dst):
+def _reference_fork(pool, page_table, lengths, refs, src, dst):
     b, m = page_table.shape
-    p, ps = refs.numel(), k_pages.shape[2]
+    p, ps = refs.numel(), pool[0].shape[2]
     table, out_len = page_table.clone(), lengths.clone()
     idx = torch.arange(src.numel(), device=src.device)
     ok = (src >= 0) & (src < b) & (dst >= 0) & (dst < b) & (src != dst)
@@ -483,21 +518,21 @@ def _reference_fork(k_pages, v_pages, page_table, lengths, refs, src, dst):
     slot = torch.arange(ps, device=src.device)[None] < rest[:, None]
     f, s = torch.nonzero(got[:, None] & slot, as_tuple=True)
     with torch.no_grad():
-        for pages in (k_pages, v_pages):
+        for pages in pool:
             pages[fresh[f].long(), :, s] = pages[last_page[f].long(), :, s]
     table[dst] = rows
     out_len[dst] = torch.where((rest > 0) & ~got, full * ps, length).to(torch.int32)
     return table, out_len, out_refs
 
 
-def _reference_compact(k_pages, v_pages, page_table, refs):
+def _reference_compact(pool, page_table, refs):
     live = refs > 0
     at = torch.arange(refs.numel(), device=refs.device)
     n = live.sum()
     movers = torch.nonzero(live & (at >= n)).reshape(-1)
     holes = torch.nonzero(~live & (at < n)).reshape(-1)
     with torch.no_grad():
-        for pages in (k_pages, v_pages):
+        for pages in pool:
             pages[holes] = pages[movers]
     where = at.clone()
     where[movers] = holes
@@ -608,6 +643,7 @@ def fork_sequences(
     src: torch.Tensor,
     dst: torch.Tensor,
     *,
+    scales: Optional[torch.Tensor] = None,
     backend: str = 'auto',
 ):
     """Makes row ``dst[i]`` a copy of row ``src[i]`` (int32 ``(n,)`` each), for
@@ -620,37 +656,33 @@ def fork_sequences(
     pages.  The target's former pages no longer count for it, but are not
     handed out by the same call.  Sources are taken as they were before the
     call.  Of several pairs with one target the last counts; ``src[i] ==
-    dst[i]`` and numbers outside the table are ignored.  Returns the new ``(page_table, lengths, refs)``."""
-    _check_pool('fork_sequences', k_pages, v_pages, written=True)
+    dst[i]`` and numbers outside the table are ignored.  Pages of
+    :mod:`nitrix_amd.quantized` come with their ``scales``.  Returns the new
+    ``(page_table, lengths, refs)``."""
+    pool = _Moved('fork_sequences', k_pages, v_pages, scales)
     dev = page_table.device
     _check_table('fork_sequences', k_pages.device, page_table,
                  lengths=(lengths, page_table.shape[:1]), refs=(refs, k_pages.shape[:1]),
                  src=(src, (None,)), dst=(dst, src.shape[:1]))
-    _check_written('fork_sequences', k_pages, v_pages)
     if page_table.shape[1] * k_pages.shape[2] >= 1 << 31:
         raise ValueError('fork_sequences: a row has room for 2^31 tokens or more.')
 
     def fused():
-        _check_fused(k_pages, v_pages)
-        lib = _lib.lib()
-        desc = _pool_desc(k_pages, v_pages)
         t, n, c, s, d = (x.contiguous() for x in (page_table, lengths, refs, src, dst))
         out = _outputs(t, n, c)
-        ws = _workspace(lib.nxa_pages_fork_workspace_bytes(t.shape[0], c.numel(), s.numel()), dev)
-        _lib.check(
-            lib.nxa_pages_fork(
-                ctypes.byref(desc), k_pages.data_ptr(), v_pages.data_ptr(), t.shape[0],
-                t.shape[1], t.data_ptr(), n.data_ptr(), c.data_ptr(), s.data_ptr(), d.data_ptr(),
-                s.numel(), *(x.data_ptr() for x in out), ws.data_ptr(), ws.numel(), _stream(dev),
-            )
+        need = _lib.lib().nxa_pages_fork_workspace_bytes(t.shape[0], c.numel(), s.numel())
+        ws = _workspace(need, dev)
+        pool.call(
+            'fork', t.shape[0], t.shape[1], t.data_ptr(), n.data_ptr(), c.data_ptr(),
+            s.data_ptr(), d.data_ptr(), s.numel(), *(x.data_ptr() for x in out), ws.data_ptr(),
+            ws.numel(), _stream(dev),
         )
-        _touched(k_pages, v_pages)
         return out
 
     return _dispatch(
         'fork_sequences', backend, dev, fused,
-        lambda: _reference_fork(k_pages, v_pages, page_table, lengths, refs, src, dst),
-        (tuple(k_pages.shape), tuple(page_table.shape)), k_pages.dtype,
+        lambda: _reference_fork(pool.tensors, page_table, lengths, refs, src, dst),
+        (tuple(k_pages.shape), tuple(page_table.shape)), pool.dtype,
     )
 
 
@@ -660,40 +692,34 @@ def compact_pages(
     page_table: torch.Tensor,
     refs: torch.Tensor,
     *,
+    scales: Optional[torch.Tensor] = None,
     backend: str = 'auto',
 ):
     """Moves the ``n`` pages in use (``refs > 0``) to the pool's first ``n``.
 
     The k-th page in use from ``n`` on is copied, in place, to the k-th free
     page below ``n``; the other pages stay where they are, and what the movers
-    leave behind is free but unchanged.  Returns the new ``(page_table, refs)``;
+    leave behind is free but unchanged.  Pages of :mod:`nitrix_amd.quantized` come
+    with their ``scales``.  Returns the new ``(page_table, refs)``;
     entries that name no page, or a free one, stay as they are."""
-    _check_pool('compact_pages', k_pages, v_pages, written=True)
+    pool = _Moved('compact_pages', k_pages, v_pages, scales)
     dev = page_table.device
     _check_table('compact_pages', k_pages.device, page_table, refs=(refs, k_pages.shape[:1]))
-    _check_written('compact_pages', k_pages, v_pages)
 
     def fused():
-        _check_fused(k_pages, v_pages)
-        lib = _lib.lib()
-        desc = _pool_desc(k_pages, v_pages)
         t, c = page_table.contiguous(), refs.contiguous()
         out = torch.empty_like(t), torch.empty_like(c)
-        ws = _workspace(lib.nxa_pages_compact_workspace_bytes(c.numel()), dev)
-        _lib.check(
-            lib.nxa_pages_compact(
-                ctypes.byref(desc), k_pages.data_ptr(), v_pages.data_ptr(), t.numel(),
-                t.data_ptr(), c.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), ws.data_ptr(),
-                ws.numel(), _stream(dev),
-            )
+        ws = _workspace(_lib.lib().nxa_pages_compact_workspace_bytes(c.numel()), dev)
+        pool.call(
+            'compact', t.numel(), t.data_ptr(), c.data_ptr(), out[0].data_ptr(),
+            out[1].data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev),
         )
-        _touched(k_pages, v_pages)
         return out
 
     return _dispatch(
         'compact_pages', backend, dev, fused,
-        lambda: _reference_compact(k_pages, v_pages, page_table, refs),
-        (tuple(k_pages.shape), tuple(page_table.shape)), k_pages.dtype,
+        lambda: _reference_compact(pool.tensors, page_table, refs),
+        (tuple(k_pages.shape), tuple(page_table.shape)), pool.dtype,
     )
 
 
@@ -718,6 +744,7 @@ def copy_pages(
     src: Union[Sequence[int], torch.Tensor],
     dst: Union[Sequence[int], torch.Tensor],
     *,
+    scales: Optional[torch.Tensor] = None,
     backend: str = 'auto',
 ) -> None:
     """Copies page ``src[i]`` to page ``dst[i]``, in place, for lists on the
@@ -725,9 +752,9 @@ def copy_pages(
 
     No page may be a target twice, or both a target and a source
     (``ValueError``): every order of the copies then gives the same.  A
-    captured graph replays the pages named at capture."""
-    _check_pool('copy_pages', k_pages, v_pages, written=True)
-    _check_written('copy_pages', k_pages, v_pages)
+    captured graph replays the pages named at capture.  Pages of
+    :mod:`nitrix_amd.quantized` come with their ``scales``."""
+    pool = _Moved('copy_pages', k_pages, v_pages, scales)
     s = _page_list('src', src, k_pages.shape[0])
     d = _page_list('dst', dst, k_pages.shape[0])
     if len(s) != len(d):
@@ -742,19 +769,11 @@ def copy_pages(
     dev = k_pages.device
 
     def fused():
-        _check_fused(k_pages, v_pages)
-        desc = _pool_desc(k_pages, v_pages)
-        _lib.check(
-            _lib.lib().nxa_pages_copy(
-                ctypes.byref(desc), k_pages.data_ptr(), v_pages.data_ptr(), s.buffer_info()[0],
-                d.buffer_info()[0], len(s), _stream(dev),
-            )
-        )
-        _touched(k_pages, v_pages)
+        pool.call('copy', s.buffer_info()[0], d.buffer_info()[0], len(s), _stream(dev))
 
     def reference():
         with torch.no_grad():
-            for pages in (k_pages, v_pages):
+            for pages in pool.tensors:
                 pages[torch.tensor(d, device=dev)] = pages[torch.tensor(s, device=dev)]
 
-    _dispatch('copy_pages', backend, dev, fused, reference, (tuple(k_pages.shape),), k_pages.dtype)
+    _dispatch('copy_pages', backend, dev, fused, reference, (tuple(k_pages.shape),), pool.dtype)

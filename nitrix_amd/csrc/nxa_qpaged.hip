@@ -4,26 +4,34 @@
 // minimum a row.
 //
 // The pages are never expanded.  Codes enter the matrix products as what they
-// are, small whole numbers, exact in bf16; the scale of a key multiplies its
-// score behind the first product, that of a value its P before the second, and the
-// minima add one number a head to the output.  So nothing of a key or value is
-// rounded, and q enters as one, two or three bf16 terms (bf16, fp16, fp32: exact).
-// P s' is the sum of two terms (fp32: three), of whose rounding 2^-17 (2^-25) is
-// left.
+// are, small whole numbers; the scale of a key multiplies its score behind the
+// first product, that of a value its P before the second, and the minima add one
+// number a head to the output.  So nothing of a key or value is rounded.  What
+// bounds the kernel is what it costs to make operands of codes (1.25 operations a
+// code of four bits in a plain form, with the HBM idle two thirds of the time), so
+// they are taken as numbers whose bits they already are:
 //
-// A code of 4 bits becomes a bf16 number by or-ing it into the mantissa of 16 (16
-// + c is exact, and nothing is converted): two operations a pair of codes.  The 16
-// is taken off again where the minima are added: -16 sum q starts the accumulator
-// of the first product, and the second's share joins the minima's.  Codes of 8
-// bits are converted through fp32.
+//  * K, 16-bit types: the byte 0000cccc is the fp8 (e4m3) number c 2^-9, whether
+//    below 8 (subnormal) or not, so codes of four bits are two masks and a shift a
+//    dword and those of eight two such halves, the upper one scaled by 16 in the
+//    product.  q is the sum of two (fp16: three) fp8 numbers, scaled so that its
+//    largest element is in 2^7 .. 2^8: exact down to 2^-10 (2^-7) of that, off by at
+//    most 2^-17 of it below.  fp32: codes in the mantissa of 16 as bf16 (16 + c), q
+//    as three bf16 numbers (exact).
+//  * V: codes in the mantissa of an fp16 64 (in bits 4 .. 7, where an element's odd
+//    codes are already) or 1024 (bits 0 .. 3, or 0 .. 7).  What is added to them is
+//    taken off at the end, by a product of ones with the very P s' that the other
+//    products saw.  P s' is one fp16 number (bf16: off by 2^-12), two (fp16: 2^-23)
+//    or three (fp32).  fp16's range is short, so the reference that P is relative to
+//    follows the largest scale as well as the largest score.
 //
 // The blocks share the work as in nxa_paged.hip (units of 128 tokens, pieces of
 // a row joined by its second kernel).  A step of a wave is 32 tokens, two halves
-// of 16: S^T = K Q^T by 16x16x32 products a half, whose accumulator holds P^T as the
-// second product reads it, O^T += V^T P^T over all 32.  Per half a lane loads a
-// quarter of one key's codes (the head dim of a product is summed in any order,
-// so q is read in the order of the codes), DP / 16 columns of four keys' values,
-// and the scales of those four keys.
+// of 16: S^T = K Q^T a half, whose accumulator holds P^T as the second product reads
+// it, O^T += V^T P^T over all 32.  Per half a lane takes a quarter of one key's
+// codes (the head dim of a product is summed in any order, so q is read in the
+// order of the codes), DP / 16 columns of four keys' values, and the scales of those
+// four keys.
 #include "nxa_quant.h"
 
 #include "nxa_paged_units.h"
@@ -36,40 +44,90 @@ namespace {
 
 constexpr int kHalfKeys = 16;
 
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
 template <typename T, int DP, int BITS>
 struct QuantStep {
   static constexpr int ES = sizeof(T);
-  static constexpr int NKW = DP * BITS / 128;      // dwords of K's codes a lane and half
-  static constexpr int NJ = DP / 32;               // products of a half's S
-  static constexpr int DPL = DP / 16;              // V columns of a lane
-  static constexpr int VB = DPL * BITS / 8;        // bytes of them a key
+  static constexpr bool FP8 = ES == 2, F16 = std::is_same<T, f16>::value;
+  static constexpr int NKW = DP * BITS / 128;       // dwords of K's codes a lane and half
+  static constexpr int NJ = FP8 ? (DP + 127) / 128 : DP / 32;  // products of a half's S
+  static constexpr int DPL = DP / 16;               // V columns of a lane
+  static constexpr int VB = DPL * BITS / 8;         // bytes of them a key
   static constexpr int NVW = VB >= 4 ? VB / 4 : 1;  // dwords
-  static constexpr int NS = ES;                    // dwords of a token's scales: 4 ES / 4
-  static constexpr int QT = ES == 4 ? 3 : std::is_same<T, f16>::value ? 2 : 1;  // terms of q
-  static constexpr int PT = ES == 4 ? 3 : 2;                                     // of P s'
+  static constexpr int NS = ES;                     // dwords of a token's scales: 4 ES / 4
+  static constexpr int QT = FP8 && !F16 ? 2 : 3;    // terms of q
+  static constexpr int PT = !FP8 ? 3 : F16 ? 2 : 1;  // of P s'
+  // What stands in for 0 in V's even and odd columns.
+  static constexpr float EVEN = BITS == 8 || (FP8 && !F16) ? 1024.f : 64.f;
+  static constexpr float ODD = BITS == 8 ? 1024.f : 64.f;
+  // A half in LDS: K's codes, V's, the scales; copies of 1 KB (scales: 256 bytes).
+  static constexpr int KC = DP * BITS <= 512 ? 1 : DP * BITS / 512;
+  static constexpr int HALF_BYTES = 2 * 1024 * KC + 256;
+  static constexpr int COPIES = 2 * KC + 1;
 };
 
+// N dwords of a lane.
+template <int N>
+struct Loaded {
+  uint32_t w[N];
+  __device__ __forceinline__ uint32_t at(int i) const { return w[i]; }
+  // From LDS (aligned to what is read, up to 16 bytes).
+  __device__ __forceinline__ void lds(uint32_t at) {
+    constexpr int W = N < 4 ? N : 4;
+    typedef uint32_t V __attribute__((ext_vector_type(W)));
+    typedef __attribute__((address_space(3))) const V lds_v;
+#pragma unroll
+    for (int i = 0; i < N; i += W) {
+      const V x = *(lds_v*)(uintptr_t)(at + 4 * i);
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[i + j] = x[j];
+    }
+  }
+};
+
+// A half's codes and scales of a lane.
 template <typename T, int DP, int BITS>
 struct HalfRegs {
   using R = QuantStep<T, DP, BITS>;
-  Words<R::NKW> k;
-  Words<R::NVW> v[4];
-  Words<R::NS> s[4];
+  Loaded<R::NKW> k;
+  Loaded<R::NVW> v[4];
+  Loaded<R::NS> s[4];
 };
 
-__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+__device__ __forceinline__ f32x4 mma_bf16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4 mma_f16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// fp8 over 128 places; UP: a's numbers times 16.
+template <bool UP>
+__device__ __forceinline__ f32x4 mma_fp8(i32x8 a, i32x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, UP ? 131 : 127, 0, 127);
+}
 
-// Two numbers as bf16, the first in the low half; and what their rounding left.
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
+// Two numbers as bf16 or fp16, the first in the low half.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   const bf16x2 r = {(bf16)a, (bf16)b};
   return __builtin_bit_cast(uint32_t, r);
 }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 r = {(f16)a, (f16)b};
+  return __builtin_bit_cast(uint32_t, r);
+}
 __device__ __forceinline__ float low_of(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ float low_f16(uint32_t w) {
+  return (float)__builtin_bit_cast(f16, (uint16_t)w);
+}
+__device__ __forceinline__ float high_f16(uint32_t w) {
+  return (float)__builtin_bit_cast(f16, (uint16_t)(w >> 16));
+}
 
 // Whole bytes of a word as floats.
 template <int B>
@@ -77,54 +135,82 @@ __device__ __forceinline__ float byte_of(uint32_t w) {
   return (float)(w >> (8 * B) & 255u);
 }
 
-// 16 + the nibbles at bits SH .. SH + 3 and SH + 16 .. SH + 19, as bf16: 16 is
-// 0x4180, and a mantissa's unit is 2^-3 there.
-template <int SH>
-__device__ __forceinline__ uint32_t nibbles(uint32_t w) {
-  const uint32_t x = SH < 3 ? w << (3 - SH) : w >> (SH - 3);
-  return (x & 0x00780078u) | 0x41804180u;
-}
+// Constants of the codes' masks, kept in registers of both kinds, so that an and
+// and an or are one operation (two constants of it cannot both be literals).
+struct CodeBits {
+  uint32_t low, high, mid, k1024, k64, k16;
+  __device__ __forceinline__ CodeBits() {
+    asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
+    asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
+    asm("s_mov_b32 %0, 0x00780078" : "=s"(mid));
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(k1024));
+    asm("v_mov_b32 %0, 0x54005400" : "=v"(k64));
+    asm("v_mov_b32 %0, 0x41804180" : "=v"(k16));
+  }
+};
 
-// Product operand j of a lane's codes of one key: eight of them.
+// 16 + the nibbles at bits SH .. SH + 3 and SH + 16 .. SH + 19, as bf16 (a
+// mantissa's unit is 2^-3 there).
+template <int SH>
+__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w, const CodeBits& cb) {
+  const uint32_t x = SH < 3 ? w << (3 - SH) : w >> (SH - 3);
+  return (x & cb.mid) | cb.k16;
+}
+// Product operand j of a lane's codes of one key, bf16: eight of them.
 template <int BITS, int N>
-__device__ __forceinline__ u32x4 key_operand(const Words<N>& k, int j) {
+__device__ __forceinline__ u32x4 key_bf16(const Loaded<N>& k, int j, const CodeBits& cb) {
   if constexpr (BITS == 4) {
-    const uint32_t w = k.w[j];
-    return u32x4{nibbles<0>(w), nibbles<4>(w), nibbles<8>(w), nibbles<12>(w)};
+    const uint32_t w = k.at(j);
+    return u32x4{nibbles_bf16<0>(w, cb), nibbles_bf16<4>(w, cb), nibbles_bf16<8>(w, cb),
+                 nibbles_bf16<12>(w, cb)};
   } else {
-    const uint32_t a = k.w[2 * j], b = k.w[2 * j + 1];
-    return u32x4{pack2(byte_of<0>(a), byte_of<1>(a)), pack2(byte_of<2>(a), byte_of<3>(a)),
-                 pack2(byte_of<0>(b), byte_of<1>(b)), pack2(byte_of<2>(b), byte_of<3>(b))};
+    const uint32_t a = k.at(2 * j), b = k.at(2 * j + 1);
+    return u32x4{pack_bf16(byte_of<0>(a), byte_of<1>(a)), pack_bf16(byte_of<2>(a), byte_of<3>(a)),
+                 pack_bf16(byte_of<0>(b), byte_of<1>(b)), pack_bf16(byte_of<2>(b), byte_of<3>(b))};
   }
 }
-// The element of the lane's eight that stands at place e of the operand.
-template <int BITS>
+// Operand j, fp8: 32 codes of four bits, or the lower or upper halves of as many of
+// eight (zeros behind the lane's last).
+template <int BITS, bool UPPER, int N>
+__device__ __forceinline__ i32x8 key_fp8(const Loaded<N>& k, int j) {
+  i32x8 r;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const int i = BITS == 4 ? 4 * j + w / 2 : 8 * j + w;
+    const bool up = BITS == 4 ? w & 1 : UPPER;
+    const uint32_t x = i < N ? k.at(i) : 0u;
+    r[w] = (int)((up ? x >> 4 : x) & 0x0f0f0f0fu);
+  }
+  return r;
+}
+// The element of eight that stands at place e of an operand.
+template <int BITS, bool FP8>
 __device__ constexpr int key_order(int e) {
-  return BITS == 4 ? (e >> 1) + 4 * (e & 1) : e;
+  if (BITS == 8) return e;
+  return FP8 ? 2 * (e & 3) + (e >> 2) : (e >> 1) + 4 * (e & 1);
 }
 
 // Scales of a token: fields k's scale and minimum, v's.
 template <typename T, int N>
-__device__ __forceinline__ float scale_field(const Words<N>& s, int f) {
-  if constexpr (std::is_same<T, float>::value) {
-    return __uint_as_float(s.w[f]);
-  } else if constexpr (std::is_same<T, f16>::value) {
-    const uint16_t h = (uint16_t)(s.w[f >> 1] >> (16 * (f & 1)));
-    return (float)__builtin_bit_cast(f16, h);
-  } else {
-    return f & 1 ? high_of(s.w[f >> 1]) : low_of(s.w[f >> 1]);
-  }
+__device__ __forceinline__ float scale_field(const Loaded<N>& s, int f) {
+  if constexpr (std::is_same<T, float>::value)
+    return __uint_as_float(s.at(f));
+  else if constexpr (std::is_same<T, f16>::value)
+    return f & 1 ? high_f16(s.at(f >> 1)) : low_f16(s.at(f >> 1));
+  else
+    return f & 1 ? high_of(s.at(f >> 1)) : low_of(s.at(f >> 1));
 }
 
 }  // namespace
 
-// Steps whose loads are in flight.
+// Steps whose copies are in flight.
 template <int DP, int BITS>
-constexpr int kQuantDepth = DP * BITS <= 512 ? 3 : 2;
+constexpr int kQuantDepth = 2;
 
-// FAST: pages hold a multiple of 16 tokens, so that a half lies in one page and
-// its address is uniform, and no lane's codes straddle a row's end; else every key
-// looks its page up and codes are loaded four bytes at a time.
+// FAST: pages hold a multiple of 16 tokens, so that a half lies in one page, and
+// codes and scales are aligned: halves are copied to LDS, each wave its own, steps
+// ahead of their use.  Else every key looks its page up and codes are loaded four
+// bytes at a time.
 template <typename T, int DP, int BITS, bool FAST>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const QuantPagedParams p) {
   using R = QuantStep<T, DP, BITS>;
@@ -134,9 +220,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
   constexpr int NB = kQuantDepth<DP, BITS>;
   constexpr int NF = DPL;  // O^T fragments: fragment f is columns DPL i + f, i = 0 .. 15
   constexpr int FIELDS = NF * 4 + 2;
-  constexpr uint32_t kNowhere = 0x7ffffff0u;  // beyond every range
-  __shared__ float ms[kWaves * FIELDS * 64];
+  constexpr int STEP_BYTES = 2 * R::HALF_BYTES, COPIES = R::COPIES;
+  constexpr int RING = FAST ? kWaves * NB * STEP_BYTES : 0, JOIN = kWaves * FIELDS * 64 * 4;
+  // (the waves' rings, then what they join)
+  __shared__ __attribute__((aligned(16))) char mem[RING > JOIN ? RING : JOIN];
   __shared__ int pre[257], wsum[kWaves];
+  float* const ms = reinterpret_cast<float*>(mem);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -180,17 +269,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
     before = __builtin_amdgcn_readfirstlane(before);
   }
   const int64_t u0 = u;
+  const CodeBits cb;
 
-  // Bytes of a row, and per-lane byte offsets inside a half: K key c, chunk g; V
-  // key 4 g + j, columns DPL c ..; scales of key 4 g + j.
+  // Bytes of a row.  A half in LDS: key c, chunk g of K; columns DPL c .. of V and
+  // the scales of keys 4 g ...
   const int kb = p.D * BITS / 8, vb = p.Dv * BITS / 8;
-  uint32_t koff, voff[4];
-  if constexpr (FAST) {
-    koff = 4 * NKW * g < kb ? (uint32_t)(c * kb + 4 * NKW * g) : kNowhere;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      voff[j] = VB * c < vb ? (uint32_t)((4 * g + j) * vb + VB * c) : kNowhere;
-  }
+  const uint32_t ring = lds_offset(mem) + wave * (NB * STEP_BYTES);
+  const uint32_t k_at = ring + c * kb + 4 * NKW * g;
+  const uint32_t v_at = ring + 1024 * R::KC + 4 * g * vb + VB * c;
+  const uint32_t s_at = ring + 2048 * R::KC + 16 * R::ES * g;
+  typedef const __attribute__((address_space(4))) int constant_int;
 
   while (u < u1) {
     const int len = __builtin_amdgcn_readfirstlane(paged_len(p, b));
@@ -209,246 +297,372 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
 
     // Q^T: column c is head h0 + c; the lane's quarter of the head dim in the
     // order of K's codes, as QT terms, and the sum of the whole row.
-    u32x4 qf[NJ][QT];
-    float qsum = 0.f;
+    u32x4 qb[R::FP8 ? 1 : NJ][QT];
+    i32x8 qe[R::FP8 ? NJ : 1][QT];
+    float qsum = 0.f, sl;
     {
       const T* qp = (const T*)p.q + b * p.q_str[0] + ((int64_t)hk * p.G + h0 + min(c, heads - 1)) * p.q_str[1];
+      float x[DP / 4], most = 0.f;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
+      for (int j = 0; j < DP / 32; ++j) {
         const int d = g * (DP / 4) + 8 * j;
-        float x[8];
+        float* y = x + 8 * j;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        for (int e = 0; e < 8; ++e) y[e] = 0.f;
         if (c < heads && d < p.D) {
           const u32x4* src = reinterpret_cast<const u32x4*>(qp + d);
           if constexpr (sizeof(T) == 4) {
             const f32x4 lo = __builtin_bit_cast(f32x4, src[0]), hi = __builtin_bit_cast(f32x4, src[1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
+            for (int e = 0; e < 4; ++e) y[e] = lo[e], y[4 + e] = hi[e];
           } else {
             struct alignas(16) Row { T x[8]; };
-            const Row y = __builtin_bit_cast(Row, src[0]);
+            const Row r = __builtin_bit_cast(Row, src[0]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (float)y.x[e];
+            for (int e = 0; e < 8; ++e) y[e] = (float)r.x[e];
           }
         }
+        // (a negative scale turns q instead, so that the largest score is that of
+        // the largest product)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) qsum += x[e];
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            float& a = x[key_order<BITS>(2 * w)];
-            float& o = x[key_order<BITS>(2 * w + 1)];
-            const uint32_t r = pack2(a, o);
-            qf[j][t][w] = r;
-            a -= low_of(r), o -= high_of(r);
-          }
+        for (int e = 0; e < 8; ++e) {
+          y[e] = p.scale_log2 < 0.f ? -y[e] : y[e];
+          qsum += y[e];
+          most = fmaxf(most, __builtin_fabsf(y[e]));
+        }
       }
       qsum += xor16(qsum);
       qsum += shfl_xor32(qsum);
+      sl = __builtin_fabsf(p.scale_log2);
+      if constexpr (R::FP8) {
+        most = fmaxf(most, xor16(most));
+        most = fmaxf(most, shfl_xor32(most));
+        // q times 2^up, its largest element in 2^7 .. 2^8, and scores in units of
+        // 2^(9 - up) (codes are c 2^-9).  NaN and infinity of q leave NaN.
+        const int up = min(8 - __builtin_amdgcn_frexp_expf(most), 100);
+        const float by = most > 0.f ? __builtin_ldexpf(1.f, up) : 1.f, unit = 512.f / by;
+        qsum = qsum / unit + (most - most) + (qsum - qsum);
+        sl *= unit;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+              // Place 4 w + i: in 4 bits the even elements of eight, then the odd.
+              int r = 0;
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                const int e0 = 32 * j + 8 * (w / 2) + key_order<BITS, true>(4 * (w & 1) + i);
+                const int e1 = 32 * j + 8 * (w / 2) + key_order<BITS, true>(4 * (w & 1) + i + 1);
+                if (e0 >= DP / 4) continue;
+                float &a = x[e0], &o = x[e1];
+                if (t == 0) a *= by, o *= by;
+                if (i == 0) r = __builtin_amdgcn_cvt_pk_fp8_f32(a, o, r, false);
+                else r = __builtin_amdgcn_cvt_pk_fp8_f32(a, o, r, true);
+                a -= i == 0 ? __builtin_amdgcn_cvt_f32_fp8(r, 0) : __builtin_amdgcn_cvt_f32_fp8(r, 2);
+                o -= i == 0 ? __builtin_amdgcn_cvt_f32_fp8(r, 1) : __builtin_amdgcn_cvt_f32_fp8(r, 3);
+              }
+              qe[j][t][w] = r;
+            }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              float& a = x[8 * j + key_order<BITS, false>(2 * w)];
+              float& o = x[8 * j + key_order<BITS, false>(2 * w + 1)];
+              const uint32_t r = pack_bf16(a, o);
+              qb[j][t][w] = r;
+              a -= low_of(r), o -= high_of(r);
+            }
+      }
+      // (one of zero is so small that all scores are zero, but for the -inf of a
+      // token that takes no part)
+      sl = fmaxf(sl, 0x1p-126f);
     }
-    const float qz = qsum * p.scale_log2;
-    const float s_init = BITS == 4 ? -16.f * qsum : 0.f;
-    f32x4 o[NF];
+    const float s_init = R::FP8 || BITS == 8 ? 0.f : -16.f * qsum;
+    f32x4 o[NF], ones_o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // (zs: what the minima, and 16 in the place of 0, add to every column)
-    float m_ref = -INFINITY, l = 0.f, zs = 0.f;
+    // P is 2^(score - ref): ref is the largest score seen, raised by more than
+    // 2^kSlack only, plus 2^s_exp that no value's scale exceeds more than fourfold
+    // (s_most), less 3: P s' is then below 2^13.  zs: what the minima add to every
+    // column.
+    float m_ref = -INFINITY, ref = -INFINITY, l = 0.f, zs = 0.f;
+    float s_most = 0.f, s_exp = -90.f;
 
     const char* kp = (const char*)p.k + hk * p.k_str[1];
     const char* vp = (const char*)p.v + hk * p.v_str[1];
-    const T* sp = (const T*)p.sc + hk * p.sc_str[1];
+    const char* sp = (const char*)p.sc + hk * p.sc_str[1] * R::ES;
     // This wave's steps: 32 tokens of each unit, up to the length.
     auto key_of = [&](int half) { return (t0 + (half >> 1)) * kPagedKeys + wave * 32 + (half & 1) * kHalfKeys; };
     int steps = t1 - t0;
     while (steps > 0 && key_of(2 * steps - 2) >= len) --steps;
-
-    for (int i0 = 0; i0 < steps; i0 += 32) {
-      const int ns = min(32, steps - i0);
-      // Lane i looks up half 2 i0 + i: its page, its slot there and the tokens it
-      // has (none where the table has no page).
-      int page = 0, slot = 0, rows = 0;
-      if (FAST && lane < 2 * ns) {
-        const int key0 = key_of(2 * i0 + lane);
-        if (key0 < len) {
-          page = p.table[b * p.table_rs + key0 / p.PS];
-          slot = key0 % p.PS;
-          if ((unsigned)page < (unsigned)p.P) rows = min(kHalfKeys, len - key0);
-          else page = 0;
+    // `mine`: tokens of the half (FAST), or a bit a token.
+    constexpr int kFull = FAST ? kHalfKeys : 0xffff;
+    auto compute = [&](const Half (&r)[2], const int (&mine)[2]) NXA_INLINE {
+      f32x4 s[2];
+      float vs[8], vz[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = f32x4{s_init, s_init, s_init, s_init};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if constexpr (R::FP8) {
+            const i32x8 a = key_fp8<BITS, false>(r[h].k, j);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) s[h] = mma_fp8<false>(a, qe[j][t], s[h]);
+            if constexpr (BITS == 8) {
+              const i32x8 a = key_fp8<BITS, true>(r[h].k, j);
+#pragma unroll
+              for (int t = 0; t < QT; ++t) s[h] = mma_fp8<true>(a, qe[j][t], s[h]);
+            }
+          } else {
+            const u32x4 a = key_bf16<BITS>(r[h].k, j, cb);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) s[h] = mma_bf16(a, qb[j][t], s[h]);
+          }
+        }
+        // Rows of the accumulator: tokens 4 g + e.
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // (a scale of infinity makes its token NaN, whatever the signs)
+          const float ks = scale_field<T>(r[h].s[e], 0), kz = scale_field<T>(r[h].s[e], 1);
+          s[h][e] = __builtin_fmaf(s[h][e], ks, __builtin_fmaf(kz, qsum, ks * 0.f));
+          vs[4 * h + e] = scale_field<T>(r[h].s[e], 2);
+          vz[4 * h + e] = scale_field<T>(r[h].s[e], 3);
         }
       }
-      Half ring[NB][2];
-      int have[NB][2];  // tokens of the half (FAST), or a bit a token
-      auto issue = [&](int hi, Half& r, int& mine) NXA_INLINE {
-        if constexpr (FAST) {
-          // (past the last step: empty ranges, so every step counts alike)
-          const int j = min(hi, 2 * ns - 1);
-          const int nr = hi < 2 * ns ? __builtin_amdgcn_readlane(rows, j) : 0;
-          const int64_t pg = __builtin_amdgcn_readlane(page, j);
-          const int64_t sl = __builtin_amdgcn_readlane(slot, j);
-          const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)(kp + pg * p.k_str[0] + sl * kb), 0, nr * kb, 0x00020000);
-          const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)(vp + pg * p.v_str[0] + sl * vb), 0, nr * vb, 0x00020000);
-          const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)(sp + pg * p.sc_str[0] + sl * 4), 0, nr * 4 * R::ES, 0x00020000);
-          r.k = buf_load<NKW>(rk, koff);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if constexpr (VB == 2)
-              r.v[x].w[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rv, voff[x], 0, kNonTemporal);
-            else
-              r.v[x] = buf_load<NVW>(rv, voff[x]);
-          }
-          // (a load a token, so that none straddles the range's end)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) r.s[x] = buf_load<NS>(rs, (4 * g + x) * 4 * R::ES);
-          mine = nr;
-        } else {
-          // Lane x < 16 looks up token x of the half; the others ask it.
-          const int key = key_of(2 * i0 + min(hi, 2 * ns - 1)) + c;
-          int pg = -1, sl = 0;
-          if (hi < 2 * ns && key < len) {
-            pg = p.table[b * p.table_rs + key / p.PS];
-            sl = key % p.PS;
-          }
-          const bool ok = (unsigned)pg < (unsigned)p.P;
-          if (!ok) pg = sl = 0;
-          mine = (int)(__ballot(ok) & 0xffff);
-          const char* kr = kp + pg * p.k_str[0] + (int64_t)sl * kb + 4 * NKW * g;
-#pragma unroll
-          for (int w = 0; w < NKW; ++w)
-            r.k.w[w] = ok && 4 * (NKW * g + w) < kb ? reinterpret_cast<const uint32_t*>(kr)[w] : 0u;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int src = 4 * g + x;
-            const bool on = mine >> src & 1;
-            const int64_t vpg = __shfl(pg, src, 64), vsl = __shfl(sl, src, 64);
-            const char* vr = vp + vpg * p.v_str[0] + vsl * vb + VB * c;
-            if constexpr (VB == 2) {
-              r.v[x].w[0] = on && VB * c < vb ? *reinterpret_cast<const uint16_t*>(vr) : 0u;
-            } else {
-#pragma unroll
-              for (int w = 0; w < NVW; ++w)
-                r.v[x].w[w] = on && VB * c + 4 * w < vb ? reinterpret_cast<const uint32_t*>(vr)[w] : 0u;
-            }
-            const uint32_t* sr = reinterpret_cast<const uint32_t*>(sp + vpg * p.sc_str[0] + vsl * 4);
-#pragma unroll
-            for (int w = 0; w < NS; ++w) r.s[x].w[w] = on ? sr[w] : 0u;
-          }
-        }
-      };
-      auto compute = [&](const Half (&r)[2], const int (&mine)[2]) NXA_INLINE {
-        f32x4 s[2];
-        float mt = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          s[h] = f32x4{s_init, s_init, s_init, s_init};
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            const u32x4 a = key_operand<BITS>(r[h].k, j);
-#pragma unroll
-            for (int t = 0; t < QT; ++t) s[h] = mma(a, qf[j][t], s[h]);
-          }
-          // Rows of the accumulator: tokens 4 g + e.
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool ok = FAST ? 4 * g + e < mine[h] : (mine[h] >> (4 * g + e) & 1) != 0;
-            // (a scale of infinity makes its token NaN, whatever the signs)
-            const float ks = scale_field<T>(r[h].s[e], 0), kz = scale_field<T>(r[h].s[e], 1);
-            const float x = __builtin_fmaf(s[h][e], ks * p.scale_log2, __builtin_fmaf(kz, qz, ks * 0.f));
-            s[h][e] = ok ? x : -INFINITY;
-            mt = fmaxf(mt, s[h][e]);
-          }
-        }
-        if (__any(mt > m_ref + kSlack)) {
-          mt = fmaxf(mt, xor16(mt));
-          mt = fmaxf(mt, shfl_xor32(mt));
-          const float mn = fmaxf(m_ref, mt);
-          const float alpha = mn > m_ref ? fast_exp2(m_ref - mn) : 1.f;
-          l *= alpha;
-          zs *= alpha;
-#pragma unroll
-          for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[f][e] *= alpha;
-          m_ref = mn;
-        }
-        const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
-        float x[8];  // P s'
+      if (((mine[0] ^ kFull) | (mine[1] ^ kFull)) != 0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float w = fast_exp2(s[h][e] + neg_m);
-            const float sc = scale_field<T>(r[h].s[e], 2), z = scale_field<T>(r[h].s[e], 3);
-            l += w;
-            x[4 * h + e] = w * sc;
-            zs = __builtin_fmaf(w, BITS == 4 ? __builtin_fmaf(-16.f, sc, z) : z, zs);
+            const bool ok = FAST ? 4 * g + e < mine[h] : (mine[h] >> (4 * g + e) & 1) != 0;
+            // (what stands there of other tokens' scales may be NaN)
+            s[h][e] = ok ? s[h][e] : -INFINITY;
+            vs[4 * h + e] = ok ? vs[4 * h + e] : 0.f;
+            vz[4 * h + e] = ok ? vz[4 * h + e] : 0.f;
           }
-        u32x4 pf[PT];
+      }
+      float mt = -INFINITY, sm = 0.f;
 #pragma unroll
-        for (int t = 0; t < PT; ++t)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            pf[t][w] = pack2(x[2 * w], x[2 * w + 1]);
-            x[2 * w] -= low_of(pf[t][w]);
-            x[2 * w + 1] -= high_of(pf[t][w]);
-          }
-        auto product = [&](int f, u32x4 a) NXA_INLINE {
+        for (int e = 0; e < 4; ++e) {
+          mt = fmaxf(mt, s[h][e]);
+          sm = fmaxf(sm, __builtin_fabsf(vs[4 * h + e]));
+        }
+      mt *= sl;
+      if (__any((mt > m_ref + kSlack) | (sm > s_most))) {
+        mt = fmaxf(mt, xor16(mt));
+        mt = fmaxf(mt, shfl_xor32(mt));
+        sm = fmaxf(sm, xor16(sm));
+        sm = fmaxf(sm, shfl_xor32(sm));
+        m_ref = fmaxf(m_ref, mt);
+        if (sm > s_most) {
+          const int e = max(__builtin_amdgcn_frexp_expf(sm), -90);
+          s_exp = fmaxf(s_exp, (float)e);
+          s_most = __builtin_ldexpf(4.f, e);
+        }
+        const float old = ref;
+        ref = m_ref + (s_exp - 3.f);
+        const float alpha = old == -INFINITY ? 1.f : fast_exp2(old - ref);
+        l *= alpha;
+        zs *= alpha;
 #pragma unroll
-          for (int t = 0; t < PT; ++t) o[f] = mma(a, pf[t], o[f]);
-        };
+        for (int e = 0; e < 4; ++e) ones_o[e] *= alpha;
 #pragma unroll
-        for (int w = 0; w < NVW; ++w)
+        for (int f = 0; f < NF; ++f)
 #pragma unroll
-          for (int y = 0; y < (VB < 4 ? VB : 4); ++y) {
-            // Byte y of word w of the lane's eight keys, in pairs.
-            const uint32_t sel = 0x0c000c00u | (uint32_t)(4 + y) << 16 | (uint32_t)y;
-            uint32_t t[4];
+          for (int e = 0; e < 4; ++e) o[f][e] *= alpha;
+      }
+      const float neg_m = ref == -INFINITY ? 0.f : -ref;
+      float x[8];  // P s'
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+      for (int i = 0; i < 8; ++i) {
+        const float w = fast_exp2(__builtin_fmaf(s[i / 4][i % 4], sl, neg_m));
+        l += w;
+        x[i] = w * vs[i];
+        zs = __builtin_fmaf(w, vz[i], zs);
+      }
+      u32x4 pf[PT];
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                t[2 * h + e] = __builtin_amdgcn_perm(r[h].v[2 * e + 1].w[w], r[h].v[2 * e].w[w], sel);
-            if constexpr (BITS == 4) {
-              product(8 * w + 2 * y, u32x4{nibbles<0>(t[0]), nibbles<0>(t[1]), nibbles<0>(t[2]), nibbles<0>(t[3])});
-              product(8 * w + 2 * y + 1, u32x4{nibbles<4>(t[0]), nibbles<4>(t[1]), nibbles<4>(t[2]), nibbles<4>(t[3])});
+      for (int t = 0; t < PT; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          pf[t][w] = pack_f16(x[2 * w], x[2 * w + 1]);
+          x[2 * w] -= low_f16(pf[t][w]);
+          x[2 * w + 1] -= high_f16(pf[t][w]);
+        }
+      auto product = [&](f32x4& acc, u32x4 a) NXA_INLINE {
+#pragma unroll
+        for (int t = 0; t < PT; ++t) acc = mma_f16(a, pf[t], acc);
+      };
+      product(ones_o, u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
+#pragma unroll
+      for (int w = 0; w < NVW; ++w)
+#pragma unroll
+        for (int y = 0; y < (VB < 4 ? VB : 4); ++y) {
+          // Byte y of word w of the lane's eight keys, in pairs.
+          const uint32_t sel = 0x0c000c00u | (uint32_t)(4 + y) << 16 | (uint32_t)y;
+          u32x4 t, a, d;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            t[i] = __builtin_amdgcn_perm(r[i / 2].v[2 * (i % 2) + 1].at(w), r[i / 2].v[2 * (i % 2)].at(w), sel);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (BITS == 8) {
+              a[i] = t[i] | cb.k1024;
             } else {
-              u32x4 a;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) a[e] = pack2(byte_of<0>(t[e]), byte_of<2>(t[e]));
-              product(4 * w + y, a);
+              a[i] = R::EVEN == 1024.f ? (t[i] & cb.low) | cb.k1024 : (t[i] << 4 & cb.high) | cb.k64;
+              d[i] = (t[i] & cb.high) | cb.k64;
             }
           }
+          if constexpr (BITS == 8) {
+            product(o[4 * w + y], a);
+          } else {
+            product(o[8 * w + 2 * y], a);
+            product(o[8 * w + 2 * y + 1], d);
+          }
+        }
+    };
+    if constexpr (FAST) {
+      // Column and slot of the next half to be issued, and its page (read a half
+      // ahead).
+      int half = 0, col, slot, page, have[NB][2];
+      const int per = p.PS >= kPagedKeys ? 0 : kPagedKeys / p.PS, rest = kPagedKeys - per * p.PS;
+      const auto* row = (constant_int*)(uintptr_t)(p.table + b * p.table_rs);
+      {
+        const int key0 = key_of(0);
+        col = __builtin_amdgcn_readfirstlane(key0 / p.PS);
+        slot = __builtin_amdgcn_readfirstlane(key0 - key0 / p.PS * p.PS);
+        page = steps > 0 ? row[col] : -1;
+      }
+      auto issue = [&](uint32_t to, int& mine) NXA_INLINE {
+        // (past the last step: empty ranges, so that every step counts alike)
+        const int key0 = key_of(half);
+        const bool ok = half < 2 * steps && (unsigned)page < (unsigned)p.P;
+        mine = ok ? max(min(kHalfKeys, len - key0), 0) : 0;
+        const uint64_t pg = ok ? (uint32_t)page : 0u;
+        const int sl = ok ? slot : 0;
+        const char* ks = kp + pg * (uint32_t)p.k16 * 16 + sl * kb;
+        const char* vs = vp + pg * (uint32_t)p.v16 * 16 + sl * vb;
+        const char* ss = sp + pg * (uint32_t)p.s16 * 16 + sl * (4 * R::ES);
+        // The next half: in this step, or at the same place 128 tokens on.
+        ++half;
+        if (half & 1) {
+          slot += kHalfKeys;
+        } else {
+          slot += rest - kHalfKeys;
+          col += per;
+          if (slot < 0) slot += p.PS, --col;
+        }
+        if (slot >= p.PS) slot -= p.PS, ++col;
+        page = half < 2 * steps && key_of(half) < len ? row[col] : -1;
+        const i32x4 rk = make_rsrc(ks, mine * kb), rv = make_rsrc(vs, mine * vb),
+                    rs = make_rsrc(ss, mine * (4 * R::ES));
+#pragma unroll
+        for (int x = 0; x < R::KC; ++x) {
+          dma16_buf_nt(rk, 16 * lane + 1024 * x, to + 1024 * x);
+          dma16_buf_nt(rv, 16 * lane + 1024 * x, to + 1024 * (R::KC + x));
+        }
+        dma4_buf(rs, 4 * lane, to + 2048 * R::KC);
+      };
+      auto fetch = [&](Half& r, uint32_t at) NXA_INLINE {
+        r.k.lds(k_at + at);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if constexpr (VB == 2)
+            r.v[x].w[0] = *(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)(v_at + at + x * vb);
+          else
+            r.v[x].lds(v_at + at + x * vb);
+          r.s[x].lds(s_at + at + 4 * R::ES * x);
+        }
       };
 #pragma unroll
       for (int x = 0; x < NB; ++x)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) issue(2 * x + h, ring[x][h], have[x][h]);
-      for (int i = 0; i < ns; i += NB)
+        for (int h = 0; h < 2; ++h) issue(ring + x * STEP_BYTES + h * R::HALF_BYTES, have[x][h]);
+      for (int i = 0; i < steps; i += NB)
 #pragma unroll
         for (int x = 0; x < NB; ++x) {
-          compute(ring[x], have[x]);
+          // (the copies of the steps behind it may be in flight)
+          __builtin_amdgcn_s_waitcnt(vmcnt_imm((NB - 1) * 2 * COPIES));
+          asm volatile("" ::: "memory");
+          Half r[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) issue(2 * (i + x + NB) + h, ring[x][h], have[x][h]);
+          for (int h = 0; h < 2; ++h) fetch(r[h], x * STEP_BYTES + h * R::HALF_BYTES);
+          // (read before the next copies to this place)
+          __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
+          asm volatile("" ::: "memory");
+          const int mine[2] = {have[x][0], have[x][1]};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) issue(ring + x * STEP_BYTES + h * R::HALF_BYTES, have[x][h]);
+          compute(r, mine);
         }
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    } else {
+      for (int i = 0; i < steps; ++i) {
+        Half r[2];
+        int mine[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // Lane x < 16 looks up token x of the half; the others ask it.
+          const int key = key_of(2 * i + h) + c;
+          int page = -1, slot = 0;
+          if (key < len) {
+            page = p.table[b * p.table_rs + key / p.PS];
+            slot = key % p.PS;
+          }
+          const bool ok = (unsigned)page < (unsigned)p.P;
+          if (!ok) page = slot = 0;
+          mine[h] = (int)(__ballot(ok) & 0xffff);
+          const char* kr = kp + page * p.k_str[0] + (int64_t)slot * kb + 4 * NKW * g;
+#pragma unroll
+          for (int w = 0; w < NKW; ++w)
+            r[h].k.w[w] = ok && 4 * (NKW * g + w) < kb ? reinterpret_cast<const uint32_t*>(kr)[w] : 0u;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int src = 4 * g + x;
+            const bool on = mine[h] >> src & 1;
+            const int64_t vpg = __shfl(page, src, 64), vsl = __shfl(slot, src, 64);
+            const char* vr = vp + vpg * p.v_str[0] + vsl * vb + VB * c;
+            if constexpr (VB == 2) {
+              r[h].v[x].w[0] = on && VB * c < vb ? *reinterpret_cast<const uint16_t*>(vr) : 0u;
+            } else {
+#pragma unroll
+              for (int w = 0; w < NVW; ++w)
+                r[h].v[x].w[w] = on && VB * c + 4 * w < vb ? reinterpret_cast<const uint32_t*>(vr)[w] : 0u;
+            }
+            const uint32_t* sr = reinterpret_cast<const uint32_t*>(
+                sp + vpg * p.sc_str[0] * R::ES + vsl * (4 * R::ES));
+#pragma unroll
+            for (int w = 0; w < NS; ++w) r[h].s[x].w[w] = on ? sr[w] : 0u;
+          }
+        }
+        compute(r, mine);
+      }
     }
     l += xor16(l);
     l += shfl_xor32(l);
     zs += xor16(zs);
     zs += shfl_xor32(zs);
 
-    // Join the waves: [wave][field][lane], field 4 f + e of O, then m and l.
+    // Join the waves: [wave][field][lane], field 4 f + e of O, then m and l (where
+    // the rings were: all copies have landed and been read).
     __syncthreads();
     {
       float* mw = ms + wave * FIELDS * 64 + lane;
 #pragma unroll
       for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mw[(4 * f + e) * 64] = o[f][e] + zs;
-      mw[(FIELDS - 2) * 64] = m_ref;
+        for (int e = 0; e < 4; ++e)
+          mw[(4 * f + e) * 64] = __builtin_fmaf(f & 1 ? -R::ODD : -R::EVEN, ones_o[e], o[f][e]) + zs;
+      mw[(FIELDS - 2) * 64] = ref;
       mw[(FIELDS - 1) * 64] = l;
     }
     __syncthreads();
@@ -498,6 +712,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
         }
       }
     }
+    if constexpr (FAST) __syncthreads();  // (the next row's copies)
     u += v1 - v0;
     if (hv == HV - 1 && v1 == n) {
       before += n;
@@ -511,12 +726,20 @@ int qpaged_dp(int m) { return m <= 64 ? 64 : m <= 128 ? 128 : 256; }
 bool qpaged_whole(int64_t room) { return room <= 1024; }
 
 template <typename T, int DP, int BITS>
-static void launch_qpaged_b(const QuantPagedParams& p, hipStream_t stream) {
+static void launch_qpaged_b(QuantPagedParams p, hipStream_t stream) {
   const dim3 grid(p.nblk ? p.nblk : p.B * p.Hk * p.strips), block(256);
   using R = QuantStep<T, DP, BITS>;
   const int kb = p.D * BITS / 8, vb = p.Dv * BITS / 8;
-  if (p.PS % kHalfKeys == 0 && kb % (4 * R::NKW) == 0 && vb % R::VB == 0)
+  const int64_t ps = p.sc_str[0] * (int)sizeof(T), hs = p.sc_str[1] * (int)sizeof(T);
+  const bool aligned = !((p.k_str[0] | p.k_str[1] | p.v_str[0] | p.v_str[1] | ps | hs) & 15);
+  const int64_t far = (int64_t)1 << 35;  // (a page stride counts 16 bytes in 31 bits)
+  if (p.PS % kHalfKeys == 0 && kb % (4 * R::NKW) == 0 && vb % R::VB == 0 && aligned &&
+      p.k_str[0] < far && p.v_str[0] < far && ps < far) {
+    p.k16 = (int)(p.k_str[0] / 16);
+    p.v16 = (int)(p.v_str[0] / 16);
+    p.s16 = (int)(ps / 16);
     hipLaunchKernelGGL((qpaged_kernel<T, DP, BITS, true>), grid, block, 0, stream, p);
+  }
   else
     hipLaunchKernelGGL((qpaged_kernel<T, DP, BITS, false>), grid, block, 0, stream, p);
 }

@@ -39,6 +39,7 @@ struct QuantPagedParams : PagedParams {  // k_str, v_str in bytes
   const void* sc;
   int64_t sc_str[2];
   int bits;
+  int k16, v16, s16;  // page strides in 16 bytes (set by the launcher)
 };
 
 int qpaged_dp(int m);  // padded head dim

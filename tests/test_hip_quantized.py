@@ -2,10 +2,24 @@
 
 Codes, scales and moved pages have to be equal.  A value read back is one
 rounding to its type (u = eps(T) / 2) of a float32 multiply-add (2^-24).
+
 Attention's tolerance is a bound per element from the roundings the kernel makes:
-float32 sums of products of whole numbers (2^-24 a step, with the 16 that codes of
-4 bits carry), P s' as two bf16 terms (2^-17, float32: three, 2^-25), and the
-output's rounding.
+
+* q, 16-bit types: fp8 terms of q scaled to a largest element of 2^7 or more.  Of
+  an element of bits b = 8 (bf16) or 11 the t = 2 or 3 terms of 4 bits leave nothing
+  but what lies below the smallest step 2^-9: at most 2^-10, that is 2^-17 of the
+  largest element; a score is off by its codes' sum times that.
+* P s' as the sum of one fp16 number (bf16: off by 2^-12 of itself), two (fp16:
+  2^-23) or three (float32: 2^-25).  The product with ones that takes off what stands
+  in for zero sees the same numbers, so the error meets the codes themselves alone.
+  The last number is off by at least 2^-25 where it is small (fp16 numbers below 2^-14
+  are 2^-24 apart); the token of the largest score has P s' = 2^3 s' / 2^e or more,
+  2^e less than twice the largest scale, so that is 2^-27 of the largest weight times
+  the largest scale.
+* float32 sums, 2^-24 a step: a wave adds up 32 tokens a step, so n / 32 + 24 of
+  them (with the join's) over codes with what stands in for zero, up to 1024, and
+  the same taken off; scores d + 8 steps, float32 over codes with 16.
+* the output's rounding, u.
 """
 
 from __future__ import annotations
@@ -47,16 +61,19 @@ def _check(out, q, pool, bits, table, lengths, scale):
     """``out`` against the plain form, on host copies of the operands."""
     dt = q.dtype
     u = torch.finfo(dt).eps / 2
-    p_err = 2.0 ** -25 if dt == torch.float32 else 2.0 ** -17
+    p_err = {torch.bfloat16: 2.0 ** -12, torch.float16: 2.0 ** -23, torch.float32: 2.0 ** -25}[dt]
+    q_err = 0.0 if dt == torch.float32 else 2.0 ** -17
     d = q.shape[2]
     sc = _n64(pool[2])
     codes = [qplain.unpack(x.cpu().numpy(), bits) for x in pool[:2]]
-    off = 16 if bits == 4 else 0
     k, v = (c * sc[..., 2 * w, None] + sc[..., 2 * w + 1, None] for w, c in enumerate(codes))
-    # What sums of a key's score and of a value's column go through: codes with
-    # the 16 they carry, the 16 taken off, the minimum, without their signs.
+    # What sums of a key's score and of a value's column go through, without signs:
+    # codes, what stands in for zero twice, and the minimum.
+    off = (32 if dt == torch.float32 and bits == 4 else 0,
+           2048 if bits == 8 or dt == torch.bfloat16 else 128)
+    kc, vc = (np.abs(sc[..., 2 * w, None]) * c for w, c in enumerate(codes))
     kab, vab = (
-        np.abs(sc[..., 2 * w, None]) * (c + 2 * off) + np.abs(sc[..., 2 * w + 1, None])
+        np.abs(sc[..., 2 * w, None]) * (c + off[w]) + np.abs(sc[..., 2 * w + 1, None])
         for w, c in enumerate(codes)
     )
     qn = _n64(q)
@@ -75,9 +92,14 @@ def _check(out, q, pool, bits, table, lengths, scale):
         for h in range(q.shape[1]):
             w, logit, _, _ = rows[i, h]
             es = (d + 8) * E24 * abs(scale) * (kab[e, h // g, s] @ np.abs(qn[i, h]))
-            es = es + 4 * E24 * np.abs(logit)
+            es += q_err * abs(scale) * kc[e, h // g, s].sum(-1) * np.abs(qn[i, h]).max()
+            es += 4 * E24 * np.abs(logit)
             rp = es + es.max() + (n + 16) * E24 + 8 * E24 * np.abs(logit).max() + 32 * E24
-            tol[i, h] = (w * (rp + p_err + (n + 16) * E24)) @ vab[e, h // g, s]
+            codes_v, all_v = vc[e, h // g, s], vab[e, h // g, s]
+            tol[i, h] = (w * (rp + 8 * E24)) @ (codes_v + np.abs(sc[e, h // g, s, 3])[:, None])
+            tol[i, h] += (w * p_err) @ codes_v
+            tol[i, h] += 2.0 ** -27 * w.max() * sc[e, h // g, s, 2].max() * codes[1].max() * len(e)
+            tol[i, h] += (n / 32 + 24) * E24 * (w @ all_v)
             tol[i, h] += (u + 8 * E24) * np.abs(want[i, h])
     tiny = 4 * (2.0 ** -24 if dt == torch.float16 else float(torch.finfo(dt).tiny))
     bad = ~(np.abs(got - want) <= tol + tiny)

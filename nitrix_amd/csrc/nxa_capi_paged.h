@@ -59,7 +59,8 @@ struct PagedPlan {
   int strips, nblk;
 };
 
-int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t), PagedPlan* plan) {
+int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t), int most,
+               PagedPlan* plan) {
   if (H <= 0 || H % Hk != 0)
     return fail(NXA_E_SHAPE, "H=%d must be a positive multiple of Hk=%d", H, Hk);
   plan->strips = (H / Hk + 15) / 16;
@@ -72,13 +73,13 @@ int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t), Page
     return fail(NXA_E_SHAPE, "%d sequences of up to %lld tokens exceed 2^31 tiles", B,
                 (long long)len);
   // (a block a row where a grid of less than 2^32 threads holds them)
-  plan->nblk =
-      whole(room) && rows < 1 << 24 ? 0 : nxa::paged_blocks(tiles * Hk * plan->strips);
+  const int64_t units = tiles * Hk * plan->strips;
+  plan->nblk = whole(room) && rows < 1 << 24 ? 0 : (int)(units < most ? units : most);
   return NXA_OK;
 }
 
 int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
-  return plan_paged(d->Hk, d->PS, B, M, H, nxa::paged_whole, plan);
+  return plan_paged(d->Hk, d->PS, B, M, H, nxa::paged_whole, nxa::kPagedBlocks, plan);
 }
 
 size_t paged_workspace(int dp, const PagedPlan& plan) {

@@ -38,13 +38,13 @@ struct PagedParams : PoolParams {
 constexpr int kPagedKeys = 128;    // keys of a work unit
 constexpr int kStartUnits = 1;     // what starting on a row costs, in units
 constexpr int kPagedBlocks = 512;  // most blocks that share the work
+constexpr int kJoinPieces = 768;   // most of any kernel whose pieces are joined
 // One partial result: [16 heads][DP] sums, then a maximum and a sum a head.
 constexpr int paged_part_floats(int dp) { return 16 * dp + 32; }
 int paged_dp(int m);               // padded head dim
 // Whether a block takes a whole row (sequence and key-value head) of up to
-// `room` tokens, and else how many share the units.
+// `room` tokens; else as many share the units as there are, at most kPagedBlocks.
 bool paged_whole(int64_t room);
-int paged_blocks(int64_t most_units);
 void launch_paged(const PagedParams& p, int io_dtype, hipStream_t stream);
 // The second kernel alone, for pieces of dp = 64, 128 or 256 columns.
 void launch_paged_join(const PagedParams& p, int io_dtype, int dp, hipStream_t stream);

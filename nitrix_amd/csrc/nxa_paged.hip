@@ -432,7 +432,7 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
 // order: block i the row that starts in block i.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p) {
-  __shared__ float wgt[kPagedBlocks * 16];
+  __shared__ float wgt[kJoinPieces * 16];
   __shared__ float inv_s[16];
   __shared__ float acc_s[256 * 4];
   const int tid = threadIdx.x, j0 = blockIdx.x;
@@ -514,10 +514,6 @@ int paged_dp(int m) { return m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
 // 31.6; 64 of up to 512 26 / 17, 1024 33 / 27, 2048 47 / 44, 4096 62 / 81; 256 of
 // up to 1024 90 / 83, 2048 139 / 138.
 bool paged_whole(int64_t room) { return room <= 1024; }
-
-int paged_blocks(int64_t most_units) {
-  return (int)(most_units < kPagedBlocks ? most_units : kPagedBlocks);
-}
 
 template <typename T, int DP>
 static void launch_paged_t(const PagedParams& p, hipStream_t stream) {

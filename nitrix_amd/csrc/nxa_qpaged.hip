@@ -204,20 +204,25 @@ __device__ __forceinline__ float scale_field(const Loaded<N>& s, int f) {
 }  // namespace
 
 // Steps whose copies are in flight.
-template <int DP, int BITS>
 constexpr int kQuantDepth = 2;
+// Blocks a CU, by registers and LDS (37 KB at 512 bits a row and less, 70 KB at
+// 1024): three where q and O leave room for it.
+constexpr int quant_blocks(int es, int dp, int bits) {
+  return dp > 128 ? 1 : dp * bits > 512 || (es == 4 && dp == 128) ? 2 : 3;
+}
 
 // FAST: pages hold a multiple of 16 tokens, so that a half lies in one page, and
 // codes and scales are aligned: halves are copied to LDS, each wave its own, steps
 // ahead of their use.  Else every key looks its page up and codes are loaded four
 // bytes at a time.
 template <typename T, int DP, int BITS, bool FAST>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const QuantPagedParams p) {
+__global__ __launch_bounds__(256, quant_blocks(sizeof(T), DP, BITS)) void
+qpaged_kernel(const QuantPagedParams p) {
   using R = QuantStep<T, DP, BITS>;
   using Half = HalfRegs<T, DP, BITS>;
   constexpr int NKW = R::NKW, NJ = R::NJ, DPL = R::DPL, VB = R::VB, NVW = R::NVW, NS = R::NS;
   constexpr int QT = R::QT, PT = R::PT;
-  constexpr int NB = kQuantDepth<DP, BITS>;
+  constexpr int NB = kQuantDepth;
   constexpr int NF = DPL;  // O^T fragments: fragment f is columns DPL i + f, i = 0 .. 15
   constexpr int FIELDS = NF * 4 + 2;
   constexpr int STEP_BYTES = 2 * R::HALF_BYTES, COPIES = R::COPIES;
@@ -391,7 +396,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
     // 2^kSlack only, plus 2^s_exp that no value's scale exceeds more than fourfold
     // (s_most), less 3: P s' is then below 2^13.  zs: what the minima add to every
     // column.
-    float m_ref = -INFINITY, ref = -INFINITY, l = 0.f, zs = 0.f;
+    float m_ref = -INFINITY, ref = -INFINITY, neg_ref = 0.f, l = 0.f, zs = 0.f;
     float s_most = 0.f, s_exp = -90.f;
 
     const char* kp = (const char*)p.k + hk * p.k_str[1];
@@ -403,7 +408,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
     while (steps > 0 && key_of(2 * steps - 2) >= len) --steps;
     // `mine`: tokens of the half (FAST), or a bit a token.
     constexpr int kFull = FAST ? kHalfKeys : 0xffff;
-    auto compute = [&](const Half (&r)[2], const int (&mine)[2]) NXA_INLINE {
+    // (`values` is called between the softmax and V's product)
+    auto compute = [&](Half (&r)[2], const int (&mine)[2], auto&& values) NXA_INLINE {
       f32x4 s[2];
       float vs[8], vz[8];
 #pragma unroll
@@ -436,7 +442,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
           vz[4 * h + e] = scale_field<T>(r[h].s[e], 3);
         }
       }
-      if (((mine[0] ^ kFull) | (mine[1] ^ kFull)) != 0) {
+      if (__builtin_expect(((mine[0] ^ kFull) | (mine[1] ^ kFull)) != 0, 0)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -457,19 +463,18 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
           sm = fmaxf(sm, __builtin_fabsf(vs[4 * h + e]));
         }
       mt *= sl;
-      if (__any((mt > m_ref + kSlack) | (sm > s_most))) {
+      if (__builtin_expect(__any((mt > m_ref + kSlack) | (sm > s_most)), 0)) {
         mt = fmaxf(mt, xor16(mt));
         mt = fmaxf(mt, shfl_xor32(mt));
         sm = fmaxf(sm, xor16(sm));
         sm = fmaxf(sm, shfl_xor32(sm));
         m_ref = fmaxf(m_ref, mt);
-        if (sm > s_most) {
-          const int e = max(__builtin_amdgcn_frexp_expf(sm), -90);
-          s_exp = fmaxf(s_exp, (float)e);
-          s_most = __builtin_ldexpf(4.f, e);
-        }
+        const int e = max(__builtin_amdgcn_frexp_expf(sm), -90);
+        s_exp = sm > s_most ? (float)e : s_exp;
+        s_most = sm > s_most ? __builtin_ldexpf(4.f, e) : s_most;
         const float old = ref;
         ref = m_ref + (s_exp - 3.f);
+        neg_ref = ref == -INFINITY ? 0.f : -ref;
         const float alpha = old == -INFINITY ? 1.f : fast_exp2(old - ref);
         l *= alpha;
         zs *= alpha;
@@ -480,11 +485,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[f][e] *= alpha;
       }
-      const float neg_m = ref == -INFINITY ? 0.f : -ref;
       float x[8];  // P s'
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float w = fast_exp2(__builtin_fmaf(s[i / 4][i % 4], sl, neg_m));
+        const float w = fast_exp2(__builtin_fmaf(s[i / 4][i % 4], sl, neg_ref));
         l += w;
         x[i] = w * vs[i];
         zs = __builtin_fmaf(w, vz[i], zs);
@@ -498,6 +502,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
           x[2 * w] -= low_f16(pf[t][w]);
           x[2 * w + 1] -= high_f16(pf[t][w]);
         }
+      values();
       auto product = [&](f32x4& acc, u32x4 a) NXA_INLINE {
 #pragma unroll
         for (int t = 0; t < PT; ++t) acc = mma_f16(a, pf[t], acc);
@@ -572,15 +577,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
         }
         dma4_buf(rs, 4 * lane, to + 2048 * R::KC);
       };
-      auto fetch = [&](Half& r, uint32_t at) NXA_INLINE {
-        r.k.lds(k_at + at);
+      auto fetch_v = [&](Half& r, uint32_t at) NXA_INLINE {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           if constexpr (VB == 2)
             r.v[x].w[0] = *(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)(v_at + at + x * vb);
           else
             r.v[x].lds(v_at + at + x * vb);
-          r.s[x].lds(s_at + at + 4 * R::ES * x);
         }
       };
 #pragma unroll
@@ -595,14 +598,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
           asm volatile("" ::: "memory");
           Half r[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) fetch(r[h], x * STEP_BYTES + h * R::HALF_BYTES);
-          // (read before the next copies to this place)
-          __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
-          asm volatile("" ::: "memory");
-          const int mine[2] = {have[x][0], have[x][1]};
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t at = x * STEP_BYTES + h * R::HALF_BYTES;
+            r[h].k.lds(k_at + at);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) issue(ring + x * STEP_BYTES + h * R::HALF_BYTES, have[x][h]);
-          compute(r, mine);
+            for (int y = 0; y < 4; ++y) r[h].s[y].lds(s_at + at + 4 * R::ES * y);
+          }
+          const int mine[2] = {have[x][0], have[x][1]};
+          compute(r, mine, [&]() NXA_INLINE {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) fetch_v(r[h], x * STEP_BYTES + h * R::HALF_BYTES);
+            // (all is read before the next copies to this place)
+            __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int h = 0; h < 2; ++h) issue(ring + x * STEP_BYTES + h * R::HALF_BYTES, have[x][h]);
+          });
         }
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     } else {
@@ -644,7 +655,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
             for (int w = 0; w < NS; ++w) r[h].s[x].w[w] = on ? sr[w] : 0u;
           }
         }
-        compute(r, mine);
+        compute(r, mine, [] {});
       }
     }
     l += xor16(l);
@@ -724,6 +735,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void qpaged_kernel(const Qu
 int qpaged_dp(int m) { return m <= 64 ? 64 : m <= 128 ? 128 : 256; }
 
 bool qpaged_whole(int64_t room) { return room <= 1024; }
+
+int qpaged_blocks(int io_dtype, int dp, int bits) {
+  return 256 * (dp > 128 ? 2 : quant_blocks(io_dtype == kF32 ? 4 : 2, dp, bits));
+}
 
 template <typename T, int DP, int BITS>
 static void launch_qpaged_b(QuantPagedParams p, hipStream_t stream) {

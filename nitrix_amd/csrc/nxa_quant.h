@@ -44,6 +44,7 @@ struct QuantPagedParams : PagedParams {  // k_str, v_str in bytes
 
 int qpaged_dp(int m);  // padded head dim
 bool qpaged_whole(int64_t room);
+int qpaged_blocks(int io_dtype, int dp, int bits);  // most blocks that share the work
 
 void launch_quant_write(const QuantMoveParams& p, int io_dtype, hipStream_t stream);
 void launch_quant_read(const QuantMoveParams& p, int io_dtype, hipStream_t stream);

@@ -60,14 +60,14 @@ struct PagedPlan {
 };
 
 int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t), int most,
-               PagedPlan* plan) {
+               int start, PagedPlan* plan) {
   if (H <= 0 || H % Hk != 0)
     return fail(NXA_E_SHAPE, "H=%d must be a positive multiple of Hk=%d", H, Hk);
   plan->strips = (H / Hk + 15) / 16;
   // Units of the largest table, in 31 bits a head.
   const int64_t room = (int64_t)M * PS;
   const int64_t len = room < INT32_MAX ? room : INT32_MAX;
-  const int64_t tiles = (int64_t)B * ((len + nxa::kPagedKeys - 1) / nxa::kPagedKeys + nxa::kStartUnits);
+  const int64_t tiles = (int64_t)B * ((len + nxa::kPagedKeys - 1) / nxa::kPagedKeys + start);
   const int64_t rows = (int64_t)B * Hk * plan->strips;
   if (tiles >= (int64_t)1 << 31 || rows >= (int64_t)1 << 31)
     return fail(NXA_E_SHAPE, "%d sequences of up to %lld tokens exceed 2^31 tiles", B,
@@ -79,7 +79,8 @@ int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t), int 
 }
 
 int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
-  return plan_paged(d->Hk, d->PS, B, M, H, nxa::paged_whole, nxa::kPagedBlocks, plan);
+  return plan_paged(d->Hk, d->PS, B, M, H, nxa::paged_whole, nxa::kPagedBlocks,
+                    nxa::kStartUnits, plan);
 }
 
 size_t paged_workspace(int dp, const PagedPlan& plan) {

@@ -102,7 +102,8 @@ int plan_quant_paged(const nxa_quant_pool_desc* d, int B, int M, int H, PagedPla
     return fail(NXA_E_SHAPE, "a row of %d pages of %d tokens has room for 2^31 or more", M, d->PS);
   const int most = nxa::qpaged_blocks(d->io_dtype, nxa::qpaged_dp(d->D > d->Dv ? d->D : d->Dv),
                                       d->bits);
-  return plan_paged(d->Hk, d->PS, B, M, H, nxa::qpaged_whole, most, plan);
+  return plan_paged(d->Hk, d->PS, B, M, H, nxa::qpaged_whole, most, nxa::kQuantStart,
+                    plan);
 }
 
 size_t quant_paged_workspace(const nxa_quant_pool_desc* d, const PagedPlan& plan) {

@@ -133,7 +133,7 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
   if (p.nblk == 0) {
     b = blockIdx.x / HV;
     before = 0;
-    const int n = paged_units(p, b), hv = blockIdx.x % HV;
+    const int n = paged_units<kStartUnits>(p, b), hv = blockIdx.x % HV;
     if (n == 0) {
       if (hv == 0) paged_zero<T>(p, b);
       return;
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
     for (int i = blockIdx.x; i < p.B; i += p.nblk)
       if (paged_len(p, i) == 0) paged_zero<T>(p, i);
     if (tid == 0) p.joins[blockIdx.x] = {0, 0, 0, 0};
-    paged_prefix(p, pre, wsum);
+    paged_prefix<kStartUnits>(p, pre, wsum);
     units = (int64_t)__builtin_amdgcn_readfirstlane(pre[256]) * HV;
     nblk = busy_blocks(p, units);
     if ((int)blockIdx.x >= nblk) return;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256, (kPagedOcc<T, DP>)) void paged_kernel(const Pa
     }
     b = lo * ((p.B + 255) / 256);
     before = pre[lo];
-    for (int n; before + (n = paged_units(p, b)) <= x; ++b) before += n;
+    for (int n; before + (n = paged_units<kStartUnits>(p, b)) <= x; ++b) before += n;
     b = __builtin_amdgcn_readfirstlane(b);
     before = __builtin_amdgcn_readfirstlane(before);
   }

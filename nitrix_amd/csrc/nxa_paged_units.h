@@ -24,19 +24,21 @@ __device__ __forceinline__ int paged_len(const PagedParams& p, int b) {
 __device__ __forceinline__ int paged_tiles(int len) {
   return (int)(((int64_t)len + kPagedKeys - 1) / kPagedKeys);
 }
-// Units of a (sequence, head): its tiles after kStartUnits for starting on it.
+// Units of a (sequence, head): its tiles after START for starting on it.
+template <int START>
 __device__ __forceinline__ int paged_units(const PagedParams& p, int b) {
   const int n = paged_tiles(paged_len(p, b));
-  return n ? n + kStartUnits : 0;
+  return n ? n + START : 0;
 }
 // Sum of the sequences' units a head before each of 256 consecutive groups of
 // sequences, into pre[0 .. 256] (LDS).
+template <int START>
 __device__ __forceinline__ void paged_prefix(const PagedParams& p, int* pre, int* wsum) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = (p.B + 255) / 256;
   int n = 0;
   for (int i = 0; i < per; ++i)
-    if (tid * per + i < p.B) n += paged_units(p, tid * per + i);
+    if (tid * per + i < p.B) n += paged_units<START>(p, tid * per + i);
   int x = n;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {

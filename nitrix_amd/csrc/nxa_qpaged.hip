@@ -243,7 +243,7 @@ qpaged_kernel(const QuantPagedParams p) {
   if (p.nblk == 0) {
     b = blockIdx.x / HV;
     before = 0;
-    const int n = paged_units(p, b), hv = blockIdx.x % HV;
+    const int n = paged_units<kQuantStart>(p, b), hv = blockIdx.x % HV;
     if (n == 0) {
       if (hv == 0) paged_zero<T>(p, b);
       return;
@@ -254,7 +254,7 @@ qpaged_kernel(const QuantPagedParams p) {
     for (int i = blockIdx.x; i < p.B; i += p.nblk)
       if (paged_len(p, i) == 0) paged_zero<T>(p, i);
     if (tid == 0) p.joins[blockIdx.x] = {0, 0, 0, 0};
-    paged_prefix(p, pre, wsum);
+    paged_prefix<kQuantStart>(p, pre, wsum);
     units = (int64_t)__builtin_amdgcn_readfirstlane(pre[256]) * HV;
     nblk = busy_blocks(p, units);
     if ((int)blockIdx.x >= nblk) return;
@@ -269,7 +269,7 @@ qpaged_kernel(const QuantPagedParams p) {
     }
     b = lo * ((p.B + 255) / 256);
     before = pre[lo];
-    for (int n; before + (n = paged_units(p, b)) <= x; ++b) before += n;
+    for (int n; before + (n = paged_units<kQuantStart>(p, b)) <= x; ++b) before += n;
     b = __builtin_amdgcn_readfirstlane(b);
     before = __builtin_amdgcn_readfirstlane(before);
   }
@@ -284,6 +284,8 @@ qpaged_kernel(const QuantPagedParams p) {
   const uint32_t v_at = ring + 1024 * R::KC + 4 * g * vb + VB * c;
   const uint32_t s_at = ring + 2048 * R::KC + 16 * R::ES * g;
   typedef const __attribute__((address_space(4))) int constant_int;
+  // Pages and slots that 128 tokens span.
+  const int per = p.PS >= kPagedKeys ? 0 : kPagedKeys / p.PS, rest = kPagedKeys - per * p.PS;
 
   while (u < u1) {
     const int len = __builtin_amdgcn_readfirstlane(paged_len(p, b));
@@ -291,15 +293,77 @@ qpaged_kernel(const QuantPagedParams p) {
       ++b;
       continue;
     }
-    const int n = paged_tiles(len) + kStartUnits;
+    const int n = paged_tiles(len) + kQuantStart;
     const int64_t rem = u - (int64_t)before * HV;
     const int hv = __builtin_amdgcn_readfirstlane((int)(rem / n));
     const int v0 = __builtin_amdgcn_readfirstlane((int)(rem % n));
     const int v1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)n, v0 + (u1 - u)));
-    const int t0 = max(v0 - kStartUnits, 0), t1 = max(v1 - kStartUnits, 0);  // tiles
+    const int t0 = max(v0 - kQuantStart, 0), t1 = max(v1 - kQuantStart, 0);  // tiles
     const int hk = hv / p.strips, h0 = (hv % p.strips) * 16;
     const int heads = min(16, p.G - h0);
 
+    const char* kp = (const char*)p.k + hk * p.k_str[1];
+    const char* vp = (const char*)p.v + hk * p.v_str[1];
+    const char* sp = (const char*)p.sc + hk * p.sc_str[1] * R::ES;
+    // This wave's steps: 32 tokens of each unit, up to the length.
+    auto key_of = [&](int half) { return (t0 + (half >> 1)) * kPagedKeys + wave * 32 + (half & 1) * kHalfKeys; };
+    int steps = t1 - t0;
+    while (steps > 0 && key_of(2 * steps - 2) >= len) --steps;
+    // Column and slot of the next half to be issued, and its page (read a half
+    // ahead).
+    int half = 0, col = 0, slot = 0, page = -1, have[NB][2];
+    const auto* row = (constant_int*)(uintptr_t)(p.table + b * p.table_rs);
+    if constexpr (FAST) {
+      const int key0 = key_of(0);
+      col = __builtin_amdgcn_readfirstlane(key0 / p.PS);
+      slot = __builtin_amdgcn_readfirstlane(key0 - key0 / p.PS * p.PS);
+      page = steps > 0 ? row[col] : -1;
+    }
+    auto issue = [&](uint32_t to, int& mine) NXA_INLINE {
+      // (past the last step: empty ranges, so that every step counts alike)
+      const int key0 = key_of(half);
+      const bool ok = half < 2 * steps && (unsigned)page < (unsigned)p.P;
+      mine = ok ? max(min(kHalfKeys, len - key0), 0) : 0;
+      const uint64_t pg = ok ? (uint32_t)page : 0u;
+      const int sl = ok ? slot : 0;
+      const char* ks = kp + pg * (uint32_t)p.k16 * 16 + sl * kb;
+      const char* vs = vp + pg * (uint32_t)p.v16 * 16 + sl * vb;
+      const char* ss = sp + pg * (uint32_t)p.s16 * 16 + sl * (4 * R::ES);
+      // The next half: in this step, or at the same place 128 tokens on.
+      ++half;
+      if (half & 1) {
+        slot += kHalfKeys;
+      } else {
+        slot += rest - kHalfKeys;
+        col += per;
+        if (slot < 0) slot += p.PS, --col;
+      }
+      if (slot >= p.PS) slot -= p.PS, ++col;
+      page = half < 2 * steps && key_of(half) < len ? row[col] : -1;
+      const i32x4 rk = make_rsrc(ks, mine * kb), rv = make_rsrc(vs, mine * vb),
+                  rs = make_rsrc(ss, mine * (4 * R::ES));
+#pragma unroll
+      for (int x = 0; x < R::KC; ++x) {
+        dma16_buf_nt(rk, 16 * lane + 1024 * x, to + 1024 * x);
+        dma16_buf_nt(rv, 16 * lane + 1024 * x, to + 1024 * (R::KC + x));
+      }
+      dma4_buf(rs, 4 * lane, to + 2048 * R::KC);
+    };
+    auto fetch_v = [&](Half& r, uint32_t at) NXA_INLINE {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if constexpr (VB == 2)
+          r.v[x].w[0] = *(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)(v_at + at + x * vb);
+        else
+          r.v[x].lds(v_at + at + x * vb);
+      }
+    };
+    // (the first copies are on their way while q is read and taken apart)
+    if constexpr (FAST)
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) issue(ring + x * STEP_BYTES + h * R::HALF_BYTES, have[x][h]);
     // Q^T: column c is head h0 + c; the lane's quarter of the head dim in the
     // order of K's codes, as QT terms, and the sum of the whole row.
     u32x4 qb[R::FP8 ? 1 : NJ][QT];
@@ -399,13 +463,6 @@ qpaged_kernel(const QuantPagedParams p) {
     float m_ref = -INFINITY, ref = -INFINITY, neg_ref = 0.f, l = 0.f, zs = 0.f;
     float s_most = 0.f, s_exp = -90.f;
 
-    const char* kp = (const char*)p.k + hk * p.k_str[1];
-    const char* vp = (const char*)p.v + hk * p.v_str[1];
-    const char* sp = (const char*)p.sc + hk * p.sc_str[1] * R::ES;
-    // This wave's steps: 32 tokens of each unit, up to the length.
-    auto key_of = [&](int half) { return (t0 + (half >> 1)) * kPagedKeys + wave * 32 + (half & 1) * kHalfKeys; };
-    int steps = t1 - t0;
-    while (steps > 0 && key_of(2 * steps - 2) >= len) --steps;
     // `mine`: tokens of the half (FAST), or a bit a token.
     constexpr int kFull = FAST ? kHalfKeys : 0xffff;
     // (`values` is called between the softmax and V's product)
@@ -536,60 +593,6 @@ qpaged_kernel(const QuantPagedParams p) {
         }
     };
     if constexpr (FAST) {
-      // Column and slot of the next half to be issued, and its page (read a half
-      // ahead).
-      int half = 0, col, slot, page, have[NB][2];
-      const int per = p.PS >= kPagedKeys ? 0 : kPagedKeys / p.PS, rest = kPagedKeys - per * p.PS;
-      const auto* row = (constant_int*)(uintptr_t)(p.table + b * p.table_rs);
-      {
-        const int key0 = key_of(0);
-        col = __builtin_amdgcn_readfirstlane(key0 / p.PS);
-        slot = __builtin_amdgcn_readfirstlane(key0 - key0 / p.PS * p.PS);
-        page = steps > 0 ? row[col] : -1;
-      }
-      auto issue = [&](uint32_t to, int& mine) NXA_INLINE {
-        // (past the last step: empty ranges, so that every step counts alike)
-        const int key0 = key_of(half);
-        const bool ok = half < 2 * steps && (unsigned)page < (unsigned)p.P;
-        mine = ok ? max(min(kHalfKeys, len - key0), 0) : 0;
-        const uint64_t pg = ok ? (uint32_t)page : 0u;
-        const int sl = ok ? slot : 0;
-        const char* ks = kp + pg * (uint32_t)p.k16 * 16 + sl * kb;
-        const char* vs = vp + pg * (uint32_t)p.v16 * 16 + sl * vb;
-        const char* ss = sp + pg * (uint32_t)p.s16 * 16 + sl * (4 * R::ES);
-        // The next half: in this step, or at the same place 128 tokens on.
-        ++half;
-        if (half & 1) {
-          slot += kHalfKeys;
-        } else {
-          slot += rest - kHalfKeys;
-          col += per;
-          if (slot < 0) slot += p.PS, --col;
-        }
-        if (slot >= p.PS) slot -= p.PS, ++col;
-        page = half < 2 * steps && key_of(half) < len ? row[col] : -1;
-        const i32x4 rk = make_rsrc(ks, mine * kb), rv = make_rsrc(vs, mine * vb),
-                    rs = make_rsrc(ss, mine * (4 * R::ES));
-#pragma unroll
-        for (int x = 0; x < R::KC; ++x) {
-          dma16_buf_nt(rk, 16 * lane + 1024 * x, to + 1024 * x);
-          dma16_buf_nt(rv, 16 * lane + 1024 * x, to + 1024 * (R::KC + x));
-        }
-        dma4_buf(rs, 4 * lane, to + 2048 * R::KC);
-      };
-      auto fetch_v = [&](Half& r, uint32_t at) NXA_INLINE {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if constexpr (VB == 2)
-            r.v[x].w[0] = *(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)(v_at + at + x * vb);
-          else
-            r.v[x].lds(v_at + at + x * vb);
-        }
-      };
-#pragma unroll
-      for (int x = 0; x < NB; ++x)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) issue(ring + x * STEP_BYTES + h * R::HALF_BYTES, have[x][h]);
       for (int i = 0; i < steps; i += NB)
 #pragma unroll
         for (int x = 0; x < NB; ++x) {

@@ -42,6 +42,10 @@ struct QuantPagedParams : PagedParams {  // k_str, v_str in bytes
   int k16, v16, s16;  // page strides in 16 bytes (set by the launcher)
 };
 
+#ifndef QSTART
+#define QSTART 5
+#endif
+constexpr int kQuantStart = QSTART;  // what starting on a row costs, in units
 int qpaged_dp(int m);  // padded head dim
 bool qpaged_whole(int64_t room);
 int qpaged_blocks(int io_dtype, int dp, int bits);  // most blocks that share the work

@@ -68,10 +68,7 @@ class _Knobs:
     @classmethod
     def read(cls) -> '_Knobs':
         env = os.environ
-        raw = env.get('NITRIX_BACKEND')
-        choice = None if raw is None else raw.strip().lower()
-        if choice is not None and choice not in _CHOICES:
-            raise _bad_choice('NITRIX_BACKEND', choice)
+        choice = env_backend()
         flag = lambda name: env.get(name, '0').lower() in _TRUTHY  # noqa: E731
         return cls(choice, flag('NITRIX_SILENCE_FALLBACK'), flag('NITRIX_STRICT_BACKEND'))
 
@@ -88,7 +85,11 @@ def strict_backend() -> bool:
 
 def env_backend() -> Optional[str]:
     """The engine named by ``NITRIX_BACKEND`` (lower-cased), or None."""
-    return _Knobs.read().backend
+    raw = os.environ.get('NITRIX_BACKEND')
+    choice = None if raw is None else raw.strip().lower()
+    if choice is not None and choice not in _CHOICES:
+        raise _bad_choice('NITRIX_BACKEND', choice)
+    return choice
 
 
 # --- reproducible mode ---------------------------------------------------------
@@ -169,7 +170,7 @@ def resolve_backend(backend: str, device: Any) -> ResolvedBackend:
         raise _bad_choice('backend', backend)
     chosen = backend
     if chosen == 'auto':
-        chosen = _Knobs.read().backend or 'auto'
+        chosen = env_backend() or 'auto'  # (the other knobs wait for a fallback)
     if chosen == 'auto':
         return auto_backend(device)
     if chosen == 'jax':

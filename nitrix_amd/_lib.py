@@ -98,7 +98,7 @@ EXPORTS = (
     'nxa_profile_reset',
 )
 
-_I64x3 = ctypes.c_int64 * 3
+_I64x3 = I64x3 = ctypes.c_int64 * 3
 I64x2 = ctypes.c_int64 * 2
 
 

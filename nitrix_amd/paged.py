@@ -40,8 +40,7 @@ import torch
 
 from . import _lib
 from ._backend import NitrixBackendError, fallback, resolve_backend
-from ._quant_pool import _check_fused as _check_fused_quantized
-from ._quant_pool import _check_quantized, _quant_desc
+from ._quant_pool import _check_quantized, _fused_pool
 from .attention import (
     _IO_DTYPES,
     _MAX_HEAD_DIM,
@@ -185,16 +184,13 @@ class _Moved:
         if self.scales is None:
             _check_fused(*self.tensors)
             desc, kind = _pool_desc(*self.tensors), 'pages'
+            ptrs = [x.data_ptr() for x in self.tensors]
         else:
             # (bytes are moved, whatever they stand for)
             bits = 4 if any(x.shape[3] % 8 for x in self.tensors[:2]) else 8
-            _check_fused_quantized(*self.tensors, bits)
-            desc, kind = _quant_desc(*self.tensors, bits), 'quant'
-        _lib.check(
-            getattr(_lib.lib(), f'nxa_{kind}_{what}')(
-                ctypes.byref(desc), *(x.data_ptr() for x in self.tensors), *args
-            )
-        )
+            desc, ptrs = _fused_pool(*self.tensors, bits)
+            kind = 'quant'
+        _lib.check(getattr(_lib.lib(), f'nxa_{kind}_{what}')(ctypes.byref(desc), *ptrs, *args))
         _touched(*self.tensors)
 
 

@@ -29,7 +29,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._quant_pool import _bits_of, _check_fused, _check_quantized, _quant_desc
+from ._quant_pool import _bits_of, _check_dtype, _check_quantized, _fused_pool
 from .attention import HipNotTileable, _has_tangent, default_scale
 from .packed import _empty_like, _kernel_layout, _stream
 from .paged import (
@@ -117,29 +117,30 @@ def _reference_write(k_pages, v_pages, scales, k, v, page_table, starts, offsets
             scales[page, :, slot, 2 * which + 1] = z[..., 0]
 
 
-def _move_args(desc, pool, k, v, page_table, starts, offsets):
-    b, m = page_table.shape
-    return (
-        ctypes.byref(desc), *(x.data_ptr() for x in pool), k.data_ptr(),
-        _lib.I64x2(*k.stride()[:2]), v.data_ptr(), _lib.I64x2(*v.stride()[:2]), k.shape[1],
-        page_table.data_ptr(), page_table.stride(0), starts.data_ptr(),
-        None if offsets is None else offsets.data_ptr(), b, m, _stream(k.device),
-    )
-
-
-def _index_layout(page_table, starts, offsets):
+def _move(entry, pool, bits, k, v, page_table, starts, offsets) -> None:
+    """Calls ``nxa_quant_write`` or ``nxa_quant_read``."""
+    desc, ptrs = _fused_pool(*pool, bits)
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
-    return page_table, starts.contiguous(), None if offsets is None else offsets.contiguous()
+    starts = starts.contiguous()
+    offsets = None if offsets is None else offsets.contiguous()
+    b, m = page_table.shape
+    ks, vs = k.stride(), v.stride()
+    _lib.check(
+        getattr(_lib.lib(), entry)(
+            ctypes.byref(desc), *ptrs, k.data_ptr(), _lib.I64x2(ks[0], ks[1]), v.data_ptr(),
+            _lib.I64x2(vs[0], vs[1]), k.shape[1], page_table.data_ptr(), page_table.stride(0),
+            starts.data_ptr(), None if offsets is None else offsets.data_ptr(), b, m,
+            _stream(k.device),
+        )
+    )
 
 
 def _write_hip(k_pages, v_pages, scales, k, v, page_table, starts, offsets, bits):
     pool = (k_pages, v_pages, scales)
-    _check_fused(*pool, bits, k, v)
+    _check_dtype(scales, k, v)
     k, v = _kernel_layout(k), _kernel_layout(v)
-    index = _index_layout(page_table, starts, offsets)
-    desc = _quant_desc(*pool, bits)
-    _lib.check(_lib.lib().nxa_quant_write(*_move_args(desc, pool, k, v, *index)))
+    _move('nxa_quant_write', pool, bits, k, v, page_table, starts, offsets)
     _touched(*pool)
 
 
@@ -216,8 +217,6 @@ def _reference_read(k_pages, v_pages, scales, page_table, starts, offsets, t, bi
 
 
 def _read_hip(k_pages, v_pages, scales, page_table, starts, offsets, t, bits):
-    pool = (k_pages, v_pages, scales)
-    _check_fused(*pool, bits)
     hk = k_pages.shape[1]
     # Tokens before heads, as a projection would leave them.
     k, v = (
@@ -225,9 +224,7 @@ def _read_hip(k_pages, v_pages, scales, page_table, starts, offsets, t, bits):
         .transpose(0, 1)
         for x in (k_pages, v_pages)
     )
-    index = _index_layout(page_table, starts, offsets)
-    desc = _quant_desc(*pool, bits)
-    _lib.check(_lib.lib().nxa_quant_read(*_move_args(desc, pool, k, v, *index)))
+    _move('nxa_quant_read', (k_pages, v_pages, scales), bits, k, v, page_table, starts, offsets)
     return k, v
 
 
@@ -312,28 +309,29 @@ def _reference_attention(q, k_pages, v_pages, scales, page_table, lengths, scale
 
 
 def _attention_hip(q, k_pages, v_pages, scales, page_table, lengths, scale, bits):
-    pool = (k_pages, v_pages, scales)
-    _check_fused(*pool, bits, q)
+    _check_dtype(scales, q)
     if torch.is_grad_enabled() and (q.requires_grad or scales.requires_grad):
         raise HipNotTileable('fused quantised attention has no backward pass.')
     if _has_tangent(q, scales):
         raise HipNotTileable('fused quantised attention has no forward-mode derivative.')
+    desc, ptrs = _fused_pool(k_pages, v_pages, scales, bits)
     q = _kernel_layout(q)
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
     lengths = lengths.contiguous()
     b, h, _ = q.shape
     m = page_table.shape[1]
-    desc = _quant_desc(*pool, bits)
     o = _empty_like(q, desc.Dv)
-    lib = _lib.lib()
-    ws = _workspace(lib.nxa_quant_paged_workspace_bytes(ctypes.byref(desc), b, m, h), q.device)
+    lib, at = _lib.lib(), ctypes.byref(desc)
+    need = lib.nxa_quant_paged_workspace_bytes(at, b, m, h)  # (0: none, or it will say why)
+    ws = _workspace(need, q.device) if need else None
+    qs, os = q.stride(), o.stride()
     _lib.check(
         lib.nxa_quant_paged_fwd(
-            ctypes.byref(desc), *(x.data_ptr() for x in pool), q.data_ptr(),
-            _lib.I64x2(*q.stride()[:2]), page_table.data_ptr(), page_table.stride(0),
-            lengths.data_ptr(), b, m, h, scale, o.data_ptr(), _lib.I64x2(*o.stride()[:2]),
-            ws.data_ptr(), ws.numel(), _stream(q.device),
+            at, *ptrs, q.data_ptr(), _lib.I64x2(qs[0], qs[1]), page_table.data_ptr(),
+            page_table.stride(0), lengths.data_ptr(), b, m, h, scale, o.data_ptr(),
+            _lib.I64x2(os[0], os[1]), None if ws is None else ws.data_ptr(), need,
+            _stream(q.device),
         )
     )
     return o

@@ -145,41 +145,45 @@ def packed_positions(
 
 
 def _validate(q, k, positions, frequencies) -> None:
-    if q.ndim < 3:
+    qs = q.shape
+    if len(qs) < 3:
         raise ValueError(f'rotary_embed: q must be (..., h, t, d); got ndim {q.ndim}.')
+    if not q.dtype.is_floating_point:
+        raise ValueError(f'rotary_embed: q must be floating-point; got {q.dtype}.')
     if k is not None:
-        same = k.ndim == q.ndim and k.shape[:-3] == q.shape[:-3] and k.shape[-2:] == q.shape[-2:]
-        if not same:
+        ks = k.shape
+        if len(ks) != len(qs) or ks[-2:] != qs[-2:] or ks[:-3] != qs[:-3]:
             raise ValueError(
                 'rotary_embed: q and k must agree in all but their heads; got '
-                f'{tuple(q.shape)} and {tuple(k.shape)}.'
+                f'{tuple(qs)} and {tuple(ks)}.'
             )
-    if not q.dtype.is_floating_point or (k is not None and k.dtype != q.dtype):
-        raise ValueError(
-            'rotary_embed: q and k must share a floating-point dtype; got '
-            f'{q.dtype}{"" if k is None else f" and {k.dtype}"}.'
-        )
+        if k.dtype != q.dtype:
+            raise ValueError(
+                f'rotary_embed: q and k must share a dtype; got {q.dtype} and {k.dtype}.'
+            )
     if frequencies.ndim != 1 or not frequencies.dtype.is_floating_point or not (
-            1 <= frequencies.shape[0] <= q.shape[-1] // 2):
+            1 <= frequencies.shape[0] <= qs[-1] // 2):
         raise ValueError(
             f'rotary_embed: frequencies must be floating-point of shape (r / 2,) with r up to '
-            f'd={q.shape[-1]}; got {frequencies.dtype} of shape {tuple(frequencies.shape)}.'
+            f'd={qs[-1]}; got {frequencies.dtype} of shape {tuple(frequencies.shape)}.'
         )
-    if positions.dtype not in (torch.int32, torch.int64):
+    if positions.dtype != torch.int32 and positions.dtype != torch.int64:
         raise ValueError(f'rotary_embed: positions must be int32 or int64; got {positions.dtype}.')
-    want = (*q.shape[:-3], q.shape[-2])
-    try:
-        ok = positions.ndim > 0 and torch.broadcast_shapes(positions.shape, want) == want
-    except RuntimeError:
-        ok = False
-    if not ok or positions.shape[-1] != want[-1]:
+    ps = positions.shape
+    # (broadcast: axes from the last on, each as long as q's or 1; every token its own)
+    if not 1 <= len(ps) <= len(qs) - 2 or ps[-1] != qs[-2] or any(
+        n != 1 and n != m for n, m in zip(ps[-2::-1], qs[-4::-1])
+    ):
         raise ValueError(
-            f'rotary_embed: positions must broadcast to {want} with one for each token; got '
-            f'{tuple(positions.shape)}.'
+            f'rotary_embed: positions must broadcast to {(*qs[:-3], qs[-2])} with one for each '
+            f'token; got {tuple(ps)}.'
         )
-    for name, x in (('k', k), ('positions', positions), ('frequencies', frequencies)):
-        if x is not None and x.device != q.device:
-            raise ValueError(f'rotary_embed: {name} is on {x.device}, q on {q.device}.')
+    device = q.device
+    if not positions.device == frequencies.device == device or (
+            k is not None and k.device != device):
+        for name, x in (('k', k), ('positions', positions), ('frequencies', frequencies)):
+            if x is not None and x.device != device:
+                raise ValueError(f'rotary_embed: {name} is on {x.device}, q on {device}.')
     if frequencies.requires_grad and torch.is_grad_enabled():
         raise ValueError('rotary_embed is not differentiable in the frequencies; detach them.')
 
@@ -207,37 +211,42 @@ def reference_rotary_embed(q, k, positions, frequencies, *, interleaved=False, s
 # ---------------------------------------------------------------------------
 
 
-def _empty_rows(x: torch.Tensor) -> torch.Tensor:
-    """Uninitialised (b, h, t, d) in the memory order of ``x``: tokens before
-    heads where a projection's output was viewed with heads first."""
-    b, h, t, d = x.shape
-    if x.stride(1) < x.stride(2):
-        return torch.empty((b, t, h, d), dtype=x.dtype, device=x.device).transpose(1, 2)
-    return torch.empty((b, h, t, d), dtype=x.dtype, device=x.device)
+def _rows(x: torch.Tensor):
+    """``x`` (h, t, d) or (b, h, t, d) with unit stride over d, its strides (batch,
+    head, token), and an uninitialised tensor of its shape in its memory order:
+    tokens before heads where a projection's output was viewed with heads first."""
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    str_ = x.stride()
+    *lead, h, t, d = x.shape
+    if str_[-3] < str_[-2]:
+        out = torch.empty((*lead, t, h, d), dtype=x.dtype, device=x.device).transpose(-3, -2)
+    else:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if lead:
+        return x, _lib.I64x3(*str_[:3]), out, _lib.I64x3(*out.stride()[:3])
+    out_str = out.stride()
+    return (x, _lib.I64x3(0, str_[0], str_[1]), out, _lib.I64x3(0, out_str[0], out_str[1]))
+
+
+_NO_STRIDES = _lib.I64x3(0, 0, 0)
 
 
 def _turn(q, k, positions, frequencies, interleaved, scale, inverse):
-    """The fused kernel on (b, h, t, d) rows, k None or of the same b, t, d."""
-    desc = _lib.NxaRotaryDesc()
-    desc.B, desc.H, desc.T, desc.D = q.shape
-    desc.R = 2 * frequencies.shape[0]
-    desc.io_dtype = _IO_DTYPES[q.dtype]
-    desc.interleaved, desc.inverse = interleaved, inverse
-    desc.pos64 = positions.dtype == torch.int64
-    desc.scale = scale
-    desc.pos_str[:] = positions.stride()
-    # (rows are read in place from any strides but those of a row's elements)
-    q = q if q.stride(3) == 1 else q.contiguous()
-    q_out = _empty_rows(q)
-    desc.q_str[:] = q.stride()[:3]
-    desc.q_out_str[:] = q_out.stride()[:3]
-    k_out = None
+    """The fused kernel on (h, t, d) or (b, h, t, d) rows, k None or of the same
+    b, t, d; positions of the batch and token axes."""
+    q, q_str, q_out, q_out_str = _rows(q)
+    k_out, hk, k_str, k_out_str = None, 0, _NO_STRIDES, _NO_STRIDES
     if k is not None:
-        k = k if k.stride(3) == 1 else k.contiguous()
-        k_out = _empty_rows(k)
-        desc.Hk = k.shape[1]
-        desc.k_str[:] = k.stride()[:3]
-        desc.k_out_str[:] = k_out.stride()[:3]
+        k, k_str, k_out, k_out_str = _rows(k)
+        hk = k.shape[-3]
+    *lead, h, t, d = q.shape
+    pos_str = positions.stride()
+    desc = _lib.NxaRotaryDesc(
+        lead[0] if lead else 1, t, h, hk, d, 2 * frequencies.shape[0], _IO_DTYPES[q.dtype],
+        interleaved, inverse, positions.dtype == torch.int64, scale,
+        _lib.I64x2(pos_str[0] if lead else 0, pos_str[-1]), q_str, k_str, q_out_str, k_out_str,
+    )
     with _on(q.device):
         _lib.check(
             _lib.lib().nxa_rotary(
@@ -256,26 +265,26 @@ class _RotaryHip(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, frequencies, interleaved, scale, inverse):
         ctx.set_materialize_grads(False)
-        ctx.args = (interleaved, scale)
-        ctx.inverse = inverse
+        ctx.args = (interleaved, scale, not inverse)
         ctx.save_for_backward(positions, frequencies)
         return _turn(q, k, positions, frequencies, interleaved, scale, inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        positions, frequencies = ctx.saved_tensors
-        for x in (dq, dk):
-            if x is not None:
-                _no_tangent_back('rotary_embed', x)
-        args = (positions, frequencies, *ctx.args, not ctx.inverse)
+        args = (*ctx.saved_tensors, *ctx.args)
         if not ctx.needs_input_grad[0]:
             dq = None
         if not ctx.needs_input_grad[1]:
             dk = None
-        if dq is None and dk is not None:
-            dk, _ = _RotaryHip.apply(dk, None, *args)
-        elif dq is not None:
-            dq, dk = _RotaryHip.apply(dq, dk, *args)
+        for x in (dq, dk):
+            if x is not None:
+                _no_tangent_back('rotary_embed', x)
+        # (a graph of the gradients themselves where one is asked for)
+        turn = _RotaryHip.apply if torch.is_grad_enabled() else _turn
+        if dq is not None:
+            dq, dk = turn(dq, dk, *args)
+        elif dk is not None:
+            dk, _ = turn(dk, None, *args)
         return dq, dk, None, None, None, None, None
 
 
@@ -284,33 +293,35 @@ def _rotary_hip(q, k, positions, frequencies, interleaved, scale):
         raise HipNotTileable(
             f'fused rotary positions support bfloat16, float16 and float32; got {q.dtype}.'
         )
-    if q.shape[-1] > _MAX_ROTARY_DIM:
+    shape = q.shape
+    if shape[-1] > _MAX_ROTARY_DIM:
         raise HipNotTileable(
-            f'fused rotary positions take head dims up to {_MAX_ROTARY_DIM}; got {q.shape[-1]}.'
+            f'fused rotary positions take head dims up to {_MAX_ROTARY_DIM}; got {shape[-1]}.'
         )
     if _has_tangent(q, k):
         raise HipNotTileable('fused rotary positions have no forward-mode derivative.')
     _lib.lib()  # a missing library is an error here, not a fallback
-    lead, t = q.shape[:-3], q.shape[-2]
-    if q.ndim == 3:
-        q4, k4 = q[None], None if k is None else k[None]
-    elif q.ndim == 4:
-        q4, k4 = q, k
-    else:
-        q4 = q.reshape(-1, *q.shape[-3:])
-        k4 = None if k is None else k.reshape(-1, *k.shape[-3:])
-    positions = positions.expand(*lead, t).reshape(q4.shape[0], t)
+    ndim = len(shape)
+    if ndim > 3:
+        positions = positions.expand(*shape[:-3], shape[-2])
+    elif positions.ndim != 1:
+        positions = positions.reshape(-1)
+    k_shape = None if k is None else k.shape
+    if ndim > 4:
+        q = q.reshape(-1, *shape[-3:])
+        k = None if k is None else k.reshape(-1, *k_shape[-3:])
+        positions = positions.reshape(-1, shape[-2])
     if frequencies.dtype != torch.float64 or not frequencies.is_contiguous():
         frequencies = frequencies.double().contiguous()
     args = (positions, frequencies, bool(interleaved), float(scale), False)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        q4, k4 = _RotaryHip.apply(q4, k4, *args)
+        q, k = _RotaryHip.apply(q, k, *args)
     else:
-        q4, k4 = _turn(q4, k4, *args)
-    if q.ndim == 4:
-        return q4, k4
-    return q4.view(q.shape) if q.ndim == 3 else q4.reshape(q.shape), (
-        None if k is None else k4.view(k.shape) if q.ndim == 3 else k4.reshape(k.shape))
+        q, k = _turn(q, k, *args)
+    if ndim > 4:
+        q = q.reshape(shape)
+        k = None if k is None else k.reshape(k_shape)
+    return q, k
 
 
 def rotary_embed(

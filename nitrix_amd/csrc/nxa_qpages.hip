@@ -1,12 +1,17 @@
 // New tokens into quantised pages and back (nxa_quant.h).
 //
-// A wave a token: it finds the token's sequence and page once and then takes the
-// rows of all heads, keys and values, LPR lanes of eight elements a row and 64 /
-// LPR rows at a time.  Bound by HBM: a row is read (written) once in the model's
-// type and written (read) once in codes.
+// A block takes kTokens tokens: a thread each finds a token's sequence and page, and
+// then a wave takes one, LPR lanes of eight elements a row (a head's key or value),
+// 64 / LPR rows at a time.  Bound by HBM: a row is read (written) once in the model's
+// type and written (read) once in codes.  What hides its latency is waves, eight a
+// SIMD: with two or four such steps loaded together a wave held 99 or more registers
+// in place of 53, and writing 16384 tokens of 8 heads of 128 in bf16 into 4 bits took
+// 39 and 47 us in place of 32; 16 tokens a block took 35, and 1024 tokens in 8 bits 13
+// in place of 9.  These 32 us are 5.3 TB/s, 17 to read them back 10 (much of it out of
+// caches), 56 for 65,664 tokens 6.1.
 //
 // Codes are rounded as the exact quotient would be, ties to even, so that they do
-// not depend on how it is taken (exact_code).
+// not depend on how it is taken (exact_code; near_code where it is as good).
 #include "nxa_quant.h"
 
 #include <type_traits>
@@ -31,29 +36,82 @@ __device__ __forceinline__ Eight<T> load_eight(const T* at) {
   return r;
 }
 
-// Sequence and position of token t (whole wave; uniform); false: of no sequence
-// or outside the table.
-__device__ __forceinline__ bool quant_find(const QuantMoveParams& p, int64_t t, int& s,
-                                           int64_t& pos) {
-  const int lane = threadIdx.x & 63;
-  s = (int)t;
-  pos = 0;
+// Past the caches: 65,664 tokens of 8 heads of 128 read back in 56 us in place of 95.
+template <typename T>
+__device__ __forceinline__ void store_eight(T* at, const Eight<T>& y) {
+  const u32x4* src = reinterpret_cast<const u32x4*>(&y);
+  u32x4* dst = reinterpret_cast<u32x4*>(at);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(y) / 16; ++i) __builtin_nontemporal_store(src[i], dst + i);
+}
+
+constexpr int kTokens = 4;  // of a block, a wave each
+
+// Where the tokens of a block are: a page (none: -1) and a slot.  Threads 0 ..
+// kTokens - 1, a token each; `ends` (LDS) holds the offsets where these are few.
+constexpr int kFewOffsets = 1024;
+struct Place {
+  int page, slot;
+};
+__device__ __forceinline__ Place quant_place(const QuantMoveParams& p, int64_t t, const int* ends) {
+  Place at = {-1, 0};
+  if (t >= p.T) return at;
+  int64_t s = t, pos = 0;
   if (p.offsets) {
+    const bool few = p.B < kFewOffsets;
     int lo = 0, hi = p.B + 1;  // last s with offsets[s] <= t
     while (hi - lo > 1) {
-      const int step = (hi - lo + 63) / 64;
-      const int x = lo + lane * step;
-      const int cnt = (int)__popcll(__ballot(x < hi && p.offsets[x] <= t));
-      if (cnt == 0) break;  // before the first sequence
-      lo += (cnt - 1) * step;
-      hi = min(lo + step, hi);
+      const int mid = (lo + hi) >> 1;
+      if ((few ? ends[mid] : p.offsets[mid]) <= t) lo = mid;
+      else hi = mid;
     }
-    s = __builtin_amdgcn_readfirstlane(lo);
-    if (s >= p.B || p.offsets[s] > t) return false;
-    pos = t - p.offsets[s];
+    const int start = few ? ends[lo] : p.offsets[lo];
+    if (lo >= p.B || start > t) return at;
+    s = lo;
+    pos = t - start;
   }
   pos += p.starts[s];
-  return pos >= 0 && pos < (int64_t)p.M * p.pool.PS;
+  if (pos < 0 || pos >= (int64_t)p.M * p.pool.PS) return at;
+  const int page = p.table[s * p.table_rs + pos / p.pool.PS];
+  if ((unsigned)page >= (unsigned)p.pool.P) return at;
+  at.page = page;
+  at.slot = (int)(pos % p.pool.PS);
+  return at;
+}
+__device__ __forceinline__ void quant_places(const QuantMoveParams& p, int64_t t0, Place* place) {
+  __shared__ int ends[kFewOffsets];
+  if (p.offsets && p.B < kFewOffsets) {
+    for (int i = threadIdx.x; i <= p.B; i += 64 * kTokens) ends[i] = p.offsets[i];
+    __syncthreads();
+  }
+  if (threadIdx.x < kTokens) place[threadIdx.x] = quant_place(p, t0 + threadIdx.x, ends);
+  __syncthreads();
+}
+
+// Reductions over the LPR lanes of a row; every lane has the result.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true);
+}
+template <int LPR, typename F>
+__device__ __forceinline__ uint32_t row_reduce(uint32_t x, F&& f) {
+  x = f(x, dpp<0xb1>(x));   // lanes 1, 0, 3, 2 of each four
+  x = f(x, dpp<0x4e>(x));   // 2, 3, 0, 1
+  x = f(x, dpp<0x141>(x));  // each eight mirrored
+  if constexpr (LPR >= 16) x = f(x, dpp<0x140>(x));  // each sixteen
+  if constexpr (LPR >= 32) x = f(x, (uint32_t)__shfl_xor((int)x, 16, 64));
+  return x;
+}
+// (as instructions: fminf would first quiet each number, which could be a NaN)
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 // rint((x - z) / s) of the exact quotient, given s and (roughly) 1 / s; zero
@@ -74,131 +132,197 @@ __device__ __forceinline__ float exact_code(float x, float z, float s, float inv
   return s > 0.f ? n : 0.f;
 }
 
+// The same where x - z is exact in fp32 and s has few bits (16-bit types, x and z
+// not too far apart): the quotient by the reciprocal, corrected by its remainder, is
+// the exact one rounded to fp32 (inv is 1 / s rounded).  A border n + 1/2 is an fp32
+// number, and (n + 1/2) s, of 20 bits or fewer, stands in the places of x - z: one
+// that is not a border differs from it by a place of x - z or more, more than half a
+// place of the quotient, and is not rounded to it.
+__device__ __forceinline__ float near_code(float diff, float s, float inv) {
+  const float q = diff * inv;
+  return __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q, s, diff), inv, q));
+}
+
 }  // namespace
 
+// Eight elements of a row of keys or values into codes at dst, by LPR lanes (those
+// behind the row's end not `mine`); the row's scale and minimum at sc.
 template <typename T, int BITS, int LPR>
-__global__ __launch_bounds__(256) void quant_write_kernel(const QuantMoveParams p) {
+__device__ __forceinline__ void write_row(const Eight<T>& y, bool mine, bool first, char* dst,
+                                          T* sc) {
   constexpr int TOP = (1 << BITS) - 1;
-  const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= p.T) return;
-  int s;
-  int64_t pos;
-  if (!quant_find(p, t, s, pos)) return;
-  const QuantPool& pool = p.pool;
-  const int page = p.table[s * p.table_rs + pos / pool.PS];
-  if ((unsigned)page >= (unsigned)pool.P) return;
-  const int slot = (int)(pos % pool.PS);
-  const int sub = lane % LPR, d = 8 * sub;
-  for (int r = lane / LPR; r < 2 * pool.Hk; r += 64 / LPR) {
-    const int which = r >= pool.Hk, h = which ? r - pool.Hk : r;
-    const int D = which ? pool.Dv : pool.D;
-    const T* src = which ? (const T*)p.vs + h * p.vs_str[0] + t * p.vs_str[1]
-                         : (const T*)p.ks + h * p.ks_str[0] + t * p.ks_str[1];
-    float x[8], lo = INFINITY, hi = -INFINITY, bad = 0.f;
-    if (d < D) {
-      const Eight<T> y = load_eight(src + d);
+  // x - z is exact where neither is 2^FAR times the other or more: 24 places less
+  // the 8 of bf16 or the 11 of fp16.
+  constexpr int FAR = std::is_same<T, f16>::value ? 12 : 15;
+  constexpr float kFar = 1 << FAR;
+  float x[8], lo = INFINITY, hi = -INFINITY;
+  uint32_t twice[8];  // twice the bits of |x|, less one (0: the most)
+  uint32_t least = 0xffffffffu, most = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = (float)y.x[e];
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-        bad = __builtin_fmaf(x[e], 0.f, bad);  // NaN where x is NaN or infinite
-      }
-    }
+  for (int e = 0; e < 8; ++e) {
+    x[e] = (float)y.x[e];
+    twice[e] = 2u * __float_as_uint(x[e]) - 1u;
+  }
 #pragma unroll
-    for (int m = 1; m < LPR; m *= 2) {
-      lo = fminf(lo, __shfl_xor(lo, m, 64));
-      hi = fmaxf(hi, __shfl_xor(hi, m, 64));
-      bad += __shfl_xor(bad, m, 64);
-    }
-    // (a row of NaN, infinity or a range past the type's reads back as NaN)
-    const float range = hi - lo;
-    bad = __builtin_fmaf(range, 0.f, bad);
-    const T zt = (T)(lo + bad), st = (T)(range * (1.f / TOP) + bad);
-    const float z = (float)zt;
-    float sf = (float)st;
-    // (quotients of tiny scales are taken 2^96 times larger)
-    const float up = sf < 0x1p-90f ? 0x1p96f : 1.f;
-    sf *= up;
-    const float inv = sf > 0.f ? 1.f / sf : 0.f;
-    uint32_t c[8];
+  for (int e = 0; e < 8; e += 2) {
+    lo = min3(lo, x[e], x[e + 1]);
+    hi = max3(hi, x[e], x[e + 1]);
+    least = min(least, min(twice[e], twice[e + 1]));
+    most = max(most, max(twice[e] + 1u, twice[e + 1] + 1u));
+  }
+  const float far = fmaxf(__builtin_fabsf(lo), __builtin_fabsf(hi));
+  if (!mine) lo = INFINITY, hi = -INFINITY, most = 0;
+  lo = __uint_as_float(row_reduce<LPR>(__float_as_uint(lo), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(min3(__uint_as_float(a), __uint_as_float(b), INFINITY));
+  }));
+  hi = __uint_as_float(row_reduce<LPR>(__float_as_uint(hi), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(max3(__uint_as_float(a), __uint_as_float(b), -INFINITY));
+  }));
+  most = row_reduce<LPR>(most, [](uint32_t a, uint32_t b) { return max(a, b); });
+  // (a row of NaN, infinity or a range past the type's reads back as NaN)
+  const float range = hi - lo;
+  const bool bad = most >= 0xff000000u || !(range < INFINITY);
+  const T zt = (T)(bad ? NAN : lo), st = (T)(bad ? NAN : range * (1.f / TOP));
+  const float z = (float)zt;
+  float sf = (float)st;
+  // (quotients of tiny scales are taken 2^96 times larger)
+  const float up = sf < 0x1p-90f ? 0x1p96f : 1.f;
+  sf *= up;
+  const float inv = sf > 0.f ? 1.f / sf : 0.f;
+  float n[8];
+  const float az = __builtin_fabsf(z);
+  const bool near = sizeof(T) == 2 && up == 1.f &&
+                    __uint_as_float((least + 1u) >> 1) >= az * (1.f / kFar) &&
+                    (far <= az * kFar || z == 0.f);
+  if (__builtin_expect(__any(!near && mine), 0)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = (uint32_t)fminf(fmaxf(exact_code(x[e] * up, z * up, sf, inv), 0.f), (float)TOP);
-    if (d < D) {
-      char* dst = which ? (char*)pool.v + page * pool.v_str[0] + h * pool.v_str[1]
-                        : (char*)pool.k + page * pool.k_str[0] + h * pool.k_str[1];
-      dst += (int64_t)slot * (D * BITS / 8) + d * BITS / 8;
-      if constexpr (BITS == 4) {
-        uint32_t w = 0;
+    for (int e = 0; e < 8; ++e) n[e] = exact_code(x[e] * up, z * up, sf, inv);
+  } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w |= c[e] << (4 * e);
-        *reinterpret_cast<uint32_t*>(dst) = w;
-      } else {
-        uint32_t w[2] = {0, 0};
+    for (int e = 0; e < 8; ++e) n[e] = near_code(x[e] - z, sf, inv);
+  }
+  // (a scale of zero or NaN gives 0, what is below the stored minimum too)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e / 4] |= c[e] << (8 * (e % 4));
-        *reinterpret_cast<uint32_t*>(dst) = w[0];
-        *reinterpret_cast<uint32_t*>(dst + 4) = w[1];
-      }
-      if (sub == 0) {
-        T* sc = (T*)pool.sc + page * pool.sc_str[0] + h * pool.sc_str[1] + 4 * (int64_t)slot;
-        sc[2 * which] = st;
-        sc[2 * which + 1] = zt;
-      }
-    }
+  for (int e = 0; e < 8; ++e) n[e] = fminf(fmaxf(n[e], 0.f), (float)TOP);
+  if (!mine) return;
+  // Codes put together as whole numbers that fp32 holds: four of 4 bits, two of 8.
+  auto pair = [&](int e) { return __builtin_fmaf(n[e + 1], (float)(TOP + 1), n[e]); };
+  if constexpr (BITS == 4) {
+    const float a = __builtin_fmaf(pair(2), 256.f, pair(0)), b = __builtin_fmaf(pair(6), 256.f, pair(4));
+    *reinterpret_cast<uint32_t*>(dst) = (uint32_t)a | (uint32_t)b << 16;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      reinterpret_cast<uint32_t*>(dst)[i] =
+          (uint32_t)pair(4 * i) | (uint32_t)pair(4 * i + 2) << 16;
+  }
+  if (first) {
+    struct alignas(2 * sizeof(T)) Scale {
+      T s, z;
+    };
+    *reinterpret_cast<Scale*>(sc) = {st, zt};
   }
 }
 
 template <typename T, int BITS, int LPR>
-__global__ __launch_bounds__(256) void quant_read_kernel(const QuantMoveParams p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= p.T) return;
+__global__ __launch_bounds__(64 * kTokens) void quant_write_kernel(const QuantMoveParams p) {
+  constexpr int RG = 64 / LPR;
+  __shared__ Place place[kTokens];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t t = (int64_t)blockIdx.x * kTokens + wave;
   const QuantPool& pool = p.pool;
-  int s, page = -1, slot = 0;
-  int64_t pos;
-  if (quant_find(p, t, s, pos)) {
-    page = p.table[s * p.table_rs + pos / pool.PS];
-    slot = (int)(pos % pool.PS);
+  const int sub = lane % LPR, d = 8 * sub, h1 = lane / LPR;
+  const bool in_k = d < pool.D, in_v = d < pool.Dv;
+  const T* ks = (const T*)p.ks + h1 * p.ks_str[0] + d;
+  const T* vs = (const T*)p.vs + h1 * p.vs_str[0] + d;
+  char* kd = (char*)pool.k + h1 * pool.k_str[1] + d * BITS / 8;
+  char* vd = (char*)pool.v + h1 * pool.v_str[1] + d * BITS / 8;
+  T* sd = (T*)pool.sc + h1 * pool.sc_str[1];
+  quant_places(p, t - wave, place);
+  if (t >= p.T) return;
+  const int page = __builtin_amdgcn_readfirstlane(place[wave].page);
+  const int slot = __builtin_amdgcn_readfirstlane(place[wave].slot);
+  if (page < 0) return;
+  const int64_t ko = page * pool.k_str[0] + (int64_t)slot * (pool.D * BITS / 8);
+  const int64_t vo = page * pool.v_str[0] + (int64_t)slot * (pool.Dv * BITS / 8);
+  const int64_t so = page * pool.sc_str[0] + 4 * (int64_t)slot;
+  const int64_t kt = t * p.ks_str[1], vt = t * p.vs_str[1];
+  for (int h = 0; h + h1 < pool.Hk; h += RG) {  // (this lane's head is h + h1)
+    Eight<T> k = {}, v = {};
+    if (in_k) k = load_eight(ks + kt + h * p.ks_str[0]);
+    if (in_v) v = load_eight(vs + vt + h * p.vs_str[0]);
+    T* sc = sd + so + h * pool.sc_str[1];
+    write_row<T, BITS, LPR>(k, in_k, sub == 0, kd + ko + h * pool.k_str[1], sc);
+    write_row<T, BITS, LPR>(v, in_v, sub == 0, vd + vo + h * pool.v_str[1], sc + 2);
   }
-  const bool held = (unsigned)page < (unsigned)pool.P;
-  const int sub = lane % LPR, d = 8 * sub;
-  for (int r = lane / LPR; r < 2 * pool.Hk; r += 64 / LPR) {
-    const int which = r >= pool.Hk, h = which ? r - pool.Hk : r;
-    const int D = which ? pool.Dv : pool.D;
-    if (d >= D) continue;
+}
+
+// A lane's eight codes and its row's scale and minimum.
+template <typename T, int BITS>
+struct HeldRow {
+  uint32_t w[BITS / 4];
+  struct alignas(2 * sizeof(T)) Scale {
+    T s, z;
+  } sc;
+  __device__ __forceinline__ void load(const char* src, const T* at) {
+#pragma unroll
+    for (int x = 0; x < BITS / 4; ++x) w[x] = reinterpret_cast<const uint32_t*>(src)[x];
+    sc = *reinterpret_cast<const Scale*>(at);
+  }
+  __device__ __forceinline__ Eight<T> values() const {
+    const float a = (float)sc.s, z = (float)sc.z;
     Eight<T> y;
-    if (held) {
-      const char* src = which ? (const char*)pool.v + page * pool.v_str[0] + h * pool.v_str[1]
-                              : (const char*)pool.k + page * pool.k_str[0] + h * pool.k_str[1];
-      src += (int64_t)slot * (D * BITS / 8) + d * BITS / 8;
-      const T* sc =
-          (const T*)pool.sc + page * pool.sc_str[0] + h * pool.sc_str[1] + 4 * (int64_t)slot;
-      const float a = (float)sc[2 * which], z = (float)sc[2 * which + 1];
-      const uint32_t w0 = *reinterpret_cast<const uint32_t*>(src);
-      const uint32_t w1 = BITS == 8 ? *reinterpret_cast<const uint32_t*>(src + 4) : 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t c = BITS == 4 ? w0 >> (4 * e) & 15 : (e < 4 ? w0 : w1) >> (8 * (e % 4)) & 255;
-        y.x[e] = (T)__builtin_fmaf((float)c, a, z);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y.x[e] = (T)0.f;
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t c = BITS == 4 ? w[0] >> (4 * e) & 15 : w[e / 4 % (BITS / 4)] >> (8 * (e % 4)) & 255;
+      y.x[e] = (T)__builtin_fmaf((float)c, a, z);
     }
-    T* dst = which ? (T*)p.vs + h * p.vs_str[0] + t * p.vs_str[1]
-                   : (T*)p.ks + h * p.ks_str[0] + t * p.ks_str[1];
-    *reinterpret_cast<Eight<T>*>(dst + d) = y;
+    return y;
+  }
+};
+
+template <typename T, int BITS, int LPR>
+__global__ __launch_bounds__(64 * kTokens) void quant_read_kernel(const QuantMoveParams p) {
+  constexpr int RG = 64 / LPR;
+  __shared__ Place place[kTokens];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t t = (int64_t)blockIdx.x * kTokens + wave;
+  const QuantPool& pool = p.pool;
+  const int sub = lane % LPR, d = 8 * sub, h1 = lane / LPR;
+  const bool in_k = d < pool.D, in_v = d < pool.Dv;
+  T* kd = (T*)p.ks + h1 * p.ks_str[0] + d;
+  T* vd = (T*)p.vs + h1 * p.vs_str[0] + d;
+  const char* ks = (const char*)pool.k + h1 * pool.k_str[1] + d * BITS / 8;
+  const char* vs = (const char*)pool.v + h1 * pool.v_str[1] + d * BITS / 8;
+  const T* ss = (const T*)pool.sc + h1 * pool.sc_str[1];
+  quant_places(p, t - wave, place);
+  if (t >= p.T) return;
+  const int page = __builtin_amdgcn_readfirstlane(place[wave].page);
+  const int slot = __builtin_amdgcn_readfirstlane(place[wave].slot);
+  const int64_t ko = page * pool.k_str[0] + (int64_t)slot * (pool.D * BITS / 8);
+  const int64_t vo = page * pool.v_str[0] + (int64_t)slot * (pool.Dv * BITS / 8);
+  const int64_t so = page * pool.sc_str[0] + 4 * (int64_t)slot;
+  const int64_t kt = t * p.ks_str[1], vt = t * p.vs_str[1];
+  for (int h = 0; h + h1 < pool.Hk; h += RG) {  // (this lane's head is h + h1)
+    HeldRow<T, BITS> k = {}, v = {};            // (zero where there is no page)
+    if (page >= 0) {
+      const T* at = ss + so + h * pool.sc_str[1];
+      if (in_k) k.load(ks + ko + h * pool.k_str[1], at);
+      if (in_v) v.load(vs + vo + h * pool.v_str[1], at + 2);
+    }
+    if (in_k) store_eight(kd + kt + h * p.ks_str[0], k.values());
+    if (in_v) store_eight(vd + vt + h * p.vs_str[0], v.values());
   }
 }
 
 template <typename T, int BITS, bool WRITE>
 static void launch_move_t(const QuantMoveParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)((p.T + 3) / 4)), block(256);
   const int most = p.pool.D > p.pool.Dv ? p.pool.D : p.pool.Dv;
   auto go = [&](auto lpr) {
     constexpr int LPR = decltype(lpr)::value;
+    const dim3 grid((unsigned)((p.T + kTokens - 1) / kTokens)), block(64 * kTokens);
     if constexpr (WRITE)
       hipLaunchKernelGGL((quant_write_kernel<T, BITS, LPR>), grid, block, 0, stream, p);
     else

@@ -16,14 +16,18 @@
 //    dword and those of eight two such halves, the upper one scaled by 16 in the
 //    product.  q is the sum of two (fp16: three) fp8 numbers, scaled so that its
 //    largest element is in 2^7 .. 2^8: exact down to 2^-10 (2^-7) of that, off by at
-//    most 2^-17 of it below.  fp32: codes in the mantissa of 16 as bf16 (16 + c), q
-//    as three bf16 numbers (exact).
+//    most 2^-17 of it below.
 //  * V: codes in the mantissa of an fp16 64 (in bits 4 .. 7, where an element's odd
 //    codes are already) or 1024 (bits 0 .. 3, or 0 .. 7).  What is added to them is
 //    taken off at the end, by a product of ones with the very P s' that the other
-//    products saw.  P s' is one fp16 number (bf16: off by 2^-12), two (fp16: 2^-23)
-//    or three (fp32).  fp16's range is short, so the reference that P is relative to
-//    follows the largest scale as well as the largest score.
+//    products saw.  P s' is one fp16 number (bf16: off by 2^-12) or two (fp16: 2^-23).
+//    fp16's range is short, so the reference that P is relative to follows the largest
+//    scale as well as the largest score.
+//  * fp32: what is added to the codes, and their minima, would cost digits: the values
+//    of a long row nearly cancel, to a root of its length, while those sums do not (8192
+//    tokens in 8 bits were off by 1.5e-5 of the output, now 4e-7).  So K's and V's codes are
+//    fp16 numbers from -8 or -128 on, one packed addition more, what they are counted
+//    from is (s 8 + z) or (s 128 + z), and q and P s' are three fp16 numbers each.
 //
 // The blocks share the work as in nxa_paged.hip (units of 128 tokens, pieces of
 // a row joined by its second kernel).  A step of a wave is 32 tokens, two halves
@@ -58,6 +62,7 @@ struct QuantStep {
   static constexpr int NS = ES;                     // dwords of a token's scales: 4 ES / 4
   static constexpr int QT = FP8 && !F16 ? 2 : 3;    // terms of q
   static constexpr int PT = !FP8 ? 3 : F16 ? 2 : 1;  // of P s'
+  static constexpr float MID = FP8 ? 0.f : BITS == 4 ? 8.f : 128.f;  // codes count from it
   // What stands in for 0 in V's even and odd columns.
   static constexpr float EVEN = BITS == 8 || (FP8 && !F16) ? 1024.f : 64.f;
   static constexpr float ODD = BITS == 8 ? 1024.f : 64.f;
@@ -95,10 +100,6 @@ struct HalfRegs {
   Loaded<R::NS> s[4];
 };
 
-__device__ __forceinline__ f32x4 mma_bf16(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 __device__ __forceinline__ f32x4 mma_f16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -109,12 +110,7 @@ __device__ __forceinline__ f32x4 mma_fp8(i32x8 a, i32x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, UP ? 131 : 127, 0, 127);
 }
 
-// Two numbers as bf16 or fp16, the first in the low half.
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 r = {(bf16)a, (bf16)b};
-  return __builtin_bit_cast(uint32_t, r);
-}
+// Two numbers as fp16, the first in the low half.
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
   const f16x2 r = {(f16)a, (f16)b};
@@ -129,44 +125,46 @@ __device__ __forceinline__ float high_f16(uint32_t w) {
   return (float)__builtin_bit_cast(f16, (uint16_t)(w >> 16));
 }
 
-// Whole bytes of a word as floats.
-template <int B>
-__device__ __forceinline__ float byte_of(uint32_t w) {
-  return (float)(w >> (8 * B) & 255u);
-}
-
 // Constants of the codes' masks, kept in registers of both kinds, so that an and
 // and an or are one operation (two constants of it cannot both be literals).
 struct CodeBits {
-  uint32_t low, high, mid, k1024, k64, k16;
+  uint32_t low, high, k1024, k64, from64, from1024;
   __device__ __forceinline__ CodeBits() {
     asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
-    asm("s_mov_b32 %0, 0x00780078" : "=s"(mid));
     asm("v_mov_b32 %0, 0x64006400" : "=v"(k1024));
     asm("v_mov_b32 %0, 0x54005400" : "=v"(k64));
-    asm("v_mov_b32 %0, 0x41804180" : "=v"(k16));
+    asm("s_mov_b32 %0, 0xd480d480" : "=s"(from64));    // -(64 + 8) twice, as fp16
+    asm("s_mov_b32 %0, 0xe480e480" : "=s"(from1024));  // -(1024 + 128)
   }
 };
 
-// 16 + the nibbles at bits SH .. SH + 3 and SH + 16 .. SH + 19, as bf16 (a
-// mantissa's unit is 2^-3 there).
-template <int SH>
-__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w, const CodeBits& cb) {
-  const uint32_t x = SH < 3 ? w << (3 - SH) : w >> (SH - 3);
-  return (x & cb.mid) | cb.k16;
+// Two fp16 sums.
+__device__ __forceinline__ uint32_t add_f16(uint32_t a, uint32_t b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, a) + __builtin_bit_cast(f16x2, b));
 }
-// Product operand j of a lane's codes of one key, bf16: eight of them.
+// The nibbles at bits SH .. SH + 3 and SH + 16 .. SH + 19 less 8, as fp16.
+template <int SH>
+__device__ __forceinline__ uint32_t nibbles_f16(uint32_t w, const CodeBits& cb) {
+  const uint32_t x = SH < 4 ? w << (4 - SH) : w >> (SH - 4);
+  return add_f16((x & cb.high) | cb.k64, cb.from64);
+}
+// Two bytes (of a word, as `sel` picks them into the low ones) less 128, as fp16.
+__device__ __forceinline__ uint32_t bytes_f16(uint32_t w, uint32_t sel, const CodeBits& cb) {
+  return add_f16(__builtin_amdgcn_perm(0u, w, sel) | cb.k1024, cb.from1024);
+}
+// Product operand j of a lane's codes of one key, fp16: eight of them.
 template <int BITS, int N>
-__device__ __forceinline__ u32x4 key_bf16(const Loaded<N>& k, int j, const CodeBits& cb) {
+__device__ __forceinline__ u32x4 key_f16(const Loaded<N>& k, int j, const CodeBits& cb) {
   if constexpr (BITS == 4) {
     const uint32_t w = k.at(j);
-    return u32x4{nibbles_bf16<0>(w, cb), nibbles_bf16<4>(w, cb), nibbles_bf16<8>(w, cb),
-                 nibbles_bf16<12>(w, cb)};
+    return u32x4{nibbles_f16<0>(w, cb), nibbles_f16<4>(w, cb), nibbles_f16<8>(w, cb),
+                 nibbles_f16<12>(w, cb)};
   } else {
     const uint32_t a = k.at(2 * j), b = k.at(2 * j + 1);
-    return u32x4{pack_bf16(byte_of<0>(a), byte_of<1>(a)), pack_bf16(byte_of<2>(a), byte_of<3>(a)),
-                 pack_bf16(byte_of<0>(b), byte_of<1>(b)), pack_bf16(byte_of<2>(b), byte_of<3>(b))};
+    return u32x4{bytes_f16(a, 0x0c010c00u, cb), bytes_f16(a, 0x0c030c02u, cb),
+                 bytes_f16(b, 0x0c010c00u, cb), bytes_f16(b, 0x0c030c02u, cb)};
   }
 }
 // Operand j, fp8: 32 codes of four bits, or the lower or upper halves of as many of
@@ -190,6 +188,12 @@ __device__ constexpr int key_order(int e) {
   return FP8 ? 2 * (e & 3) + (e >> 2) : (e >> 1) + 4 * (e & 1);
 }
 
+// What a row's codes, as a product has them, count from.
+template <typename T, int BITS>
+__device__ __forceinline__ float from_mid(float s, float z) {
+  using R = QuantStep<T, 16, BITS>;
+  return R::MID == 0.f ? z : __builtin_fmaf(s, R::MID, z);
+}
 // Scales of a token: fields k's scale and minimum, v's.
 template <typename T, int N>
 __device__ __forceinline__ float scale_field(const Loaded<N>& s, int f) {
@@ -403,15 +407,17 @@ qpaged_kernel(const QuantPagedParams p) {
       qsum += xor16(qsum);
       qsum += shfl_xor32(qsum);
       sl = __builtin_fabsf(p.scale_log2);
+      most = fmaxf(most, xor16(most));
+      most = fmaxf(most, shfl_xor32(most));
+      // q times 2^up, its largest element in 2^7 .. 2^8 (fp32: 2^13 .. 2^14, so that
+      // three fp16 numbers hold it down to 2^-24), and scores in units of 2^(9 - up)
+      // (codes are c 2^-9 as fp8; 2^-up).  NaN and infinity of q leave NaN.
+      const int up = min((R::FP8 ? 8 : 14) - __builtin_amdgcn_frexp_expf(most), 100);
+      const float by = most > 0.f ? __builtin_ldexpf(1.f, up) : 1.f;
+      const float unit = (R::FP8 ? 512.f : 1.f) / by;
+      qsum = qsum / unit + (most - most) + (qsum - qsum);
+      sl *= unit;
       if constexpr (R::FP8) {
-        most = fmaxf(most, xor16(most));
-        most = fmaxf(most, shfl_xor32(most));
-        // q times 2^up, its largest element in 2^7 .. 2^8, and scores in units of
-        // 2^(9 - up) (codes are c 2^-9).  NaN and infinity of q leave NaN.
-        const int up = min(8 - __builtin_amdgcn_frexp_expf(most), 100);
-        const float by = most > 0.f ? __builtin_ldexpf(1.f, up) : 1.f, unit = 512.f / by;
-        qsum = qsum / unit + (most - most) + (qsum - qsum);
-        sl *= unit;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -443,16 +449,16 @@ qpaged_kernel(const QuantPagedParams p) {
             for (int w = 0; w < 4; ++w) {
               float& a = x[8 * j + key_order<BITS, false>(2 * w)];
               float& o = x[8 * j + key_order<BITS, false>(2 * w + 1)];
-              const uint32_t r = pack_bf16(a, o);
+              if (t == 0) a *= by, o *= by;
+              const uint32_t r = pack_f16(a, o);
               qb[j][t][w] = r;
-              a -= low_of(r), o -= high_of(r);
+              a -= low_f16(r), o -= high_f16(r);
             }
       }
       // (one of zero is so small that all scores are zero, but for the -inf of a
       // token that takes no part)
       sl = fmaxf(sl, 0x1p-126f);
     }
-    const float s_init = R::FP8 || BITS == 8 ? 0.f : -16.f * qsum;
     f32x4 o[NF], ones_o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[f] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -471,7 +477,8 @@ qpaged_kernel(const QuantPagedParams p) {
       float vs[8], vz[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        s[h] = f32x4{s_init, s_init, s_init, s_init};
+        s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 rest = s[h];  // fp32: of all terms of q but the first
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           if constexpr (R::FP8) {
@@ -484,19 +491,24 @@ qpaged_kernel(const QuantPagedParams p) {
               for (int t = 0; t < QT; ++t) s[h] = mma_fp8<true>(a, qe[j][t], s[h]);
             }
           } else {
-            const u32x4 a = key_bf16<BITS>(r[h].k, j, cb);
+            const u32x4 a = key_f16<BITS>(r[h].k, j, cb);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) s[h] = mma_bf16(a, qb[j][t], s[h]);
+            for (int t = 1; t < QT; ++t) rest = mma_f16(a, qb[j][t], rest);
+            s[h] = mma_f16(a, qb[j][0], s[h]);
           }
         }
+        if constexpr (!R::FP8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[h][e] += rest[e];
         // Rows of the accumulator: tokens 4 g + e.
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           // (a scale of infinity makes its token NaN, whatever the signs)
-          const float ks = scale_field<T>(r[h].s[e], 0), kz = scale_field<T>(r[h].s[e], 1);
+          const float ks = scale_field<T>(r[h].s[e], 0);
+          const float kz = from_mid<T, BITS>(ks, scale_field<T>(r[h].s[e], 1));
           s[h][e] = __builtin_fmaf(s[h][e], ks, __builtin_fmaf(kz, qsum, ks * 0.f));
           vs[4 * h + e] = scale_field<T>(r[h].s[e], 2);
-          vz[4 * h + e] = scale_field<T>(r[h].s[e], 3);
+          vz[4 * h + e] = from_mid<T, BITS>(vs[4 * h + e], scale_field<T>(r[h].s[e], 3));
         }
       }
       if (__builtin_expect(((mine[0] ^ kFull) | (mine[1] ^ kFull)) != 0, 0)) {
@@ -549,6 +561,9 @@ qpaged_kernel(const QuantPagedParams p) {
         l += w;
         x[i] = w * vs[i];
         zs = __builtin_fmaf(w, vz[i], zs);
+        // (its first term is to be that of the rounded product, which the next is
+        // taken from; the compiler would round the exact one to fp16 for it)
+        if constexpr (PT > 1) asm("" : "+v"(x[i]));
       }
       u32x4 pf[PT];
 #pragma unroll
@@ -564,7 +579,7 @@ qpaged_kernel(const QuantPagedParams p) {
 #pragma unroll
         for (int t = 0; t < PT; ++t) acc = mma_f16(a, pf[t], acc);
       };
-      product(ones_o, u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
+      if constexpr (R::FP8) product(ones_o, u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
 #pragma unroll
       for (int w = 0; w < NVW; ++w)
 #pragma unroll
@@ -579,9 +594,11 @@ qpaged_kernel(const QuantPagedParams p) {
           for (int i = 0; i < 4; ++i) {
             if constexpr (BITS == 8) {
               a[i] = t[i] | cb.k1024;
+              if constexpr (!R::FP8) a[i] = add_f16(a[i], cb.from1024);
             } else {
               a[i] = R::EVEN == 1024.f ? (t[i] & cb.low) | cb.k1024 : (t[i] << 4 & cb.high) | cb.k64;
               d[i] = (t[i] & cb.high) | cb.k64;
+              if constexpr (!R::FP8) a[i] = add_f16(a[i], cb.from64), d[i] = add_f16(d[i], cb.from64);
             }
           }
           if constexpr (BITS == 8) {
@@ -675,7 +692,8 @@ qpaged_kernel(const QuantPagedParams p) {
       for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          mw[(4 * f + e) * 64] = __builtin_fmaf(f & 1 ? -R::ODD : -R::EVEN, ones_o[e], o[f][e]) + zs;
+          mw[(4 * f + e) * 64] =
+              (R::FP8 ? __builtin_fmaf(f & 1 ? -R::ODD : -R::EVEN, ones_o[e], o[f][e]) : o[f][e]) + zs;
       mw[(FIELDS - 2) * 64] = ref;
       mw[(FIELDS - 1) * 64] = l;
     }

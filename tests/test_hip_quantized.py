@@ -18,7 +18,9 @@ Attention's tolerance is a bound per element from the roundings the kernel makes
   the largest scale.
 * float32 sums, 2^-24 a step: a wave adds up 32 tokens a step, so n / 32 + 24 of
   them (with the join's) over codes with what stands in for zero, up to 1024, and
-  the same taken off; scores d + 8 steps, float32 over codes with 16.
+  the same taken off; scores d + 8 steps.  (For float32 operands, whose codes count
+  from their middle, that allows more than there is; ``test_float32_keeps_its_digits``
+  holds them to less.)
 * the output's rounding, u.
 """
 
@@ -283,6 +285,40 @@ def test_one_long_sequence(dtype, bits):
     q = _rand((1, 6, 64), DT[dtype], 5)
     out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32(lens), backend='hip')
     _check(out, q, pool, bits, table, lens, 0.125)
+
+
+@pytest.mark.parametrize('bits, lens, hk, d', [
+    (4, [700, 90, 333], 4, 64), (8, [8192, 5000], 2, 128), (4, [60000], 1, 64), (8, [2371, 197], 2, 256),
+    (4, [484, 1100], 3, 32),
+])
+def test_float32_keeps_its_digits(bits, lens, hk, d):
+    """Values of random sign nearly cancel in a long row, and an error that does not
+    (one of the codes' middle, of a single weight) stands out.  Each weight may be off
+    by its score's and its exponent's roundings: 3 d / 32 products' sums, half a step
+    of a score below 8 each, half a step of an exponent below 32, and 8 steps of 2^-24
+    for the exponential, the products behind it and the sums' share: (12 d / 128) 2^-22
+    + 2^-20 + 2^-21, at most 4.5 2^-20 (d = 256; below 128 3 2^-20).  These are as
+    random as the values, so that the whole output is off by no more than that share
+    of its norm."""
+    pool, table = _setup(torch.float32, lens, hk, d, d, 16, bits)
+    x = torch.randn(*pool[2].shape[:3], 2, 2, d, generator=torch.Generator().manual_seed(8))
+    top = (1 << bits) - 1
+    lo, hi = x[..., 0, :, :].amin(-1), x[..., 0, :, :].amax(-1)
+    pool[2][..., 0::2] = ((hi - lo) / top).to(pool[2])
+    pool[2][..., 1::2] = lo.to(pool[2])
+    codes = ((x[..., 0, :, :] - lo[..., None]) / (hi - lo)[..., None] * top).round().to(torch.uint8)
+    for i in range(2):
+        c = codes[..., i, :]
+        pool[i].copy_(c if bits == 8 else c[..., ::2] | c[..., 1::2] << 4)
+    q = _rand((len(lens), 2 * hk, d), torch.float32, 5)
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32(lens), backend='hip')
+    sc = _n64(pool[2])
+    k, v = (qplain.values(y.cpu().numpy(), sc, i, bits) for i, y in enumerate(pool[:2]))
+    want, _ = plain.attention(_n64(q), k, v, table, lens, 1 / math.sqrt(d))
+    for i in range(len(lens)):
+        for h in range(2 * hk):
+            off = np.linalg.norm(_n64(out[i, h]) - want[i, h]) / np.linalg.norm(want[i, h])
+            assert off <= (4.5 if d > 128 else 3) * 2.0 ** -20, (lens[i], h, off)
 
 
 def test_many_sequences():

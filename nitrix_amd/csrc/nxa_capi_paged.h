@@ -59,7 +59,7 @@ struct PagedPlan {
   int strips, nblk;
 };
 
-int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t), int most,
+int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t, int64_t), int most,
                int start, PagedPlan* plan) {
   if (H <= 0 || H % Hk != 0)
     return fail(NXA_E_SHAPE, "H=%d must be a positive multiple of Hk=%d", H, Hk);
@@ -74,13 +74,14 @@ int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t), int 
                 (long long)len);
   // (a block a row where a grid of less than 2^32 threads holds them)
   const int64_t units = tiles * Hk * plan->strips;
-  plan->nblk = whole(room) && rows < 1 << 24 ? 0 : (int)(units < most ? units : most);
+  plan->nblk = whole(room, rows) && rows < 1 << 24 ? 0 : (int)(units < most ? units : most);
   return NXA_OK;
 }
 
 int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
-  return plan_paged(d->Hk, d->PS, B, M, H, nxa::paged_whole, nxa::kPagedBlocks,
-                    nxa::kStartUnits, plan);
+  return plan_paged(
+      d->Hk, d->PS, B, M, H, [](int64_t room, int64_t) { return nxa::paged_whole(room); },
+      nxa::kPagedBlocks, nxa::kStartUnits, plan);
 }
 
 size_t paged_workspace(int dp, const PagedPlan& plan) {

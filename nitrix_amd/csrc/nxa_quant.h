@@ -48,7 +48,7 @@ struct QuantPagedParams : PagedParams {  // k_str, v_str in bytes
 // 132 / 131 / 129.
 constexpr int kQuantStart = 5;
 int qpaged_dp(int m);  // padded head dim
-bool qpaged_whole(int64_t room);
+bool qpaged_whole(int64_t room, int64_t rows);  // a block a row (sequence and head)
 int qpaged_blocks(int io_dtype, int dp, int bits);  // most blocks that share the work
 
 void launch_quant_write(const QuantMoveParams& p, int io_dtype, hipStream_t stream);

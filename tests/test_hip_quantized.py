@@ -331,6 +331,17 @@ def test_many_sequences():
     _check(out, q, pool, 4, table, lens, 1 / math.sqrt(32))
 
 
+@pytest.mark.parametrize('rows, longest', [(130, 1500), (127, 1500), (130, 2500)])
+def test_rows_shared_by_blocks_or_a_block_each(rows, longest):
+    rng = np.random.default_rng(rows)
+    lens = [int(x) for x in rng.integers(0, 60, rows)]
+    lens[7], lens[8], lens[rows - 1] = longest, 0, 129
+    pool, table = _setup(torch.bfloat16, lens, 2, 64, 64, 16, 4)
+    q = _rand((rows, 2, 64), torch.bfloat16, 6)
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32(lens), backend='hip')
+    _check(out, q, pool, 4, table, lens, 0.125)
+
+
 def test_operand_layouts():
     lens = [70, 3]
     pool, table = _setup(torch.bfloat16, lens, 2, 64, 64, 16, 4)

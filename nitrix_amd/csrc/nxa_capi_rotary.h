@@ -12,8 +12,9 @@ int check_rotary(const nxa_rotary_desc* d) {
   if (d->B <= 0 || d->T <= 0 || d->H <= 0 || d->Hk < 0)
     return fail(NXA_E_SHAPE, "extents must be positive (B=%d T=%d H=%d Hk=%d)", d->B, d->T, d->H,
                 d->Hk);
-  if (d->H > 1 << 20 || d->Hk > 1 << 20)
-    return fail(NXA_E_SHAPE, "H=%d, Hk=%d: at most 2^20 heads", d->H, d->Hk);
+  // (a block counts its tokens' elements in 31 bits)
+  if ((int64_t)d->H + d->Hk > 1 << 20)
+    return fail(NXA_E_SHAPE, "H=%d, Hk=%d: at most 2^20 heads together", d->H, d->Hk);
   if (d->D <= 0 || d->D > nxa::kRotaryMaxDim)
     return fail(NXA_E_UNSUPPORTED, "head dim D=%d is outside 1 .. %d", d->D, nxa::kRotaryMaxDim);
   if (d->R <= 0 || d->R > d->D || d->R % 2)

@@ -7,10 +7,13 @@
 //
 // Bound by HBM: 6 operations on 4 bytes read and 4 written (16 bits).  What
 // could cost more is the sine and cosine of each pair, which all heads of a
-// token share: a block takes a few tokens with all their heads, forms each pair's
-// once and keeps them in LDS.  Angles are turns in 64 bits, p (w / 2 pi), of which
+// token share: a block takes a token or a few with all their heads, forms each
+// pair's once and keeps them in LDS.  Angles are turns in 64 bits, p (w / 2 pi), of which
 // the fraction goes on in 32 bits: a position of 10^9 costs no accuracy.
+// 16384 tokens of 40 heads of 128 in bf16 take 61 us (5.5 TB/s).
 #include "nxa_rotary.h"
+
+#include <type_traits>
 
 namespace nxa {
 
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
 }
 
 // Any head dim, rotated part, strides and alignment: a pair or an element an
-// item.
+// item (173 us where chunks take 65).
 template <typename T, int TB>
 __global__ __launch_bounds__(256) void rotary_any_kernel(const RotaryParams p) {
   __shared__ float2 cs[TB * kRotaryMaxDim / 2];
@@ -130,11 +133,23 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(const RotaryParams p) {
 
 template <typename T>
 static void launch_rotary_t(const RotaryParams& p, bool chunks, hipStream_t stream) {
-  constexpr int TB = 4;
-  const dim3 grid((unsigned)((int64_t)p.B * ((p.T + TB - 1) / TB))), block(256);
-  if (!chunks) hipLaunchKernelGGL((rotary_any_kernel<T, TB>), grid, block, 0, stream, p);
-  else if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, true, TB>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((rotary_kernel<T, false, TB>), grid, block, 0, stream, p);
+  auto go = [&](auto tb) {
+    constexpr int TB = decltype(tb)::value;
+    const dim3 grid((unsigned)((int64_t)p.B * ((p.T + TB - 1) / TB))), block(256);
+    if (!chunks) hipLaunchKernelGGL((rotary_any_kernel<T, TB>), grid, block, 0, stream, p);
+    else if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, true, TB>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((rotary_kernel<T, false, TB>), grid, block, 0, stream, p);
+  };
+  // A token a block where its chunks are a thread's each, and where there are few
+  // tokens; else four, whose blocks take longer than their dispatch (0.9 ns each).  us
+  // at 128 dims in bf16, one / four: 16384 tokens of 40 heads 60.8 / 65.3, 20000 of 20
+  // heads 35.0 / 33.3, of 8 heads 23.4 / 16.1; 64 tokens of 40 heads 4.0 / 5.5, 1000 of
+  // 10 heads of 64 in fp32 4.8 / 4.6.  (Grids stay below 2^32 threads.)
+  const int chunks_of_token = (p.H[0] + p.H[1]) * p.D * (int)sizeof(T) / 32;
+  const int64_t tokens = (int64_t)p.B * p.T;
+  if (tokens <= 512 || (chunks_of_token >= 256 && tokens < 1 << 24))
+    go(std::integral_constant<int, 1>());
+  else go(std::integral_constant<int, 4>());
 }
 
 void launch_rotary(const RotaryParams& p, int io_dtype, bool chunks, hipStream_t stream) {

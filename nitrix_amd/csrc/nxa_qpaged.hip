@@ -188,6 +188,14 @@ __device__ constexpr int key_order(int e) {
   return FP8 ? 2 * (e & 3) + (e >> 2) : (e >> 1) + 4 * (e & 1);
 }
 
+// The lane eight columns on (of sixteen).
+__device__ __forceinline__ uint32_t other_eight(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true);
+}
+__device__ __forceinline__ float other_eight(float x) {
+  return __uint_as_float(other_eight(__float_as_uint(x)));
+}
+
 // What a row's codes, as a product has them, count from.
 template <typename T, int BITS>
 __device__ __forceinline__ float from_mid(float s, float z) {
@@ -220,7 +228,10 @@ constexpr int quant_blocks(int es, int dp, int bits) {
 // codes and scales are aligned: halves are copied to LDS, each wave its own, steps
 // ahead of their use.  Else every key looks its page up and codes are loaded four
 // bytes at a time.
-template <typename T, int DP, int BITS, bool FAST>
+// PAIR: eight heads a key head or fewer leave half of a product's columns idle.  q
+// then stands in both halves, and columns from 8 on take the softmax of the second
+// half's keys, whose weights go back to the heads' columns for V's product.
+template <typename T, int DP, int BITS, bool FAST, bool PAIR>
 __global__ __launch_bounds__(256, quant_blocks(sizeof(T), DP, BITS)) void
 qpaged_kernel(const QuantPagedParams p) {
   using R = QuantStep<T, DP, BITS>;
@@ -228,6 +239,7 @@ qpaged_kernel(const QuantPagedParams p) {
   constexpr int NKW = R::NKW, NJ = R::NJ, DPL = R::DPL, VB = R::VB, NVW = R::NVW, NS = R::NS;
   constexpr int QT = R::QT, PT = R::PT;
   constexpr int NB = kQuantDepth;
+  constexpr int SC = PAIR ? 4 : 8;  // scores of a lane and step
   constexpr int NF = DPL;  // O^T fragments: fragment f is columns DPL i + f, i = 0 .. 15
   constexpr int FIELDS = NF * 4 + 2;
   constexpr int STEP_BYTES = 2 * R::HALF_BYTES, COPIES = R::COPIES;
@@ -240,6 +252,7 @@ qpaged_kernel(const QuantPagedParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
+  const bool upper = c >= 8;
   const int HV = p.Hk * p.strips;
 
   // The units of this block, u .. u1 (as in paged_kernel).
@@ -287,7 +300,7 @@ qpaged_kernel(const QuantPagedParams p) {
   const uint32_t ring = lds_offset(mem) + wave * (NB * STEP_BYTES);
   const uint32_t k_at = ring + c * kb + 4 * NKW * g;
   const uint32_t v_at = ring + 1024 * R::KC + 4 * g * vb + VB * c;
-  const uint32_t s_at = ring + 2048 * R::KC + 16 * R::ES * g;
+  const uint32_t s_at = ring + 2048 * R::KC + 16 * R::ES * g + (PAIR && upper ? R::HALF_BYTES : 0);
   typedef const __attribute__((address_space(4))) int constant_int;
   // Pages and slots that 128 tokens span.
   const int per = p.PS >= kPagedKeys ? 0 : kPagedKeys / p.PS, rest = kPagedKeys - per * p.PS;
@@ -375,7 +388,8 @@ qpaged_kernel(const QuantPagedParams p) {
     i32x8 qe[R::FP8 ? NJ : 1][QT];
     float qsum = 0.f, sl;
     {
-      const T* qp = (const T*)p.q + b * p.q_str[0] + ((int64_t)hk * p.G + h0 + min(c, heads - 1)) * p.q_str[1];
+      const int cq = PAIR ? c & 7 : c;
+      const T* qp = (const T*)p.q + b * p.q_str[0] + ((int64_t)hk * p.G + h0 + min(cq, heads - 1)) * p.q_str[1];
       float x[DP / 4], most = 0.f;
 #pragma unroll
       for (int j = 0; j < DP / 32; ++j) {
@@ -383,7 +397,7 @@ qpaged_kernel(const QuantPagedParams p) {
         float* y = x + 8 * j;
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = 0.f;
-        if (c < heads && d < p.D) {
+        if (cq < heads && d < p.D) {
           const u32x4* src = reinterpret_cast<const u32x4*>(qp + d);
           if constexpr (sizeof(T) == 4) {
             const f32x4 lo = __builtin_bit_cast(f32x4, src[0]), hi = __builtin_bit_cast(f32x4, src[1]);
@@ -474,70 +488,73 @@ qpaged_kernel(const QuantPagedParams p) {
     constexpr int kFull = FAST ? kHalfKeys : 0xffff;
     // (`values` is called between the softmax and V's product)
     auto compute = [&](Half (&r)[2], const int (&mine)[2], auto&& values) NXA_INLINE {
-      f32x4 s[2];
-      float vs[8], vz[8];
+      f32x4 dots[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-        f32x4 rest = s[h];  // fp32: of all terms of q but the first
+        dots[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 rest = dots[h];  // fp32: of all terms of q but the first
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           if constexpr (R::FP8) {
             const i32x8 a = key_fp8<BITS, false>(r[h].k, j);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) s[h] = mma_fp8<false>(a, qe[j][t], s[h]);
+            for (int t = 0; t < QT; ++t) dots[h] = mma_fp8<false>(a, qe[j][t], dots[h]);
             if constexpr (BITS == 8) {
               const i32x8 a = key_fp8<BITS, true>(r[h].k, j);
 #pragma unroll
-              for (int t = 0; t < QT; ++t) s[h] = mma_fp8<true>(a, qe[j][t], s[h]);
+              for (int t = 0; t < QT; ++t) dots[h] = mma_fp8<true>(a, qe[j][t], dots[h]);
             }
           } else {
             const u32x4 a = key_f16<BITS>(r[h].k, j, cb);
 #pragma unroll
             for (int t = 1; t < QT; ++t) rest = mma_f16(a, qb[j][t], rest);
-            s[h] = mma_f16(a, qb[j][0], s[h]);
+            dots[h] = mma_f16(a, qb[j][0], dots[h]);
           }
         }
         if constexpr (!R::FP8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[h][e] += rest[e];
-        // Rows of the accumulator: tokens 4 g + e.
+          for (int e = 0; e < 4; ++e) dots[h][e] += rest[e];
+      }
+      // Rows of the accumulator: tokens 4 g + e.
+      float s[SC], vs[SC], vz[SC];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          // (a scale of infinity makes its token NaN, whatever the signs)
-          const float ks = scale_field<T>(r[h].s[e], 0);
-          const float kz = from_mid<T, BITS>(ks, scale_field<T>(r[h].s[e], 1));
-          s[h][e] = __builtin_fmaf(s[h][e], ks, __builtin_fmaf(kz, qsum, ks * 0.f));
-          vs[4 * h + e] = scale_field<T>(r[h].s[e], 2);
-          vz[4 * h + e] = from_mid<T, BITS>(vs[4 * h + e], scale_field<T>(r[h].s[e], 3));
-        }
+      for (int i = 0; i < SC; ++i) {
+        const auto& sc = r[i / 4].s[i % 4];
+        // (a scale of infinity makes its token NaN, whatever the signs)
+        const float ks = scale_field<T>(sc, 0);
+        const float kz = from_mid<T, BITS>(ks, scale_field<T>(sc, 1));
+        const float dot = PAIR && upper ? dots[1][i % 4] : dots[i / 4][i % 4];
+        s[i] = __builtin_fmaf(dot, ks, __builtin_fmaf(kz, qsum, ks * 0.f));
+        vs[i] = scale_field<T>(sc, 2);
+        vz[i] = from_mid<T, BITS>(vs[i], scale_field<T>(sc, 3));
       }
       if (__builtin_expect(((mine[0] ^ kFull) | (mine[1] ^ kFull)) != 0, 0)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool ok = FAST ? 4 * g + e < mine[h] : (mine[h] >> (4 * g + e) & 1) != 0;
-            // (what stands there of other tokens' scales may be NaN)
-            s[h][e] = ok ? s[h][e] : -INFINITY;
-            vs[4 * h + e] = ok ? vs[4 * h + e] : 0.f;
-            vz[4 * h + e] = ok ? vz[4 * h + e] : 0.f;
-          }
+        for (int i = 0; i < SC; ++i) {
+          const int e = i % 4, there = PAIR && upper ? mine[1] : mine[i / 4];
+          const bool ok = FAST ? 4 * g + e < there : (there >> (4 * g + e) & 1) != 0;
+          // (what stands there of other tokens' scales may be NaN)
+          s[i] = ok ? s[i] : -INFINITY;
+          vs[i] = ok ? vs[i] : 0.f;
+          vz[i] = ok ? vz[i] : 0.f;
+        }
       }
       float mt = -INFINITY, sm = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          mt = fmaxf(mt, s[h][e]);
-          sm = fmaxf(sm, __builtin_fabsf(vs[4 * h + e]));
-        }
+      for (int i = 0; i < SC; ++i) {
+        mt = fmaxf(mt, s[i]);
+        sm = fmaxf(sm, __builtin_fabsf(vs[i]));
+      }
       mt *= sl;
       if (__builtin_expect(__any((mt > m_ref + kSlack) | (sm > s_most)), 0)) {
         mt = fmaxf(mt, xor16(mt));
         mt = fmaxf(mt, shfl_xor32(mt));
         sm = fmaxf(sm, xor16(sm));
         sm = fmaxf(sm, shfl_xor32(sm));
+        if constexpr (PAIR) {
+          mt = fmaxf(mt, other_eight(mt));
+          sm = fmaxf(sm, other_eight(sm));
+        }
         m_ref = fmaxf(m_ref, mt);
         const int e = max(__builtin_amdgcn_frexp_expf(sm), -90);
         s_exp = sm > s_most ? (float)e : s_exp;
@@ -555,10 +572,10 @@ qpaged_kernel(const QuantPagedParams p) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[f][e] *= alpha;
       }
-      float x[8];  // P s'
+      float x[SC];  // P s'
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = fast_exp2(__builtin_fmaf(s[i / 4][i % 4], sl, neg_ref));
+      for (int i = 0; i < SC; ++i) {
+        const float w = fast_exp2(__builtin_fmaf(s[i], sl, neg_ref));
         l += w;
         x[i] = w * vs[i];
         zs = __builtin_fmaf(w, vz[i], zs);
@@ -570,8 +587,9 @@ qpaged_kernel(const QuantPagedParams p) {
 #pragma unroll
       for (int t = 0; t < PT; ++t)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < SC / 2; ++w) {
           pf[t][w] = pack_f16(x[2 * w], x[2 * w + 1]);
+          if constexpr (PAIR) pf[t][2 + w] = other_eight(pf[t][w]);
           x[2 * w] -= low_f16(pf[t][w]);
           x[2 * w + 1] -= high_f16(pf[t][w]);
         }
@@ -623,7 +641,7 @@ qpaged_kernel(const QuantPagedParams p) {
             const uint32_t at = x * STEP_BYTES + h * R::HALF_BYTES;
             r[h].k.lds(k_at + at);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) r[h].s[y].lds(s_at + at + 4 * R::ES * y);
+            for (int y = 0; y < (PAIR && h ? 0 : 4); ++y) r[h].s[y].lds(s_at + at + 4 * R::ES * y);
           }
           const int mine[2] = {have[x][0], have[x][1]};
           compute(r, mine, [&]() NXA_INLINE {
@@ -683,6 +701,10 @@ qpaged_kernel(const QuantPagedParams p) {
     l += shfl_xor32(l);
     zs += xor16(zs);
     zs += shfl_xor32(zs);
+    if constexpr (PAIR) {
+      l += other_eight(l);
+      zs += other_eight(zs);
+    }
 
     // Join the waves: [wave][field][lane], field 4 f + e of O, then m and l (where
     // the rings were: all copies have landed and been read).
@@ -781,10 +803,13 @@ static void launch_qpaged_b(QuantPagedParams p, hipStream_t stream) {
     p.k16 = (int)(p.k_str[0] / 16);
     p.v16 = (int)(p.v_str[0] / 16);
     p.s16 = (int)(ps / 16);
-    hipLaunchKernelGGL((qpaged_kernel<T, DP, BITS, true>), grid, block, 0, stream, p);
+    if (p.G <= 8)
+      hipLaunchKernelGGL((qpaged_kernel<T, DP, BITS, true, true>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((qpaged_kernel<T, DP, BITS, true, false>), grid, block, 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((qpaged_kernel<T, DP, BITS, false, false>), grid, block, 0, stream, p);
   }
-  else
-    hipLaunchKernelGGL((qpaged_kernel<T, DP, BITS, false>), grid, block, 0, stream, p);
 }
 
 template <typename T, int BITS>

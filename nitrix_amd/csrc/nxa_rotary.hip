@@ -40,6 +40,15 @@ struct alignas(16) Chunk {
   T x[N];
 };
 
+// Sixteen bytes to memory, of many tokens past the caches: us called in turn with /
+// without, 8192 tokens of 40 heads of 128 in fp16 28.6 / 35.0, 16384 in bf16 53 / 66.
+template <int TB, typename C>
+__device__ __forceinline__ void put(void* at, const C& x) {
+  u32x4* to = reinterpret_cast<u32x4*>(at);
+  if (TB > 1) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, x), to);
+  else *to = __builtin_bit_cast(u32x4, x);
+}
+
 }  // namespace
 
 // Rows as 16-byte chunks: an item is a pair of chunks that turn together (half
@@ -70,7 +79,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
     const float2* at = cs + t * (kRotaryMaxDim / 2);
     if (c >= turned) {
       const int d = p.R + (c - turned) * N;
-      *reinterpret_cast<u32x4*>(y + d) = *reinterpret_cast<const u32x4*>(x + d);
+      put<TB>(y + d, *reinterpret_cast<const u32x4*>(x + d));
     } else if (IL) {
       Chunk<T> a = *reinterpret_cast<const Chunk<T>*>(x + c * N);
 #pragma unroll
@@ -80,7 +89,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
         a.x[2 * e] = (T)(u * k.x - v * k.y);
         a.x[2 * e + 1] = (T)(v * k.x + u * k.y);
       }
-      *reinterpret_cast<Chunk<T>*>(y + c * N) = a;
+      put<TB>(y + c * N, a);
     } else {
       Chunk<T> a = *reinterpret_cast<const Chunk<T>*>(x + c * N);
       Chunk<T> o = *reinterpret_cast<const Chunk<T>*>(x + half + c * N);
@@ -91,14 +100,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
         a.x[e] = (T)(u * k.x - v * k.y);
         o.x[e] = (T)(v * k.x + u * k.y);
       }
-      *reinterpret_cast<Chunk<T>*>(y + c * N) = a;
-      *reinterpret_cast<Chunk<T>*>(y + half + c * N) = o;
+      put<TB>(y + c * N, a);
+      put<TB>(y + half + c * N, o);
     }
   }
 }
 
 // Any head dim, rotated part, strides and alignment: a pair or an element an
-// item (173 us where chunks take 65).
+// item (173 us where chunks take 61).
 template <typename T, int TB>
 __global__ __launch_bounds__(256) void rotary_any_kernel(const RotaryParams p) {
   __shared__ float2 cs[TB * kRotaryMaxDim / 2];
@@ -140,14 +149,11 @@ static void launch_rotary_t(const RotaryParams& p, bool chunks, hipStream_t stre
     else if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, true, TB>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((rotary_kernel<T, false, TB>), grid, block, 0, stream, p);
   };
-  // A token a block where its chunks are a thread's each, and where there are few
-  // tokens; else four, whose blocks take longer than their dispatch (0.9 ns each).  us
-  // at 128 dims in bf16, one / four: 16384 tokens of 40 heads 60.8 / 65.3, 20000 of 20
-  // heads 35.0 / 33.3, of 8 heads 23.4 / 16.1; 64 tokens of 40 heads 4.0 / 5.5, 1000 of
-  // 10 heads of 64 in fp32 4.8 / 4.6.  (Grids stay below 2^32 threads.)
-  const int chunks_of_token = (p.H[0] + p.H[1]) * p.D * (int)sizeof(T) / 32;
-  const int64_t tokens = (int64_t)p.B * p.T;
-  if (tokens <= 512 || (chunks_of_token >= 256 && tokens < 1 << 24))
+  // A token a block where there are few tokens, whose blocks run at once, else four.
+  // us, one / four: 64 tokens of 40 heads of 128 in bf16 4.0 / 5.5, 1000 of 10 heads of 64
+  // in fp32 4.8 / 4.6, 20000 of 8 heads of 128 23.4 / 16.1, 8192 of 40 heads in fp16
+  // 31.9 / 30.4 (called in turn 39.0 / 35.0; all before put).
+  if ((int64_t)p.B * p.T <= 512)
     go(std::integral_constant<int, 1>());
   else go(std::integral_constant<int, 4>());
 }

@@ -2,13 +2,14 @@
 //
 // A block takes kTokens tokens: a thread each finds a token's sequence and page, and
 // then a wave takes one, LPR lanes of eight elements a row (a head's key or value),
-// 64 / LPR rows at a time.  Bound by HBM: a row is read (written) once in the model's
-// type and written (read) once in codes.  What hides its latency is waves, eight a
-// SIMD: with two or four such steps loaded together a wave held 99 or more registers
-// in place of 53, and writing 16384 tokens of 8 heads of 128 in bf16 into 4 bits took
-// 39 and 47 us in place of 32; 16 tokens a block took 35, and 1024 tokens in 8 bits 13
-// in place of 9.  These 32 us are 5.3 TB/s, 17 to read them back 10 (much of it out of
-// caches), 56 for 65,664 tokens 6.1.
+// 64 / LPR rows at a time.  A row is read (written) once in the model's type and
+// written (read) once in codes.  Reading back is bound by HBM: 65,664 tokens of 8 heads
+// of 128 in bf16 and 4 bits 56 us, 6.1 TB/s, 16384 tokens 17 us.  Writing 16384 takes 31
+// us (2.7 TB/s): some 200 vector operations for a lane's eight elements, which keep
+// the SIMDs busy for two thirds of it.  What hides latency is waves, eight a SIMD: with
+// two or four such steps loaded together a wave held 99 or more registers in place of 53,
+// and writing took 39 and 47 us; 16 tokens a block took 35, and 1024 tokens in 8 bits 13 in
+// place of 9.
 //
 // Codes are rounded as the exact quotient would be, ties to even, so that they do
 // not depend on how it is taken (exact_code; near_code where it is as good).

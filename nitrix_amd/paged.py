@@ -26,7 +26,8 @@ engine has no derivatives.  The reference has no counterpart; engines and
 (``'jax'``: the same functions in stock tensor ops).
 
 Page contents change in place (a cache fills most of the memory); tables,
-lengths and counts are returned anew.
+lengths and counts are returned anew.  :mod:`nitrix_amd.quantized` holds the same
+pages in 4 or 8 bits an element.
 """
 
 from __future__ import annotations

@@ -352,8 +352,8 @@ def quantized_paged_attention(
 
     :func:`~nitrix_amd.paged.paged_attention` of what the codes stand for: q
     ``(b, h, d)`` in the scales' dtype, the result ``(b, h, d_v)``.  Bits a code (4
-    or 8) follow from ``d`` and the pages' width.  Neither codes, minima nor scales
-    are rounded on the way; tokens in no page, lengths outside the table's room and
+    or 8) follow from ``d`` and the pages' width.  Keys and values are not rounded
+    to the type on the way; tokens in no page, lengths outside the table's room and
     rows without tokens are treated as there.  A page row has room for less than
     2^31 - 4096 tokens.
 

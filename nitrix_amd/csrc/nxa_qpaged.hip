@@ -488,7 +488,7 @@ qpaged_kernel(const QuantPagedParams p) {
     // (s_most), less 3: P s' is then below 2^13.  zs: what the minima add to every
     // column.
     float m_ref = -INFINITY, ref = -INFINITY, neg_ref = 0.f, l = 0.f, zs = 0.f;
-    float s_most = 0.f, s_exp = -90.f;
+    float s_most = 0.f, s_exp = 0.f;  // (0 while all scales are: zs holds any minimum)
 
     // `mine`: tokens of the half (FAST), or a bit a token.
     constexpr int kFull = FAST ? kHalfKeys : 0xffff;

@@ -162,8 +162,8 @@ def write_quantized_pages(
     ``starts`` and ``offsets`` as in :func:`~nitrix_amd.paged.write_pages`; bits a
     code (4 or 8) follow from the widths of the pages.  Of each row ``z`` is the
     minimum, ``s`` the range times ``1 / (2^bits - 1)`` (both in float32), rounded to
-    the scales' dtype, and codes are the exact quotients ``(x - z) / s`` rounded to the nearest, ties to
-    even.  A row that holds NaN or infinity, or whose range exceeds float32's, is
+    the scales' dtype, and codes are the exact quotients ``(x - z) / s`` rounded to
+    the nearest, ties to even.  A row that holds NaN or infinity, or whose range exceeds float32's, is
     NaN when it is read; a constant row is exact.
 
     The fused engine takes bfloat16, float16 and float32 and head dims up to 256

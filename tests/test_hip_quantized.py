@@ -277,6 +277,23 @@ def test_large_and_small_rows():
         _check(out, q, (pool[0], pool[1], sc), 4, table, lens, 0.125)
 
 
+@pytest.mark.parametrize('dtype, value', [('bf16', 1e30), ('f16', 3e4), ('f32', -1e25), ('bf16', 0.0)])
+def test_rows_of_one_value(dtype, value):
+    """Constant values have a scale of zero, whatever they are; half of the second
+    sequence's, of the first's all."""
+    lens = [300, 200]
+    pool, table = _setup(DT[dtype], lens, 1, 64, 64, 16, 4)
+    for j in list(table[0, :19]) + list(table[1, :6]):
+        pool[2][int(j), ..., 2] = 0
+        pool[2][int(j), ..., 3] = value
+    q = _rand((2, 3, 64), DT[dtype], 4)
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32(lens), backend='hip')
+    z = pool[2][int(table[0, 0]), 0, 0, 3].item()
+    # (the sum of weights times the value over the sum of weights, 300 steps each)
+    assert (out[0].double() - z).abs().max() <= abs(z) * (600 * E24 + torch.finfo(DT[dtype]).eps / 2)
+    _check(out, q, pool, 4, table, lens, 0.125)
+
+
 @pytest.mark.parametrize('dtype, bits', [('bf16', 4), ('f32', 8)])
 def test_one_long_sequence(dtype, bits):
     """Every block a piece of the same rows."""

@@ -4,12 +4,12 @@
 // then a wave takes one, LPR lanes of eight elements a row (a head's key or value),
 // 64 / LPR rows at a time.  A row is read (written) once in the model's type and
 // written (read) once in codes.  Reading back is bound by HBM: 65,664 tokens of 8 heads
-// of 128 in bf16 and 4 bits 56 us, 6.1 TB/s, 16384 tokens 17 us.  Writing 16384 takes 31
-// us (2.7 TB/s): some 200 vector operations for a lane's eight elements, which keep
-// the SIMDs busy for two thirds of it.  What hides latency is waves, eight a SIMD: with
+// of 128 in bf16 and 4 bits 56 us, 6.1 TB/s, 16384 tokens 17 us.  Writing 16384 takes 28
+// us (3.1 TB/s): some 170 vector operations for a lane's eight elements, which keep
+// the SIMDs busy for three quarters of it.  What hides latency is waves, eight a SIMD: with
 // two or four such steps loaded together a wave held 99 or more registers in place of 53,
-// and writing took 39 and 47 us; 16 tokens a block took 35, and 1024 tokens in 8 bits 13 in
-// place of 9.
+// and writing took 39 and 47 us, 31 then; 16 tokens a block took 35, and 1024 tokens in 8
+// bits 13 in place of 9.
 //
 // Codes are rounded as the exact quotient would be, ties to even, so that they do
 // not depend on how it is taken (exact_code; near_code where it is as good).
@@ -103,15 +103,15 @@ __device__ __forceinline__ uint32_t row_reduce(uint32_t x, F&& f) {
   if constexpr (LPR >= 32) x = f(x, (uint32_t)__shfl_xor((int)x, 16, 64));
   return x;
 }
-// (as instructions: fminf would first quiet each number, which could be a NaN)
+// (NaN where one of them is)
 __device__ __forceinline__ float min3(float a, float b, float c) {
   float r;
-  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  asm("v_minimum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
 
@@ -135,10 +135,11 @@ __device__ __forceinline__ float exact_code(float x, float z, float s, float inv
 
 // The same where x - z is exact in fp32 and s has few bits (16-bit types, x and z
 // not too far apart): the quotient by the reciprocal, corrected by its remainder, is
-// the exact one rounded to fp32 (inv is 1 / s rounded).  A border n + 1/2 is an fp32
-// number, and (n + 1/2) s, of 20 bits or fewer, stands in the places of x - z: one
-// that is not a border differs from it by a place of x - z or more, more than half a
-// place of the quotient, and is not rounded to it.
+// the exact one but for 2^-45 of it, rounded to fp32 (inv is off by a place or two).
+// A border n + 1/2 is an fp32 number, and (n + 1/2) s, of 20 bits or fewer, stands in
+// the places of x - z: one that is not a border differs from it by a place of x - z or
+// more, at least 1 + 2^-11 times half a place of the quotient (s has 11 bits or fewer),
+// and is not rounded to it.
 __device__ __forceinline__ float near_code(float diff, float s, float inv) {
   const float q = diff * inv;
   return __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q, s, diff), inv, q));
@@ -157,39 +158,37 @@ __device__ __forceinline__ void write_row(const Eight<T>& y, bool mine, bool fir
   constexpr int FAR = std::is_same<T, f16>::value ? 12 : 15;
   constexpr float kFar = 1 << FAR;
   float x[8], lo = INFINITY, hi = -INFINITY;
-  uint32_t twice[8];  // twice the bits of |x|, less one (0: the most)
-  uint32_t least = 0xffffffffu, most = 0;
+  uint32_t least = 0xffffffffu;  // twice the bits of the least |x| but 0, less one
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    x[e] = (float)y.x[e];
-    twice[e] = 2u * __float_as_uint(x[e]) - 1u;
-  }
+  for (int e = 0; e < 8; ++e) x[e] = (float)y.x[e];
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     lo = min3(lo, x[e], x[e + 1]);
     hi = max3(hi, x[e], x[e + 1]);
-    least = min(least, min(twice[e], twice[e + 1]));
-    most = max(most, max(twice[e] + 1u, twice[e + 1] + 1u));
+    least = min(least, min(2u * __float_as_uint(x[e]) - 1u, 2u * __float_as_uint(x[e + 1]) - 1u));
   }
   const float far = fmaxf(__builtin_fabsf(lo), __builtin_fabsf(hi));
-  if (!mine) lo = INFINITY, hi = -INFINITY, most = 0;
+  if (!mine) lo = INFINITY, hi = -INFINITY;
   lo = __uint_as_float(row_reduce<LPR>(__float_as_uint(lo), [](uint32_t a, uint32_t b) {
     return __float_as_uint(min3(__uint_as_float(a), __uint_as_float(b), INFINITY));
   }));
   hi = __uint_as_float(row_reduce<LPR>(__float_as_uint(hi), [](uint32_t a, uint32_t b) {
     return __float_as_uint(max3(__uint_as_float(a), __uint_as_float(b), -INFINITY));
   }));
-  most = row_reduce<LPR>(most, [](uint32_t a, uint32_t b) { return max(a, b); });
   // (a row of NaN, infinity or a range past the type's reads back as NaN)
   const float range = hi - lo;
-  const bool bad = most >= 0xff000000u || !(range < INFINITY);
+  const bool bad = !(range < INFINITY);
   const T zt = (T)(bad ? NAN : lo), st = (T)(bad ? NAN : range * (1.f / TOP));
   const float z = (float)zt;
   float sf = (float)st;
   // (quotients of tiny scales are taken 2^96 times larger)
   const float up = sf < 0x1p-90f ? 0x1p96f : 1.f;
   sf *= up;
-  const float inv = sf > 0.f ? 1.f / sf : 0.f;
+  // (the hardware's reciprocal, off by a place or so, and a step that leaves next to
+  // nothing of that)
+  const float near_inv = __builtin_amdgcn_rcpf(sf);
+  const float inv =
+      sf > 0.f ? __builtin_fmaf(__builtin_fmaf(-sf, near_inv, 1.f), near_inv, near_inv) : 0.f;
   float n[8];
   const float az = __builtin_fabsf(z);
   const bool near = sizeof(T) == 2 && up == 1.f &&

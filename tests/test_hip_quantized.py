@@ -174,6 +174,13 @@ CASES = [
     ('f32', 4, 2, 1, 256, 256, 32, 'heads'),
     ('bf16', 4, 40, 1, 32, 32, 128, 'wide'),
     ('bf16', 4, 6, 2, 96, 8, 16, 'heads'),
+    # more than eight heads a key head: whole products
+    ('bf16', 4, 16, 1, 128, 128, 16, 'heads'),
+    ('f32', 4, 12, 1, 128, 128, 16, 'heads'),
+    ('bf16', 8, 32, 2, 128, 128, 32, 'heads'),
+    ('f16', 8, 9, 1, 256, 256, 16, 'heads'),
+    ('f32', 8, 10, 1, 64, 64, 16, 'heads'),
+    ('f16', 4, 20, 1, 128, 96, 16, 'wide'),
     ('bf16', 8, 8, 2, 128, 128, 16, 'heads'),
     ('f16', 8, 6, 3, 64, 128, 32, 'wide'),
     ('f32', 8, 4, 2, 128, 128, 16, 'heads'),

@@ -11,12 +11,13 @@
 // code of four bits in a plain form, with the HBM idle two thirds of the time), so
 // they are taken as numbers whose bits they already are:
 //
-//  * K, 16-bit types: the byte 0000cccc is the fp8 (e4m3) number c 2^-9, whether
-//    below 8 (subnormal) or not, so codes of four bits are two masks and a shift a
-//    dword and those of eight two such halves, the upper one scaled by 16 in the
-//    product.  q is the sum of two (fp16: three) fp8 numbers, scaled so that its
-//    largest element is in 2^7 .. 2^8: exact down to 2^-10 (2^-7) of that, off by at
-//    most 2^-17 of it below.
+//  * K: codes in the mantissa of an fp16 64 (4 bits) or 1024 (8 bits).  What is added
+//    to them is what a product's sum starts from, -64 (1024) sum q: a score loses
+//    some 2^-24 of 64 |sum q|, no more than its codes' own sum would.  q is scaled to a
+//    largest element of 2^14 or more and then is one fp16 number, exact down to 2^-29 of
+//    that.  (fp8 numbers need no 64, c 2^-9 being their bits, and 2 operations less for
+//    8 codes.  But their products keep 13 bits below the largest of eight and drop
+//    the others' rest, and q takes two or three of them.)
 //  * V: codes in the mantissa of an fp16 64 (in bits 4 .. 7, where an element's odd
 //    codes are already) or 1024 (bits 0 .. 3, or 0 .. 7).  What is added to them is
 //    taken off at the end, by a product of ones with the very P s' that the other
@@ -53,23 +54,22 @@ namespace {
 
 constexpr int kHalfKeys = 16;
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
 template <typename T, int DP, int BITS>
 struct QuantStep {
   static constexpr int ES = sizeof(T);
-  static constexpr bool FP8 = ES == 2, F16 = std::is_same<T, f16>::value;
+  static constexpr bool F32 = ES == 4, F16 = std::is_same<T, f16>::value;
   static constexpr int NKW = DP * BITS / 128;       // dwords of K's codes a lane and half
-  static constexpr int NJ = FP8 ? (DP + 127) / 128 : DP / 32;  // products of a half's S
+  static constexpr int NJ = DP / 32;                // products of a half's S
   static constexpr int DPL = DP / 16;               // V columns of a lane
   static constexpr int VB = DPL * BITS / 8;         // bytes of them a key
   static constexpr int NVW = VB >= 4 ? VB / 4 : 1;  // dwords
   static constexpr int NS = ES;                     // dwords of a token's scales: 4 ES / 4
-  static constexpr int QT = FP8 && !F16 ? 2 : 3;    // terms of q
-  static constexpr int PT = !FP8 ? 3 : F16 ? 2 : 1;  // of P s'
-  static constexpr float MID = FP8 ? 0.f : BITS == 4 ? 8.f : 128.f;  // codes count from it
-  // What stands in for 0 in V's even and odd columns.
-  static constexpr float EVEN = BITS == 8 || (FP8 && !F16) ? 1024.f : 64.f;
+  static constexpr int QT = F32 ? 3 : 1;            // terms of q
+  static constexpr int PT = F32 ? 3 : F16 ? 2 : 1;  // of P s'
+  static constexpr float MID = !F32 ? 0.f : BITS == 4 ? 8.f : 128.f;  // codes count from it
+  static constexpr float ZERO = BITS == 4 ? 64.f : 1024.f;  // what stands in for 0 in K (16 bits)
+  // and in V's even and odd columns.
+  static constexpr float EVEN = BITS == 8 || !(F32 || F16) ? 1024.f : 64.f;
   static constexpr float ODD = BITS == 8 ? 1024.f : 64.f;
   // A half in LDS: K's codes, V's, the scales; copies of 1 KB (scales: 256 bytes).
   static constexpr int KC = DP * BITS <= 512 ? 1 : DP * BITS / 512;
@@ -109,12 +109,6 @@ __device__ __forceinline__ f32x4 mma_f16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// fp8 over 128 places; UP: a's numbers times 16.
-template <bool UP>
-__device__ __forceinline__ f32x4 mma_fp8(i32x8 a, i32x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, UP ? 131 : 127, 0, 127);
-}
-
 // Two numbers as fp16, the first in the low half.
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -149,48 +143,38 @@ __device__ __forceinline__ uint32_t add_f16(uint32_t a, uint32_t b) {
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, a) + __builtin_bit_cast(f16x2, b));
 }
-// The nibbles at bits SH .. SH + 3 and SH + 16 .. SH + 19 less 8, as fp16.
+// The nibbles at bits SH .. SH + 3 and SH + 16 .. SH + 19 as fp16, more by 64.
 template <int SH>
 __device__ __forceinline__ uint32_t nibbles_f16(uint32_t w, const CodeBits& cb) {
-  const uint32_t x = SH < 4 ? w << (4 - SH) : w >> (SH - 4);
-  return add_f16((x & cb.high) | cb.k64, cb.from64);
+  return ((SH < 4 ? w << (4 - SH) : w >> (SH - 4)) & cb.high) | cb.k64;
 }
-// Two bytes (of a word, as `sel` picks them into the low ones) less 128, as fp16.
+// Two bytes (of a word, as `sel` picks them into the low ones), more by 1024.
 __device__ __forceinline__ uint32_t bytes_f16(uint32_t w, uint32_t sel, const CodeBits& cb) {
-  return add_f16(__builtin_amdgcn_perm(0u, w, sel) | cb.k1024, cb.from1024);
+  return __builtin_amdgcn_perm(0u, w, sel) | cb.k1024;
 }
-// Product operand j of a lane's codes of one key, fp16: eight of them.
-template <int BITS, int N>
+// Product operand j of a lane's codes of one key, eight of them; MID: from their
+// middle, else more by what stands in for 0.
+template <int BITS, bool MID, int N>
 __device__ __forceinline__ u32x4 key_f16(const Loaded<N>& k, int j, const CodeBits& cb) {
+  u32x4 r;
   if constexpr (BITS == 4) {
     const uint32_t w = k.at(j);
-    return u32x4{nibbles_f16<0>(w, cb), nibbles_f16<4>(w, cb), nibbles_f16<8>(w, cb),
-                 nibbles_f16<12>(w, cb)};
+    r = u32x4{nibbles_f16<0>(w, cb), nibbles_f16<4>(w, cb), nibbles_f16<8>(w, cb),
+              nibbles_f16<12>(w, cb)};
   } else {
     const uint32_t a = k.at(2 * j), b = k.at(2 * j + 1);
-    return u32x4{bytes_f16(a, 0x0c010c00u, cb), bytes_f16(a, 0x0c030c02u, cb),
-                 bytes_f16(b, 0x0c010c00u, cb), bytes_f16(b, 0x0c030c02u, cb)};
+    r = u32x4{bytes_f16(a, 0x0c010c00u, cb), bytes_f16(a, 0x0c030c02u, cb),
+              bytes_f16(b, 0x0c010c00u, cb), bytes_f16(b, 0x0c030c02u, cb)};
   }
-}
-// Operand j, fp8: 32 codes of four bits, or the lower or upper halves of as many of
-// eight (zeros behind the lane's last).
-template <int BITS, bool UPPER, int N>
-__device__ __forceinline__ i32x8 key_fp8(const Loaded<N>& k, int j) {
-  i32x8 r;
+  if constexpr (MID)
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const int i = BITS == 4 ? 4 * j + w / 2 : 8 * j + w;
-    const bool up = BITS == 4 ? w & 1 : UPPER;
-    const uint32_t x = i < N ? k.at(i) : 0u;
-    r[w] = (int)((up ? x >> 4 : x) & 0x0f0f0f0fu);
-  }
+    for (int i = 0; i < 4; ++i) r[i] = add_f16(r[i], BITS == 4 ? cb.from64 : cb.from1024);
   return r;
 }
 // The element of eight that stands at place e of an operand.
-template <int BITS, bool FP8>
+template <int BITS>
 __device__ constexpr int key_order(int e) {
-  if (BITS == 8) return e;
-  return FP8 ? 2 * (e & 3) + (e >> 2) : (e >> 1) + 4 * (e & 1);
+  return BITS == 8 ? e : (e >> 1) + 4 * (e & 1);
 }
 
 // The lane eight columns on (of sixteen).
@@ -390,8 +374,7 @@ qpaged_kernel(const QuantPagedParams p) {
         for (int h = 0; h < 2; ++h) issue(ring + x * STEP_BYTES + h * R::HALF_BYTES, have[x][h]);
     // Q^T: column c is head h0 + c; the lane's quarter of the head dim in the
     // order of K's codes, as QT terms, and the sum of the whole row.
-    u32x4 qb[R::FP8 ? 1 : NJ][QT];
-    i32x8 qe[R::FP8 ? NJ : 1][QT];
+    u32x4 qb[NJ][QT];
     float qsum = 0.f, sl;
     {
       const int cq = PAIR ? c & 7 : c;
@@ -421,61 +404,37 @@ qpaged_kernel(const QuantPagedParams p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           y[e] = p.scale_log2 < 0.f ? -y[e] : y[e];
-          qsum += y[e];
           most = fmaxf(most, __builtin_fabsf(y[e]));
         }
       }
-      qsum += xor16(qsum);
-      qsum += shfl_xor32(qsum);
-      sl = __builtin_fabsf(p.scale_log2);
       most = fmaxf(most, xor16(most));
       most = fmaxf(most, shfl_xor32(most));
-      // q times 2^up, its largest element in 2^7 .. 2^8 (fp32: 2^13 .. 2^14, so that
-      // three fp16 numbers hold it down to 2^-24), and scores in units of 2^(9 - up)
-      // (codes are c 2^-9 as fp8; 2^-up).  NaN and infinity of q leave NaN.
-      const int up = min((R::FP8 ? 8 : 14) - __builtin_amdgcn_frexp_expf(most), 100);
+      // q times 2^up, its largest element in 2^14 .. 2^15: as fp16 exact down to 2^-29
+      // of that (16-bit types), in three terms to 2^-24 of each element and 2^-39 of the
+      // largest (fp32).  Scores in units of 2^-up.  NaN and infinity of q leave NaN.
+      const int up = min(15 - __builtin_amdgcn_frexp_expf(most), 100);
       const float by = most > 0.f ? __builtin_ldexpf(1.f, up) : 1.f;
-      const float unit = (R::FP8 ? 512.f : 1.f) / by;
-      qsum = qsum / unit + (most - most) + (qsum - qsum);
-      sl *= unit;
-      if constexpr (R::FP8) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int w = 0; w < 8; ++w) {
-              // Place 4 w + i: in 4 bits the even elements of eight, then the odd.
-              int r = 0;
-#pragma unroll
-              for (int i = 0; i < 4; i += 2) {
-                const int e0 = 32 * j + 8 * (w / 2) + key_order<BITS, true>(4 * (w & 1) + i);
-                const int e1 = 32 * j + 8 * (w / 2) + key_order<BITS, true>(4 * (w & 1) + i + 1);
-                if (e0 >= DP / 4) continue;
-                float &a = x[e0], &o = x[e1];
-                if (t == 0) a *= by, o *= by;
-                if (i == 0) r = __builtin_amdgcn_cvt_pk_fp8_f32(a, o, r, false);
-                else r = __builtin_amdgcn_cvt_pk_fp8_f32(a, o, r, true);
-                a -= i == 0 ? __builtin_amdgcn_cvt_f32_fp8(r, 0) : __builtin_amdgcn_cvt_f32_fp8(r, 2);
-                o -= i == 0 ? __builtin_amdgcn_cvt_f32_fp8(r, 1) : __builtin_amdgcn_cvt_f32_fp8(r, 3);
-              }
-              qe[j][t][w] = r;
-            }
-      } else {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              float& a = x[8 * j + key_order<BITS, false>(2 * w)];
-              float& o = x[8 * j + key_order<BITS, false>(2 * w + 1)];
-              if (t == 0) a *= by, o *= by;
-              const uint32_t r = pack_f16(a, o);
-              qb[j][t][w] = r;
-              a -= low_f16(r), o -= high_f16(r);
-            }
+      for (int e = 0; e < DP / 4; ++e) {
+        x[e] *= by;
+        qsum += x[e];
       }
+      qsum += xor16(qsum);
+      qsum += shfl_xor32(qsum);
+      qsum += (most - most) + (qsum - qsum);
+      sl = __builtin_fabsf(p.scale_log2) / by;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            float& a = x[8 * j + key_order<BITS>(2 * w)];
+            float& o = x[8 * j + key_order<BITS>(2 * w + 1)];
+            const uint32_t r = pack_f16(a, o);
+            qb[j][t][w] = r;
+            a -= low_f16(r), o -= high_f16(r);
+          }
       // (one of zero is so small that all scores are zero, but for the -inf of a
       // token that takes no part)
       sl = fmaxf(sl, 0x1p-126f);
@@ -497,27 +456,18 @@ qpaged_kernel(const QuantPagedParams p) {
       f32x4 dots[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        dots[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-        f32x4 rest = dots[h];  // fp32: of all terms of q but the first
+        // (what stands in for 0 in the codes is taken off to begin with)
+        const float from = R::F32 ? 0.f : -R::ZERO * qsum;
+        dots[h] = f32x4{from, from, from, from};
+        f32x4 rest = {0.f, 0.f, 0.f, 0.f};  // fp32: of all terms of q but the first
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          if constexpr (R::FP8) {
-            const i32x8 a = key_fp8<BITS, false>(r[h].k, j);
+          const u32x4 a = key_f16<BITS, R::F32>(r[h].k, j, cb);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) dots[h] = mma_fp8<false>(a, qe[j][t], dots[h]);
-            if constexpr (BITS == 8) {
-              const i32x8 a = key_fp8<BITS, true>(r[h].k, j);
-#pragma unroll
-              for (int t = 0; t < QT; ++t) dots[h] = mma_fp8<true>(a, qe[j][t], dots[h]);
-            }
-          } else {
-            const u32x4 a = key_f16<BITS>(r[h].k, j, cb);
-#pragma unroll
-            for (int t = 1; t < QT; ++t) rest = mma_f16(a, qb[j][t], rest);
-            dots[h] = mma_f16(a, qb[j][0], dots[h]);
-          }
+          for (int t = 1; t < QT; ++t) rest = mma_f16(a, qb[j][t], rest);
+          dots[h] = mma_f16(a, qb[j][0], dots[h]);
         }
-        if constexpr (!R::FP8)
+        if constexpr (R::F32)
 #pragma unroll
           for (int e = 0; e < 4; ++e) dots[h][e] += rest[e];
       }
@@ -604,7 +554,7 @@ qpaged_kernel(const QuantPagedParams p) {
 #pragma unroll
         for (int t = 0; t < PT; ++t) acc = mma_f16(a, pf[t], acc);
       };
-      if constexpr (R::FP8) product(ones_o, u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
+      if constexpr (!R::F32) product(ones_o, u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
 #pragma unroll
       for (int w = 0; w < NVW; ++w)
 #pragma unroll
@@ -619,11 +569,11 @@ qpaged_kernel(const QuantPagedParams p) {
           for (int i = 0; i < 4; ++i) {
             if constexpr (BITS == 8) {
               a[i] = t[i] | cb.k1024;
-              if constexpr (!R::FP8) a[i] = add_f16(a[i], cb.from1024);
+              if constexpr (R::F32) a[i] = add_f16(a[i], cb.from1024);
             } else {
               a[i] = R::EVEN == 1024.f ? (t[i] & cb.low) | cb.k1024 : (t[i] << 4 & cb.high) | cb.k64;
               d[i] = (t[i] & cb.high) | cb.k64;
-              if constexpr (!R::FP8) a[i] = add_f16(a[i], cb.from64), d[i] = add_f16(d[i], cb.from64);
+              if constexpr (R::F32) a[i] = add_f16(a[i], cb.from64), d[i] = add_f16(d[i], cb.from64);
             }
           }
           if constexpr (BITS == 8) {
@@ -722,7 +672,7 @@ qpaged_kernel(const QuantPagedParams p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           mw[(4 * f + e) * 64] =
-              (R::FP8 ? __builtin_fmaf(f & 1 ? -R::ODD : -R::EVEN, ones_o[e], o[f][e]) : o[f][e]) + zs;
+              (!R::F32 ? __builtin_fmaf(f & 1 ? -R::ODD : -R::EVEN, ones_o[e], o[f][e]) : o[f][e]) + zs;
       mw[(FIELDS - 2) * 64] = ref;
       mw[(FIELDS - 1) * 64] = l;
     }

@@ -21,9 +21,8 @@
 //  * V: codes in the mantissa of an fp16 64 (in bits 4 .. 7, where an element's odd
 //    codes are already) or 1024 (bits 0 .. 3, or 0 .. 7).  What is added to them is
 //    taken off at the end, by a product of ones with the very P s' that the other
-//    products saw.  P s' is one fp16 number (bf16: off by 2^-12) or two (fp16: 2^-23).
-//    fp16's range is short, so the reference that P is relative to follows the largest
-//    scale as well as the largest score.
+//    products saw.  P s' is one fp16 number (bf16: off by 2^-12) or two (fp16: 2^-23),
+//    times a power of two that keeps the largest of them near the top of fp16's range.
 //  * fp32: what is added to the codes, and their minima, would cost digits: the values
 //    of a long row nearly cancel, to a root of its length, while those sums do not (8192
 //    tokens in 8 bits were off by 1.5e-5 of the output, now 4e-7).  So K's and V's codes are
@@ -442,12 +441,23 @@ qpaged_kernel(const QuantPagedParams p) {
     f32x4 o[NF], ones_o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // P is 2^(score - ref): ref is the largest score seen, raised by more than
-    // 2^kSlack only, plus 2^s_exp that no value's scale exceeds more than fourfold
-    // (s_most), less 3: P s' is then below 2^13.  zs: what the minima add to every
-    // column.
-    float m_ref = -INFINITY, ref = -INFINITY, neg_ref = 0.f, l = 0.f, zs = 0.f;
-    float s_most = 0.f, s_exp = 0.f;  // (0 while all scales are: zs holds any minimum)
+    // P is 2^(score - m_ref): m_ref is the largest score seen, rounded up so that it
+    // moves by whole powers of two, and raised by more than 2^kSlack only.  l sums P, zs
+    // what the minima add to every column.  P s' goes to fp16 times 2^x_exp, whose
+    // range is short: the exponent follows the largest P s' itself, which then is in 2^9
+    // .. 2^15 (rows of large scales and no weight do not count), up to 2^kMostExp, past
+    // which P 2^x_exp would leave fp32.
+    constexpr float kMostExp = 100.f;
+    float m_ref = -INFINITY, neg_m = 0.f, l = 0.f, zs = 0.f, x_exp = kMostExp, x_by = 0x1p100f;
+    // (over the lanes of a head)
+    auto most_of = [&](float x) NXA_INLINE {
+      x = fmaxf(x, xor16(x));
+      x = fmaxf(x, shfl_xor32(x));
+      if constexpr (PAIR) x = fmaxf(x, other_eight(x));
+      return x;
+    };
+    // 2^e of a whole number e at most 0, however small.
+    auto shrink = [](float e) NXA_INLINE { return __builtin_ldexpf(1.f, (int)fmaxf(e, -200.f)); };
 
     // `mine`: tokens of the half (FAST), or a bit a token.
     constexpr int kFull = FAST ? kHalfKeys : 0xffff;
@@ -495,50 +505,59 @@ qpaged_kernel(const QuantPagedParams p) {
           vz[i] = ok ? vz[i] : 0.f;
         }
       }
-      float mt = -INFINITY, sm = 0.f;
+      float mt = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < SC; ++i) {
-        mt = fmaxf(mt, s[i]);
-        sm = fmaxf(sm, __builtin_fabsf(vs[i]));
-      }
+      for (int i = 0; i < SC; ++i) mt = fmaxf(mt, s[i]);
       mt *= sl;
-      if (__builtin_expect(__any((mt > m_ref + kSlack) | (sm > s_most)), 0)) {
-        mt = fmaxf(mt, xor16(mt));
-        mt = fmaxf(mt, shfl_xor32(mt));
-        sm = fmaxf(sm, xor16(sm));
-        sm = fmaxf(sm, shfl_xor32(sm));
-        if constexpr (PAIR) {
-          mt = fmaxf(mt, other_eight(mt));
-          sm = fmaxf(sm, other_eight(sm));
-        }
-        m_ref = fmaxf(m_ref, mt);
-        const int e = max(__builtin_amdgcn_frexp_expf(sm), -90);
-        s_exp = sm > s_most ? (float)e : s_exp;
-        s_most = sm > s_most ? __builtin_ldexpf(4.f, e) : s_most;
-        const float old = ref;
-        ref = m_ref + (s_exp - 3.f);
-        neg_ref = ref == -INFINITY ? 0.f : -ref;
-        const float alpha = old == -INFINITY ? 1.f : fast_exp2(old - ref);
+      float o_by = 1.f;
+      if (__builtin_expect(__any(mt > m_ref + kSlack), 0)) {
+        const float old = m_ref;
+        m_ref = fmaxf(m_ref, __builtin_ceilf(most_of(mt)));
+        neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+        // (from -inf on, where nothing has been summed: by 0)
+        const float up = m_ref > old ? m_ref - old : 0.f, alpha = shrink(-up);
         l *= alpha;
         zs *= alpha;
+        // P s' keeps its power of two, what P loses x_exp gains.
+        x_exp += up;
+        o_by = shrink(fminf(kMostExp - x_exp, 0.f));
+        x_exp = fminf(x_exp, kMostExp);
+        x_by = __builtin_ldexpf(1.f, (int)x_exp);
+      }
+      float w[SC], x[SC], xm = 0.f;  // P and P s'
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ones_o[e] *= alpha;
+      for (int i = 0; i < SC; ++i) {
+        w[i] = fast_exp2(__builtin_fmaf(s[i], sl, neg_m));
+        l += w[i];
+        zs = __builtin_fmaf(w[i], vz[i], zs);
+        x[i] = w[i] * x_by * vs[i];
+        xm = fmaxf(xm, __builtin_fabsf(x[i]));
+      }
+      if (__builtin_expect(__any((xm > 0x1p15f) | (o_by < 1.f)), 0)) {
+        float e = -1000.f;
+#pragma unroll
+        for (int i = 0; i < SC; ++i)
+          if (x[i] != 0.f)
+            e = fmaxf(e, (float)(__builtin_amdgcn_frexp_expf(w[i]) + __builtin_amdgcn_frexp_expf(vs[i])));
+        // (the largest P s' is then in 2^9 .. 2^11)
+        const float to = fminf(x_exp, 11.f - most_of(e));
+        o_by *= shrink(to - x_exp);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ones_o[e] *= o_by;
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[f][e] *= alpha;
-      }
-      float x[SC];  // P s'
+          for (int e = 0; e < 4; ++e) o[f][e] *= o_by;
+        x_exp = to;
+        x_by = __builtin_ldexpf(1.f, (int)x_exp);
 #pragma unroll
-      for (int i = 0; i < SC; ++i) {
-        const float w = fast_exp2(__builtin_fmaf(s[i], sl, neg_ref));
-        l += w;
-        x[i] = w * vs[i];
-        zs = __builtin_fmaf(w, vz[i], zs);
-        // (its first term is to be that of the rounded product, which the next is
-        // taken from; the compiler would round the exact one to fp16 for it)
-        if constexpr (PT > 1) asm("" : "+v"(x[i]));
+        for (int i = 0; i < SC; ++i) x[i] = w[i] * x_by * vs[i];
       }
+      // (a term is to be that of the rounded product, which the next is taken from;
+      // the compiler would round the exact one to fp16 for it)
+      if constexpr (PT > 1)
+#pragma unroll
+        for (int i = 0; i < SC; ++i) asm("" : "+v"(x[i]));
       u32x4 pf[PT];
 #pragma unroll
       for (int t = 0; t < PT; ++t)
@@ -672,8 +691,9 @@ qpaged_kernel(const QuantPagedParams p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           mw[(4 * f + e) * 64] =
-              (!R::F32 ? __builtin_fmaf(f & 1 ? -R::ODD : -R::EVEN, ones_o[e], o[f][e]) : o[f][e]) + zs;
-      mw[(FIELDS - 2) * 64] = ref;
+              __builtin_ldexpf(!R::F32 ? __builtin_fmaf(f & 1 ? -R::ODD : -R::EVEN, ones_o[e], o[f][e]) : o[f][e],
+                               -(int)x_exp) + zs;
+      mw[(FIELDS - 2) * 64] = m_ref;
       mw[(FIELDS - 1) * 64] = l;
     }
     __syncthreads();

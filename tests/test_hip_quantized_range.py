@@ -44,6 +44,161 @@ def _off(out, want):
     return (np.linalg.norm(got - want, axis=-1) / np.linalg.norm(want, axis=-1)).max()
 
 
+@pytest.mark.parametrize('dtype', ['bf16', 'f32'])
+@pytest.mark.parametrize('size', [1e20, 3e28])
+def test_constant_rows_beside_one_of_a_tiny_scale(dtype, size):
+    """199 rows of one value (scale 0) and one that is 1e40 times smaller: the sum of
+    the constant rows is no weight times a power that the tiny scale asks for.  The
+    output is the values' mean but for the scores' roundings, which leave the
+    weights' sum what they are: 200 steps of 2^-24 each way and the type's."""
+    t, d = 200, 64
+    v = torch.full((1, t, d), size)
+    v[0, 77] = torch.linspace(0, 1e-19, d)
+    k = torch.randn(1, t, d, generator=torch.Generator().manual_seed(1))
+    pool, table = _written_pool(DT[dtype], k, v, 4)
+    q = _rand((1, 2, d), DT[dtype], 2)
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32([t]), backend='hip')
+    hk, hv = _held(pool, 4)
+    want, rows = plain.attention(_n64(q), hk, hv, table, [t], 0.125)
+    # (the tiny row's weight is off by its score's roundings, 2^-14 or less of it)
+    u = torch.finfo(DT[dtype]).eps / 2
+    assert (np.abs(_n64(out) - want) <= np.abs(want) * (u + 400 * E24 + 2.0 ** -14 / 4)).all()
+
+
+def _float32_pool(lens, hk, d, bits, sizes):
+    """As rows of random values times ``sizes`` (lengths' sum) give."""
+    pool, table = _setup(torch.float32, lens, hk, d, d, 16, bits)
+    x = torch.randn(*pool[2].shape[:3], 2, d, generator=torch.Generator().manual_seed(8))
+    x[..., 1, :] *= sizes
+    top = (1 << bits) - 1
+    lo, hi = x.amin(-1), x.amax(-1)
+    pool[2][..., 0::2] = ((hi - lo) / top).to(pool[2])
+    pool[2][..., 1::2] = lo.to(pool[2])
+    codes = ((x - lo[..., None]) / (hi - lo)[..., None] * top).round().to(torch.uint8)
+    for i in range(2):
+        c = codes[..., i, :]
+        pool[i].copy_(c if bits == 8 else c[..., ::2] | c[..., 1::2] << 4)
+    return pool, table
+
+
+def _float32_off(pool, table, q, lens, bits):
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32(lens), backend='hip')
+    k, v = _held(pool, bits)
+    want, _ = plain.attention(_n64(q), k, v, table, lens, 1 / math.sqrt(q.shape[2]))
+    return max(_off(out[i], want[i]) for i in range(len(lens)))
+
+
+@pytest.mark.parametrize('bits, d', [(4, 64), (8, 64), (8, 128), (4, 256), (8, 32)])
+@pytest.mark.parametrize('ratio', [32, 1024, 2.0 ** 20])
+def test_float32_beside_large_values_of_no_weight(bits, d, ratio):
+    """A few value rows ``ratio`` times larger than the rest, early in the sequence, at
+    scores that leave them no weight: the others keep their digits.  The bound is that
+    of ``test_float32_keeps_its_digits``: (12 d / 128) 2^-22 + 2^-20 + 2^-21 of the
+    norm, for the scores', the exponentials' and the sums' roundings."""
+    lens, hk = [500, 1300], 2
+    held, table = _setup(torch.float32, lens, hk, d, d, 16, bits)
+    sizes = torch.ones(held[2].shape[0], hk, 16, 1)
+    big = [(int(row[0]), s) for row in table for s in (1, 2, 7)]
+    for e, s in big:
+        sizes[e, :, s] = ratio
+    pool, table = _float32_pool(lens, hk, d, bits, sizes)
+    for e, s in big:  # keys of one value: q is positive, so that their scores are -100 or less
+        pool[2][e, :, s, 0], pool[2][e, :, s, 1] = 0, -16
+    q = _rand((2, 2 * hk, d), torch.float32, 5).abs()
+    assert float(16 * q.sum(-1).min() / math.sqrt(d)) > 50
+    off = _float32_off(pool, table, q, lens, bits)
+    assert off <= (12 * d / 128) * 2.0 ** -22 + 2.0 ** -20 + 2.0 ** -21, off
+
+
+@pytest.mark.parametrize('bits, d', [(4, 64), (8, 128)])
+@pytest.mark.parametrize('own', [1.0, 2.0 ** -10])
+def test_float32_tail_of_one_large_score(bits, d, own):
+    """One token of most of the weight and 20000 that share 2^-6 of it, all of one
+    value: their sum keeps its digits though each is 2^-20 of the largest; also where
+    the token's own row is 2^-10 as large, so that the tail is what the output is made
+    of."""
+    n, hk = 20000, 1
+    held, table = _setup(torch.float32, [n], hk, d, d, 16, bits)
+    sizes = torch.ones(held[2].shape[0], hk, 16, 1)
+    first = (int(table[0, 0]), 3)
+    sizes[first[0], :, first[1]] = own
+    pool, table = _float32_pool([n], hk, d, bits, sizes)
+    # (keys of one value each: scores of 0 and of ln(2^20))
+    pool[2][..., :2] = torch.where(torch.isnan(pool[2][..., :2]), math.nan, 0)
+    q = _rand((1, 2, d), torch.float32, 5).abs()
+    q *= math.sqrt(d) / q.sum(-1, keepdim=True)
+    pool[2][first[0], :, first[1], 1] = 20 * math.log(2)
+    # every token of the tail has the value of the first
+    row, one = (int(table[0, 0]), 0, 0), (first[0], 0, first[1])
+    tail = ~torch.isnan(pool[2][..., 0])
+    tail[one] = False
+    pool[1][tail] = pool[1][row].clone()
+    pool[2][..., 2:][tail] = pool[2][row][2:].clone()
+    off = _float32_off(pool, table, q, [n], bits)
+    # (the sums of 20000 equal weights go one way: 157 steps of a wave and the join's)
+    assert off <= (12 * d / 128) * 2.0 ** -22 + 2.0 ** -20 + 2.0 ** -21 + 180 * E24, off
+
+
+@pytest.mark.parametrize('dtype, bits, h, d', [
+    ('bf16', 4, 4, 64), ('f16', 4, 4, 128), ('bf16', 8, 12, 128), ('f16', 8, 2, 256),
+    ('bf16', 4, 2, 40),
+])
+@pytest.mark.parametrize('ratio', [2.0 ** 6, 2.0 ** 12])
+def test_16_bits_beside_large_values_of_no_weight(dtype, bits, h, d, ratio):
+    """As in float32: rows 2^12 times larger (2^24 in bfloat16) at no weight.  Per element
+    the output is off by u of itself and, of the values' sizes w |v|, by the scores'
+    roundings (q within 2^-22 of its largest element: the codes' sum times that, d + 8
+    steps of 2^-24 of a score's terms) and 2^-21 for the weights."""
+    ratio = ratio ** 2 if dtype == 'bf16' else ratio
+    dt, n = DT[dtype], 700
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(1, n, d, generator=g) for _ in range(2))
+    for j in (0, 3, 200):
+        k[0, j] = -16
+        v[0, j] *= ratio
+    pool, table = _written_pool(dt, k, v, bits)
+    q = _rand((1, h, d), dt, 2).abs()
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32([n]), backend='hip')
+    hk, hv = _held(pool, bits)
+    want, rows = plain.attention(_n64(q), hk, hv, table, [n], 1 / math.sqrt(d))
+    kf, vf = (x[:, 0].reshape(-1, d)[:n] for x in (hk, hv))
+    sc = _n64(pool[2])[:, 0].reshape(-1, 4)[:n]
+    qn = _n64(q)[0]
+    u = torch.finfo(dt).eps / 2
+    tiny = 4 * (2.0 ** -24 if dt == torch.float16 else float(torch.finfo(dt).tiny))
+    for i in range(h):
+        w = rows[0, i][0]
+        size = np.abs(kf) + 2 * np.abs(sc[:, 1:2])
+        es = ((d + 8) * E24 * (size @ np.abs(qn[i])) + 2.0 ** -22 * np.abs(qn[i]).max() *
+              size.sum(-1)) / math.sqrt(d)
+        rel = es + (w @ es) + 2.0 ** -21
+        tol = (w * rel) @ (np.abs(vf) + 2 * np.abs(sc[:, 3:])) + u * np.abs(want[0, i])
+        assert (np.abs(_n64(out)[0, i] - want[0, i]) <= tol + tiny).all(), (
+            i, (np.abs(_n64(out)[0, i] - want[0, i]) / (tol + tiny)).max())
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16', 'f32'])
+@pytest.mark.parametrize('step', [0.75, 40.0, -40.0])
+def test_scores_that_climb(dtype, step):
+    """Scores that grow (fall) by ``step`` a token, over hundreds of powers of two, with
+    constant rows (scale 0) among ordinary ones: the last (first) tokens alone are left.
+    Scores are one product, exact but for 2^-22 of itself."""
+    dt, n, d = DT[dtype], 300, 64
+    g = torch.Generator().manual_seed(7)
+    v = torch.randn(1, n, d, generator=g)
+    v[0, ::3] = 2.5
+    v[0, n - 8:n - 2] = -1.5
+    k = (torch.arange(n) * step / 8)[None, :, None].expand(1, n, d)
+    pool, table = _written_pool(dt, k, v, 4)
+    q = torch.full((1, 3, d), 1.0, dtype=dt, device=_dev())
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32([n]), backend='hip')
+    hk, hv = _held(pool, 4)
+    want, _ = plain.attention(_n64(q), hk, hv, table, [n], 0.125)
+    # (weights of tokens with the largest scores, off by those scores' 2^-22)
+    off = 2.0 ** -22 * n * abs(step) * 2 + 2.0 ** -19
+    assert np.abs(_n64(out) - want).max() <= (off + torch.finfo(dt).eps / 2) * 4
+
+
 @pytest.mark.parametrize('dtype, bits, h, d, ps', [
     ('f16', 4, 4, 128, 16), ('f16', 8, 12, 128, 16), ('f16', 4, 2, 256, 12), ('bf16', 4, 4, 64, 16),
     ('bf16', 8, 2, 256, 16), ('f16', 8, 3, 80, 24),

@@ -18,16 +18,17 @@
 //    that.  (fp8 numbers need no 64, c 2^-9 being their bits, and 2 operations less for
 //    8 codes.  But their products keep 13 bits below the largest of eight and drop
 //    the others' rest, and q takes two or three of them.)
-//  * V: codes in the mantissa of an fp16 64 (in bits 4 .. 7, where an element's odd
-//    codes are already) or 1024 (bits 0 .. 3, or 0 .. 7).  What is added to them is
-//    taken off at the end, by a product of ones with the very P s' that the other
-//    products saw.  P s' is one fp16 number (bf16: off by 2^-12) or two (fp16: 2^-23),
-//    times a power of two that keeps the largest of them near the top of fp16's range.
-//  * fp32: what is added to the codes, and their minima, would cost digits: the values
-//    of a long row nearly cancel, to a root of its length, while those sums do not (8192
-//    tokens in 8 bits were off by 1.5e-5 of the output, now 4e-7).  So K's and V's codes are
-//    fp16 numbers from -8 or -128 on, one packed addition more, what they are counted
-//    from is (s 8 + z) or (s 128 + z), and q and P s' are three fp16 numbers each.
+//  * V: the same, in pairs of one column's keys.  What is added to the codes would cost
+//    digits: the values of a long row nearly cancel, to a root of its length, while
+//    their sum with 64 or 1024 does not (65536 tokens of equal weight in bf16 and 4 bits were
+//    off by 2.8e-2 of the output, 1.8e-3 now, its own rounding).  So it comes off every
+//    four steps, with the codes' middle, by a product of ones with the very P s' that the
+//    other products saw; the rest of a value is s 8 + z (s 128 + z).  P s' is one fp16
+//    number (bf16: off by 2^-12) or two (fp16: 2^-23), times a power of two that keeps
+//    the largest of them near the top of fp16's range.
+//  * fp32: four steps' sums of 64s would cost digits too.  So K's and V's codes are fp16
+//    numbers from -8 or -128 on, one packed addition more, what they are counted from is
+//    (s 8 + z) or (s 128 + z), and q and P s' are three fp16 numbers each.
 //
 // The blocks share the work as in nxa_paged.hip (units of 128 tokens, pieces of
 // a row joined by its second kernel).  A step of a wave is 32 tokens, two halves
@@ -65,11 +66,8 @@ struct QuantStep {
   static constexpr int NS = ES;                     // dwords of a token's scales: 4 ES / 4
   static constexpr int QT = F32 ? 3 : 1;            // terms of q
   static constexpr int PT = F32 ? 3 : F16 ? 2 : 1;  // of P s'
-  static constexpr float MID = !F32 ? 0.f : BITS == 4 ? 8.f : 128.f;  // codes count from it
-  static constexpr float ZERO = BITS == 4 ? 64.f : 1024.f;  // what stands in for 0 in K (16 bits)
-  // and in V's even and odd columns.
-  static constexpr float EVEN = BITS == 8 || !(F32 || F16) ? 1024.f : 64.f;
-  static constexpr float ODD = BITS == 8 ? 1024.f : 64.f;
+  static constexpr float MID = BITS == 4 ? 8.f : 128.f;     // V's codes count from it (fp32: K's too)
+  static constexpr float ZERO = BITS == 4 ? 64.f : 1024.f;  // what stands in for 0 (16-bit types)
   // A half in LDS: K's codes, V's, the scales; copies of 1 KB (scales: 256 bytes).
   static constexpr int KC = DP * BITS <= 512 ? 1 : DP * BITS / 512;
   static constexpr int HALF_BYTES = 2 * 1024 * KC + 256;
@@ -126,9 +124,8 @@ __device__ __forceinline__ float high_f16(uint32_t w) {
 // Constants of the codes' masks, kept in registers of both kinds, so that an and
 // and an or are one operation (two constants of it cannot both be literals).
 struct CodeBits {
-  uint32_t low, high, k1024, k64, from64, from1024;
+  uint32_t high, k1024, k64, from64, from1024;
   __device__ __forceinline__ CodeBits() {
-    asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
     asm("v_mov_b32 %0, 0x64006400" : "=v"(k1024));
     asm("v_mov_b32 %0, 0x54005400" : "=v"(k64));
@@ -184,11 +181,10 @@ __device__ __forceinline__ float other_eight(float x) {
   return __uint_as_float(other_eight(__float_as_uint(x)));
 }
 
-// What a row's codes, as a product has them, count from.
+// What the middle of a row's codes stands for.
 template <typename T, int BITS>
 __device__ __forceinline__ float from_mid(float s, float z) {
-  using R = QuantStep<T, 16, BITS>;
-  return R::MID == 0.f ? z : __builtin_fmaf(s, R::MID, z);
+  return __builtin_fmaf(s, QuantStep<T, 16, BITS>::MID, z);
 }
 // Scales of a token: fields k's scale and minimum, v's.
 template <typename T, int N>
@@ -488,7 +484,7 @@ qpaged_kernel(const QuantPagedParams p) {
         const auto& sc = r[i / 4].s[i % 4];
         // (a scale of infinity makes its token NaN, whatever the signs)
         const float ks = scale_field<T>(sc, 0);
-        const float kz = from_mid<T, BITS>(ks, scale_field<T>(sc, 1));
+        const float z = scale_field<T>(sc, 1), kz = R::F32 ? from_mid<T, BITS>(ks, z) : z;
         const float dot = PAIR && upper ? dots[1][i % 4] : dots[i / 4][i % 4];
         s[i] = __builtin_fmaf(dot, ks, __builtin_fmaf(kz, qsum, ks * 0.f));
         vs[i] = scale_field<T>(sc, 2);
@@ -590,7 +586,7 @@ qpaged_kernel(const QuantPagedParams p) {
               a[i] = t[i] | cb.k1024;
               if constexpr (R::F32) a[i] = add_f16(a[i], cb.from1024);
             } else {
-              a[i] = R::EVEN == 1024.f ? (t[i] & cb.low) | cb.k1024 : (t[i] << 4 & cb.high) | cb.k64;
+              a[i] = (t[i] << 4 & cb.high) | cb.k64;
               d[i] = (t[i] & cb.high) | cb.k64;
               if constexpr (R::F32) a[i] = add_f16(a[i], cb.from64), d[i] = add_f16(d[i], cb.from64);
             }
@@ -603,8 +599,18 @@ qpaged_kernel(const QuantPagedParams p) {
           }
         }
     };
+    // What stands in for 0 and the codes' middle off O (16-bit types): before every
+    // fourth step, so that the sums stay as small as the values they are made of.
+    auto settle = [&]() NXA_INLINE {
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[f][e] = __builtin_fmaf(-(R::ZERO + R::MID), ones_o[e], o[f][e]);
+      ones_o = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
     if constexpr (FAST) {
-      for (int i = 0; i < steps; i += NB)
+      for (int i = 0; i < steps; i += NB) {
+        if (!R::F32 && i % 4 == 0) settle();
 #pragma unroll
         for (int x = 0; x < NB; ++x) {
           // (the copies of the steps behind it may be in flight)
@@ -629,9 +635,11 @@ qpaged_kernel(const QuantPagedParams p) {
             for (int h = 0; h < 2; ++h) issue(ring + x * STEP_BYTES + h * R::HALF_BYTES, have[x][h]);
           });
         }
+      }
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     } else {
       for (int i = 0; i < steps; ++i) {
+        if (!R::F32 && i % 4 == 0) settle();
         Half r[2];
         int mine[2];
 #pragma unroll
@@ -672,6 +680,7 @@ qpaged_kernel(const QuantPagedParams p) {
         compute(r, mine, [] {});
       }
     }
+    if constexpr (!R::F32) settle();
     l += xor16(l);
     l += shfl_xor32(l);
     zs += xor16(zs);
@@ -690,9 +699,7 @@ qpaged_kernel(const QuantPagedParams p) {
       for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          mw[(4 * f + e) * 64] =
-              __builtin_ldexpf(!R::F32 ? __builtin_fmaf(f & 1 ? -R::ODD : -R::EVEN, ones_o[e], o[f][e]) : o[f][e],
-                               -(int)x_exp) + zs;
+          mw[(4 * f + e) * 64] = __builtin_ldexpf(o[f][e], -(int)x_exp) + zs;
       mw[(FIELDS - 2) * 64] = m_ref;
       mw[(FIELDS - 1) * 64] = l;
     }

@@ -245,3 +245,31 @@ def test_q_next_to_the_largest_number(dtype):
     # (scores below 2^4, off by 16 2^-24 of their terms; values below 4)
     u = torch.finfo(dt).eps / 2
     assert (np.abs(_n64(out) - want) <= u * np.abs(want) + 4 * 2.0 ** -15).all()
+
+
+@pytest.mark.parametrize('dtype, bits, h', [('bf16', 4, 1), ('f16', 4, 1), ('bf16', 8, 1), ('f16', 8, 1),
+                                            ('bf16', 4, 12)])
+def test_long_even_rows_nearly_cancel(dtype, bits, h):
+    """65536 tokens of equal weight, whose values are random: the output is 1/256 of
+    them, and a block takes a whole row, 512 steps a wave (96 sequences of the same
+    pages).  Of the codes' sum each step may lose 2^-24 of itself; these are random
+    but for half of one, a few 2^-24 sqrt(512) in all: 2^-17 of the values' size, 2^-9 of
+    the output's, beside its own rounding u."""
+    dt, n, hk, d, ps = DT[dtype], 65536, 8, 64, 128
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(2, hk, n, d, generator=g)
+    pool, table = _written_pool(dt, x[0], x[1], bits, ps)
+    rows = 96
+    q = torch.zeros(rows, hk * h, d, dtype=dt, device=_dev())
+    t = _i32(np.repeat(table, rows, 0))
+    out = nx.quantized_paged_attention(q, *pool, t, _i32([n] * rows), backend='hip')
+    assert torch.equal(out[0], out[rows - 1])
+    top = (1 << bits) - 1
+    sc = pool[2].double()
+    c = pool[1] if bits == 8 else torch.stack((pool[1] & 15, pool[1] >> 4), -1).flatten(-2)
+    held = c.double() * sc[..., 2, None] + sc[..., 3, None]
+    want = held.transpose(0, 1).reshape(hk, n, d).mean(1).cpu().numpy().repeat(h, 0)
+    u = torch.finfo(dt).eps / 2
+    off = _off(out[0], want)
+    print(f'[case] off {off:.2e} at {top} codes', flush=True)
+    assert off <= u + 2.0 ** -9, off

@@ -23,9 +23,10 @@
 //    their sum with 64 or 1024 does not (65536 tokens of equal weight in bf16 and 4 bits were
 //    off by 2.8e-2 of the output, 1.8e-3 now, its own rounding).  So it comes off every
 //    four steps, with the codes' middle, by a product of ones with the very P s' that the
-//    other products saw; the rest of a value is s 8 + z (s 128 + z).  P s' is one fp16
-//    number (bf16: off by 2^-12) or two (fp16: 2^-23), times a power of two that keeps
-//    the largest of them near the top of fp16's range.
+//    other products saw; the rest of a value is s 8 + z (s 128 + z).  P s' is two fp16
+//    numbers (off by 2^-23; one, in bf16, would take 2 us of 49 less and be off by
+//    2^-12), times a power of two that keeps the largest of them near the top of
+//    fp16's range.
 //  * fp32: four steps' sums of 64s would cost digits too.  So K's and V's codes are fp16
 //    numbers from -8 or -128 on, one packed addition more, what they are counted from is
 //    (s 8 + z) or (s 128 + z), and q and P s' are three fp16 numbers each.
@@ -65,7 +66,7 @@ struct QuantStep {
   static constexpr int NVW = VB >= 4 ? VB / 4 : 1;  // dwords
   static constexpr int NS = ES;                     // dwords of a token's scales: 4 ES / 4
   static constexpr int QT = F32 ? 3 : 1;            // terms of q
-  static constexpr int PT = F32 ? 3 : F16 ? 2 : 1;  // of P s'
+  static constexpr int PT = F32 ? 3 : 2;            // of P s'
   static constexpr float MID = BITS == 4 ? 8.f : 128.f;     // V's codes count from it (fp32: K's too)
   static constexpr float ZERO = BITS == 4 ? 64.f : 1024.f;  // what stands in for 0 (16-bit types)
   // A half in LDS: K's codes, V's, the scales; copies of 1 KB (scales: 256 bytes).

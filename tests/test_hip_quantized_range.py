@@ -177,6 +177,34 @@ def test_16_bits_beside_large_values_of_no_weight(dtype, bits, h, d, ratio):
             i, (np.abs(_n64(out)[0, i] - want[0, i]) / (tol + tiny)).max())
 
 
+@pytest.mark.parametrize('dtype, bits, h', [
+    ('bf16', 4, 4), ('f16', 4, 4), ('f32', 4, 4), ('bf16', 8, 12), ('f16', 8, 1), ('f32', 8, 12),
+])
+def test_rows_of_every_size(dtype, bits, h):
+    """Value rows times powers of two over most of the type's range, at scores of some
+    3, so that a few rows make the output.  Per element: the weights within 2^-19 (a
+    score's and its exponential's roundings) of what they are, of the values' sizes w
+    |v|, the sums 2^-20 of the largest w s' times the codes, and u of the output."""
+    dt, n, d = DT[dtype], 500, 64
+    g = torch.Generator().manual_seed(7)
+    k, v = (torch.randn(1, n, d, generator=g) for _ in range(2))
+    span = 9 if dtype == 'f16' else 80
+    v *= 2.0 ** torch.randint(-span, span + 1, (1, n, 1), generator=g)
+    pool, table = _written_pool(dt, k, v, bits)
+    q = _rand((1, h, d), dt, 2)
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32([n]), backend='hip')
+    hk, hv = _held(pool, bits)
+    want, rows = plain.attention(_n64(q), hk, hv, table, [n], 0.125)
+    vf, sc = hv[:, 0].reshape(-1, d)[:n], _n64(pool[2])[:, 0].reshape(-1, 4)[:n]
+    u = torch.finfo(dt).eps / 2
+    for i in range(h):
+        w = rows[0, i][0]
+        tol = 2.0 ** -19 * (w @ (np.abs(vf) + 2 * np.abs(sc[:, 3:]))) + u * np.abs(want[0, i])
+        tol += 2.0 ** -20 * (w * sc[:, 2]).max() * (15 if bits == 4 else 255) + 2.0 ** -24 * (span == 9)
+        assert (np.abs(_n64(out)[0, i] - want[0, i]) <= tol).all(), (
+            i, (np.abs(_n64(out)[0, i] - want[0, i]) / tol).max())
+
+
 @pytest.mark.parametrize('dtype', ['bf16', 'f16', 'f32'])
 @pytest.mark.parametrize('step', [0.75, 40.0, -40.0])
 def test_scores_that_climb(dtype, step):
@@ -273,3 +301,21 @@ def test_long_even_rows_nearly_cancel(dtype, bits, h):
     off = _off(out[0], want)
     print(f'[case] off {off:.2e} at {top} codes', flush=True)
     assert off <= u + 2.0 ** -9, off
+
+
+@pytest.mark.parametrize('dtype, bits', [('bf16', 4), ('f16', 4), ('bf16', 8), ('f16', 8)])
+def test_weights_are_pairs(dtype, bits):
+    """Two tokens of nearly equal weights and opposite values, of which a hundredth is
+    left: weights are held within 2^-22, the sums lose 2^-24 a few times, and the output
+    is off by 2^-20 of the values' sizes beside u of itself."""
+    dt, d = DT[dtype], 64
+    v = torch.randn(1, 2, d, generator=torch.Generator().manual_seed(7))
+    v[0, 1] = -v[0, 0]
+    k = torch.tensor([0.0, 0.02])[None, :, None].expand(1, 2, d)
+    pool, table = _written_pool(dt, k, v, bits)
+    q = torch.full((1, 2, d), 0.125, dtype=dt, device=_dev())
+    out = nx.quantized_paged_attention(q, *pool, _i32(table), _i32([2]), backend='hip')
+    hk, hv = _held(pool, bits)
+    want, _ = plain.attention(_n64(q), hk, hv, table, [2], 0.125)
+    tol = 2.0 ** -20 * 2 * np.abs(hv).max() + torch.finfo(dt).eps / 2 * np.abs(want)
+    assert (np.abs(_n64(out) - want) <= tol).all()

@@ -329,9 +329,9 @@ qpaged_kernel(const QuantPagedParams p) {
       const bool ok = half < 2 * steps && (unsigned)page < (unsigned)p.P;
       mine = ok ? max(min(kHalfKeys, len - key0), 0) : 0;
       const uint64_t pg = ok ? (uint32_t)page : 0u;
-      const int sl = ok ? slot : 0;
-      const char* ks = kp + pg * (uint32_t)p.k16 * 16 + sl * kb;
-      const char* vs = vp + pg * (uint32_t)p.v16 * 16 + sl * vb;
+      const uint64_t sl = ok ? (uint32_t)slot : 0u;  // (times a row's bytes: past 32 bits)
+      const char* ks = kp + pg * (uint32_t)p.k16 * 16 + sl * (uint32_t)kb;
+      const char* vs = vp + pg * (uint32_t)p.v16 * 16 + sl * (uint32_t)vb;
       const char* ss = sp + pg * (uint32_t)p.s16 * 16 + sl * (4 * R::ES);
       // The next half: in this step, or at the same place 128 tokens on.
       ++half;

@@ -319,3 +319,26 @@ def test_weights_are_pairs(dtype, bits):
     want, _ = plain.attention(_n64(q), hk, hv, table, [2], 0.125)
     tol = 2.0 ** -20 * 2 * np.abs(hv).max() + torch.finfo(dt).eps / 2 * np.abs(want)
     assert (np.abs(_n64(out) - want) <= tol).all()
+
+
+def test_a_page_past_2_31_bytes():
+    """One page of more than 2^23 slots of 256 bytes: the last tokens' rows start past
+    2^31 bytes of it.  Their keys alone have a score (200), so that they alone count."""
+    ps, d, dv, tail = (1 << 23) + 4096, 256, 16, 40
+    k = torch.zeros(2, 1, ps, d, dtype=torch.uint8, device=_dev())
+    v = torch.zeros(2, 1, ps, dv, dtype=torch.uint8, device=_dev())
+    sc = torch.zeros(2, 1, ps, 4, dtype=torch.bfloat16, device=_dev())
+    new = [_rand((1, tail, n), torch.bfloat16, s) for n, s in ((d, 1), (dv, 2))]
+    n = ps - 3
+    table, start, off = _i32([[1]]), _i32([n - tail]), _i32([0, tail])
+    nx.write_quantized_pages(k, v, sc, *new, table, start, off, backend='hip')
+    sc[1, 0, n - tail:n, 1] += 200 / 16
+    q = torch.ones(1, 2, d, dtype=torch.bfloat16, device=_dev())
+    out = nx.quantized_paged_attention(q, k, v, sc, table, _i32([n]), backend='hip')
+    near = [x[1:, :, n - tail:n].cpu() for x in (k, v, sc)]
+    hk, hv = _held(near, 8)
+    want, _ = plain.attention(_n64(q), hk, hv, np.array([[0]]), [tail], 1 / 16)
+    # (scores of 200, 264 steps of 2^-24 of them)
+    assert np.abs(_n64(out) - want).max() <= 4 * (2.0 ** -8 + 264 * 200 * E24)
+    got = nx.read_quantized_pages(k, v, sc, table, start, off, tail, bits=8, backend='hip')
+    assert np.abs(_n64(got[1])[0] - hv[0, 0]).max() <= 2.0 ** -8 * 4

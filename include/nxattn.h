@@ -365,7 +365,7 @@ int nxa_paged_fwd(const nxa_pool_desc* desc, const void* k_pages, const void* v_
  * pages.  With offsets (B + 1, as nxa_packed_desc) token t of sequence s goes
  * to position starts[s] + t - offsets[s]; without (T = B) token s to
  * starts[s].  Tokens of no sequence, outside the table or in no page are
- * dropped.  T < 2^26.  Of tokens meant for one slot (rows that share a page there) either
+ * dropped.  T <= 2^26 - 4.  Of tokens meant for one slot (rows that share a page there) either
  * may stay, by 16-byte chunks. */
 int nxa_pages_write(const nxa_pool_desc* desc, void* k_pages, void* v_pages, const void* k,
                     const int64_t* k_str, const void* v, const int64_t* v_str, int64_t T,

@@ -8,8 +8,8 @@ namespace {
 
 // (page and slot numbers plus what a block steps by stay in 31 bits)
 constexpr int kMostPages = 1 << 30;
-// (a grid holds less than 2^32 threads: 64 a token written, 256 a listed row)
-constexpr int kMostTokens = 1 << 26, kMostListed = 1 << 24;
+// (a grid holds less than 2^32 threads: 256 for four tokens written, 256 a listed row)
+constexpr int kMostTokens = (1 << 26) - 4, kMostListed = 1 << 24;
 
 int check_pool(const nxa_pool_desc* d) {
   if (!d) return fail(NXA_E_ARG, "pool descriptor is NULL");
@@ -287,8 +287,8 @@ int nxa_pages_write(const nxa_pool_desc* d, void* k_pages, void* v_pages, const 
   if (rc) return rc;
   if (!table || !starts || !k_str || !v_str)
     return fail(NXA_E_ARG, "table, starts and the strides must not be NULL");
-  if (T <= 0 || T >= kMostTokens)
-    return fail(NXA_E_SHAPE, "T=%lld: 1 to 2^26 - 1 tokens a call", (long long)T);
+  if (T <= 0 || T > kMostTokens)
+    return fail(NXA_E_SHAPE, "T=%lld: 1 to 2^26 - 4 tokens a call", (long long)T);
   if (!offsets && T != B)
     return fail(NXA_E_SHAPE, "without offsets one token a sequence is written: T=%lld, B=%d",
                 (long long)T, B);

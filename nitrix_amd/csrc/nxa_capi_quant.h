@@ -66,8 +66,8 @@ int quant_move(const char* name, bool write, const nxa_quant_pool_desc* d, const
   if (rc) return rc;
   if (!table || !starts || !k_str || !v_str)
     return fail(NXA_E_ARG, "table, starts and the strides must not be NULL");
-  if (T <= 0 || T >= kMostTokens)
-    return fail(NXA_E_SHAPE, "T=%lld: 1 to 2^26 - 1 tokens a call", (long long)T);
+  if (T <= 0 || T > kMostTokens)
+    return fail(NXA_E_SHAPE, "T=%lld: 1 to 2^26 - 4 tokens a call", (long long)T);
   if (!offsets && T != B)
     return fail(NXA_E_SHAPE, "without offsets there is one token a sequence: T=%lld, B=%d",
                 (long long)T, B);

@@ -1,0 +1,43 @@
+"""The largest calls of the paged caches and the rotary positions: refused before
+anything is launched where a grid or a number would not hold them (CPU only)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import nitrix_amd as nx
+from nitrix_amd import _lib
+
+OK = 1 << 20  # a pointer that no check looks behind
+
+
+def _quant(Hk=2, PS=16, D=64, Dv=64):
+    d = _lib.NxaQuantPoolDesc()
+    d.P, d.Hk, d.PS, d.D, d.Dv, d.io_dtype, d.bits = 8, Hk, PS, D, Dv, _lib.NXA_BF16, 4
+    d.k_str[:] = (Hk * PS * D // 2, PS * D // 2)
+    d.v_str[:] = (Hk * PS * Dv // 2, PS * Dv // 2)
+    d.s_str[:] = (Hk * PS * 4, PS * 4)
+    return d
+
+
+def _plain(Hk=2, PS=16, D=64, Dv=64):
+    d = _lib.NxaPoolDesc()
+    d.P, d.Hk, d.PS, d.D, d.Dv, d.io_dtype = 8, Hk, PS, D, Dv, _lib.NXA_BF16
+    d.k_str[:] = (Hk * PS * D, PS * D, D)
+    d.v_str[:] = (Hk * PS * Dv, PS * Dv, Dv)
+    return d
+
+
+@pytest.mark.parametrize('t', [(1 << 26) - 3, (1 << 26) - 1])
+def test_tokens_whose_grid_has_2_32_threads(t):
+    """Four tokens a block of 256 threads: 2^24 blocks are one too many."""
+    lib, s2 = _lib.lib(), _lib.I64x2(64, 128)
+    q, p = ctypes.byref(_quant()), ctypes.byref(_plain())
+    for move in (lib.nxa_quant_write, lib.nxa_quant_read):
+        assert move(q, OK, OK, OK, OK, s2, OK, s2, t, OK, 3, OK, OK, 2, 3,
+                    None) == _lib.NXA_E_SHAPE
+    assert lib.nxa_pages_write(p, OK, OK, OK, s2, OK, s2, t, OK, 3, OK, OK, 2, 3,
+                               None) == _lib.NXA_E_SHAPE

@@ -353,8 +353,8 @@ int nxa_pool_check(const nxa_pool_desc* desc);
  * v over the first lengths[b] tokens of sequence b (at most M * PS; a negative
  * length is zero), key-value head h / (H / Hk).  q [B, H, D], o [B, H, Dv]
  * with sequence and head strides.  Tokens in no page take no part; a row
- * without tokens (or whose scores are all -inf) is zero.  The workspace
- * (16-byte aligned) is scratch of one call. */
+ * without tokens (or whose scores are all -inf) is zero.  H * Dv <= 2^31 - 256.
+ * The workspace (16-byte aligned) is scratch of one call. */
 size_t nxa_paged_workspace_bytes(const nxa_pool_desc* desc, int32_t B, int32_t M, int32_t H);
 int nxa_paged_fwd(const nxa_pool_desc* desc, const void* k_pages, const void* v_pages,
                   const void* q, const int64_t* q_str, const int32_t* table, int64_t table_rs,

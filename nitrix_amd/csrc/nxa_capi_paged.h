@@ -59,10 +59,13 @@ struct PagedPlan {
   int strips, nblk;
 };
 
-int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t, int64_t), int most,
-               int start, PagedPlan* plan) {
+int plan_paged(int Hk, int PS, int Dv, int B, int M, int H, bool (*whole)(int64_t, int64_t),
+               int most, int start, PagedPlan* plan) {
   if (H <= 0 || H % Hk != 0)
     return fail(NXA_E_SHAPE, "H=%d must be a positive multiple of Hk=%d", H, Hk);
+  // (zeros of a sequence without tokens are counted in 31 bits, 256 at a time)
+  if ((int64_t)H * Dv > ((int64_t)1 << 31) - 256)
+    return fail(NXA_E_SHAPE, "H=%d heads of %d: more than 2^31 - 256 elements a sequence", H, Dv);
   plan->strips = (H / Hk + 15) / 16;
   // Units of the largest table, in 31 bits a head.
   const int64_t room = (int64_t)M * PS;
@@ -80,7 +83,7 @@ int plan_paged(int Hk, int PS, int B, int M, int H, bool (*whole)(int64_t, int64
 
 int plan_paged(const nxa_pool_desc* d, int B, int M, int H, PagedPlan* plan) {
   return plan_paged(
-      d->Hk, d->PS, B, M, H, [](int64_t room, int64_t) { return nxa::paged_whole(room); },
+      d->Hk, d->PS, d->Dv, B, M, H, [](int64_t room, int64_t) { return nxa::paged_whole(room); },
       nxa::kPagedBlocks, nxa::kStartUnits, plan);
 }
 

@@ -100,12 +100,9 @@ int plan_quant_paged(const nxa_quant_pool_desc* d, int B, int M, int H, PagedPla
   // (a wave steps past a row's last token: what it adds stays in 31 bits)
   if ((int64_t)M * d->PS >= ((int64_t)1 << 31) - 4096)
     return fail(NXA_E_SHAPE, "a row of %d pages of %d tokens has room for 2^31 or more", M, d->PS);
-  // (zeros of a sequence without tokens are counted in 31 bits)
-  if ((int64_t)H * d->Dv >= (int64_t)1 << 31)
-    return fail(NXA_E_SHAPE, "H=%d heads of %d: 2^31 elements a sequence or more", H, d->Dv);
   const int most = nxa::qpaged_blocks(d->io_dtype, nxa::qpaged_dp(d->D > d->Dv ? d->D : d->Dv),
                                       d->bits);
-  return plan_paged(d->Hk, d->PS, B, M, H, nxa::qpaged_whole, most, nxa::kQuantStart,
+  return plan_paged(d->Hk, d->PS, d->Dv, B, M, H, nxa::qpaged_whole, most, nxa::kQuantStart,
                     plan);
 }
 

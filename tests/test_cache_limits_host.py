@@ -41,3 +41,20 @@ def test_tokens_whose_grid_has_2_32_threads(t):
                     None) == _lib.NXA_E_SHAPE
     assert lib.nxa_pages_write(p, OK, OK, OK, s2, OK, s2, t, OK, 3, OK, OK, 2, 3,
                                None) == _lib.NXA_E_SHAPE
+
+
+@pytest.mark.parametrize('h', [(1 << 23) - 1, 1 << 23, (1 << 23) + 1, 1 << 24])
+def test_heads_whose_zeros_pass_2_31(h):
+    """A sequence without tokens is zeroed by 256 threads, whose count of H Dv
+    elements steps past the last by up to 255."""
+    lib, s2 = _lib.lib(), _lib.I64x2(64, 128)
+    q, p = (ctypes.byref(f(Hk=1, D=256, Dv=256)) for f in (_quant, _plain))
+    fits = h * 256 <= (1 << 31) - 256
+    # (a table of 2 pages: a block a row in each, no workspace; of 200: some)
+    assert (lib.nxa_quant_paged_workspace_bytes(q, 1, 200, h) > 0) == fits
+    assert (lib.nxa_paged_workspace_bytes(p, 1, 200, h) > 0) == fits
+    if not fits:
+        assert lib.nxa_quant_paged_fwd(q, OK, OK, OK, OK, s2, OK, 2, OK, 1, 2, h, 1.0, OK, s2, None,
+                                       0, None) == _lib.NXA_E_SHAPE
+        assert lib.nxa_paged_fwd(p, OK, OK, OK, s2, OK, 2, OK, 1, 2, h, 1.0, OK, s2, None, 0,
+                                 None) == _lib.NXA_E_SHAPE

@@ -258,6 +258,9 @@ def _reference_paged(q, k_pages, v_pages, page_table, lengths, scale):
 
 def _paged_hip(q, k_pages, v_pages, page_table, lengths, scale):
     _check_fused(k_pages, v_pages, q)
+    b, h, _ = q.shape
+    if (b | h) >> 31:
+        raise HipNotTileable('fused paged attention numbers sequences and heads in 31 bits.')
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k_pages, v_pages)):
         raise HipNotTileable('fused paged attention has no backward pass.')
     if _has_tangent(q, k_pages, v_pages):
@@ -266,7 +269,6 @@ def _paged_hip(q, k_pages, v_pages, page_table, lengths, scale):
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
     lengths = lengths.contiguous()
-    b, h, _ = q.shape
     m = page_table.shape[1]
     o = _empty_like(q, v_pages.shape[3])
     lib = _lib.lib()

@@ -310,6 +310,9 @@ def _reference_attention(q, k_pages, v_pages, scales, page_table, lengths, scale
 
 def _attention_hip(q, k_pages, v_pages, scales, page_table, lengths, scale, bits):
     _check_dtype(scales, q)
+    b, h, _ = q.shape
+    if (b | h) >> 31:
+        raise HipNotTileable('fused quantised attention numbers sequences and heads in 31 bits.')
     if torch.is_grad_enabled() and (q.requires_grad or scales.requires_grad):
         raise HipNotTileable('fused quantised attention has no backward pass.')
     if _has_tangent(q, scales):
@@ -319,7 +322,6 @@ def _attention_hip(q, k_pages, v_pages, scales, page_table, lengths, scale, bits
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
     lengths = lengths.contiguous()
-    b, h, _ = q.shape
     m = page_table.shape[1]
     o = _empty_like(q, desc.Dv)
     lib, at = _lib.lib(), ctypes.byref(desc)

@@ -298,6 +298,9 @@ def _rotary_hip(q, k, positions, frequencies, interleaved, scale):
         raise HipNotTileable(
             f'fused rotary positions take head dims up to {_MAX_ROTARY_DIM}; got {shape[-1]}.'
         )
+    if q.numel() >> 31 and max(math.prod(shape[:-3]), *shape[-3:]) >> 31 or (
+            k is not None and k.shape[-3] >> 31):
+        raise HipNotTileable('fused rotary positions number sequences, heads and tokens in 31 bits.')
     if _has_tangent(q, k):
         raise HipNotTileable('fused rotary positions have no forward-mode derivative.')
     _lib.lib()  # a missing library is an error here, not a fallback

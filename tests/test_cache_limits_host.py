@@ -58,3 +58,31 @@ def test_heads_whose_zeros_pass_2_31(h):
                                        0, None) == _lib.NXA_E_SHAPE
         assert lib.nxa_paged_fwd(p, OK, OK, OK, s2, OK, 2, OK, 1, 2, h, 1.0, OK, s2, None, 0,
                                  None) == _lib.NXA_E_SHAPE
+
+
+def test_extents_past_31_bits_are_declined():
+    """The C ABI's extents are 32-bit: 2^32 + 1 must not arrive as 1 (expanded
+    tensors, so that nothing is that large)."""
+    from nitrix_amd import paged, quantized, rotary
+    from nitrix_amd.attention import HipNotTileable
+
+    most, bf16 = (1 << 32) + 1, torch.bfloat16
+    x = torch.zeros(1, 1, 1, 8, dtype=bf16)
+    pos, freq = torch.zeros(1, dtype=torch.int32), torch.ones(4, dtype=torch.float64)
+    for q, k in (
+        (x.expand(most, 1, 1, 8), None), (x.expand(1, most, 1, 8), None),
+        (x.expand(1, 1, most, 8), None), (x[0], x[0].expand(most, 1, 8)),
+        (x.expand(1 << 16, 1, 1, 8)[:, None].expand(1 << 16, 1 << 16, 1, 1, 8), None),
+    ):
+        p = pos.expand(q.shape[-2])
+        with pytest.raises(HipNotTileable, match='31 bits'):
+            rotary._rotary_hip(q, k, p, freq, False, 1.0)
+    pages = torch.zeros(2, 1, 16, 8, dtype=bf16)
+    codes, sc = torch.zeros(2, 1, 16, 8, dtype=torch.uint8), torch.zeros(2, 1, 16, 4, dtype=bf16)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    for b, h in ((most, 1), (1, most)):
+        q, t, n = x[0].expand(b, h, 8), table.expand(b, 1), pos.expand(b)
+        with pytest.raises(HipNotTileable, match='31 bits'):
+            paged._paged_hip(q, pages, pages, t, n, 1.0)
+        with pytest.raises(HipNotTileable, match='31 bits'):
+            quantized._attention_hip(q, codes, codes, sc, t, n, 1.0, 8)

@@ -267,7 +267,12 @@ class _RotaryHip(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.args = (interleaved, scale, not inverse)
         ctx.save_for_backward(positions, frequencies)
-        return _turn(q, k, positions, frequencies, interleaved, scale, inverse)
+        out = _turn(q, k, positions, frequencies, interleaved, scale, inverse)
+        # (keys of a frozen projection beside queries that are trained)
+        ctx.mark_non_differentiable(*(
+            y for y, need in zip(out, ctx.needs_input_grad) if y is not None and not need
+        ))
+        return out
 
     @staticmethod
     def backward(ctx, dq, dk):

@@ -259,3 +259,24 @@ def test_declined_calls_fall_back_loudly():
     assert y.requires_grad and y.dtype == torch.float64
     empty = nx.rotary_embed(wide[:, :0], None, pos[:0], freq)[0]
     assert empty.shape == (1, 0, 264)
+
+
+def test_only_what_is_trained_has_a_gradient():
+    """As in the other engine: the output of an input without a gradient has none,
+    and may go into a cache."""
+    h, t, d = 2, 5, 16
+    freq, pos = nx.rotary_frequencies(d, device=_dev()), torch.arange(t, device=_dev())
+    for which in range(2):
+        x = [_rand((h, t, d), torch.float32, s) for s in (1, 2)]
+        x[which].requires_grad_(True)
+        for backend in ('hip', 'jax'):
+            out = nx.rotary_embed(*x, pos, freq, backend=backend)
+            assert [y.requires_grad for y in out] == [which == 0, which == 1]
+            out[which].sum().backward()
+    pages = [torch.zeros(1, h, 16, d, device=_dev()) for _ in range(2)]
+    i32 = dict(dtype=torch.int32, device=_dev())
+    q, k = (_rand((h, t, d), torch.float32, s) for s in (1, 2))
+    _, turned = nx.rotary_embed(q.requires_grad_(True), k, pos, freq, backend='hip')
+    nx.write_pages(*pages, turned, k, torch.zeros(1, 1, **i32), torch.zeros(1, **i32),
+                   torch.tensor([0, t], **i32), backend='hip')
+    assert torch.equal(pages[0][0, :, :t], turned)

@@ -8,8 +8,9 @@
 // Bound by HBM: 6 operations on 4 bytes read and 4 written (16 bits).  What
 // could cost more is the sine and cosine of each pair, which all heads of a
 // token share: a block takes a token or a few with all their heads, forms each
-// pair's once and keeps them in LDS.  Angles are turns in 64 bits, p (w / 2 pi), of which
-// the fraction goes on in 32 bits: a position of 10^9 costs no accuracy.
+// pair's once and keeps them in LDS.  Angles are turns, p w / (2 pi) with what the two
+// products in 64 bits round off, of which the fraction goes on in 32 bits: positions
+// up to 2^53 cost no accuracy (p (w / 2 pi) alone would be off by 2^-51 p w / 2 pi turns).
 // 16384 tokens of 40 heads of 128 in bf16 take 61 us (5.5 TB/s).
 #include "nxa_rotary.h"
 
@@ -26,9 +27,12 @@ __device__ __forceinline__ int64_t rotary_position(const RotaryParams& p, int b,
 
 // c cos and c sin of pair i at a position.
 __device__ __forceinline__ float2 rotary_turn(const RotaryParams& p, int64_t pos, int i) {
-  constexpr double kInvTwoPi = 0.15915494309189533577;
-  const double turns = (double)pos * (p.freq[i] * kInvTwoPi);
-  const float f = (float)(2.0 * (turns - __builtin_rint(turns)));
+  // (1 / (2 pi) in two numbers)
+  constexpr double kInvTwoPi = 0x1.45f306dc9c883p-3, kInvRest = -0x1.6b01ec5417056p-57;
+  const double w = p.freq[i], a = (double)pos * w, a_rest = __builtin_fma((double)pos, w, -a);
+  const double whole = __builtin_rint(a * kInvTwoPi);
+  const double rest = __builtin_fma(a, kInvRest, a_rest * kInvTwoPi);
+  const float f = (float)(2.0 * (__builtin_fma(a, kInvTwoPi, -whole) + rest));
   float s, c;
   sincospif(f, &s, &c);
   return float2{c * p.scale, (p.inverse ? -s : s) * p.scale};

@@ -355,8 +355,10 @@ def rotary_embed(
     ``scale``; elements from ``r`` on are copied.  Returns ``(q', k')`` (None for
     None).
 
-    Angles are formed in float64, the rotation in float32 (float64 inputs, which
-    the reference engine takes: float64) and rounded once.  Differentiable in q and
+    Angles are formed in float64 (off by 2^-53 of themselves in the reference engine,
+    by less than a float32's last place in the fused one up to positions of 2^53), the
+    rotation in float32 (float64 inputs, which the reference engine takes: float64) and
+    rounded once.  Differentiable in q and
     k, any number of times; forward-mode derivatives are left to the reference
     engine.  The fused engine takes bfloat16, float16 and float32 and head dims up
     to 256; ``d`` and ``r`` (half layout: ``r / 2``) in whole 16-byte chunks are

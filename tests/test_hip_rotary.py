@@ -7,6 +7,8 @@ signs (2^-20 of it bounds the sum of them), and one rounding to the type.
 
 from __future__ import annotations
 
+from fractions import Fraction
+
 import _quant_plain as qplain
 import numpy as np
 import pytest
@@ -280,3 +282,21 @@ def test_only_what_is_trained_has_a_gradient():
     nx.write_pages(*pages, turned, k, torch.zeros(1, 1, **i32), torch.zeros(1, **i32),
                    torch.tensor([0, t], **i32), backend='hip')
     assert torch.equal(pages[0][0, :, :t], turned)
+
+
+@pytest.mark.parametrize('inter', [False, True])
+def test_far_positions_to_the_last_digit(inter):
+    """Against turns in whole fractions.  In float32 a half turn is off by 2^-25 of
+    itself (2^-23.3 rad), sine and cosine by 2^-23, the products and their sum by 2^-24
+    each: 2^-21 of the terms' size covers them, wherever a token stands."""
+    pi = Fraction('3.14159265358979323846264338327950288419716939937510582097494459')
+    pos = [10 ** 9, 2 ** 31 - 1, 2 ** 40 + 12345, -2 ** 45 - 7, 2 ** 52 + 1]
+    freq = nx.rotary_frequencies(64, device=_dev())
+    x = _rand((2, len(pos), 64), torch.float32, 1)
+    got, _ = nx.rotary_embed(x, None, torch.tensor(pos, device=_dev()), freq, interleaved=inter,
+                             backend='hip')
+    turns = [[float(p * Fraction(w) / (2 * pi) % 1) for w in freq.tolist()] for p in pos]
+    # (as angles of position 1, a token at a time)
+    for i, t in enumerate(turns):
+        want, size = qplain.rotate(_n64(x)[:, i:i + 1], [1], 2 * np.pi * np.array(t), inter, 1.0)
+        assert (np.abs(_n64(got)[:, i:i + 1] - want) <= 2.0 ** -21 * size).all(), pos[i]

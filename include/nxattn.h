@@ -444,7 +444,8 @@ int nxa_quant_write(const nxa_quant_pool_desc* desc, void* k_pages, void* v_page
                     const int32_t* offsets, int32_t B, int32_t M, void* stream);
 
 /* The tokens that nxa_quant_write's arguments name, back into k [Hk, T, D] and v
- * [Hk, T, Dv]; zero for tokens of no sequence, outside the table or in no page. */
+ * [Hk, T, Dv], at most the type's largest number where s and z are finite; zero for
+ * tokens of no sequence, outside the table or in no page. */
 int nxa_quant_read(const nxa_quant_pool_desc* desc, const void* k_pages, const void* v_pages,
                    const void* scales, void* k, const int64_t* k_str, void* v,
                    const int64_t* v_str, int64_t T, const int32_t* table, int64_t table_rs,

@@ -175,7 +175,7 @@ __device__ __forceinline__ void write_row(const Eight<T>& y, bool mine, bool fir
   hi = __uint_as_float(row_reduce<LPR>(__float_as_uint(hi), [](uint32_t a, uint32_t b) {
     return __float_as_uint(max3(__uint_as_float(a), __uint_as_float(b), -INFINITY));
   }));
-  // (a row of NaN, infinity or a range past the type's reads back as NaN)
+  // (a row of NaN, infinity or a range past fp32's reads back as NaN)
   const float range = hi - lo;
   const bool bad = !(range < INFINITY);
   const T zt = (T)(bad ? NAN : lo), st = (T)(bad ? NAN : range * (1.f / TOP));
@@ -272,11 +272,15 @@ struct HeldRow {
   }
   __device__ __forceinline__ Eight<T> values() const {
     const float a = (float)sc.s, z = (float)sc.z;
+    // (a scale is rounded, up too, so that the largest code of a row that ends near the
+    // type's largest number may stand for more than that)
+    constexpr float MOST = std::is_same<T, f16>::value ? 65504.f : sizeof(T) == 2 ? 0x1.fep127f : 0x1.fffffep127f;
+    const float lim = a < INFINITY && z < INFINITY ? MOST : INFINITY;
     Eight<T> y;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t c = BITS == 4 ? w[0] >> (4 * e) & 15 : w[e / 4 % (BITS / 4)] >> (8 * (e % 4)) & 255;
-      y.x[e] = (T)__builtin_fmaf((float)c, a, z);
+      y.x[e] = (T)min3(__builtin_fmaf((float)c, a, z), lim, lim);
     }
     return y;
   }

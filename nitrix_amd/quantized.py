@@ -211,7 +211,11 @@ def _reference_read(k_pages, v_pages, scales, page_table, starts, offsets, t, bi
         sc = scales[page, :, slot]
         out = []
         for which, pages in enumerate((k_pages, v_pages)):
-            x = _values(pages[page, :, slot], sc, which, bits).to(scales.dtype)
+            x = _values(pages[page, :, slot], sc, which, bits)
+            # (a scale rounded up takes the largest code past the type's largest number)
+            finite = (sc[..., 2 * which:2 * which + 2] < math.inf).all(-1, keepdim=True)
+            top = torch.where(finite, torch.finfo(scales.dtype).max, math.inf).to(x.dtype)
+            x = torch.minimum(x, top).to(scales.dtype)
             out.append(torch.where(ok[:, None, None], x, 0).transpose(0, 1))
     return tuple(out)
 
@@ -246,7 +250,8 @@ def read_quantized_pages(
     The mirror of :func:`write_quantized_pages`: with ``offsets`` ``(b + 1,)`` and
     the number ``t`` of tokens, token ``offsets[i] + j`` is the one at position
     ``starts[i] + j`` of sequence ``i``; without, there is one a sequence, at
-    ``starts[i]``.  ``z + s c`` is rounded once.  Tokens of no sequence, outside the
+    ``starts[i]``.  ``z + s c`` is rounded once, and where the rounding of ``s`` took it
+    past the type's largest number it is that.  Tokens of no sequence, outside the
     table or in no page are zero.  For packed attention over tokens that a cache
     holds already, and for attention over what the cache holds of new ones.
     """

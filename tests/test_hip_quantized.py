@@ -672,3 +672,28 @@ def test_declined_calls_fall_back_loudly():
     gap = torch.zeros(3, 1, 32, 8, dtype=torch.uint8, device=_dev())[:, :, ::2]
     with pytest.warns(nx.NitrixBackendFallback):
         nx.read_quantized_pages(gap, gap.clone(), sc, _i32([[2]]), _i32([3]))
+
+@pytest.mark.parametrize('bits', [4, 8])
+@pytest.mark.parametrize('dtype', ['bf16', 'f16', 'f32'])
+def test_rows_up_to_the_largest_number_read_back_finite(dtype, bits):
+    """A scale rounded up takes the last code past the type's largest number: it reads
+    back as that, within the step and the scale's rounding; infinite scales and
+    minima stay what they are."""
+    dt, top = DT[dtype], (1 << bits) - 1
+    most = float(torch.finfo(dt).max)
+    lo = -most if dtype == 'f16' else 0.0
+    x = torch.linspace(0, 1, 32, dtype=torch.float64)[None, None] * (most - lo) + lo
+    x = x.to(dt).repeat(1, 5, 1).to(_dev())
+    pool = _pool(dt, 3, 1, 16, 32, 32, bits)
+    table, starts, off = _i32([[1]]), _i32([2]), _i32([0, 5])
+    nx.write_quantized_pages(*pool, x, x, table, starts, off, backend='hip')
+    sc = pool[2]
+    sc[1, 0, 4, 0], sc[1, 0, 5, 1], sc[1, 0, 6, 2] = math.inf, math.inf, math.nan
+    k, v = nx.read_quantized_pages(*pool, table, starts, off, 5, bits=bits, backend='hip')
+    for y in (k[:, :2], v[:, :4]):
+        assert torch.isfinite(y).all() and float(y.max()) == most
+        off_by = (y.double() - x[:, :y.shape[1]].double()).abs().max()
+        step = (most - lo) / top
+        assert off_by <= step / 2 + (most - lo) * torch.finfo(dt).eps
+    assert not torch.isfinite(k[0, 2]).any() and (k[0, 3] == math.inf).all()
+    assert torch.isnan(v[0, 4]).all()

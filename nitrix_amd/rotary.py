@@ -96,7 +96,8 @@ def rotary_frequencies(
                 for t in (fast_turns, slow_turns)
             )
             lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), dims - 1)
-            slow = ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+            # (no pair turns even slow_turns times: all are divided)
+            slow = torch.ones_like(i) if hi <= 0 else ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
         else:
             turns = original_length * w / (2 * math.pi)
             slow = ((fast_turns - turns) / (fast_turns - slow_turns)).clamp(0, 1)

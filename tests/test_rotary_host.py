@@ -74,6 +74,20 @@ def test_frequencies():
         torch.testing.assert_close(same, plain, rtol=1e-15, atol=0)
 
 
+@pytest.mark.parametrize('scaling', ['ramp', 'bands'])
+@pytest.mark.parametrize('length', [1, 6, 10, 64, 300, 10 ** 9, 10 ** 14])
+def test_pairs_at_either_end(scaling, length):
+    """Pairs that turn 32 times or more stay, those of one turn or less are divided,
+    also where all of them do."""
+    plain = nx.rotary_frequencies(16)
+    ratio = nx.rotary_frequencies(16, scaling=scaling, factor=4.0, original_length=length) / plain
+    turns = length * plain / (2 * math.pi)
+    assert (ratio[turns >= 32 * (1 + 1e-12)] == 1).all()
+    slow = ratio[turns <= 1 - 1e-12]
+    torch.testing.assert_close(slow, torch.full_like(slow, 0.25))
+    assert (ratio >= 0.25 - 1e-12).all() and (ratio <= 1).all()
+
+
 def test_frequency_refusals():
     for kw in (
         {'dims': 7}, {'dims': 0}, {'dims': 8, 'base': 0.0}, {'dims': 8, 'factor': -1.0},

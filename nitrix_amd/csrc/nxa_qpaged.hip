@@ -13,11 +13,11 @@
 //
 //  * K: codes in the mantissa of an fp16 64 (4 bits) or 1024 (8 bits).  What is added
 //    to them is what a product's sum starts from, -64 (1024) sum q: a score loses
-//    some 2^-24 of 64 |sum q|, no more than its codes' own sum would.  q is scaled to a
-//    largest element of 2^14 or more and then is one fp16 number, exact down to 2^-29 of
-//    that.  (fp8 numbers need no 64, c 2^-9 being their bits, and 2 operations less for
-//    8 codes.  But their products keep 13 bits below the largest of eight and drop
-//    the others' rest, and q takes two or three of them.)
+//    some 2^-24 of s times 64 (1024) |sum q|, eight times what its codes' own sum would.
+//    q is scaled to a largest element of 2^14 or more and then is one fp16 number, exact
+//    down to 2^-29 of that.  (fp8 numbers need no 64, c 2^-9 being their bits, and three
+//    operations for 8 codes in place of seven.  But their products keep 13 bits below
+//    the largest of eight and drop the others' rest, and q takes two or three of them.)
 //  * V: the same, in pairs of one column's keys.  What is added to the codes would cost
 //    digits: the values of a long row nearly cancel, to a root of its length, while
 //    their sum with 64 or 1024 does not (65536 tokens of equal weight in bf16 and 4 bits were
@@ -40,9 +40,9 @@
 // four keys.
 //
 // At head dim 128 and 8 key heads, kernel without the join: two sequences, 582,048
-// tokens together, in 4 bits (633 MB) 113 us, 5.6 TB/s, nine tenths of the rate of
-// reading alone; 64 of up to 8192 (154 MB) 43 us, of which starting on rows and the
-// first copies' latency are some 15; in 8 bits (351 MB) 73 us, 4.8 TB/s.
+// tokens together, in 4 bits (633 MB) 116 us, 5.5 TB/s, nine tenths of the rate of
+// reading alone; 64 of up to 8192 (154 MB) 47 us, of which starting on rows and the
+// first copies' latency are some 15; in 8 bits (351 MB) 75 us, 4.7 TB/s.
 #include "nxa_quant.h"
 
 #include "nxa_paged_units.h"
@@ -204,7 +204,8 @@ __device__ __forceinline__ float scale_field(const Loaded<N>& s, int f) {
 constexpr int kQuantDepth = 2;
 // Blocks a CU, by registers and LDS (37 KB at 512 bits a row and less, 70 KB at
 // 1024): three where q and O leave room for it (64 sequences of up to 8192, 4 bits,
-// three / two: 44.2 / 47.6 us).
+// three / two: 53.6 / 57.0 us a call; more than eight heads a key head, where three
+// spill 12 registers, 93 / 107).
 constexpr int quant_blocks(int es, int dp, int bits) {
   return dp > 128 ? 1 : dp * bits > 512 || (es == 4 && dp == 128) ? 2 : 3;
 }
@@ -212,11 +213,11 @@ constexpr int quant_blocks(int es, int dp, int bits) {
 // FAST: pages hold a multiple of 16 tokens, so that a half lies in one page, and
 // codes and scales are aligned: halves are copied to LDS, each wave its own, steps
 // ahead of their use.  Else every key looks its page up and codes are loaded four
-// bytes at a time (64 sequences of up to 8192, 4 bits, 44 / 71 us, 8 bits 73 / 160).
+// bytes at a time (64 sequences of up to 8192, 4 bits, 54 / 79 us, 8 bits 73 / 162).
 // PAIR: eight heads a key head or fewer leave half of a product's columns idle.  q
 // then stands in both halves, and columns from 8 on take the softmax of the second
 // half's keys, whose weights go back to the heads' columns for V's product (two
-// sequences of up to 400000, four heads a key head, with / without 114 / 126 us).
+// sequences of up to 400000, four heads a key head, with / without 130 / 146 us).
 template <typename T, int DP, int BITS, bool FAST, bool PAIR>
 __global__ __launch_bounds__(256, quant_blocks(sizeof(T), DP, BITS)) void
 qpaged_kernel(const QuantPagedParams p) {
@@ -763,9 +764,9 @@ qpaged_kernel(const QuantPagedParams p) {
 int qpaged_dp(int m) { return m <= 64 ? 64 : m <= 128 ? 128 : 256; }
 
 // Rows a block each, of tables this short, against rows cut into equal work and
-// joined.  us at head dim 128, 4 bits: 32 rows of 700 tokens 12.8 / 16.8, of 1000 15.4 /
-// 17.1, of 2000 23.1 / 20.9; 256 rows of up to 2048 24 / 30, 512 30 / 38 (one of 2048
-// among short ones 23.6 / 24.9); 512 of up to 4096 48.5 / 47.6 (one of 4096 38 / 25).
+// joined.  us a call at head dim 128, 4 bits: 32 rows of 700 or 1000 tokens 18 / 23, of
+// 2000 25.3 / 22.8; 256 rows of up to 2048 25.6 / 30.3, 512 33.4 / 38.6; 512 of up to
+// 4096 54 / 48.
 bool qpaged_whole(int64_t room, int64_t rows) {
   return room <= (rows < 256 ? 1024 : 2304);
 }

@@ -43,9 +43,9 @@ struct QuantPagedParams : PagedParams {  // k_str, v_str in bytes
 };
 
 // What starting on a row costs a block, in units of 128 tokens (its first page ids,
-// copies and q, with nothing to work on meanwhile).  us with 1 / 3 / 5: 48 rows of up to
-// 8192 tokens, 4 bits, 54.5 / 45.4 / 44.6, 8 bits 86.4 / 74.9 / 73.3; 2 rows of 131072
-// 132 / 131 / 129.
+// copies and q, with nothing to work on meanwhile).  us a call with 1 / 3 / 5 / 8: 64
+// sequences of up to 8192 tokens, 4 bits, 61 / 54 / 54 / 56, 8 bits 88 / 73 / 73 / 78; two
+// of up to 400000 135 / 134 / 130 / 129.
 constexpr int kQuantStart = 5;
 int qpaged_dp(int m);  // padded head dim
 bool qpaged_whole(int64_t room, int64_t rows);  // a block a row (sequence and head)

@@ -697,3 +697,25 @@ def test_rows_up_to_the_largest_number_read_back_finite(dtype, bits):
         assert off_by <= step / 2 + (most - lo) * torch.finfo(dt).eps
     assert not torch.isfinite(k[0, 2]).any() and (k[0, 3] == math.inf).all()
     assert torch.isnan(v[0, 4]).all()
+
+
+@pytest.mark.parametrize('b', [1023, 1024, 3000])
+def test_many_sequences_written_and_read(b):
+    """Offsets that are kept on the chip and ones that are not; empty sequences."""
+    rng = np.random.default_rng(b)
+    new = rng.integers(0, 4, b)
+    off = np.concatenate([[2], 2 + np.cumsum(new)]).astype(np.int32)
+    t, hk, d = int(off[-1]) + 3, 1, 16
+    starts = rng.integers(0, 30, b).astype(np.int32)
+    table = rng.permutation(3 * b).reshape(b, 3).astype(np.int32)
+    pools = [_pool(torch.float16, 3 * b, hk, 16, d, d, 8) for _ in range(2)]
+    x, y = (_rand((hk, t, d), torch.float16, s) for s in (1, 2))
+    args = _i32(table), _i32(starts), _i32(off)
+    held = []
+    for pool, backend in zip(pools, ('hip', 'jax')):
+        nx.write_quantized_pages(*pool, x, y, *args, backend=backend)
+        held.append(nx.read_quantized_pages(*pool, *args, t, bits=8, backend=backend))
+    assert all(torch.equal(a, b) for a, b in zip(*pools))
+    for got, want in zip(*held):
+        torch.testing.assert_close(got, want, rtol=2.0 ** -10, atol=2.0 ** -24)
+    assert (held[0][0][:, :2] == 0).all() and (held[0][0][:, -3:] == 0).all()

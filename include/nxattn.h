@@ -437,7 +437,8 @@ typedef struct {
 /* Host-only validation (no GPU needed). */
 int nxa_quant_pool_check(const nxa_quant_pool_desc* desc);
 
-/* New tokens into their pages as nxa_pages_write does, quantised. */
+/* New tokens into their pages as nxa_pages_write does, quantised (T <= 2^26 - 4; of
+ * tokens meant for one slot codes and scales may be either's). */
 int nxa_quant_write(const nxa_quant_pool_desc* desc, void* k_pages, void* v_pages, void* scales,
                     const void* k, const int64_t* k_str, const void* v, const int64_t* v_str,
                     int64_t T, const int32_t* table, int64_t table_rs, const int32_t* starts,

@@ -163,12 +163,13 @@ def write_quantized_pages(
     code (4 or 8) follow from the widths of the pages.  Of each row ``z`` is the
     minimum, ``s`` the range times ``1 / (2^bits - 1)`` (both in float32), rounded to
     the scales' dtype, and codes are the exact quotients ``(x - z) / s`` rounded to
-    the nearest, ties to even.  A row that holds NaN or infinity, or whose range exceeds float32's, is
-    NaN when it is read; a constant row is exact.
+    the nearest, ties to even.  A row that holds NaN or infinity, or whose range
+    exceeds float32's, is NaN when it is read; a constant row is exact.
 
     The fused engine takes bfloat16, float16 and float32 and head dims up to 256
     in multiples of 8.  Two rows that share the page a token goes to write over
-    each other: which of them a slot ends up with is not defined.
+    each other: which of them a slot ends up with, codes and scales each, is not
+    defined.
     """
     name = 'write_quantized_pages'
     _check_quantized(name, k_pages, v_pages, scales, written=True)
@@ -360,9 +361,11 @@ def quantized_paged_attention(
     :func:`~nitrix_amd.paged.paged_attention` of what the codes stand for: q
     ``(b, h, d)`` in the scales' dtype, the result ``(b, h, d_v)``.  Bits a code (4
     or 8) follow from ``d`` and the pages' width.  Keys and values are not rounded
-    to the type on the way; tokens in no page, lengths outside the table's room and
-    rows without tokens are treated as there.  A page row has room for less than
-    2^31 - 4096 tokens.
+    to the type on the way, and scores, weights and sums are float32's; tokens in no
+    page, lengths outside the table's room and rows without tokens are treated as
+    there.  A page row has room for less than 2^31 - 4096 tokens.  Keys past 2^100, and
+    values whose sum over the tokens passes 2^119, leave float32; of values' scales
+    below 2^-90 digits are lost.
 
     The fused engine takes bfloat16, float16 and float32, head dims up to 256 in
     multiples of 8 and pages of any number of slots (a multiple of 16 is fastest, as

@@ -58,7 +58,7 @@ constexpr int kHalfKeys = 16;
 template <typename T, int DP, int BITS>
 struct QuantStep {
   static constexpr int ES = sizeof(T);
-  static constexpr bool F32 = ES == 4, F16 = std::is_same<T, f16>::value;
+  static constexpr bool F32 = ES == 4;
   static constexpr int NKW = DP * BITS / 128;       // dwords of K's codes a lane and half
   static constexpr int NJ = DP / 32;                // products of a half's S
   static constexpr int DPL = DP / 16;               // V columns of a lane
@@ -553,9 +553,8 @@ qpaged_kernel(const QuantPagedParams p) {
       }
       // (a term is to be that of the rounded product, which the next is taken from;
       // the compiler would round the exact one to fp16 for it)
-      if constexpr (PT > 1)
 #pragma unroll
-        for (int i = 0; i < SC; ++i) asm("" : "+v"(x[i]));
+      for (int i = 0; i < SC; ++i) asm("" : "+v"(x[i]));
       u32x4 pf[PT];
 #pragma unroll
       for (int t = 0; t < PT; ++t)

@@ -10,7 +10,7 @@
 // token share: a block takes a token or a few with all their heads, forms each
 // pair's once and keeps them in LDS.  Angles are turns, p w / (2 pi) with what the two
 // products in 64 bits round off, of which the fraction goes on in 32 bits: positions
-// up to 2^53 cost no accuracy (p (w / 2 pi) alone would be off by 2^-51 p w / 2 pi turns).
+// up to 2^53 cost no accuracy (p (w / 2 pi) alone would be off by 2^-53 of itself).
 // 16384 tokens of 40 heads of 128 in bf16 take 61 us (5.5 TB/s).
 #include "nxa_rotary.h"
 

@@ -63,7 +63,7 @@ CASES = [
     ('f32', 3, 1, 11, 7, 6, False),
     ('bf16', 1, 1, 3, 2, 2, True),
     ('f16', 2, 1, 5, 255, 254, False),
-    # many tokens: a block takes four, or one of many heads
+    # many tokens: a block takes four
     ('bf16', 3, 1, 1031, 128, 64, False),
     ('f16', 4, 4, 514, 64, 64, True),
     ('f32', 1, 1, 2001, 32, 20, False),
